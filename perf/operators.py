@@ -1,0 +1,432 @@
+"""Performance cases of attention's backward pass and of the 4-bit key/value cache.
+
+Three operators: the gradients of one attention call (`flash_atten.attention_backward`), the append of new
+key/value rows to a cache that holds them in 4 bits (`kv4.Kv4Cache.append`), and attention over that cache
+(`flash_atten.sdpa_kv4`). Sizes are those of the benchmark, the tests and the decode and prefill harnesses,
+and generic odd ones.
+
+The cache format: each row of D channels is cut into blocks of 32. A block keeps one scale byte e, standing
+for 2^(e - 127), and 32 codes of 4 bits (sign, 2 exponent bits, 1 mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6),
+channel 2i in the low half of byte i. With `a` the block's largest magnitude, e is the exponent byte of
+float32(a) with a carry from mantissas of 1.75 and up, less 2, and at least the type's floor; a value becomes
+the code nearest to value / 2^(e - 127), ties to the even code, at most 6. A block with an infinity or NaN gets
+e = 255, and all of it stands for NaN.
+"""
+from __future__ import annotations
+
+import math
+import sys
+from pathlib import Path
+
+import torch
+
+own = False
+
+_PKG = str(Path(__file__).resolve().parent.parent / "flash-attn-economical-gpu_amd")
+_DTYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
+_FLOOR = {torch.float16: 104, torch.bfloat16: 2}  # scale bytes below these would leave the type's range
+_BLOCK = 32
+_CODES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def _modules():
+    if _PKG not in sys.path:
+        sys.path.insert(0, _PKG)
+    import flash_atten
+    import kv4
+
+    return flash_atten, kv4
+
+
+def _bwd(name, dtype, B, H, H_kv, M, N, D, causal=False, views=False):
+    case = {"op": "backward", "dtype": dtype, "B": B, "H": H, "H_kv": H_kv, "M": M, "N": N, "D": D, "causal": causal,
+            "views": views}
+    return case if name is None else {"name": name, **case}
+
+
+def _append(name, dtype, B, H_kv, rows, capacity, D, ragged=False):
+    case = {"op": "append", "dtype": dtype, "B": B, "H_kv": H_kv, "rows": rows, "capacity": capacity, "D": D,
+            "ragged": ragged}
+    return case if name is None else {"name": name, **case}
+
+
+def _attend(name, dtype, B, H, H_kv, M, capacity, D, ragged=False, lse=False):
+    case = {"op": "attend", "dtype": dtype, "B": B, "H": H, "H_kv": H_kv, "M": M, "capacity": capacity, "D": D,
+            "ragged": ragged, "lse": lse}
+    return case if name is None else {"name": name, **case}
+
+
+def listed():
+    return [
+        # gradients at the smallest attention configuration (latency and launch cost)
+        _bwd("bwd_f16_d64_512", "f16", 1, 4, 4, 512, 512, 64),
+        # a training step's causal layer
+        _bwd("bwd_f16_d128_2k_causal", "f16", 4, 32, 32, 2048, 2048, 128, True),
+        # the benchmark's headline shape, backwards (the largest call)
+        _bwd("bwd_f16_d128_8k", "f16", 4, 32, 32, 8192, 8192, 128),
+        # one 4096-token sequence in a grouped-query decoder: strided projection views, few key/value heads
+        _bwd("bwd_bf16_gqa_4k_causal", "bf16", 1, 12, 2, 4096, 4096, 128, True, True),
+        # the benchmark's large head dimension
+        _bwd("bwd_bf16_d256_2k", "bf16", 2, 16, 16, 2048, 2048, 256),
+        # cross-attention of odd lengths
+        _bwd("bwd_bf16_d64_777x1283", "bf16", 2, 16, 16, 777, 1283, 64),
+        # one new token for each sequence of a serving batch (latency)
+        _append("append_bf16_b32_token", "bf16", 32, 8, 1, 8192, 128),
+        # prompts of unequal lengths enter the cache; the layer goes on with the values that the cache now holds
+        _append("append_bf16_b4_prompts", "bf16", 4, 8, 4096, 8192, 128, True),
+        # decode step of a single sequence against 8k cached tokens
+        _attend("attend_bf16_b1_8k", "bf16", 1, 32, 8, 1, 8192, 128),
+        # decode step of a serving batch with long caches of unequal lengths (bandwidth)
+        _attend("attend_bf16_b8_32k", "bf16", 8, 32, 8, 1, 32768, 128, True),
+        # four drafted tokens are checked at once, head dimension 64, log-sum-exp kept
+        _attend("attend_f16_d64_m4", "f16", 4, 16, 2, 4, 65536, 64, True, True),
+        # a chunk of a long prompt attends to what is cached and to itself
+        _attend("attend_f16_chunk_509", "f16", 2, 28, 4, 509, 16384, 128, True),
+    ]
+
+
+def _log_uniform(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+_MAX_PAIRS = 4 * 32 * 8192 * 8192 * 128  # B H M N D of the largest listed case
+
+
+def draw(rng):
+    op = rng.choice(["backward", "backward", "backward", "append", "attend", "attend"])
+    dtype = rng.choice(["f16", "bf16"])
+    D = rng.choice([64, 128, 128, 256])
+    if op == "backward":
+        H_kv = rng.choice([1, 2, 4, 8, 16])
+        H = H_kv * rng.choice([1, 1, 2, 4, 7])
+        B = rng.choice([1, 1, 2, 3, 4])
+        N = _log_uniform(rng, 128, 8192)
+        M = N if rng.random() < 0.6 else _log_uniform(rng, 16, 8192)
+        while B * H * M * N * D > _MAX_PAIRS // 4:
+            M, N = (M + 1) // 2, (N + 1) // 2
+        return _bwd(None, dtype, B, H, H_kv, M, N, D, rng.random() < 0.5, rng.random() < 0.5)
+    H_kv = rng.choice([1, 2, 4, 8])
+    if op == "append":
+        B = rng.choice([1, 2, 4, 8, 32])
+        rows = rng.choice([1, 1, 4, _log_uniform(rng, 16, 8192), _log_uniform(rng, 16, 8192)])
+        while B * H_kv * rows * D > 1 << 26:
+            rows = (rows + 1) // 2
+        return _append(None, dtype, B, H_kv, rows, rows + _log_uniform(rng, 64, 8192), D, rng.random() < 0.5)
+    H = H_kv * rng.choice([1, 2, 4, 6, 7, 8])
+    B = rng.choice([1, 1, 2, 4, 8, 16])
+    capacity = _log_uniform(rng, 64, 131072)
+    while B * H_kv * capacity * D > 8 * 8 * 32768 * 128:
+        capacity = (capacity + 1) // 2
+    M = rng.choice([1, 1, 1, 3, 8, _log_uniform(rng, 16, 1024)])
+    M = min(M, capacity)
+    while B * H * M * capacity * D > _MAX_PAIRS // 64:
+        M = (M + 1) // 2
+    return _attend(None, dtype, B, H, H_kv, M, capacity, D, rng.random() < 0.5, M <= 8 and rng.random() < 0.5)
+
+
+def _lengths(case):
+    """Cached tokens of each sequence, new ones included, and how many of the rows given are new tokens."""
+    B, capacity = case["B"], case["capacity"]
+    rows = case["M"] if case["op"] == "attend" else case["rows"]
+    out = []
+    for b in range(B):
+        total = capacity - (capacity // 2) * b // B if case["ragged"] else capacity
+        total = max(total, 1)
+        new = min(rows, total)
+        if case["ragged"] and rows > 16:
+            new = max(1, min(new, rows - (rows // 2) * b // B))
+        out.append((total, new))
+    return out
+
+
+def _heads(x, H):
+    return x.repeat_interleave(H // x.shape[1], dim=1)
+
+
+def _chunks(B, H, per_head):
+    """Ranges over flattened (batch, head) pairs whose score matrices fit a few GB together."""
+    step = max(1, min(B * H, (1 << 28) // max(1, per_head)))
+    return [(i, min(i + step, B * H)) for i in range(0, B * H, step)]
+
+
+def _hidden(M, N, device):
+    return torch.arange(N, device=device)[None, :] > torch.arange(M, device=device)[:, None]
+
+
+def _quantize(x):
+    """Scale bytes [..., D / 32] and codes [..., D / 2] (two in a byte) of x."""
+    f = x.float().unflatten(-1, (-1, _BLOCK))
+    bits = f.abs().amax(dim=-1).view(torch.int32)
+    e = (((bits + 0x200000) >> 23) - 2).clamp(min=_FLOOR[x.dtype])
+    bad = bits >= 0x7F800000
+    y = (f * ((254 - e) << 23).view(torch.float32)[..., None]).masked_fill_(bad[..., None], 0.0)
+    a = y.abs()
+    code = ((a > 0.25).to(torch.uint8) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0))
+    code = (code | (torch.signbit(f) & ~bad[..., None]).to(torch.uint8) << 3).flatten(-2)
+    return torch.where(bad, 255, e).to(torch.uint8), code[..., 0::2] | code[..., 1::2] << 4
+
+
+def _dequantize(scales, codes):
+    """float32 values that scale bytes and codes stand for."""
+    table = torch.tensor(_CODES + tuple(-c for c in _CODES), device=codes.device)
+    pair = torch.stack((codes & 15, codes >> 4), dim=-1).flatten(-2)
+    e = scales.to(torch.int32)
+    scale = (e << 23).view(torch.float32).masked_fill(e == 255, math.nan)
+    return (table[pair.int()].unflatten(-1, (-1, _BLOCK)) * scale[..., None]).flatten(-2)
+
+
+def _inputs(case, seed):
+    """The case's tensors: the same values for prepare() and exact()."""
+    dev = torch.device("cuda")
+    gen = torch.Generator(device=dev).manual_seed(seed)
+    dtype = _DTYPES[case["dtype"]]
+    B, D = case["B"], case["D"]
+
+    def normal(*shape, sigma=1.0):
+        return (torch.randn(shape, device=dev, generator=gen) * sigma).to(dtype)
+
+    if case["op"] == "backward":
+        H, H_kv, M, N = (case[x] for x in ("H", "H_kv", "M", "N"))
+        sigma = 0.5 if D == 256 else 1.0
+        if case["views"]:  # projection outputs [B, S, heads, D], seen by the layer as [B, heads, S, D]
+            q, k, v, do = (normal(B, s, h, D, sigma=f).transpose(1, 2)
+                           for s, h, f in ((M, H, sigma), (N, H_kv, sigma), (N, H_kv, sigma), (M, H, 0.02)))
+        else:
+            q, k, v, do = (normal(B, h, s, D, sigma=f)
+                           for s, h, f in ((M, H, sigma), (N, H_kv, sigma), (N, H_kv, sigma), (M, H, 0.02)))
+        o = torch.empty_like(q)
+        lse = torch.empty(B, H, M, device=dev)
+        qf = q.float().reshape(B * H, M, D)
+        kt = _heads(k.float(), H).reshape(B * H, N, D).transpose(1, 2).contiguous()
+        vf = _heads(v.float(), H).reshape(B * H, N, D)
+        of, lf = torch.empty_like(qf), lse.view(B * H, M)
+        for i, j in _chunks(B, H, M * N):
+            s = (qf[i:j] @ kt[i:j]).mul_(D ** -0.5)
+            if case["causal"]:
+                s.masked_fill_(_hidden(M, N, dev), -math.inf)
+            lf[i:j] = torch.logsumexp(s, dim=-1)
+            of[i:j] = s.sub_(lf[i:j, :, None]).exp_() @ vf[i:j]
+        o.copy_(of.view(B, H, M, D))
+        return do, q, k, v, o, lse
+
+    H_kv, lengths = case["H_kv"], _lengths(case)
+    order = torch.randperm(B, device=dev, generator=gen).tolist()
+    total = [lengths[b][0] for b in order]
+    new = [lengths[b][1] for b in order]
+    start = torch.tensor([t - n for t, n in zip(total, new)], device=dev, dtype=torch.int32)
+    count = torch.tensor(new, device=dev, dtype=torch.int32)
+    # channels of keys differ in size by a factor of ten or so, those of values less
+    k_size = (torch.randn(H_kv, 1, D, device=dev, generator=gen) * 0.6).exp()
+    v_size = (torch.randn(H_kv, 1, D, device=dev, generator=gen) * 0.2).exp()
+    if case["op"] == "append":
+        rows = case["rows"]
+        k, v = ((torch.randn(B, rows, H_kv, D, device=dev, generator=gen).transpose(1, 2) * s).to(dtype)
+                for s in (k_size, v_size))
+        return k, v, start, count
+    capacity = case["capacity"]
+    cache = []
+    for size in (k_size, v_size):
+        parts = [_quantize((torch.randn(H_kv, capacity, D, device=dev, generator=gen) * size).to(dtype)) for _ in range(B)]
+        cache += [torch.stack([p[0] for p in parts]), torch.stack([p[1] for p in parts])]
+    q = (torch.randn(B, case["M"], case["H"], D, device=dev, generator=gen).to(dtype)).transpose(1, 2)
+    return (q, *cache, start, count)
+
+
+def prepare(case, seed):
+    x = _inputs(case, seed)
+    state = {"case": case, "in": x}
+    if case["op"] == "backward":
+        return state
+    B, H_kv, capacity, D = (case[n] for n in ("B", "H_kv", "capacity", "D"))
+    if own:
+        _, kv4 = _modules()
+        cache = state["cache"] = kv4.Kv4Cache(B, H_kv, capacity, D, dtype=_DTYPES[case["dtype"]], device=x[0].device)
+        if case["op"] == "attend":
+            for buffer, held in zip((cache.k_scales, cache.k_codes, cache.v_scales, cache.v_codes), x[1:5]):
+                buffer.copy_(held)
+            state["in"] = (x[0], None, None, None, None, x[5], x[6])
+    elif case["op"] == "append":
+        state["cache"] = [torch.zeros(B, H_kv, capacity, n, device=x[0].device, dtype=torch.uint8)
+                          for n in (D // _BLOCK, D // 2, D // _BLOCK, D // 2)]
+    return state
+
+
+def _plain_backward(case, do, q, k, v, o, lse):
+    B, H, H_kv, M, N, D = (case[x] for x in ("B", "H", "H_kv", "M", "N", "D"))
+    scale = D ** -0.5
+    delta = (do.float() * o.float()).sum(dim=-1).reshape(B * H, M, 1)
+    qf, dof = q.float().reshape(B * H, M, D), do.float().reshape(B * H, M, D)
+    kf, vf = (_heads(t.float(), H).reshape(B * H, N, D) for t in (k, v))
+    kt, vt = kf.transpose(1, 2).contiguous(), vf.transpose(1, 2).contiguous()
+    lf = lse.reshape(B * H, M, 1)
+    dq, dk, dv = torch.empty_like(qf), torch.empty_like(kf), torch.empty_like(vf)
+    for i, j in _chunks(B, H, M * N):
+        p = (qf[i:j] @ kt[i:j]).mul_(scale).sub_(lf[i:j]).exp_()
+        if case["causal"]:
+            p.masked_fill_(_hidden(M, N, p.device), 0.0)
+        ds = (dof[i:j] @ vt[i:j]).sub_(delta[i:j]).mul_(p)
+        dq[i:j] = (ds @ kf[i:j]).mul_(scale)
+        dk[i:j] = (ds.transpose(1, 2).contiguous() @ qf[i:j]).mul_(scale)
+        dv[i:j] = p.transpose(1, 2).contiguous() @ dof[i:j]
+    dk, dv = (t.view(B, H_kv, H // H_kv, N, D).sum(dim=2) for t in (dk, dv))
+    return dq.view(B, H, M, D).to(q.dtype), dk.to(k.dtype), dv.to(v.dtype)
+
+
+def _plain_append(case, cache, k, v, start, count):
+    """Rows of k and v into the cache. Returns what those rows now stand for (zeros in rows that are no new
+    token) and the cache."""
+    B, H_kv, rows, _ = k.shape
+    row = torch.arange(rows, device=k.device)
+    held = (row[None, :] < count[:, None])[:, None, :, None]
+    at = (start[:, None] + row[None, :]).clamp(max=case["capacity"] - 1)[:, None, :, None].long()
+    out = []
+    for x, scales, codes in ((k, cache[0], cache[1]), (v, cache[2], cache[3])):
+        e, c = _quantize(x)
+        for buffer, new in ((scales, e), (codes, c)):
+            index = at.expand(new.shape)
+            buffer.scatter_(2, index, torch.where(held, new, buffer.gather(2, index)))
+        out.append(_dequantize(e, c).masked_fill(~held, 0.0).to(x.dtype))
+    return (*out, *cache)
+
+
+def _plain_attend(case, q, k_scales, k_codes, v_scales, v_codes, start, count):
+    B, H, M, D = q.shape
+    H_kv, N = k_codes.shape[1], k_codes.shape[2]
+    out = torch.empty(B, H, M, D, device=q.device, dtype=q.dtype)
+    lse = torch.empty(B, H, M, device=q.device)
+    row = torch.arange(M, device=q.device)
+    column = torch.arange(N, device=q.device)
+    for b in range(B):
+        kf, vf = _dequantize(k_scales[b], k_codes[b]), _dequantize(v_scales[b], v_codes[b])
+        used = (column < start[b] + count[b])[None, :, None]
+        kt = kf.masked_fill_(~used, 0.0).transpose(1, 2).contiguous()
+        vf.masked_fill_(~used, 0.0)
+        seen = (column[None, :] <= (start[b] + row)[:, None]) & (row < count[b])[:, None]
+        for h in range(H_kv):
+            heads = slice(h * (H // H_kv), (h + 1) * (H // H_kv))
+            qf = q[b, heads].float().reshape(-1, D)
+            s = (qf @ kt[h]).mul_(D ** -0.5).view(-1, M, N).masked_fill_(~seen, -math.inf)
+            top = s.amax(dim=-1, keepdim=True).clamp(min=torch.finfo(torch.float32).min)
+            p = s.sub_(top).exp_()
+            total = p.sum(dim=-1, keepdim=True)
+            lse[b, heads] = (top + total.log())[..., 0]
+            o = (p.view(-1, N) @ vf[h]).view(-1, M, D) / total
+            out[b, heads] = o.masked_fill(total == 0, 0.0).to(q.dtype)
+    return (out, lse) if case["lse"] else out
+
+
+def run(state):
+    case, x = state["case"], state["in"]
+    if case["op"] == "backward":
+        if own:
+            return _modules()[0].attention_backward(*x, causal=case["causal"])
+        return _plain_backward(case, *x)
+    if case["op"] == "append":
+        cache = state["cache"]
+        if own:
+            values = cache.append(*x[:3], count=x[3], return_values=True)
+            return (*values, cache.k_scales, cache.k_codes, cache.v_scales, cache.v_codes)
+        return _plain_append(case, cache, *x)
+    if own:
+        return _modules()[0].sdpa_kv4(x[0], state["cache"], x[5], count=x[6], return_lse=case["lse"])
+    return _plain_attend(case, *x)
+
+
+def work(case):
+    B, D = case["B"], case["D"]
+    if case["op"] == "backward":
+        H, H_kv, M, N = (case[x] for x in ("H", "H_kv", "M", "N"))
+        pairs = sum(min(i + 1, N) for i in range(M)) if case["causal"] else M * N
+        # q, o, do, dq; k, v, dk, dv; lse. Products: scores, dP, dV, dQ, dK.
+        return {"bytes": 2 * (4 * B * H * M * D + 4 * B * H_kv * N * D) + 4 * B * H * M, "flops": 10 * B * H * pairs * D}
+    H_kv = case["H_kv"]
+    packed = D // 2 + D // _BLOCK  # bytes of one cached row of keys or values
+    if case["op"] == "append":
+        new = sum(n for _, n in _lengths(case))
+        return {"bytes": 2 * H_kv * (new * (2 * D + packed) + 2 * B * case["rows"] * D),
+                "flops": 4 * H_kv * new * D}
+    H, M = case["H"], case["M"]
+    keys = pairs = 0
+    for total, new in _lengths(case):
+        keys += total
+        pairs += sum(total - new + i + 1 for i in range(new))
+    return {"bytes": 2 * H_kv * keys * packed + 4 * B * H * M * D + (4 * B * H * M if case["lse"] else 0),
+            "flops": 4 * H * pairs * D}
+
+
+def _exact_backward(case, do, q, k, v, o, lse):
+    B, H, H_kv, M, N, D = (case[x] for x in ("B", "H", "H_kv", "M", "N", "D"))
+    group, scale = H // H_kv, 1.0 / math.sqrt(D)
+    dq = torch.empty(B, H, M, D, device=q.device, dtype=torch.float64)
+    dk = torch.zeros(B, H_kv, N, D, device=q.device, dtype=torch.float64)
+    dv = torch.zeros_like(dk)
+    for b in range(B):
+        for h in range(H):
+            keys, values = k[b, h // group].double().contiguous(), v[b, h // group].double().contiguous()
+            queries, g = q[b, h].double().contiguous(), do[b, h].double().contiguous()
+            p = torch.exp(queries @ keys.t().contiguous() * scale - lse[b, h].double()[:, None])
+            if case["causal"]:
+                p = p.tril()
+            slope = p * (g @ values.t().contiguous() - torch.linalg.vecdot(g, o[b, h].double())[:, None])
+            dq[b, h] = slope @ keys * scale
+            dk[b, h // group] += slope.t().contiguous() @ queries * scale
+            dv[b, h // group] += p.t().contiguous() @ g
+    return dq, dk, dv
+
+
+def _exact_values(x):
+    """64-bit values that the cache holds for x, by the distances to all codes."""
+    f = x.double().unflatten(-1, (-1, _BLOCK))
+    a = f.abs().amax(dim=-1, keepdim=True)
+    mantissa, exponent = torch.frexp(a)  # a = mantissa 2^exponent, mantissa in [0.5, 1)
+    power = torch.where(a > 0, exponent - 3 + (mantissa >= 0.875), -1000).clamp(min=_FLOOR[x.dtype] - 127).double()
+    step = torch.pow(torch.tensor(2.0, device=x.device, dtype=torch.float64), power)
+    y = (f / step).abs()
+    best = torch.zeros_like(y)
+    gap = y.clone()
+    for n, c in enumerate(_CODES[1:], start=1):
+        d = (y - c).abs()
+        nearer = (d < gap) | ((d == gap) & (n % 2 == 0))
+        best, gap = torch.where(nearer, c, best), torch.where(nearer, d, gap)
+    value = torch.where(f < 0, -best, best) * step
+    return torch.where(torch.isfinite(a), value, math.nan).flatten(-2)
+
+
+def _exact_attend(case, q, k_scales, k_codes, v_scales, v_codes, start, count):
+    B, H, M, D = q.shape
+    group = H // case["H_kv"]
+    out = torch.zeros(B, H, M, D, device=q.device, dtype=torch.float64)
+    lse = torch.full((B, H, M), -math.inf, device=q.device, dtype=torch.float64)
+    magnitude = torch.tensor(_CODES, device=q.device, dtype=torch.float64)
+
+    def values(scales, codes):
+        x = torch.empty(codes.shape[0], 2 * codes.shape[1], device=q.device, dtype=torch.float64)
+        for half in (0, 1):
+            c = (codes >> (4 * half)).long() & 15
+            x[:, half::2] = magnitude[c & 7] * (1 - 2 * (c >> 3))
+        return x * torch.pow(2.0, scales.double() - 127.0).repeat_interleave(_BLOCK, dim=1)
+
+    for b in range(B):
+        first, new = int(start[b]), int(count[b])
+        n = first + new
+        for h in range(H):
+            keys = values(k_scales[b, h // group, :n], k_codes[b, h // group, :n])
+            held = values(v_scales[b, h // group, :n], v_codes[b, h // group, :n])
+            s = q[b, h, :new].double() @ keys.t().contiguous() / math.sqrt(D)
+            s = s.masked_fill(torch.ones(new, n, device=q.device, dtype=torch.bool).triu(first + 1), -math.inf)
+            out[b, h, :new] = torch.softmax(s, dim=1) @ held
+            lse[b, h, :new] = torch.logsumexp(s, dim=1)
+    return (out, lse) if case["lse"] else out
+
+
+def exact(case, seed):
+    x = _inputs(case, seed)
+    if case["op"] == "backward":
+        return _exact_backward(case, *x)
+    if case["op"] == "attend":
+        return _exact_attend(case, *x)
+    k, v, _, count = x
+    row = torch.arange(case["rows"], device=k.device)
+    held = (row[None, :] < count[:, None])[:, None, :, None]
+    # the cache's own bytes are whole numbers: equal to the plain form's, or wrong
+    return (*(_exact_values(t).masked_fill(~held, 0.0) for t in (k, v)), None, None, None, None)
