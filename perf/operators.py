@@ -8,8 +8,8 @@ and generic odd ones.
 The cache format: each row of D channels is cut into blocks of 32. A block keeps one scale byte e, standing
 for 2^(e - 127), and 32 codes of 4 bits (sign, 2 exponent bits, 1 mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6),
 channel 2i in the low half of byte i. With `a` the block's largest magnitude, e is the exponent byte of
-float32(a) with a carry from mantissas of 1.75 and up, less 2, and at least the type's floor; a value becomes
-the code nearest to value / 2^(e - 127), ties to the even code, at most 6. A block with an infinity or NaN gets
+float32(a) with a carry from mantissas of 1.75 and up, less 2, kept where the type holds half a step and six
+steps; a value becomes the code nearest to value / 2^(e - 127), ties to the even code, at most 6. A block with an infinity or NaN gets
 e = 255, and all of it stands for NaN.
 """
 from __future__ import annotations
@@ -24,7 +24,7 @@ own = False
 
 _PKG = str(Path(__file__).resolve().parent.parent / "flash-attn-economical-gpu_amd")
 _DTYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
-_FLOOR = {torch.float16: 104, torch.bfloat16: 2}  # scale bytes below these would leave the type's range
+_RANGE = {torch.float16: (104, 140), torch.bfloat16: (2, 252)}  # of scale bytes: 0.5 and 6 times them fit the type
 _BLOCK = 32
 _CODES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
@@ -157,7 +157,7 @@ def _quantize(x):
     """Scale bytes [..., D / 32] and codes [..., D / 2] (two in a byte) of x."""
     f = x.float().unflatten(-1, (-1, _BLOCK))
     bits = f.abs().amax(dim=-1).view(torch.int32)
-    e = (((bits + 0x200000) >> 23) - 2).clamp(min=_FLOOR[x.dtype])
+    e = (((bits + 0x200000) >> 23) - 2).clamp(*_RANGE[x.dtype])
     bad = bits >= 0x7F800000
     y = (f * ((254 - e) << 23).view(torch.float32)[..., None]).masked_fill_(bad[..., None], 0.0)
     a = y.abs()
@@ -379,7 +379,8 @@ def _exact_values(x):
     f = x.double().unflatten(-1, (-1, _BLOCK))
     a = f.abs().amax(dim=-1, keepdim=True)
     mantissa, exponent = torch.frexp(a)  # a = mantissa 2^exponent, mantissa in [0.5, 1)
-    power = torch.where(a > 0, exponent - 3 + (mantissa >= 0.875), -1000).clamp(min=_FLOOR[x.dtype] - 127).double()
+    power = torch.where(a > 0, exponent - 3 + (mantissa >= 0.875), -1000).clamp(
+        *(e - 127 for e in _RANGE[x.dtype])).double()
     step = torch.pow(torch.tensor(2.0, device=x.device, dtype=torch.float64), power)
     y = (f / step).abs()
     best = torch.zeros_like(y)
