@@ -21,11 +21,10 @@
 constexpr int64_t kScratchBytes = FA_NOALLOC_SCRATCH_BYTES;
 static __device__ __align__(256) unsigned char scratch[kScratchBytes];
 
-namespace {
+static thread_local std::string g_last_error;
 
-thread_local std::string g_last_error;
+namespace fa {
 
-int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int fail(int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
@@ -40,6 +39,13 @@ int ok() {
   g_last_error.clear();
   return FA_OK;
 }
+
+}  // namespace fa
+
+namespace {
+
+using fa::fail;
+using fa::ok;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -1,0 +1,527 @@
+// Attention backward for gfx950: dQ, dK and dV of O = softmax(scale Q K^T) V, recomputing P from the
+// forward's log-sum-exp.
+//
+//   P = exp(scale Q K^T - lse)            (0 above the diagonal when causal)
+//   delta_i = sum_d dO_id O_id - dlse_i,  dP = dO V^T,  dS = P (dP - delta)
+//   dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K      (dK, dV summed over a group's query heads)
+//
+// Three products share each operand tile's two readings (rows for the products over D, transposed for the
+// products over rows), and none of P, dP, dS leaves the registers:
+//  * dK/dV blocks own 32 keys per wave. S = Q K^T with Q as the A operand gives each lane one key
+//    (lane & 15) and four consecutive query rows per 16x16 tile, which is the B operand of
+//    dV^T = dO^T P and dK^T = Q^T dS as it stands (two 16-row tiles make one k = 32 operand; the transposing
+//    LDS read ds_read_b64_tr_b16 takes the matching rows). K, V and both sums stay in registers; Q and dO
+//    tiles of 32 rows pass through LDS.
+//  * dQ blocks own 32 query rows per wave: S^T = K Q^T, then dQ^T = K^T dS^T, with Q, dO and dQ in registers
+//    and K, V tiles of 32 keys passing through LDS.
+// Recomputing S and dP for dQ costs two more products than the five of a single pass, and buys sums in a
+// fixed order (no atomics), no fp32 dQ in memory and no third pass to convert it.
+//
+// fp16 range. P and dS enter the second products as 16-bit values. With fp16, P of long rows and dS of small
+// gradients would fall under 2^-14 and lose bits, so P is scaled by 2^15 (in the exponent's offset, free)
+// and dS by a power of two from a bound on |dP - delta| (row norms of dO and V, |delta|) that puts it under
+// 2^15; the sums are scaled back in fp32. bf16 has fp32's range and takes neither.
+#include "fa_common.h"
+#include "fa_kernels.h"
+#include "../../include/fa_gfx950.h"
+
+namespace fa {
+
+template <typename Tag>
+struct BwdTraits;
+template <>
+struct BwdTraits<f16_t> {
+  static constexpr bool kScaled = true;
+  static constexpr float kPBias = 15.f;           // log2 of P's scale
+  static constexpr float kPUnscale = 1.f / 32768.f;
+};
+template <>
+struct BwdTraits<bf16_t> {
+  static constexpr bool kScaled = false;
+  static constexpr float kPBias = 0.f;
+  static constexpr float kPUnscale = 1.f;
+};
+
+// Per-row terms in the workspace, in groups of 32 rows (one LDS-DMA of 4 bytes per lane):
+// nd[bh][row / 32][0][32] = P's scale in log2 units - lse * log2(e) (-inf: the row has no P: padding, or a row without keys),
+// nd[bh][row / 32][1][32] = -delta.
+__device__ inline int64_t nd_index(const BwdParams& p, int64_t bh, int row) {
+  return (bh * p.row_groups + (row >> 5)) * 64 + (row & 31);
+}
+
+constexpr int kPrepRows = 64;  // rows per block of the row-term kernel
+
+// Row terms, and for fp16 the block maxima behind dS's scale: bound[0][bh][block] = max |dO row|^2,
+// bound[1][bh][block] = max |delta|, vbound[b * Hkv + h][block] = max |V row|^2. Rows that are not finite
+// are left out (their gradients are not finite whatever the scale is). Bound by memory: dO and O are read once.
+template <typename Tag, int D>
+__global__ __launch_bounds__(256) void fa_bwd_prep_kernel(BwdParams p) {
+  constexpr int LPR = D / 8;          // lanes per row (16-byte loads)
+  constexpr int RPP = 256 / LPR;      // rows per pass
+  const int t = threadIdx.x, part = t % LPR, r0 = t / LPR;
+  __shared__ float red[8];
+  const int qblocks = p.prep_blocks;
+  const int64_t nq = (int64_t)p.B * p.H * qblocks;
+  const int64_t id = blockIdx.x;
+  float top = 0.f, topd = 0.f;
+  if (id < nq) {
+    const int64_t bh = id / qblocks;
+    const int blk = (int)(id % qblocks);
+    const int b = (int)(bh / p.H), h = (int)(bh % p.H);
+    for (int i = r0; i < kPrepRows; i += RPP) {
+      const int row = blk * kPrepRows + i;
+      float dot = 0.f, sq = 0.f;
+      if (row < p.M) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(p.o + b * p.so[0] + h * p.so[1] + row * p.so[2] + part * 8);
+        const u32x4 y = *reinterpret_cast<const u32x4*>(p.dout + b * p.sdo[0] + h * p.sdo[1] + row * p.sdo[2] + part * 8);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float y0 = DT<Tag>::to_float((uint16_t)y[j]), y1 = DT<Tag>::to_float((uint16_t)(y[j] >> 16));
+          dot += DT<Tag>::to_float((uint16_t)x[j]) * y0;
+          dot += DT<Tag>::to_float((uint16_t)(x[j] >> 16)) * y1;
+          sq += y0 * y0;
+          sq += y1 * y1;
+        }
+      }
+#pragma unroll
+      for (int s = 1; s < LPR; s *= 2) {
+        dot += __shfl_xor(dot, s, 64);
+        sq += __shfl_xor(sq, s, 64);
+      }
+      float nl = FA_NEG_INF;
+      if (row < p.M) {
+        const float lse = p.lse[b * p.sl[0] + h * p.sl[1] + row * p.sl[2]];
+        if (p.dlse != nullptr) dot -= p.dlse[b * p.sdl[0] + h * p.sdl[1] + row * p.sdl[2]];
+        nl = lse == FA_NEG_INF ? FA_NEG_INF : BwdTraits<Tag>::kPBias - lse * 1.4426950408889634f;
+      }
+      if (part == 0) {
+        float* nd = p.nd + nd_index(p, bh, row);
+        nd[0] = nl;
+        nd[32] = -dot;
+      }
+      if ((__float_as_uint(sq) & 0x7fffffffu) < 0x7f800000u) top = fmaxf(top, sq);
+      if ((__float_as_uint(dot) & 0x7fffffffu) < 0x7f800000u) topd = fmaxf(topd, fabsf(dot));
+    }
+  } else {
+    const int64_t v = id - nq;
+    const int64_t bh = v / p.vblocks;
+    const int blk = (int)(v % p.vblocks);
+    const int b = (int)(bh / p.Hkv), h = (int)(bh % p.Hkv);
+    for (int i = r0; i < kPrepRows; i += RPP) {
+      const int row = blk * kPrepRows + i;
+      float sq = 0.f;
+      if (row < p.N) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(p.v + b * p.sv[0] + h * p.sv[1] + row * p.sv[2] + part * 8);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x0 = DT<Tag>::to_float((uint16_t)x[j]), x1 = DT<Tag>::to_float((uint16_t)(x[j] >> 16));
+          sq += x0 * x0;
+          sq += x1 * x1;
+        }
+      }
+#pragma unroll
+      for (int s = 1; s < LPR; s *= 2) sq += __shfl_xor(sq, s, 64);
+      if ((__float_as_uint(sq) & 0x7fffffffu) < 0x7f800000u) top = fmaxf(top, sq);
+    }
+  }
+  if constexpr (BwdTraits<Tag>::kScaled) {
+#pragma unroll
+    for (int s = 32; s >= 1; s /= 2) {
+      top = fmaxf(top, __shfl_xor(top, s, 64));
+      topd = fmaxf(topd, __shfl_xor(topd, s, 64));
+    }
+    if (t % 64 == 0) {
+      red[t / 64] = top;
+      red[4 + t / 64] = topd;
+    }
+    __syncthreads();
+    if (t == 0) {
+      const float a = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+      const float d = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
+      if (id < nq) {
+        p.bound[id] = a;
+        p.bound[nq + id] = d;
+      } else {
+        p.bound[2 * nq + (id - nq)] = a;
+      }
+    }
+  }
+}
+
+template <typename Tag, int D>
+struct Bwd {
+  static constexpr int WAVES = 4;
+  static constexpr int T = 32;               // rows of a tile passing through LDS, and rows owned per wave
+  static constexpr int BLOCK = WAVES * 32;   // rows owned per workgroup
+  static constexpr int KS = D / 32;          // k = 32 steps over D
+  static constexpr int DT16 = D / 16;        // 16-wide tiles over D
+  static constexpr int ROWB = 2 * D;         // bytes of an LDS row
+  static constexpr int CPR = D / 8;          // 16-byte chunks of a row
+  // LDS rows are unpadded (LDS-DMA writes 1 KiB blocks); chunk c of row r lies at c ^ (r & SWZ), so that the
+  // 16 rows of a fragment read fall on different banks.
+  static constexpr int SWZ = CPR < 16 ? CPR - 1 : 15;
+  static constexpr int TILEB = T * ROWB;
+  static constexpr int STAGEB = 2 * TILEB + 256;  // two tiles and a group of row terms
+  static constexpr int SMEM = 2 * STAGEB;
+  typedef DT<Tag> N_;
+
+  // Rows [row0, row0 + 32) of a matrix into an LDS tile; rows at or past `rows` read as zeros.
+  __device__ static inline void load_tile(const uint16_t* base, int64_t stride, int row0, int rows, uint32_t lds,
+                                          int wave, int lane) {
+    const int left = rows - row0;
+    const uint32_t sb = (uint32_t)stride * 2u;
+    const uint32_t bytes = left <= 0 ? 0u : (uint32_t)((left < T ? left : T) - 1) * sb + (uint32_t)ROWB;
+    const u32x4 rsrc = make_rsrc(base + row0 * stride, bytes);
+    constexpr int RPB = 1024 / ROWB, NB = TILEB / 1024;
+#pragma unroll
+    for (int i = 0; i < NB / WAVES; ++i) {
+      const int blk = wave + i * WAVES;
+      const int row = blk * RPB + lane / CPR;
+      const uint32_t off = (uint32_t)row * sb + (uint32_t)(((lane % CPR) ^ (row & SWZ)) * 16);
+      buffer_load16_to_lds<0, true>(rsrc, off, lds + (uint32_t)blk * 1024u);
+    }
+  }
+
+  // The 32 rows' two terms (256 bytes), by one wave.
+  __device__ static inline void load_terms(const float* nd, uint32_t lds, int lane) {
+    const u32x4 rsrc = make_rsrc(nd, 256);
+    const uint32_t dst = __builtin_amdgcn_readfirstlane(lds);
+    asm volatile("s_nop 4\n\ts_mov_b32 m0, %1\n\tbuffer_load_dword %0, %2, 0 offen lds"
+                 :
+                 : "v"((uint32_t)lane * 4u), "s"(dst), "s"(rsrc)
+                 : "memory", "m0");
+  }
+
+  // Byte offset in a tile of a lane's row fragment (row lane & 15, channels 8 (lane >> 4) ..): step ks is at
+  // off ^ (ks << 6), row tile i at + i * 16 * ROWB.
+  __device__ static inline uint32_t row_off(int lane) {
+    const int r = lane & 15, g = lane >> 4;
+    return (uint32_t)(r * ROWB + ((g ^ (r & SWZ)) << 4));
+  }
+  // Byte offset of a lane's transposing read (rows 4 (lane >> 4) .. + 3, its 4 of 16 columns): columns
+  // 16 dt .. are at off ^ (dt << 5), row tile i at + i * 16 * ROWB.
+  __device__ static inline uint32_t tr_off(int lane) {
+    const int L = lane & 15, r = 4 * (lane >> 4) + (L >> 2);
+    return (uint32_t)(r * ROWB + ((((L & 3) >> 1) ^ (r & SWZ)) << 4) + ((L & 1) << 3));
+  }
+  __device__ static inline u32x4 frag(const char* tile, uint32_t off) {
+    return *reinterpret_cast<const u32x4*>(tile + off);
+  }
+  __device__ static inline u32x4 tfrag(const char* tile, uint32_t off) {
+    const u32x2 a = lds_read_tr16(reinterpret_cast<const uint16_t*>(tile + off));
+    const u32x2 b = lds_read_tr16(reinterpret_cast<const uint16_t*>(tile + off + 16 * ROWB));
+    return (u32x4){a[0], a[1], b[0], b[1]};
+  }
+
+  // 32 rows' fragments (two 16-row tiles) straight from memory, zeros past `rows`.
+  __device__ static inline void load_frags(u32x4 (&f)[2][KS], const uint16_t* base, int64_t stride, int row0, int rows,
+                                           int lane) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = row0 + 16 * i + (lane & 15);
+      const uint16_t* src = base + row * stride + 8 * (lane >> 4);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        f[i][ks] = (u32x4){0, 0, 0, 0};
+        if (row < rows) f[i][ks] = *reinterpret_cast<const u32x4*>(src + 32 * ks);
+      }
+    }
+  }
+
+  // Power of two that brings |dP - delta| under 1 (fp16), from the bounds of this kv head's rows.
+  __device__ static inline int scale_exponent(const BwdParams& p, int b, int hk, float* red) {
+    const int t = threadIdx.x;
+    const int64_t nq = (int64_t)p.B * p.H * p.prep_blocks;
+    const int64_t first = ((int64_t)b * p.H + (int64_t)hk * p.group) * p.prep_blocks;
+    const int count = p.group * p.prep_blocks;
+    float o2 = 0.f, dl = 0.f, v2 = 0.f;
+    for (int i = t; i < count; i += WAVES * 64) {
+      o2 = fmaxf(o2, p.bound[first + i]);
+      dl = fmaxf(dl, p.bound[nq + first + i]);
+    }
+    const float* vb = p.bound + 2 * nq + ((int64_t)b * p.Hkv + hk) * p.vblocks;
+    for (int i = t; i < p.vblocks; i += WAVES * 64) v2 = fmaxf(v2, vb[i]);
+#pragma unroll
+    for (int s = 32; s >= 1; s /= 2) {
+      o2 = fmaxf(o2, __shfl_xor(o2, s, 64));
+      dl = fmaxf(dl, __shfl_xor(dl, s, 64));
+      v2 = fmaxf(v2, __shfl_xor(v2, s, 64));
+    }
+    if (t % 64 == 0) {
+      red[t / 64] = o2;
+      red[4 + t / 64] = dl;
+      red[8 + t / 64] = v2;
+    }
+    __syncthreads();
+    o2 = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    dl = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
+    v2 = fmaxf(fmaxf(red[8], red[9]), fmaxf(red[10], red[11]));
+    __syncthreads();
+    const float bound = sqrtf(o2) * sqrtf(v2) + dl;
+    const int e = (int)(__float_as_uint(bound) >> 23) - 126;  // 2^e > bound
+    return e < -100 ? -100 : (e > 100 ? 100 : e);
+  }
+  __device__ static inline float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+  __device__ static void dkdv(const BwdParams& p, char* smem, int id) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c16 = lane & 15, g = lane >> 4;
+    const int hkb = id / p.nblocks, nb = id % p.nblocks;
+    const int b = hkb / p.Hkv, hk = hkb % p.Hkv;
+    const int k0 = nb * BLOCK, kw = k0 + 32 * wave;  // first key of the block, of the wave
+    float sc = 1.f, unscale = 1.f;
+    if constexpr (BwdTraits<Tag>::kScaled) {
+      const int e = scale_exponent(p, b, hk, reinterpret_cast<float*>(smem));
+      sc = pow2(-e);
+      unscale = pow2(e);
+    }
+    u32x4 kf[2][KS], vf[2][KS];
+    load_frags(kf, p.k + b * p.sk[0] + hk * p.sk[1], p.sk[2], kw, p.N, lane);
+    load_frags(vf, p.v + b * p.sv[0] + hk * p.sv[1], p.sv[2], kw, p.N, lane);
+    floatx4 dk[DT16][2], dv[DT16][2];
+#pragma unroll
+    for (int d = 0; d < DT16; ++d)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) dk[d][i] = dv[d][i] = (floatx4){0.f, 0.f, 0.f, 0.f};
+
+    const uint32_t lds = lds_address(smem);
+    const uint32_t ro = row_off(lane), to = tr_off(lane);
+    const int qt_all = (p.M + T - 1) / T;
+    const int qt0 = p.causal ? k0 / T : 0;  // rows above the block's first key see none of its keys
+    const int per_head = qt_all > qt0 ? qt_all - qt0 : 0;
+    const int total = per_head * p.group;
+
+    int lh = 0, lt = qt0;  // head and tile of the next load
+    auto load_next = [&](int stage) {
+      const int h = hk * p.group + lh;
+      const uint32_t dst = lds + (uint32_t)(stage * STAGEB);
+      load_tile(p.q + b * p.sq[0] + h * p.sq[1], p.sq[2], lt * T, p.M, dst, wave, lane);
+      load_tile(p.dout + b * p.sdo[0] + h * p.sdo[1], p.sdo[2], lt * T, p.M, dst + TILEB, wave, lane);
+      if (wave == 0) load_terms(p.nd + (((int64_t)b * p.H + h) * p.row_groups + lt) * 64, dst + 2 * TILEB, lane);
+      if (++lt == qt_all) {
+        lt = qt0;
+        ++lh;
+      }
+    };
+    if (total > 0) load_next(0);
+    int ct = qt0;
+    for (int it = 0; it < total; ++it) {
+      wait_vm_lds_barrier<0>();
+      if (it + 1 < total) load_next((it + 1) & 1);
+      const char* qs = smem + (it & 1) * STAGEB;
+      const char* os = qs + TILEB;
+      const float* nd = reinterpret_cast<const float*>(qs + 2 * TILEB);
+      const int q0 = ct * T;
+      if (++ct == qt_all) ct = qt0;
+      if (p.causal && q0 + T - 1 < kw) continue;
+      floatx4 s[2][2], dp[2][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const floatx4 nd1 = *reinterpret_cast<const floatx4*>(nd + 32 + 16 * i + 4 * g);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          s[i][j] = (floatx4){0.f, 0.f, 0.f, 0.f};
+          dp[i][j] = nd1;
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const u32x4 a = frag(qs + i * 16 * ROWB, ro ^ (ks << 6));
+          const u32x4 o = frag(os + i * 16 * ROWB, ro ^ (ks << 6));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            s[i][j] = N_::mfma16(a, kf[j][ks], s[i][j]);
+            dp[i][j] = N_::mfma16(o, vf[j][ks], dp[i][j]);
+          }
+        }
+      }
+      const bool edge = p.causal && q0 < kw + 31;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const floatx4 nl = *reinterpret_cast<const floatx4*>(nd + 16 * i + 4 * g);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float e = fast_exp2(fmaf(p.c, s[i][j][r], nl[r]));
+            float d = BwdTraits<Tag>::kScaled ? e * (dp[i][j][r] * sc) : e * dp[i][j][r];
+            if (edge && kw + 16 * j + c16 > q0 + 16 * i + 4 * g + r) e = d = 0.f;
+            s[i][j][r] = e;
+            dp[i][j][r] = d;
+          }
+      }
+      u32x4 pb[2], sb[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        pb[j] = (u32x4){N_::pack2(s[0][j][0], s[0][j][1]), N_::pack2(s[0][j][2], s[0][j][3]),
+                        N_::pack2(s[1][j][0], s[1][j][1]), N_::pack2(s[1][j][2], s[1][j][3])};
+        sb[j] = (u32x4){N_::pack2(dp[0][j][0], dp[0][j][1]), N_::pack2(dp[0][j][2], dp[0][j][3]),
+                        N_::pack2(dp[1][j][0], dp[1][j][1]), N_::pack2(dp[1][j][2], dp[1][j][3])};
+      }
+#pragma unroll
+      for (int d = 0; d < DT16; ++d) {
+        const u32x4 ot = tfrag(os, to ^ (d << 5));
+        const u32x4 qt = tfrag(qs, to ^ (d << 5));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          dv[d][j] = N_::mfma16(ot, pb[j], dv[d][j]);
+          dk[d][j] = N_::mfma16(qt, sb[j], dk[d][j]);
+        }
+      }
+    }
+    const float fk = p.scale * unscale * BwdTraits<Tag>::kPUnscale, fv = BwdTraits<Tag>::kPUnscale;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int key = kw + 16 * j + c16;
+      if (key >= p.N) continue;
+      uint16_t* ok = p.dk + b * p.sdk[0] + hk * p.sdk[1] + key * p.sdk[2] + 4 * g;
+      uint16_t* ov = p.dv + b * p.sdv[0] + hk * p.sdv[1] + key * p.sdv[2] + 4 * g;
+#pragma unroll
+      for (int d = 0; d < DT16; ++d) {
+        const floatx4 a = dk[d][j] * fk, v = dv[d][j] * fv;
+        *reinterpret_cast<u32x2*>(ok + 16 * d) = (u32x2){N_::pack2(a[0], a[1]), N_::pack2(a[2], a[3])};
+        *reinterpret_cast<u32x2*>(ov + 16 * d) = (u32x2){N_::pack2(v[0], v[1]), N_::pack2(v[2], v[3])};
+      }
+    }
+  }
+
+  __device__ static void dq(const BwdParams& p, char* smem, int id) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c16 = lane & 15, g = lane >> 4;
+    const int bh = id / p.mblocks;
+    // causal: the heaviest block (most keys) of a head first
+    const int mb = p.causal ? p.mblocks - 1 - id % p.mblocks : id % p.mblocks;
+    const int b = bh / p.H, h = bh % p.H, hk = h / p.group;
+    const int m0 = mb * BLOCK, mw = m0 + 32 * wave;
+    float sc = 1.f, unscale = 1.f;
+    if constexpr (BwdTraits<Tag>::kScaled) {
+      const int e = scale_exponent(p, b, hk, reinterpret_cast<float*>(smem));
+      sc = pow2(-e);
+      unscale = pow2(e);
+    }
+    u32x4 qf[2][KS], of[2][KS];
+    load_frags(qf, p.q + b * p.sq[0] + h * p.sq[1], p.sq[2], mw, p.M, lane);
+    load_frags(of, p.dout + b * p.sdo[0] + h * p.sdo[1], p.sdo[2], mw, p.M, lane);
+    float nl[2], nd[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = mw + 16 * i + c16;
+      nl[i] = FA_NEG_INF;
+      nd[i] = 0.f;
+      if (row < p.M) {
+        const float* src = p.nd + nd_index(p, bh, row);
+        nl[i] = src[0];
+        nd[i] = src[32];
+      }
+    }
+    floatx4 acc[DT16][2];
+#pragma unroll
+    for (int d = 0; d < DT16; ++d)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) acc[d][i] = (floatx4){0.f, 0.f, 0.f, 0.f};
+    const uint32_t lds = lds_address(smem);
+    const uint32_t ro = row_off(lane), to = tr_off(lane);
+    const int n_end = p.causal && m0 + BLOCK < p.N ? m0 + BLOCK : p.N;
+    const int tiles = (n_end + T - 1) / T;
+    const uint16_t* kb = p.k + b * p.sk[0] + hk * p.sk[1];
+    const uint16_t* vb = p.v + b * p.sv[0] + hk * p.sv[1];
+    auto load = [&](int t) {
+      const uint32_t dst = lds + (uint32_t)((t & 1) * STAGEB);
+      load_tile(kb, p.sk[2], t * T, p.N, dst, wave, lane);
+      load_tile(vb, p.sv[2], t * T, p.N, dst + TILEB, wave, lane);
+    };
+    if (tiles > 0) load(0);
+    for (int t = 0; t < tiles; ++t) {
+      wait_vm_lds_barrier<0>();
+      if (t + 1 < tiles) load(t + 1);
+      const char* ks_ = smem + (t & 1) * STAGEB;
+      const char* vs_ = ks_ + TILEB;
+      const int n0 = t * T;
+      if (p.causal && n0 > mw + 31) continue;
+      floatx4 s[2][2], dp[2][2];  // [key tile][row tile]
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          s[i][j] = (floatx4){0.f, 0.f, 0.f, 0.f};
+          dp[i][j] = (floatx4){nd[j], nd[j], nd[j], nd[j]};
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const u32x4 a = frag(ks_ + i * 16 * ROWB, ro ^ (ks << 6));
+          const u32x4 v = frag(vs_ + i * 16 * ROWB, ro ^ (ks << 6));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            s[i][j] = N_::mfma16(a, qf[j][ks], s[i][j]);
+            dp[i][j] = N_::mfma16(v, of[j][ks], dp[i][j]);
+          }
+        }
+      }
+      const bool edge = (p.causal && n0 + T - 1 > mw) || n0 + T > p.N;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float e = fast_exp2(fmaf(p.c, s[i][j][r], nl[j]));
+            float d = BwdTraits<Tag>::kScaled ? e * (dp[i][j][r] * sc) : e * dp[i][j][r];
+            if (edge) {
+              const int key = n0 + 16 * i + 4 * g + r;
+              if (key >= p.N || (p.causal && key > mw + 16 * j + c16)) d = 0.f;
+            }
+            dp[i][j][r] = d;
+          }
+      u32x4 sb[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        sb[j] = (u32x4){N_::pack2(dp[0][j][0], dp[0][j][1]), N_::pack2(dp[0][j][2], dp[0][j][3]),
+                        N_::pack2(dp[1][j][0], dp[1][j][1]), N_::pack2(dp[1][j][2], dp[1][j][3])};
+#pragma unroll
+      for (int d = 0; d < DT16; ++d) {
+        const u32x4 kt = tfrag(ks_, to ^ (d << 5));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[d][j] = N_::mfma16(kt, sb[j], acc[d][j]);
+      }
+    }
+    const float f = p.scale * unscale * BwdTraits<Tag>::kPUnscale;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int row = mw + 16 * j + c16;
+      if (row >= p.M) continue;
+      uint16_t* out = p.dq + b * p.sdq[0] + h * p.sdq[1] + row * p.sdq[2] + 4 * g;
+#pragma unroll
+      for (int d = 0; d < DT16; ++d) {
+        const floatx4 a = acc[d][j] * f;
+        *reinterpret_cast<u32x2*>(out + 16 * d) = (u32x2){N_::pack2(a[0], a[1]), N_::pack2(a[2], a[3])};
+      }
+    }
+  }
+};
+
+// dK/dV blocks first (they are the longer ones), then dQ blocks, in one grid: small problems fill more of
+// the chip, large ones drain together.
+template <typename Tag, int D>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void fa_bwd_kernel(BwdParams p) {
+  __shared__ __align__(1024) char smem[Bwd<Tag, D>::SMEM];
+  const int id = blockIdx.x;
+  if (id < p.kv_total)
+    Bwd<Tag, D>::dkdv(p, smem, xcd_remap(id, p.kv_total));
+  else
+    Bwd<Tag, D>::dq(p, smem, xcd_remap(id - p.kv_total, p.q_total));
+}
+
+#define FA_BWD_ENTRY(TAG, DTYPE, D) \
+  {DTYPE, D, (const void*)&fa_bwd_prep_kernel<TAG, D>, (const void*)&fa_bwd_kernel<TAG, D>, Bwd<TAG, D>::BLOCK, kPrepRows}
+
+static const BwdKernelEntry kBwdEntries[] = {
+    FA_BWD_ENTRY(f16_t, FA_DTYPE_F16, 64),   FA_BWD_ENTRY(f16_t, FA_DTYPE_F16, 128),
+    FA_BWD_ENTRY(f16_t, FA_DTYPE_F16, 256),  FA_BWD_ENTRY(bf16_t, FA_DTYPE_BF16, 64),
+    FA_BWD_ENTRY(bf16_t, FA_DTYPE_BF16, 128), FA_BWD_ENTRY(bf16_t, FA_DTYPE_BF16, 256),
+};
+
+const BwdKernelEntry* fa_bwd_registry(int* count) {
+  *count = (int)(sizeof(kBwdEntries) / sizeof(kBwdEntries[0]));
+  return kBwdEntries;
+}
+
+}  // namespace fa

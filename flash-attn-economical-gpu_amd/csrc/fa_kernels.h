@@ -74,6 +74,95 @@ struct FaMergeEntry {
   const void* fn;
 };
 
+// One attention-backward launch (row-term kernel, then dK/dV and dQ blocks in one grid). Strides
+// are in elements: batch, head, row.
+struct BwdParams {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  const uint16_t* o;
+  const uint16_t* dout;
+  const float* lse;
+  const float* dlse;  // nullable
+  uint16_t* dq;
+  uint16_t* dk;
+  uint16_t* dv;
+  int64_t sq[3], sk[3], sv[3], so[3], sdo[3], sl[3], sdl[3], sdq[3], sdk[3], sdv[3];
+  float* nd;     // workspace: two fp32 terms per query row, in groups of 32 rows
+  float* bound;  // workspace: block maxima behind fp16's dS scale
+  int32_t B, H, Hkv, M, N, group;
+  int32_t row_groups;   // 32-row groups of a head's row terms
+  int32_t prep_blocks;  // row-term blocks of a query head
+  int32_t vblocks;      // V-norm blocks of a kv head (fp16; 0 otherwise)
+  int32_t nblocks, mblocks;   // dK/dV blocks of a kv head, dQ blocks of a query head
+  int32_t kv_total, q_total;  // blocks of each kind
+  int32_t causal;
+  float c;      // scale * log2(e)
+  float scale;
+};
+
+struct BwdKernelEntry {
+  int32_t dtype;
+  int32_t D;
+  const void* prep;
+  const void* main;
+  int32_t block;      // keys (dK/dV) and query rows (dQ) of a workgroup
+  int32_t prep_rows;  // rows of a row-term block
+};
+
+const BwdKernelEntry* fa_bwd_registry(int* count);
+
+// The 4-bit cache (kv4.hip). Code and scale strides are in bytes: batch, head; cached rows are dense.
+struct Kv4AppendParams {
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* k_values;  // nullable (both): what the appended rows now stand for
+  uint16_t* v_values;
+  uint8_t* k_codes;
+  uint8_t* k_scales;
+  uint8_t* v_codes;
+  uint8_t* v_scales;
+  const int32_t* start;
+  const int32_t* count;  // nullable: all rows
+  int64_t sk[3], sv[3], skv[3], svv[3];
+  int64_t code_stride[2], scale_stride[2];
+  int32_t B, Hkv, D, rows, capacity;
+};
+
+struct Kv4AttendParams {
+  const uint16_t* q;
+  uint16_t* o;
+  float* lse;  // nullable
+  const uint8_t* k_codes;
+  const uint8_t* k_scales;
+  const uint8_t* v_codes;
+  const uint8_t* v_scales;
+  const int32_t* start;
+  const int32_t* count;  // nullable: all rows
+  float* ws_o;           // splits > 1: unnormalised partial sums [splits][B * H * M][D]
+  float* ws_ml;          // splits > 1: their row maximum (log2 units) and sum [splits][B * H * M][2]
+  int64_t sq[3], so[3], sl[3];
+  int64_t code_stride[2], scale_stride[2];
+  int32_t B, H, Hkv, M, group, capacity;
+  int32_t causal, splits, min_tiles, row_blocks;
+  float c;  // scale * log2(e)
+};
+
+struct Kv4KernelEntry {
+  int32_t dtype;
+  int32_t D;
+  const void* append;
+  const void* merge;
+  const void* attend[3];  // 16 rows shared by a workgroup's waves, 32 rows shared, own rows per wave
+  int32_t chunk_tiles;    // 16-row tiles per wave of the last
+};
+
+const Kv4KernelEntry* kv4_registry(int* count);
+
+// The last error of the calling thread (fa_last_error), shared by the files that implement the C ABI.
+int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+int ok();
+
 const FaKernelEntry* fa_fwd_registry(int* count);
 const FaKernelEntry* fa_fwd16_registry(int* count);
 const FaMergeEntry* fa_merge_registry(int* count);

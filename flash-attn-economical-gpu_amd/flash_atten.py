@@ -27,6 +27,7 @@ import torch
 
 import gfx950_configs as cfgs
 import hip_lib
+import kv4
 from tuner import FlashAttentionLaunchSpec
 
 logger = logging.getLogger(__name__)
@@ -296,6 +297,104 @@ def sdpa(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, is_caus
     workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
     hip_lib.fa_fwd_planned(block, query, key, value, out, None, workspace, query.device.index)
     return out
+
+
+def attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
+                       lse: torch.Tensor, *, causal: bool = False, sm_scale: float | None = None,
+                       dlse: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients (dq, dk, dv) of attention from its inputs, its output o and log-sum-exp lse (what
+    `attention(..., return_lse=True)` gives), the gradient `do` of o and, where the lse was used, `dlse` of lse.
+
+    k/v may have fewer heads (GQA): their gradients are summed over the query heads they serve. Operands are
+    read through their strides (unit head-dim stride; others are copied first), gradients come in their
+    operand's layout. Repeated calls give the same bits; nothing synchronises, and the call can be captured
+    into a HIP graph."""
+    do, q, k, v, o = (hip_lib.operand(t, name) for name, t in (("do", do), ("q", q), ("k", k), ("v", v), ("o", o)))
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    key = ("backward", _form(do), _form(q), _form(k), _form(v), _form(o), _form(lse),
+           None if dlse is None else _form(dlse), bool(causal), None if sm_scale is None else float(sm_scale))
+    plan = _plans.get(key)
+    if plan is None:
+        scale = q.shape[3] ** -0.5 if sm_scale is None else float(sm_scale)
+        plan = (hip_lib.bwd_plan(do, q, k, v, o, lse, dlse, dq, dk, dv, sm_scale=scale, causal=bool(causal)),
+                hip_lib.bwd_workspace_bytes(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2]))
+        _keep_plan(key, plan)
+    block, need = plan
+    workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    hip_lib.fa_bwd_planned(block, do, q, k, v, o, lse, dlse, dq, dk, dv, workspace)
+    return dq, dk, dv
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, causal, sm_scale):
+        q, k, v = (hip_lib.operand(t, name) for name, t in (("q", q), ("k", k), ("v", v)))
+        B, H, M, D = q.shape
+        o = torch.empty_strided((B, H, M, D), (max(M, 1) * H * D, D, H * D, 1), device=q.device, dtype=q.dtype)
+        lse = torch.empty(B, H, M, device=q.device, dtype=torch.float32)
+        key = ("differentiable", _form(q), _form(k), _form(v), causal, sm_scale)
+        plan = _plans.get(key)
+        if plan is None:
+            tile = _tile_for(hip_lib.FA_VARIANT_OPT, q.dtype, D, causal, B, H, M, k.shape[2], {})
+            plan = (hip_lib.fwd_plan(q, k, v, o, lse, sm_scale=D ** -0.5 if sm_scale is None else sm_scale, causal=causal,
+                                     variant=hip_lib.FA_VARIANT_OPT, tile=tile.to_c()),)
+            _keep_plan(key, plan)
+        hip_lib.fa_fwd_planned(plan[0], q, k, v, o, lse, None, q.device.index)
+        ctx.save_for_backward(q, k, v, o, lse)
+        ctx.causal, ctx.sm_scale = causal, sm_scale
+        ctx.set_materialize_grads(False)
+        return o, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do, dlse):
+        q, k, v, o, lse = ctx.saved_tensors
+        if do is None:
+            if dlse is None:
+                return None, None, None, None, None
+            do = torch.zeros_like(o)
+        grads = attention_backward(do, q, k, v, o, lse, causal=ctx.causal, sm_scale=ctx.sm_scale, dlse=dlse)
+        return (*grads, None, None)
+
+
+def differentiable_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = False,
+                             sm_scale: float | None = None, return_lse: bool = False):
+    """Attention for training: the optimized forward, whose result takes part in autograd (both o and, with
+    return_lse, the log-sum-exp). q [B, H, M, D] and k/v [B, H_kv, N, D] are read through their strides; o is a
+    [B, H, M, D] view of memory laid out [B, M, H, D], as from `sdpa`. First derivatives only."""
+    o, lse = _Attention.apply(q, k, v, bool(causal), None if sm_scale is None else float(sm_scale))
+    return (o, lse) if return_lse else o
+
+
+def sdpa_kv4(query: torch.Tensor, cache: kv4.Kv4Cache, start: torch.Tensor, *, count: torch.Tensor | None = None,
+             is_causal: bool = True, scale: float | None = None, return_lse: bool = False):
+    """Attention of new tokens' queries [B, H, M, D] over a 4-bit cache that already holds their keys.
+
+    Row i of sequence b stands at position start[b] + i and sees the cached tokens up to and including it
+    (is_causal), or all start[b] + count[b] of them. Rows i >= count[b] (none without a count) and rows that
+    see nothing come out as zeros, their lse as -inf. H is a multiple of the cache's heads. M = 1 is a decode
+    step, a few rows a draft being checked, many a chunk of a prompt. start and count are int32 [B] on the GPU;
+    nothing synchronises, and the call can be captured into a HIP graph. The result has `sdpa`'s layout."""
+    if query.dim() != 4:
+        raise ValueError(f"query must be 4-D [batch, heads, seq, head_dim], got {tuple(query.shape)}")
+    B, H, M, D = query.shape
+    if B != cache.batch or D != cache.head_dim or H < 1 or H % cache.kv_heads:
+        raise ValueError(f"query {tuple(query.shape)} does not fit a cache of {cache.batch} sequences, {cache.kv_heads} "
+                         f"heads of {cache.head_dim}")
+    if query.dtype != cache.dtype or query.device != cache.device:
+        raise ValueError(f"query is {query.dtype} on {query.device}, the cache {cache.dtype} on {cache.device}")
+    if start is None:
+        raise ValueError("start is required")
+    start, count = (kv4._positions(t, name, B, cache.device) for name, t in (("start", start), ("count", count)))
+    query = hip_lib.operand(query, "query")
+    o = torch.empty_strided((B, H, M, D), (max(M, 1) * H * D, D, H * D, 1), device=query.device, dtype=query.dtype)
+    lse = torch.empty(B, H, M, device=query.device, dtype=torch.float32) if return_lse else None
+    splits = kv4.choose_splits(B, H, cache.kv_heads, M, D, cache.capacity)
+    need = hip_lib.kv4_attend_workspace_bytes(B, H, M, D, splits)
+    workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
+    hip_lib.kv4_attend(cache._args, query, o, lse, workspace, start, count, sm_scale=D ** -0.5 if scale is None else scale,
+                       causal=is_causal, splits=splits)
+    return (o, lse) if return_lse else o
 
 
 __all__ = [

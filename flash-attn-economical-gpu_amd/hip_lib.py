@@ -18,7 +18,7 @@ import torch
 HERE = Path(__file__).resolve().parent
 LIB_PATH = HERE / "libfa_gfx950.so"
 RESOURCES_PATH = HERE / "kernel_resources.json"
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 FA_OK, FA_EINVAL, FA_ENOTSUP, FA_EHIP, FA_EWORKSPACE = 0, 1, 2, 3, 4
 FA_DTYPE_F16, FA_DTYPE_BF16 = 0, 1
@@ -102,6 +102,66 @@ class FaDeviceLimits(ctypes.Structure):
     ]
 
 
+class FaBwdArgs(ctypes.Structure):
+    _fields_ = [
+        *((name, ctypes.c_void_p) for name in ("q", "k", "v", "o", "dout", "lse", "dlse", "dq", "dk", "dv", "workspace")),
+        ("workspace_bytes", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64 * 4),
+        ("k_stride", ctypes.c_int64 * 4),
+        ("v_stride", ctypes.c_int64 * 4),
+        ("o_stride", ctypes.c_int64 * 4),
+        ("dout_stride", ctypes.c_int64 * 4),
+        ("lse_stride", ctypes.c_int64 * 3),
+        ("dlse_stride", ctypes.c_int64 * 3),
+        ("dq_stride", ctypes.c_int64 * 4),
+        ("dk_stride", ctypes.c_int64 * 4),
+        ("dv_stride", ctypes.c_int64 * 4),
+        *((name, ctypes.c_int32) for name in ("B", "H", "H_kv", "M", "N", "D")),
+        ("sm_scale", ctypes.c_float),
+        ("dtype", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+    ]
+
+
+class Kv4CacheArgs(ctypes.Structure):
+    _fields_ = [
+        *((name, ctypes.c_void_p) for name in ("k_codes", "k_scales", "v_codes", "v_scales")),
+        ("code_stride", ctypes.c_int64 * 2),
+        ("scale_stride", ctypes.c_int64 * 2),
+        *((name, ctypes.c_int32) for name in ("B", "H_kv", "D", "dtype", "rows", "capacity")),
+    ]
+
+
+class Kv4AppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", Kv4CacheArgs),
+        *((name, ctypes.c_void_p) for name in ("k", "v", "k_values", "v_values", "start", "count")),
+        ("k_stride", ctypes.c_int64 * 4),
+        ("v_stride", ctypes.c_int64 * 4),
+        ("k_values_stride", ctypes.c_int64 * 4),
+        ("v_values_stride", ctypes.c_int64 * 4),
+        ("rows", ctypes.c_int32),
+    ]
+
+
+class Kv4AttendArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", Kv4CacheArgs),
+        *((name, ctypes.c_void_p) for name in ("q", "o", "lse", "workspace")),
+        ("workspace_bytes", ctypes.c_int64),
+        ("start", ctypes.c_void_p),
+        ("count", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 4),
+        ("o_stride", ctypes.c_int64 * 4),
+        ("lse_stride", ctypes.c_int64 * 3),
+        ("H", ctypes.c_int32),
+        ("M", ctypes.c_int32),
+        ("sm_scale", ctypes.c_float),
+        ("causal", ctypes.c_int32),
+        ("splits", ctypes.c_int32),
+    ]
+
+
 # Every symbol include/fa_gfx950.h declares, with its ctypes signature.
 SIGNATURES = {
     "fa_abi_version": (ctypes.c_int, []),
@@ -159,6 +219,11 @@ SIGNATURES = {
         ],
     ),
     "fa_device_limits": (ctypes.c_int, [ctypes.c_int32, ctypes.POINTER(FaDeviceLimits)]),
+    "fa_bwd": (ctypes.c_int, [ctypes.POINTER(FaBwdArgs), ctypes.c_void_p]),
+    "fa_bwd_workspace_bytes": (ctypes.c_int64, [ctypes.c_int32] * 5),
+    "kv4_append": (ctypes.c_int, [ctypes.POINTER(Kv4AppendArgs), ctypes.c_void_p]),
+    "kv4_attend": (ctypes.c_int, [ctypes.POINTER(Kv4AttendArgs), ctypes.c_void_p]),
+    "kv4_attend_workspace_bytes": (ctypes.c_int64, [ctypes.c_int32] * 5),
 }
 
 
@@ -463,3 +528,129 @@ def fwd_kernel_symbol(variant: int, dtype: torch.dtype, D: int, tile: FaTile) ->
 def gemm_kernel_symbol(tile: GemmTile) -> str:
     """Mangled name of the GEMM kernel a tile runs (its default deep-ring kernel); needs no device."""
     return _kernel_symbol(1, 0, torch.float16, 0, None, tile)
+
+
+def operand(t: torch.Tensor, name: str) -> torch.Tensor:
+    """t as the backward and cache kernels read it: a [batch, heads, rows, D] GPU tensor with a unit head-dim
+    stride, rows that do not overlap and 16-byte alignment; copied where it is laid out otherwise (the
+    gradient of a sum, say, whose strides are zero)."""
+    if t.dim() != 4:
+        raise ValueError(f"{name} must be 4-D [batch, heads, seq, head_dim], got {tuple(t.shape)}")
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be a GPU tensor, got device {t.device}")
+    B, H, S, D = t.shape
+    b, h, r, d = t.stride()
+    if ((d == 1 or D == 1) and (S == 1 or D <= r <= 1 << 22 and r % 8 == 0) and (B == 1 or b % 8 == 0)
+            and (H == 1 or h % 8 == 0) and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides4_of(t: torch.Tensor):
+    """Strides with those of dimensions of size 1, which are never used, replaced by valid ones."""
+    B, H, S, D = t.shape
+    b, h, r, d = t.stride()
+    return _I64x4(b if B > 1 else 0, h if H > 1 else 0, r if S > 1 else D, d if D > 1 else 1)
+
+
+def _launch(fn, args, device: torch.device, what: str) -> None:
+    """One C entry on the tensors' device and its current stream."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        code = fn(ctypes.byref(args), _stream_ptr(device))
+    else:
+        with torch.cuda.device(index):
+            code = fn(ctypes.byref(args), _stream_ptr(device))
+    if code:
+        check(code, what)
+
+
+@functools.lru_cache(maxsize=4096)
+def bwd_workspace_bytes(B: int, H: int, H_kv: int, M: int, N: int) -> int:
+    return int(load().fa_bwd_workspace_bytes(B, H, H_kv, M, N))
+
+
+def bwd_plan(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
+             dlse: torch.Tensor | None, dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, *, sm_scale: float,
+             causal: bool) -> bytes:
+    """fa_bwd's argument block for these tensors' shapes, strides, types and devices, after the checks on
+    them. As with fwd_plan, it holds no address that fa_bwd_planned uses."""
+    B, H, M, D = q.shape
+    Bk, H_kv, N, Dk = k.shape
+    if not (q.dtype == k.dtype == v.dtype == o.dtype == do.dtype):
+        raise ValueError(f"q/k/v/o/do dtypes differ: {q.dtype} {k.dtype} {v.dtype} {o.dtype} {do.dtype}")
+    dtype = dtype_code(q.dtype)
+    if tuple(v.shape) != tuple(k.shape):
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} shapes differ")
+    if Bk != B or Dk != D or o.shape != q.shape or do.shape != q.shape:
+        raise ValueError(f"incompatible shapes q={tuple(q.shape)} k={tuple(k.shape)} o={tuple(o.shape)} do={tuple(do.shape)}")
+    for name, t in (("lse", lse), ("dlse", dlse)):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (B, H, M)):
+            raise ValueError(f"{name} must be float32 [{B}, {H}, {M}], got {t.dtype} {tuple(t.shape)}")
+    for name, t in (("k", k), ("v", v), ("o", o), ("do", do), ("lse", lse), ("dlse", dlse)):
+        if t is not None and t.device != q.device:
+            raise ValueError(f"{name} is on {t.device}, q on {q.device}")
+    args = FaBwdArgs()
+    for name, t in (("q", q), ("k", k), ("v", v), ("o", o), ("dout", do), ("dq", dq), ("dk", dk), ("dv", dv)):
+        setattr(args, name + "_stride", _strides4_of(t))
+    args.lse_stride = (ctypes.c_int64 * 3)(*lse.stride())
+    if dlse is not None:
+        args.dlse_stride = (ctypes.c_int64 * 3)(*dlse.stride())
+    args.B, args.H, args.H_kv, args.M, args.N, args.D = B, H, H_kv, M, N, D
+    args.sm_scale, args.dtype, args.causal = float(sm_scale), dtype, int(bool(causal))
+    return bytes(args)
+
+
+def fa_bwd_planned(plan: bytes, do, q, k, v, o, lse, dlse, dq, dk, dv, workspace) -> None:
+    """fa_bwd with the argument block of bwd_plan. The caller has matched the tensors to the plan."""
+    args = FaBwdArgs.from_buffer_copy(plan)
+    args.q, args.k, args.v, args.o, args.dout = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), do.data_ptr()
+    args.lse = lse.data_ptr()
+    if dlse is not None:
+        args.dlse = dlse.data_ptr()
+    args.dq, args.dk, args.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    if workspace is not None:
+        args.workspace = workspace.data_ptr()
+        args.workspace_bytes = workspace.numel()
+    _launch(load().fa_bwd, args, q.device, "fa_bwd")
+
+
+@functools.lru_cache(maxsize=4096)
+def kv4_attend_workspace_bytes(B: int, H: int, M: int, D: int, splits: int) -> int:
+    return int(load().kv4_attend_workspace_bytes(B, H, M, D, splits))
+
+
+def kv4_append(cache: Kv4CacheArgs, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, count: torch.Tensor | None,
+               k_values: torch.Tensor | None, v_values: torch.Tensor | None) -> None:
+    """Append rows to a 4-bit cache on the current stream; the caller has matched the tensors to the cache."""
+    args = Kv4AppendArgs()
+    args.cache = cache
+    args.k, args.v, args.start = k.data_ptr(), v.data_ptr(), start.data_ptr()
+    if count is not None:
+        args.count = count.data_ptr()
+    args.k_stride, args.v_stride = _strides4_of(k), _strides4_of(v)
+    if k_values is not None:
+        args.k_values, args.v_values = k_values.data_ptr(), v_values.data_ptr()
+        args.k_values_stride, args.v_values_stride = _strides4_of(k_values), _strides4_of(v_values)
+    args.rows = k.shape[2]
+    _launch(load().kv4_append, args, k.device, "kv4_append")
+
+
+def kv4_attend(cache: Kv4CacheArgs, q: torch.Tensor, o: torch.Tensor, lse: torch.Tensor | None,
+               workspace: torch.Tensor | None, start: torch.Tensor, count: torch.Tensor | None, *, sm_scale: float,
+               causal: bool, splits: int) -> None:
+    """Attention over a 4-bit cache on the current stream; the caller has matched the tensors to the cache."""
+    args = Kv4AttendArgs()
+    args.cache = cache
+    args.q, args.o, args.start = q.data_ptr(), o.data_ptr(), start.data_ptr()
+    if count is not None:
+        args.count = count.data_ptr()
+    if lse is not None:
+        args.lse = lse.data_ptr()
+        args.lse_stride = (ctypes.c_int64 * 3)(*lse.stride())
+    if workspace is not None:
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    args.q_stride, args.o_stride = _strides4_of(q), _strides4_of(o)
+    args.H, args.M = q.shape[1], q.shape[2]
+    args.sm_scale, args.causal, args.splits = float(sm_scale), int(bool(causal)), int(splits)
+    _launch(load().kv4_attend, args, q.device, "kv4_attend")

@@ -20,6 +20,7 @@
  *   fa_kernel_resources                <- Triton compile metadata (shared, n_regs)          tuner.py:341-376
  *   fa_kernel_symbol                   <- the compiled kernel that metadata belongs to      tuner.py:356-357
  *   fa_fwd_noalloc                     (no counterpart: fa_fwd for callers that cannot allocate)
+ *   fa_bwd, kv4_append, kv4_attend     (no counterpart: the reference has forward attention only)
  */
 #ifndef FA_GFX950_H
 #define FA_GFX950_H
@@ -30,7 +31,7 @@
 extern "C" {
 #endif
 
-#define FA_ABI_VERSION 6
+#define FA_ABI_VERSION 7
 
 enum {
   FA_OK = 0,
@@ -237,6 +238,108 @@ int fa_kernel_symbol(int32_t op, int32_t variant, int32_t dtype, int32_t D, cons
                      const gemm_tile* gtile, char* buf, int32_t buf_bytes);
 
 int fa_device_limits(int32_t device, fa_device_limits_t* out);
+
+/* Attention backward: dq, dk and dv of fa_fwd's output, from its inputs, output and log-sum-exp. Tensors and
+ * strides as in fa_fwd_args (row strides at least D and at most 2^22 elements); dout is the gradient of o,
+ * dlse (nullable) that of lse. dq has q's shape, dk and dv k's: a kv head's gradients are summed over its
+ * query heads. Causal is top-left as in the forward. A row whose lse is -inf (no keys) has zero gradients.
+ * workspace: fa_bwd_workspace_bytes(), 256-byte aligned; nothing in it is kept between calls. Results do not
+ * depend on the order in which the GPU runs the work. No counterpart in the reference. */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* o;
+  const void* dout;
+  const float* lse;
+  const float* dlse;
+  void* dq;
+  void* dk;
+  void* dv;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t q_stride[4];
+  int64_t k_stride[4];
+  int64_t v_stride[4];
+  int64_t o_stride[4];
+  int64_t dout_stride[4];
+  int64_t lse_stride[3];
+  int64_t dlse_stride[3];
+  int64_t dq_stride[4];
+  int64_t dk_stride[4];
+  int64_t dv_stride[4];
+  int32_t B, H, H_kv, M, N, D;
+  float sm_scale;
+  int32_t dtype;
+  int32_t causal;
+} fa_bwd_args;
+
+int fa_bwd(const fa_bwd_args* args, void* stream);
+int64_t fa_bwd_workspace_bytes(int32_t B, int32_t H, int32_t H_kv, int32_t M, int32_t N);
+
+/* Key/value cache of 4-bit codes. A row of D channels is D / 2 bytes of codes (channel 2i in the low half of
+ * byte i: sign, two exponent bits, one mantissa bit, that is 0, .5, 1, 1.5, 2, 3, 4, 6) and D / 32 scale
+ * bytes, one for 32 channels: e stands for 2^(e - 127), 255 for a block that is NaN throughout. Rows of one
+ * (batch, kv head) are dense; batch and head strides are in bytes, multiples of 16, alike for keys and values.
+ * `rows` rows are allocated (a multiple of 32: whole tiles are read, whatever the rows behind a sequence
+ * hold), `capacity` of them may be used. dtype is the type of the rows that go in and of the queries. */
+typedef struct {
+  uint8_t* k_codes;
+  uint8_t* k_scales;
+  uint8_t* v_codes;
+  uint8_t* v_scales;
+  int64_t code_stride[2];
+  int64_t scale_stride[2];
+  int32_t B, H_kv, D, dtype;
+  int32_t rows, capacity;
+} kv4_cache;
+
+/* Rows t < count[b] (all `rows` without a count) of k and v [B, H_kv, rows, D] become cached rows
+ * start[b] + t; rows that would fall outside [0, capacity) are dropped, cached rows that are not written stay
+ * as they are. start and count are int32 [B] in device memory. k_values and v_values (both or neither) receive
+ * what the appended rows now stand for, in k's type, and zeros in rows that were not written. */
+typedef struct {
+  kv4_cache cache;
+  const void* k;
+  const void* v;
+  void* k_values;
+  void* v_values;
+  const int32_t* start;
+  const int32_t* count;
+  int64_t k_stride[4];
+  int64_t v_stride[4];
+  int64_t k_values_stride[4];
+  int64_t v_values_stride[4];
+  int32_t rows;
+} kv4_append_args;
+
+int kv4_append(const kv4_append_args* args, void* stream);
+
+/* Attention of q [B, H, M, D] over the cache. Row i < count[b] (all M without a count) of sequence b stands at
+ * position start[b] + i and sees the cached rows up to and including it (causal), or all
+ * start[b] + count[b] (otherwise), never past the capacity. Rows that see nothing, and rows at or behind
+ * count[b], are zeros with lse = -inf. lse (nullable): fp32 [B, H, M]. splits > 1 splits each sequence's keys over that
+ * many workgroups, with a workspace of kv4_attend_workspace_bytes() and a second launch that joins them. */
+typedef struct {
+  kv4_cache cache;
+  const void* q;
+  void* o;
+  float* lse;
+  void* workspace;
+  int64_t workspace_bytes;
+  const int32_t* start;
+  const int32_t* count;
+  int64_t q_stride[4];
+  int64_t o_stride[4];
+  int64_t lse_stride[3];
+  int32_t H, M;
+  float sm_scale;
+  int32_t causal;
+  int32_t splits;
+} kv4_attend_args;
+
+int kv4_attend(const kv4_attend_args* args, void* stream);
+int64_t kv4_attend_workspace_bytes(int32_t B, int32_t H, int32_t M, int32_t D, int32_t splits);
 
 #ifdef __cplusplus
 }
