@@ -71,17 +71,41 @@ int launch(const void* fn, int64_t blocks, int64_t y, int threads, void* params,
 
 constexpr int kBwdPrepRows = 64;
 
+constexpr int kBwdBlock = 128;
+
 struct BwdSizes {
-  int64_t row_groups, prep_blocks, vblocks, nd_bytes, bound_bytes;
+  int64_t row_groups, prep_blocks, vblocks, nblocks, mblocks;
+  int64_t kv_splits, q_splits;
+  int64_t bound_at, dk_at, dv_at, dq_at, bytes;  // workspace offsets and size
 };
 
-BwdSizes bwd_sizes(int64_t B, int64_t H, int64_t Hkv, int64_t M, int64_t N) {
+// How many workgroups share a block's steps. A step is a 32-row tile against a block of 128: four products for
+// dK/dV, three for dQ. The chip holds kSlots workgroups; a block that is longer than an even share of all
+// work (and than kMinWork, below which the sums' extra pass costs more than it gives) is split to that.
+BwdSizes bwd_sizes(int64_t B, int64_t H, int64_t Hkv, int64_t M, int64_t N, int64_t D, bool causal) {
+  constexpr int64_t kMinWork = 32;
+  const int64_t kSlots = D == 256 ? 256 : 512;
   BwdSizes s;
   s.prep_blocks = (M + kBwdPrepRows - 1) / kBwdPrepRows;
   s.row_groups = s.prep_blocks * (kBwdPrepRows / 32);
   s.vblocks = (N + kBwdPrepRows - 1) / kBwdPrepRows;
-  s.nd_bytes = align256(B * H * s.row_groups * 64 * 4);
-  s.bound_bytes = align256((2 * B * H * s.prep_blocks + B * Hkv * s.vblocks) * 4);
+  s.nblocks = (N + kBwdBlock - 1) / kBwdBlock;
+  s.mblocks = (M + kBwdBlock - 1) / kBwdBlock;
+  const int64_t qt = (M + 31) / 32, kt = (N + 31) / 32;
+  const int64_t kv_work = 4 * (H / Hkv) * qt, q_work = 3 * kt;  // of the longest block
+  const int64_t all = B * Hkv * s.nblocks * kv_work + B * H * s.mblocks * q_work;
+  int64_t even = (causal ? all / 2 : all) / kSlots;
+  if (even < kMinWork) even = kMinWork;
+  s.kv_splits = 2 * kv_work > 3 * even ? (kv_work + even - 1) / even : 1;
+  s.q_splits = 2 * q_work > 3 * even ? (q_work + even - 1) / even : 1;
+  int64_t at = align256(B * H * s.row_groups * 64 * 4);
+  s.bound_at = at;
+  at += align256((2 * B * H * s.prep_blocks + B * Hkv * s.vblocks) * 4);
+  const int64_t kv_bytes = s.kv_splits > 1 ? align256(s.kv_splits * B * Hkv * N * D * 4) : 0;
+  s.dk_at = at;
+  s.dv_at = at + kv_bytes;
+  s.dq_at = at + 2 * kv_bytes;
+  s.bytes = s.dq_at + (s.q_splits > 1 ? s.q_splits * B * H * M * D * 4 : 0);
   return s;
 }
 
@@ -106,10 +130,9 @@ int check_cache(const kv4_cache* c) {
 
 extern "C" {
 
-int64_t fa_bwd_workspace_bytes(int32_t B, int32_t H, int32_t H_kv, int32_t M, int32_t N) {
-  if (B <= 0 || H <= 0 || H_kv <= 0 || M < 0 || N < 0) return 0;
-  const BwdSizes s = bwd_sizes(B, H, H_kv, M, N);
-  return s.nd_bytes + s.bound_bytes;
+int64_t fa_bwd_workspace_bytes(int32_t B, int32_t H, int32_t H_kv, int32_t M, int32_t N, int32_t D, int32_t causal) {
+  if (B <= 0 || H <= 0 || H_kv <= 0 || M < 0 || N < 0 || D <= 0) return 0;
+  return bwd_sizes(B, H, H_kv, M, N, D, causal != 0).bytes;
 }
 
 int fa_bwd(const fa_bwd_args* a, void* stream) {
@@ -136,15 +159,15 @@ int fa_bwd(const fa_bwd_args* a, void* stream) {
     if ((code = check_tensor("dk", a->dk, a->dk_stride, a->D, 4)) != FA_OK) return code;
     if ((code = check_tensor("dv", a->dv, a->dv_stride, a->D, 4)) != FA_OK) return code;
   }
-  const int64_t need = fa_bwd_workspace_bytes(a->B, a->H, a->H_kv, a->M, a->N);
+  const int64_t need = fa_bwd_workspace_bytes(a->B, a->H, a->H_kv, a->M, a->N, a->D, a->causal);
   if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need))
     return fail(FA_EWORKSPACE, "backward workspace of %lld bytes needed, got %lld", (long long)need,
                 (long long)a->workspace_bytes);
   if (!aligned(a->workspace, 256)) return fail(FA_EINVAL, "workspace must be 256-byte aligned");
   const fa::BwdKernelEntry* e = find_bwd(a->dtype, a->D);
   if (e == nullptr) return fail(FA_ENOTSUP, "backward kernels for dtype=%d D=%d are not built", a->dtype, a->D);
-  if (e->prep_rows != kBwdPrepRows) return fail(FA_ENOTSUP, "row-term blocks of %d rows", e->prep_rows);
-  const BwdSizes s = bwd_sizes(a->B, a->H, a->H_kv, a->M, a->N);
+  if (e->prep_rows != kBwdPrepRows || e->block != kBwdBlock) return fail(FA_ENOTSUP, "backward kernels of other blocks");
+  const BwdSizes s = bwd_sizes(a->B, a->H, a->H_kv, a->M, a->N, a->D, a->causal != 0);
 
   fa::BwdParams p;
   std::memset(&p, 0, sizeof(p));
@@ -169,18 +192,25 @@ int fa_bwd(const fa_bwd_args* a, void* stream) {
   copy3(p.sdk, a->dk_stride);
   copy3(p.sdv, a->dv_stride);
   p.nd = static_cast<float*>(a->workspace);
-  p.bound = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + s.nd_bytes);
+  char* ws = static_cast<char*>(a->workspace);
+  p.bound = reinterpret_cast<float*>(ws + s.bound_at);
+  p.ws_dk = reinterpret_cast<float*>(ws + s.dk_at);
+  p.ws_dv = reinterpret_cast<float*>(ws + s.dv_at);
+  p.ws_dq = reinterpret_cast<float*>(ws + s.dq_at);
   p.B = a->B; p.H = a->H; p.Hkv = a->H_kv; p.M = a->M; p.N = a->N;
   p.group = a->H / a->H_kv;
   p.row_groups = (int32_t)s.row_groups;
   p.prep_blocks = (int32_t)s.prep_blocks;
   p.vblocks = a->dtype == FA_DTYPE_F16 ? (int32_t)s.vblocks : 0;
-  p.nblocks = (a->N + e->block - 1) / e->block;
-  p.mblocks = (a->M + e->block - 1) / e->block;
+  p.nblocks = (int32_t)s.nblocks;
+  p.mblocks = (int32_t)s.mblocks;
+  p.kv_splits = (int32_t)s.kv_splits;
+  p.q_splits = (int32_t)s.q_splits;
   p.causal = a->causal ? 1 : 0;
   p.scale = a->sm_scale;
   p.c = a->sm_scale * 1.4426950408889634f;
-  const int64_t kv_total = (int64_t)a->B * a->H_kv * p.nblocks, q_total = (int64_t)a->B * a->H * p.mblocks;
+  const int64_t kv_total = (int64_t)a->B * a->H_kv * s.nblocks * s.kv_splits;
+  const int64_t q_total = (int64_t)a->B * a->H * s.mblocks * s.q_splits;
   if (kv_total + q_total > 0x7fffffffLL || (int64_t)p.group * p.prep_blocks > 0x7fffffffLL)
     return fail(FA_EINVAL, "backward grid too large (%lld workgroups)", (long long)(kv_total + q_total));
   p.kv_total = (int32_t)kv_total;
@@ -188,6 +218,9 @@ int fa_bwd(const fa_bwd_args* a, void* stream) {
   const int64_t prep = (int64_t)a->B * a->H * p.prep_blocks + (int64_t)a->B * a->H_kv * p.vblocks;
   if (prep > 0 && (code = launch(e->prep, prep, 1, 256, &p, stream, "row-term")) != FA_OK) return code;
   if ((code = launch(e->main, kv_total + q_total, 1, 256, &p, stream, "backward")) != FA_OK) return code;
+  const int64_t sums = ((s.kv_splits > 1 ? 2 * (int64_t)a->B * a->H_kv * a->N : 0) +
+                        (s.q_splits > 1 ? (int64_t)a->B * a->H * a->M : 0)) * (a->D / 4);
+  if (sums > 0 && (code = launch(e->reduce, (sums + 255) / 256, 1, 256, &p, stream, "gradient sum")) != FA_OK) return code;
   return ok();
 }
 

@@ -165,22 +165,26 @@ struct Bwd {
   static constexpr int SMEM = 2 * STAGEB;
   typedef DT<Tag> N_;
 
-  // Rows [row0, row0 + 32) of a matrix into an LDS tile; rows at or past `rows` read as zeros.
-  __device__ static inline void load_tile(const uint16_t* base, int64_t stride, int row0, int rows, uint32_t lds,
-                                          int wave, int lane) {
-    const int left = rows - row0;
-    const uint32_t sb = (uint32_t)stride * 2u;
-    const uint32_t bytes = left <= 0 ? 0u : (uint32_t)((left < T ? left : T) - 1) * sb + (uint32_t)ROWB;
-    const u32x4 rsrc = make_rsrc(base + row0 * stride, bytes);
-    constexpr int RPB = 1024 / ROWB, NB = TILEB / 1024;
+  // Tiles of 32 rows of a matrix into LDS; rows at or past the matrix's end read as zeros.
+  struct Loader {
+    static constexpr int RPB = 1024 / ROWB, NB = TILEB / 1024 / WAVES;  // rows of a 1 KiB block, blocks of a wave
+    uint32_t off[NB], pitch;
+    __device__ inline Loader(int64_t stride, int wave, int lane) {
+      pitch = (uint32_t)stride * 2u;
 #pragma unroll
-    for (int i = 0; i < NB / WAVES; ++i) {
-      const int blk = wave + i * WAVES;
-      const int row = blk * RPB + lane / CPR;
-      const uint32_t off = (uint32_t)row * sb + (uint32_t)(((lane % CPR) ^ (row & SWZ)) * 16);
-      buffer_load16_to_lds<0, true>(rsrc, off, lds + (uint32_t)blk * 1024u);
+      for (int i = 0; i < NB; ++i) {
+        const int row = (wave + i * WAVES) * RPB + lane / CPR;
+        off[i] = (uint32_t)row * pitch + (uint32_t)(((lane % CPR) ^ (row & SWZ)) * 16);
+      }
     }
-  }
+    // `base`: the tile's first row, `left`: rows from there to the end (> 0)
+    __device__ inline void load(const uint16_t* base, int left, uint32_t lds, int wave) const {
+      const u32x4 rsrc = make_rsrc(base, (uint32_t)((left < T ? left : T) - 1) * pitch + (uint32_t)ROWB);
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+        buffer_load16_to_lds<0, true>(rsrc, off[i], lds + (uint32_t)(wave + i * WAVES) * 1024u);
+    }
+  };
 
   // The 32 rows' two terms (256 bytes), by one wave.
   __device__ static inline void load_terms(const float* nd, uint32_t lds, int lane) {
@@ -261,13 +265,16 @@ struct Bwd {
     const int e = (int)(__float_as_uint(bound) >> 23) - 126;  // 2^e > bound
     return e < -100 ? -100 : (e > 100 ? 100 : e);
   }
+  __device__ static inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
   __device__ static inline float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
   __device__ static void dkdv(const BwdParams& p, char* smem, int id) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g = lane >> 4;
-    const int hkb = id / p.nblocks, nb = id % p.nblocks;
-    const int b = hkb / p.Hkv, hk = hkb % p.Hkv;
+    // key blocks innermost: those running together read the same query rows
+    const int nb = uniform(id % p.nblocks), part = uniform(id / p.nblocks % p.kv_splits);
+    const int hkb = uniform(id / p.nblocks / p.kv_splits);
+    const int b = uniform(hkb / p.Hkv), hk = uniform(hkb % p.Hkv);
     const int k0 = nb * BLOCK, kw = k0 + 32 * wave;  // first key of the block, of the wave
     float sc = 1.f, unscale = 1.f;
     if constexpr (BwdTraits<Tag>::kScaled) {
@@ -289,22 +296,31 @@ struct Bwd {
     const int qt_all = (p.M + T - 1) / T;
     const int qt0 = p.causal ? k0 / T : 0;  // rows above the block's first key see none of its keys
     const int per_head = qt_all > qt0 ? qt_all - qt0 : 0;
-    const int total = per_head * p.group;
+    // this split's share of the (query head, row tile) steps
+    const int all = per_head * p.group, share = (all + p.kv_splits - 1) / p.kv_splits;
+    const int first = part * share, total = first >= all ? 0 : (all - first < share ? all - first : share);
+    const int h0 = total > 0 ? uniform(first / per_head) : 0, ht0 = qt0 + first - h0 * per_head;
 
-    int lh = 0, lt = qt0;  // head and tile of the next load
+    const Loader lq(p.sq[2], wave, lane), lo(p.sdo[2], wave, lane);
+    const int hq = hk * p.group + h0;
+    const uint16_t* qh = p.q + b * p.sq[0] + hq * p.sq[1];  // the next load's head
+    const uint16_t* oh = p.dout + b * p.sdo[0] + hq * p.sdo[1];
+    const float* nh = p.nd + ((int64_t)b * p.H + hq) * p.row_groups * 64;
+    int lt = ht0;  // and its tile
     auto load_next = [&](int stage) {
-      const int h = hk * p.group + lh;
       const uint32_t dst = lds + (uint32_t)(stage * STAGEB);
-      load_tile(p.q + b * p.sq[0] + h * p.sq[1], p.sq[2], lt * T, p.M, dst, wave, lane);
-      load_tile(p.dout + b * p.sdo[0] + h * p.sdo[1], p.sdo[2], lt * T, p.M, dst + TILEB, wave, lane);
-      if (wave == 0) load_terms(p.nd + (((int64_t)b * p.H + h) * p.row_groups + lt) * 64, dst + 2 * TILEB, lane);
+      lq.load(qh + lt * (T * p.sq[2]), p.M - lt * T, dst, wave);
+      lo.load(oh + lt * (T * p.sdo[2]), p.M - lt * T, dst + TILEB, wave);
+      if (wave == 0) load_terms(nh + (int64_t)lt * 64, dst + 2 * TILEB, lane);
       if (++lt == qt_all) {
         lt = qt0;
-        ++lh;
+        qh += p.sq[1];
+        oh += p.sdo[1];
+        nh += (int64_t)p.row_groups * 64;
       }
     };
     if (total > 0) load_next(0);
-    int ct = qt0;
+    int ct = ht0;
     for (int it = 0; it < total; ++it) {
       wait_vm_lds_barrier<0>();
       if (it + 1 < total) load_next((it + 1) & 1);
@@ -314,14 +330,17 @@ struct Bwd {
       const int q0 = ct * T;
       if (++ct == qt_all) ct = qt0;
       if (p.causal && q0 + T - 1 < kw) continue;
-      floatx4 s[2][2], dp[2][2];
+      const bool edge = p.causal && q0 < kw + 31;
+      u32x4 pb[2], sb[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        const floatx4 nl = *reinterpret_cast<const floatx4*>(nd + 16 * i + 4 * g);
         const floatx4 nd1 = *reinterpret_cast<const floatx4*>(nd + 32 + 16 * i + 4 * g);
+        floatx4 s[2], dp[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          s[i][j] = (floatx4){0.f, 0.f, 0.f, 0.f};
-          dp[i][j] = nd1;
+          s[j] = (floatx4){0.f, 0.f, 0.f, 0.f};
+          dp[j] = nd1;
         }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -329,33 +348,25 @@ struct Bwd {
           const u32x4 o = frag(os + i * 16 * ROWB, ro ^ (ks << 6));
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            s[i][j] = N_::mfma16(a, kf[j][ks], s[i][j]);
-            dp[i][j] = N_::mfma16(o, vf[j][ks], dp[i][j]);
+            s[j] = N_::mfma16(a, kf[j][ks], s[j]);
+            dp[j] = N_::mfma16(o, vf[j][ks], dp[j]);
           }
         }
-      }
-      const bool edge = p.causal && q0 < kw + 31;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const floatx4 nl = *reinterpret_cast<const floatx4*>(nd + 16 * i + 4 * g);
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            float e = fast_exp2(fmaf(p.c, s[i][j][r], nl[r]));
-            float d = BwdTraits<Tag>::kScaled ? e * (dp[i][j][r] * sc) : e * dp[i][j][r];
+            float e = fast_exp2(fmaf(p.c, s[j][r], nl[r]));
+            float d = BwdTraits<Tag>::kScaled ? e * (dp[j][r] * sc) : e * dp[j][r];
             if (edge && kw + 16 * j + c16 > q0 + 16 * i + 4 * g + r) e = d = 0.f;
-            s[i][j][r] = e;
-            dp[i][j][r] = d;
+            s[j][r] = e;
+            dp[j][r] = d;
           }
-      }
-      u32x4 pb[2], sb[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        pb[j] = (u32x4){N_::pack2(s[0][j][0], s[0][j][1]), N_::pack2(s[0][j][2], s[0][j][3]),
-                        N_::pack2(s[1][j][0], s[1][j][1]), N_::pack2(s[1][j][2], s[1][j][3])};
-        sb[j] = (u32x4){N_::pack2(dp[0][j][0], dp[0][j][1]), N_::pack2(dp[0][j][2], dp[0][j][3]),
-                        N_::pack2(dp[1][j][0], dp[1][j][1]), N_::pack2(dp[1][j][2], dp[1][j][3])};
+          pb[j][2 * i] = N_::pack2(s[j][0], s[j][1]);
+          pb[j][2 * i + 1] = N_::pack2(s[j][2], s[j][3]);
+          sb[j][2 * i] = N_::pack2(dp[j][0], dp[j][1]);
+          sb[j][2 * i + 1] = N_::pack2(dp[j][2], dp[j][3]);
+        }
       }
 #pragma unroll
       for (int d = 0; d < DT16; ++d) {
@@ -373,6 +384,15 @@ struct Bwd {
     for (int j = 0; j < 2; ++j) {
       const int key = kw + 16 * j + c16;
       if (key >= p.N) continue;
+      if (p.kv_splits > 1) {
+        const int64_t w = ((int64_t)(part * p.B + b) * p.Hkv + hk) * p.N + key;
+#pragma unroll
+        for (int d = 0; d < DT16; ++d) {
+          *reinterpret_cast<floatx4*>(p.ws_dk + w * D + 16 * d + 4 * g) = dk[d][j] * fk;
+          *reinterpret_cast<floatx4*>(p.ws_dv + w * D + 16 * d + 4 * g) = dv[d][j] * fv;
+        }
+        continue;
+      }
       uint16_t* ok = p.dk + b * p.sdk[0] + hk * p.sdk[1] + key * p.sdk[2] + 4 * g;
       uint16_t* ov = p.dv + b * p.sdv[0] + hk * p.sdv[1] + key * p.sdv[2] + 4 * g;
 #pragma unroll
@@ -387,10 +407,10 @@ struct Bwd {
   __device__ static void dq(const BwdParams& p, char* smem, int id) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g = lane >> 4;
-    const int bh = id / p.mblocks;
-    // causal: the heaviest block (most keys) of a head first
-    const int mb = p.causal ? p.mblocks - 1 - id % p.mblocks : id % p.mblocks;
-    const int b = bh / p.H, h = bh % p.H, hk = h / p.group;
+    const int at = id % p.mblocks, part = uniform(id / p.mblocks % p.q_splits);
+    const int bh = uniform(id / p.mblocks / p.q_splits);
+    const int mb = uniform(p.causal ? p.mblocks - 1 - at : at);  // causal: the block with the most keys first
+    const int b = uniform(bh / p.H), h = uniform(bh % p.H), hk = uniform(h / p.group);
     const int m0 = mb * BLOCK, mw = m0 + 32 * wave;
     float sc = 1.f, unscale = 1.f;
     if constexpr (BwdTraits<Tag>::kScaled) {
@@ -421,29 +441,33 @@ struct Bwd {
     const uint32_t lds = lds_address(smem);
     const uint32_t ro = row_off(lane), to = tr_off(lane);
     const int n_end = p.causal && m0 + BLOCK < p.N ? m0 + BLOCK : p.N;
-    const int tiles = (n_end + T - 1) / T;
+    const int all = (n_end + T - 1) / T, share = (all + p.q_splits - 1) / p.q_splits;
+    const int first = part * share, tiles = first >= all ? first : (all - first < share ? all : first + share);
     const uint16_t* kb = p.k + b * p.sk[0] + hk * p.sk[1];
     const uint16_t* vb = p.v + b * p.sv[0] + hk * p.sv[1];
+    const Loader lk(p.sk[2], wave, lane), lv(p.sv[2], wave, lane);
     auto load = [&](int t) {
       const uint32_t dst = lds + (uint32_t)((t & 1) * STAGEB);
-      load_tile(kb, p.sk[2], t * T, p.N, dst, wave, lane);
-      load_tile(vb, p.sv[2], t * T, p.N, dst + TILEB, wave, lane);
+      lk.load(kb + t * (T * p.sk[2]), p.N - t * T, dst, wave);
+      lv.load(vb + t * (T * p.sv[2]), p.N - t * T, dst + TILEB, wave);
     };
-    if (tiles > 0) load(0);
-    for (int t = 0; t < tiles; ++t) {
+    if (first < tiles) load(first);
+    for (int t = first; t < tiles; ++t) {
       wait_vm_lds_barrier<0>();
       if (t + 1 < tiles) load(t + 1);
       const char* ks_ = smem + (t & 1) * STAGEB;
       const char* vs_ = ks_ + TILEB;
       const int n0 = t * T;
       if (p.causal && n0 > mw + 31) continue;
-      floatx4 s[2][2], dp[2][2];  // [key tile][row tile]
+      const bool edge = (p.causal && n0 + T - 1 > mw) || n0 + T > p.N;
+      u32x4 sb[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        floatx4 s[2], dp[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          s[i][j] = (floatx4){0.f, 0.f, 0.f, 0.f};
-          dp[i][j] = (floatx4){nd[j], nd[j], nd[j], nd[j]};
+          s[j] = (floatx4){0.f, 0.f, 0.f, 0.f};
+          dp[j] = (floatx4){nd[j], nd[j], nd[j], nd[j]};
         }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -451,31 +475,26 @@ struct Bwd {
           const u32x4 v = frag(vs_ + i * 16 * ROWB, ro ^ (ks << 6));
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            s[i][j] = N_::mfma16(a, qf[j][ks], s[i][j]);
-            dp[i][j] = N_::mfma16(v, of[j][ks], dp[i][j]);
+            s[j] = N_::mfma16(a, qf[j][ks], s[j]);
+            dp[j] = N_::mfma16(v, of[j][ks], dp[j]);
           }
         }
-      }
-      const bool edge = (p.causal && n0 + T - 1 > mw) || n0 + T > p.N;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float e = fast_exp2(fmaf(p.c, s[i][j][r], nl[j]));
-            float d = BwdTraits<Tag>::kScaled ? e * (dp[i][j][r] * sc) : e * dp[i][j][r];
+            const float e = fast_exp2(fmaf(p.c, s[j][r], nl[j]));
+            float d = BwdTraits<Tag>::kScaled ? e * (dp[j][r] * sc) : e * dp[j][r];
             if (edge) {
               const int key = n0 + 16 * i + 4 * g + r;
               if (key >= p.N || (p.causal && key > mw + 16 * j + c16)) d = 0.f;
             }
-            dp[i][j][r] = d;
+            dp[j][r] = d;
           }
-      u32x4 sb[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        sb[j] = (u32x4){N_::pack2(dp[0][j][0], dp[0][j][1]), N_::pack2(dp[0][j][2], dp[0][j][3]),
-                        N_::pack2(dp[1][j][0], dp[1][j][1]), N_::pack2(dp[1][j][2], dp[1][j][3])};
+          sb[j][2 * i] = N_::pack2(dp[j][0], dp[j][1]);
+          sb[j][2 * i + 1] = N_::pack2(dp[j][2], dp[j][3]);
+        }
+      }
 #pragma unroll
       for (int d = 0; d < DT16; ++d) {
         const u32x4 kt = tfrag(ks_, to ^ (d << 5));
@@ -488,6 +507,12 @@ struct Bwd {
     for (int j = 0; j < 2; ++j) {
       const int row = mw + 16 * j + c16;
       if (row >= p.M) continue;
+      if (p.q_splits > 1) {
+        const int64_t w = ((int64_t)(part * p.B + b) * p.H + h) * p.M + row;
+#pragma unroll
+        for (int d = 0; d < DT16; ++d) *reinterpret_cast<floatx4*>(p.ws_dq + w * D + 16 * d + 4 * g) = acc[d][j] * f;
+        continue;
+      }
       uint16_t* out = p.dq + b * p.sdq[0] + h * p.sdq[1] + row * p.sdq[2] + 4 * g;
 #pragma unroll
       for (int d = 0; d < DT16; ++d) {
@@ -510,8 +535,44 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void fa_bwd_kernel(BwdParams
     Bwd<Tag, D>::dq(p, smem, xcd_remap(id - p.kv_total, p.q_total));
 }
 
+// Sums of the splits' partial gradients, in split order: a thread takes four channels of one row.
+template <typename Tag, int D>
+__global__ __launch_bounds__(256) void fa_bwd_reduce_kernel(BwdParams p) {
+  const int64_t kv_rows = p.kv_splits > 1 ? (int64_t)p.B * p.Hkv * p.N : 0;
+  const int64_t q_rows = p.q_splits > 1 ? (int64_t)p.B * p.H * p.M : 0;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  int64_t row = id / (D / 4);
+  const int d = (int)(id % (D / 4)) * 4;
+  if (row >= 2 * kv_rows + q_rows) return;
+  const float* src;
+  uint16_t* out;
+  const int64_t* st;
+  int64_t rows;
+  int splits, heads, len;
+  if (row < 2 * kv_rows) {
+    const bool second = row >= kv_rows;
+    row -= second ? kv_rows : 0;
+    src = second ? p.ws_dv : p.ws_dk;
+    out = second ? p.dv : p.dk;
+    st = second ? p.sdv : p.sdk;
+    rows = kv_rows, splits = p.kv_splits, heads = p.Hkv, len = p.N;
+  } else {
+    row -= 2 * kv_rows;
+    src = p.ws_dq;
+    out = p.dq;
+    st = p.sdq;
+    rows = q_rows, splits = p.q_splits, heads = p.H, len = p.M;
+  }
+  floatx4 sum = *reinterpret_cast<const floatx4*>(src + row * D + d);
+  for (int i = 1; i < splits; ++i) sum += *reinterpret_cast<const floatx4*>(src + (i * rows + row) * D + d);
+  const int64_t bh = row / len;
+  out += bh / heads * st[0] + bh % heads * st[1] + row % len * st[2] + d;
+  *reinterpret_cast<u32x2*>(out) = (u32x2){DT<Tag>::pack2(sum[0], sum[1]), DT<Tag>::pack2(sum[2], sum[3])};
+}
+
 #define FA_BWD_ENTRY(TAG, DTYPE, D) \
-  {DTYPE, D, (const void*)&fa_bwd_prep_kernel<TAG, D>, (const void*)&fa_bwd_kernel<TAG, D>, Bwd<TAG, D>::BLOCK, kPrepRows}
+  {DTYPE, D, (const void*)&fa_bwd_prep_kernel<TAG, D>, (const void*)&fa_bwd_kernel<TAG, D>, \
+   (const void*)&fa_bwd_reduce_kernel<TAG, D>, Bwd<TAG, D>::BLOCK, kPrepRows}
 
 static const BwdKernelEntry kBwdEntries[] = {
     FA_BWD_ENTRY(f16_t, FA_DTYPE_F16, 64),   FA_BWD_ENTRY(f16_t, FA_DTYPE_F16, 128),

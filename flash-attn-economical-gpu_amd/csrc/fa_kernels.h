@@ -90,12 +90,16 @@ struct BwdParams {
   int64_t sq[3], sk[3], sv[3], so[3], sdo[3], sl[3], sdl[3], sdq[3], sdk[3], sdv[3];
   float* nd;     // workspace: two fp32 terms per query row, in groups of 32 rows
   float* bound;  // workspace: block maxima behind fp16's dS scale
+  float* ws_dk;  // workspace: partial gradients [kv_splits][B * Hkv][N][D] (kv_splits > 1)
+  float* ws_dv;
+  float* ws_dq;  // workspace: partial gradients [q_splits][B * H][M][D] (q_splits > 1)
   int32_t B, H, Hkv, M, N, group;
   int32_t row_groups;   // 32-row groups of a head's row terms
   int32_t prep_blocks;  // row-term blocks of a query head
   int32_t vblocks;      // V-norm blocks of a kv head (fp16; 0 otherwise)
   int32_t nblocks, mblocks;   // dK/dV blocks of a kv head, dQ blocks of a query head
-  int32_t kv_total, q_total;  // blocks of each kind
+  int32_t kv_splits, q_splits;  // workgroups that share a block's steps
+  int32_t kv_total, q_total;    // workgroups of each kind
   int32_t causal;
   float c;      // scale * log2(e)
   float scale;
@@ -106,6 +110,7 @@ struct BwdKernelEntry {
   int32_t D;
   const void* prep;
   const void* main;
+  const void* reduce;
   int32_t block;      // keys (dK/dV) and query rows (dQ) of a workgroup
   int32_t prep_rows;  // rows of a row-term block
 };

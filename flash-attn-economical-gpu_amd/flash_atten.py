@@ -317,7 +317,7 @@ def attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: to
     if plan is None:
         scale = q.shape[3] ** -0.5 if sm_scale is None else float(sm_scale)
         plan = (hip_lib.bwd_plan(do, q, k, v, o, lse, dlse, dq, dk, dv, sm_scale=scale, causal=bool(causal)),
-                hip_lib.bwd_workspace_bytes(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2]))
+                hip_lib.bwd_workspace_bytes(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], bool(causal)))
         _keep_plan(key, plan)
     block, need = plan
     workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None

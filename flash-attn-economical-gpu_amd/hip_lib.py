@@ -220,7 +220,7 @@ SIGNATURES = {
     ),
     "fa_device_limits": (ctypes.c_int, [ctypes.c_int32, ctypes.POINTER(FaDeviceLimits)]),
     "fa_bwd": (ctypes.c_int, [ctypes.POINTER(FaBwdArgs), ctypes.c_void_p]),
-    "fa_bwd_workspace_bytes": (ctypes.c_int64, [ctypes.c_int32] * 5),
+    "fa_bwd_workspace_bytes": (ctypes.c_int64, [ctypes.c_int32] * 7),
     "kv4_append": (ctypes.c_int, [ctypes.POINTER(Kv4AppendArgs), ctypes.c_void_p]),
     "kv4_attend": (ctypes.c_int, [ctypes.POINTER(Kv4AttendArgs), ctypes.c_void_p]),
     "kv4_attend_workspace_bytes": (ctypes.c_int64, [ctypes.c_int32] * 5),
@@ -566,8 +566,8 @@ def _launch(fn, args, device: torch.device, what: str) -> None:
 
 
 @functools.lru_cache(maxsize=4096)
-def bwd_workspace_bytes(B: int, H: int, H_kv: int, M: int, N: int) -> int:
-    return int(load().fa_bwd_workspace_bytes(B, H, H_kv, M, N))
+def bwd_workspace_bytes(B: int, H: int, H_kv: int, M: int, N: int, D: int, causal: bool) -> int:
+    return int(load().fa_bwd_workspace_bytes(B, H, H_kv, M, N, D, int(causal)))
 
 
 def bwd_plan(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,

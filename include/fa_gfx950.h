@@ -275,7 +275,7 @@ typedef struct {
 } fa_bwd_args;
 
 int fa_bwd(const fa_bwd_args* args, void* stream);
-int64_t fa_bwd_workspace_bytes(int32_t B, int32_t H, int32_t H_kv, int32_t M, int32_t N);
+int64_t fa_bwd_workspace_bytes(int32_t B, int32_t H, int32_t H_kv, int32_t M, int32_t N, int32_t D, int32_t causal);
 
 /* Key/value cache of 4-bit codes. A row of D channels is D / 2 bytes of codes (channel 2i in the low half of
  * byte i: sign, two exponent bits, one mantissa bit, that is 0, .5, 1, 1.5, 2, 3, 4, 6) and D / 32 scale

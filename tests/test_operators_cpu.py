@@ -76,7 +76,7 @@ def test_empty_calls_do_nothing():
     assert lib.fa_bwd(None, None) == lib.kv4_append(None, None) == lib.kv4_attend(None, None) == hip_lib.FA_EINVAL
     assert lib.kv4_append(ctypes.byref(_append(rows=0)), None) == hip_lib.FA_OK
     assert lib.kv4_attend(ctypes.byref(_attend(M=0)), None) == hip_lib.FA_OK
-    assert lib.fa_bwd_workspace_bytes(0, 1, 1, 1, 1) == lib.kv4_attend_workspace_bytes(1, 1, 1, 64, 1) == 0
+    assert lib.fa_bwd_workspace_bytes(0, 1, 1, 1, 1, 64, 0) == lib.kv4_attend_workspace_bytes(1, 1, 1, 64, 1) == 0
     assert lib.kv4_attend_workspace_bytes(2, 4, 3, 64, 5) == 5 * 24 * (64 * 4 + 8)
 
 
