@@ -71,30 +71,29 @@ int launch(const void* fn, int64_t blocks, int64_t y, int threads, void* params,
 
 constexpr int kBwdPrepRows = 64;
 
-constexpr int kBwdBlock = 128;
-
 struct BwdSizes {
   int64_t row_groups, prep_blocks, vblocks, nblocks, mblocks;
   int64_t kv_splits, q_splits;
   int64_t bound_at, dk_at, dv_at, dq_at, bytes;  // workspace offsets and size
 };
 
-// How many workgroups share a block's steps. A step is a 32-row tile against a block of 128: four products for
-// dK/dV, three for dQ. The chip holds kSlots workgroups; a block that is longer than an even share of all
+// How many workgroups share a block's steps. A step is a 32-row tile against a block: four products for dK/dV,
+// three for dQ. The chip (256 CUs) holds `slots` workgroups; a block that is longer than an even share of all
 // work (and than kMinWork, below which the sums' extra pass costs more than it gives) is split to that.
-BwdSizes bwd_sizes(int64_t B, int64_t H, int64_t Hkv, int64_t M, int64_t N, int64_t D, bool causal) {
+BwdSizes bwd_sizes(const fa::BwdKernelEntry* e, int64_t B, int64_t H, int64_t Hkv, int64_t M, int64_t N, int64_t D,
+                   bool causal) {
   constexpr int64_t kMinWork = 32;
-  const int64_t kSlots = D == 256 ? 256 : 512;
+  const int64_t slots = 256 * e->per_cu;
   BwdSizes s;
   s.prep_blocks = (M + kBwdPrepRows - 1) / kBwdPrepRows;
   s.row_groups = s.prep_blocks * (kBwdPrepRows / 32);
   s.vblocks = (N + kBwdPrepRows - 1) / kBwdPrepRows;
-  s.nblocks = (N + kBwdBlock - 1) / kBwdBlock;
-  s.mblocks = (M + kBwdBlock - 1) / kBwdBlock;
+  s.nblocks = (N + e->block - 1) / e->block;
+  s.mblocks = (M + e->block - 1) / e->block;
   const int64_t qt = (M + 31) / 32, kt = (N + 31) / 32;
   const int64_t kv_work = 4 * (H / Hkv) * qt, q_work = 3 * kt;  // of the longest block
   const int64_t all = B * Hkv * s.nblocks * kv_work + B * H * s.mblocks * q_work;
-  int64_t even = (causal ? all / 2 : all) / kSlots;
+  int64_t even = (causal ? all / 2 : all) / slots;
   if (even < kMinWork) even = kMinWork;
   s.kv_splits = 2 * kv_work > 3 * even ? (kv_work + even - 1) / even : 1;
   s.q_splits = 2 * q_work > 3 * even ? (q_work + even - 1) / even : 1;
@@ -131,8 +130,9 @@ int check_cache(const kv4_cache* c) {
 extern "C" {
 
 int64_t fa_bwd_workspace_bytes(int32_t B, int32_t H, int32_t H_kv, int32_t M, int32_t N, int32_t D, int32_t causal) {
-  if (B <= 0 || H <= 0 || H_kv <= 0 || M < 0 || N < 0 || D <= 0) return 0;
-  return bwd_sizes(B, H, H_kv, M, N, D, causal != 0).bytes;
+  const fa::BwdKernelEntry* e = find_bwd(FA_DTYPE_F16, D);  // blocks are alike for both types
+  if (e == nullptr || B <= 0 || H <= 0 || H_kv <= 0 || M < 0 || N < 0) return 0;
+  return bwd_sizes(e, B, H, H_kv, M, N, D, causal != 0).bytes;
 }
 
 int fa_bwd(const fa_bwd_args* a, void* stream) {
@@ -166,8 +166,8 @@ int fa_bwd(const fa_bwd_args* a, void* stream) {
   if (!aligned(a->workspace, 256)) return fail(FA_EINVAL, "workspace must be 256-byte aligned");
   const fa::BwdKernelEntry* e = find_bwd(a->dtype, a->D);
   if (e == nullptr) return fail(FA_ENOTSUP, "backward kernels for dtype=%d D=%d are not built", a->dtype, a->D);
-  if (e->prep_rows != kBwdPrepRows || e->block != kBwdBlock) return fail(FA_ENOTSUP, "backward kernels of other blocks");
-  const BwdSizes s = bwd_sizes(a->B, a->H, a->H_kv, a->M, a->N, a->D, a->causal != 0);
+  if (e->prep_rows != kBwdPrepRows) return fail(FA_ENOTSUP, "row-term blocks of %d rows", e->prep_rows);
+  const BwdSizes s = bwd_sizes(e, a->B, a->H, a->H_kv, a->M, a->N, a->D, a->causal != 0);
 
   fa::BwdParams p;
   std::memset(&p, 0, sizeof(p));

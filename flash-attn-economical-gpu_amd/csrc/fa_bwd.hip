@@ -21,6 +21,8 @@
 // gradients would fall under 2^-14 and lose bits, so P is scaled by 2^15 (in the exponent's offset, free)
 // and dS by a power of two from a bound on |dP - delta| (row norms of dO and V, |delta|) that puts it under
 // 2^15; the sums are scaled back in fp32. bf16 has fp32's range and takes neither.
+#include <type_traits>
+
 #include "fa_common.h"
 #include "fa_kernels.h"
 #include "../../include/fa_gfx950.h"
@@ -148,47 +150,51 @@ __global__ __launch_bounds__(256) void fa_bwd_prep_kernel(BwdParams p) {
   }
 }
 
-template <typename Tag, int D>
+template <typename Tag, int D, int KT>
 struct Bwd {
   static constexpr int WAVES = 4;
-  static constexpr int T = 32;               // rows of a tile passing through LDS, and rows owned per wave
-  static constexpr int BLOCK = WAVES * 32;   // rows owned per workgroup
+  static constexpr int T = 32;                   // rows of a tile passing through LDS
+  static constexpr int OWN = 16 * KT;            // rows owned per wave
+  static constexpr int BLOCK = WAVES * OWN;      // rows owned per workgroup
   static constexpr int KS = D / 32;          // k = 32 steps over D
   static constexpr int DT16 = D / 16;        // 16-wide tiles over D
   static constexpr int ROWB = 2 * D;         // bytes of an LDS row
   static constexpr int CPR = D / 8;          // 16-byte chunks of a row
-  // LDS rows are unpadded (LDS-DMA writes 1 KiB blocks); chunk c of row r lies at c ^ (r & SWZ), so that the
-  // 16 rows of a fragment read fall on different banks.
-  static constexpr int SWZ = CPR < 16 ? CPR - 1 : 15;
   static constexpr int TILEB = T * ROWB;
   static constexpr int STAGEB = 2 * TILEB + 256;  // two tiles and a group of row terms
-  static constexpr int SMEM = 2 * STAGEB;
+  // A ring of four stages: a tile's loads are issued three steps before its use.
+  static constexpr int STAGES = 4;
+  static constexpr int SMEM = STAGES * STAGEB;
+  static constexpr int NB = TILEB / 1024 / WAVES;  // LDS-DMA instructions of a wave per tile
+
+  // LDS rows are unpadded (LDS-DMA writes 1 KiB blocks); chunk c of row r lies at c ^ swz(r). The LDS serves 256
+  // bytes a cycle: 16 lanes of a row-fragment read (one chunk of 16 rows) and 32 lanes of a transposing read
+  // (an even chunk and the next, of 8 rows). Both fall on different banks when rows 0 .. 7 differ in the chunk
+  // pair and r, r + 8 in the place within it (D = 64, two rows to 256 bytes: rows 0, 2, 4, 6).
+  __device__ static inline int swz(int r) {
+    return D == 64 ? (r & 6) : (r & 7) << 1;
+  }
   typedef DT<Tag> N_;
 
-  // Tiles of 32 rows of a matrix into LDS; rows at or past the matrix's end read as zeros.
-  struct Loader {
-    static constexpr int RPB = 1024 / ROWB, NB = TILEB / 1024 / WAVES;  // rows of a 1 KiB block, blocks of a wave
-    uint32_t off[NB], pitch;
-    __device__ inline Loader(int64_t stride, int wave, int lane) {
-      pitch = (uint32_t)stride * 2u;
+  // A tile of 32 rows (`base`: its first row, `left`: rows from there to the matrix's end, past which zeros are
+  // read) into LDS. The lanes' offsets are worked out anew for every tile: held across the loop they
+  // are spilled (D = 128 has no register free), and a reload from scratch stalls the loads behind it.
+  __device__ static inline void load_tile(const uint16_t* base, int64_t stride, int left, uint32_t lds, int wave, int lane) {
+    constexpr int RPB = 1024 / ROWB;  // rows of a 1 KiB block
+    const uint32_t pitch = (uint32_t)stride * 2u;
+    const u32x4 rsrc = make_rsrc(base, left <= 0 ? 0u : (uint32_t)((left < T ? left : T) - 1) * pitch + (uint32_t)ROWB);
+    asm volatile("" : "+v"(lane));
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const int row = (wave + i * WAVES) * RPB + lane / CPR;
-        off[i] = (uint32_t)row * pitch + (uint32_t)(((lane % CPR) ^ (row & SWZ)) * 16);
-      }
+    for (int i = 0; i < NB; ++i) {
+      const uint32_t row = (wave + i * WAVES) * RPB + lane / CPR;
+      const uint32_t off = row * pitch + (((lane % CPR) ^ swz(row)) * 16u);
+      buffer_load16_to_lds<0, true>(rsrc, off, lds + (uint32_t)(wave + i * WAVES) * 1024u);
     }
-    // `base`: the tile's first row, `left`: rows from there to the end (> 0)
-    __device__ inline void load(const uint16_t* base, int left, uint32_t lds, int wave) const {
-      const u32x4 rsrc = make_rsrc(base, (uint32_t)((left < T ? left : T) - 1) * pitch + (uint32_t)ROWB);
-#pragma unroll
-      for (int i = 0; i < NB; ++i)
-        buffer_load16_to_lds<0, true>(rsrc, off[i], lds + (uint32_t)(wave + i * WAVES) * 1024u);
-    }
-  };
+  }
 
-  // The 32 rows' two terms (256 bytes), by one wave.
-  __device__ static inline void load_terms(const float* nd, uint32_t lds, int lane) {
-    const u32x4 rsrc = make_rsrc(nd, 256);
+  // The 32 rows' two terms (256 bytes). Every wave loads them, so that all have the same loads in flight.
+  __device__ static inline void load_terms(const float* nd, bool live, uint32_t lds, int lane) {
+    const u32x4 rsrc = make_rsrc(nd, live ? 256 : 0);
     const uint32_t dst = __builtin_amdgcn_readfirstlane(lds);
     asm volatile("s_nop 4\n\ts_mov_b32 m0, %1\n\tbuffer_load_dword %0, %2, 0 offen lds"
                  :
@@ -200,13 +206,13 @@ struct Bwd {
   // off ^ (ks << 6), row tile i at + i * 16 * ROWB.
   __device__ static inline uint32_t row_off(int lane) {
     const int r = lane & 15, g = lane >> 4;
-    return (uint32_t)(r * ROWB + ((g ^ (r & SWZ)) << 4));
+    return (uint32_t)(r * ROWB + ((g ^ swz(r)) << 4));
   }
   // Byte offset of a lane's transposing read (rows 4 (lane >> 4) .. + 3, its 4 of 16 columns): columns
   // 16 dt .. are at off ^ (dt << 5), row tile i at + i * 16 * ROWB.
   __device__ static inline uint32_t tr_off(int lane) {
     const int L = lane & 15, r = 4 * (lane >> 4) + (L >> 2);
-    return (uint32_t)(r * ROWB + ((((L & 3) >> 1) ^ (r & SWZ)) << 4) + ((L & 1) << 3));
+    return (uint32_t)(r * ROWB + ((((L & 3) >> 1) ^ swz(r)) << 4) + ((L & 1) << 3));
   }
   __device__ static inline u32x4 frag(const char* tile, uint32_t off) {
     return *reinterpret_cast<const u32x4*>(tile + off);
@@ -217,11 +223,11 @@ struct Bwd {
     return (u32x4){a[0], a[1], b[0], b[1]};
   }
 
-  // 32 rows' fragments (two 16-row tiles) straight from memory, zeros past `rows`.
-  __device__ static inline void load_frags(u32x4 (&f)[2][KS], const uint16_t* base, int64_t stride, int row0, int rows,
+  // The owned rows' fragments straight from memory, zeros past `rows`.
+  __device__ static inline void load_frags(u32x4 (&f)[KT][KS], const uint16_t* base, int64_t stride, int row0, int rows,
                                            int lane) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < KT; ++i) {
       const int row = row0 + 16 * i + (lane & 15);
       const uint16_t* src = base + row * stride + 8 * (lane >> 4);
 #pragma unroll
@@ -263,7 +269,7 @@ struct Bwd {
     __syncthreads();
     const float bound = sqrtf(o2) * sqrtf(v2) + dl;
     const int e = (int)(__float_as_uint(bound) >> 23) - 126;  // 2^e > bound
-    return e < -100 ? -100 : (e > 100 ? 100 : e);
+    return uniform(e < -100 ? -100 : (e > 100 ? 100 : e));
   }
   __device__ static inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
   __device__ static inline float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
@@ -275,21 +281,21 @@ struct Bwd {
     const int nb = uniform(id % p.nblocks), part = uniform(id / p.nblocks % p.kv_splits);
     const int hkb = uniform(id / p.nblocks / p.kv_splits);
     const int b = uniform(hkb / p.Hkv), hk = uniform(hkb % p.Hkv);
-    const int k0 = nb * BLOCK, kw = k0 + 32 * wave;  // first key of the block, of the wave
+    const int k0 = nb * BLOCK, kw = k0 + OWN * wave;  // first key of the block, of the wave
     float sc = 1.f, unscale = 1.f;
     if constexpr (BwdTraits<Tag>::kScaled) {
       const int e = scale_exponent(p, b, hk, reinterpret_cast<float*>(smem));
       sc = pow2(-e);
       unscale = pow2(e);
     }
-    u32x4 kf[2][KS], vf[2][KS];
+    u32x4 kf[KT][KS], vf[KT][KS];
     load_frags(kf, p.k + b * p.sk[0] + hk * p.sk[1], p.sk[2], kw, p.N, lane);
     load_frags(vf, p.v + b * p.sv[0] + hk * p.sv[1], p.sv[2], kw, p.N, lane);
-    floatx4 dk[DT16][2], dv[DT16][2];
+    floatx4 dk[DT16][KT], dv[DT16][KT];
 #pragma unroll
     for (int d = 0; d < DT16; ++d)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) dk[d][i] = dv[d][i] = (floatx4){0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < KT; ++i) dk[d][i] = dv[d][i] = (floatx4){0.f, 0.f, 0.f, 0.f};
 
     const uint32_t lds = lds_address(smem);
     const uint32_t ro = row_off(lane), to = tr_off(lane);
@@ -301,44 +307,47 @@ struct Bwd {
     const int first = part * share, total = first >= all ? 0 : (all - first < share ? all - first : share);
     const int h0 = total > 0 ? uniform(first / per_head) : 0, ht0 = qt0 + first - h0 * per_head;
 
-    const Loader lq(p.sq[2], wave, lane), lo(p.sdo[2], wave, lane);
     const int hq = hk * p.group + h0;
     const uint16_t* qh = p.q + b * p.sq[0] + hq * p.sq[1];  // the next load's head
     const uint16_t* oh = p.dout + b * p.sdo[0] + hq * p.sdo[1];
     const float* nh = p.nd + ((int64_t)b * p.H + hq) * p.row_groups * 64;
     int lt = ht0;  // and its tile
-    auto load_next = [&](int stage) {
-      const uint32_t dst = lds + (uint32_t)(stage * STAGEB);
-      lq.load(qh + lt * (T * p.sq[2]), p.M - lt * T, dst, wave);
-      lo.load(oh + lt * (T * p.sdo[2]), p.M - lt * T, dst + TILEB, wave);
-      if (wave == 0) load_terms(nh + (int64_t)lt * 64, dst + 2 * TILEB, lane);
-      if (++lt == qt_all) {
+    // Behind the last step the loads go on with nothing in range: the waits count on a fixed number in flight.
+    auto load_next = [&](int step) {
+      const uint32_t dst = lds + (uint32_t)((step % STAGES) * STAGEB);
+      const int left = step < total ? p.M - lt * T : 0;
+      load_tile(qh + lt * (T * p.sq[2]), p.sq[2], left, dst, wave, lane);
+      load_tile(oh + lt * (T * p.sdo[2]), p.sdo[2], left, dst + TILEB, wave, lane);
+      load_terms(nh + (int64_t)lt * 64, left > 0, dst + 2 * TILEB, lane);
+      if (step < total && ++lt == qt_all) {
         lt = qt0;
         qh += p.sq[1];
         oh += p.sdo[1];
         nh += (int64_t)p.row_groups * 64;
       }
     };
-    if (total > 0) load_next(0);
-    int ct = ht0;
-    for (int it = 0; it < total; ++it) {
-      wait_vm_lds_barrier<0>();
-      if (it + 1 < total) load_next((it + 1) & 1);
-      const char* qs = smem + (it & 1) * STAGEB;
+    if (total > 0)
+      for (int i = 0; i < STAGES - 1; ++i) load_next(i);
+    int it = 0, ct = ht0;
+    auto step = [&](auto edge_tile) {
+      constexpr bool EDGE = decltype(edge_tile)::value;
+      wait_vm_lds_barrier<(STAGES - 2) * (2 * NB + 1)>();
+      load_next(it + STAGES - 1);
+      const char* qs = smem + (it % STAGES) * STAGEB;
       const char* os = qs + TILEB;
       const float* nd = reinterpret_cast<const float*>(qs + 2 * TILEB);
       const int q0 = ct * T;
-      if (++ct == qt_all) ct = qt0;
-      if (p.causal && q0 + T - 1 < kw) continue;
-      const bool edge = p.causal && q0 < kw + 31;
-      u32x4 pb[2], sb[2];
+      ++it;
+      ++ct;
+      if (EDGE && q0 + T - 1 < kw) return;
+      u32x4 pb[KT], sb[KT];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const floatx4 nl = *reinterpret_cast<const floatx4*>(nd + 16 * i + 4 * g);
         const floatx4 nd1 = *reinterpret_cast<const floatx4*>(nd + 32 + 16 * i + 4 * g);
-        floatx4 s[2], dp[2];
+        floatx4 s[KT], dp[KT];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < KT; ++j) {
           s[j] = (floatx4){0.f, 0.f, 0.f, 0.f};
           dp[j] = nd1;
         }
@@ -347,20 +356,19 @@ struct Bwd {
           const u32x4 a = frag(qs + i * 16 * ROWB, ro ^ (ks << 6));
           const u32x4 o = frag(os + i * 16 * ROWB, ro ^ (ks << 6));
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
+          for (int j = 0; j < KT; ++j) {
             s[j] = N_::mfma16(a, kf[j][ks], s[j]);
             dp[j] = N_::mfma16(o, vf[j][ks], dp[j]);
           }
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < KT; ++j) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            float e = fast_exp2(fmaf(p.c, s[j][r], nl[r]));
-            float d = BwdTraits<Tag>::kScaled ? e * (dp[j][r] * sc) : e * dp[j][r];
-            if (edge && kw + 16 * j + c16 > q0 + 16 * i + 4 * g + r) e = d = 0.f;
-            s[j][r] = e;
-            dp[j][r] = d;
+            float x = fmaf(p.c, s[j][r], nl[r]);
+            if (EDGE && kw + 16 * j + c16 > q0 + 16 * i + 4 * g + r) x = FA_NEG_INF;
+            s[j][r] = fast_exp2(x);
+            dp[j][r] = BwdTraits<Tag>::kScaled ? s[j][r] * (dp[j][r] * sc) : s[j][r] * dp[j][r];
           }
           pb[j][2 * i] = N_::pack2(s[j][0], s[j][1]);
           pb[j][2 * i + 1] = N_::pack2(s[j][2], s[j][3]);
@@ -373,15 +381,24 @@ struct Bwd {
         const u32x4 ot = tfrag(os, to ^ (d << 5));
         const u32x4 qt = tfrag(qs, to ^ (d << 5));
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < KT; ++j) {
           dv[d][j] = N_::mfma16(ot, pb[j], dv[d][j]);
           dk[d][j] = N_::mfma16(qt, sb[j], dk[d][j]);
         }
       }
+    };
+    // head by head: first the tiles on the diagonal, then those that all the block's keys precede
+    while (it < total) {
+      const int left = total - it, edge_end = p.causal ? qt0 + BLOCK / T : 0;
+      for (int n = ct < edge_end ? (left < edge_end - ct ? left : edge_end - ct) : 0; n > 0 && ct < qt_all; --n)
+        step(std::true_type{});
+      for (int n = total - it < qt_all - ct ? total - it : qt_all - ct; n > 0; --n) step(std::false_type{});
+      ct = qt0;
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may reach LDS after the workgroup's end
     const float fk = p.scale * unscale * BwdTraits<Tag>::kPUnscale, fv = BwdTraits<Tag>::kPUnscale;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < KT; ++j) {
       const int key = kw + 16 * j + c16;
       if (key >= p.N) continue;
       if (p.kv_splits > 1) {
@@ -411,19 +428,19 @@ struct Bwd {
     const int bh = uniform(id / p.mblocks / p.q_splits);
     const int mb = uniform(p.causal ? p.mblocks - 1 - at : at);  // causal: the block with the most keys first
     const int b = uniform(bh / p.H), h = uniform(bh % p.H), hk = uniform(h / p.group);
-    const int m0 = mb * BLOCK, mw = m0 + 32 * wave;
+    const int m0 = mb * BLOCK, mw = m0 + OWN * wave;
     float sc = 1.f, unscale = 1.f;
     if constexpr (BwdTraits<Tag>::kScaled) {
       const int e = scale_exponent(p, b, hk, reinterpret_cast<float*>(smem));
       sc = pow2(-e);
       unscale = pow2(e);
     }
-    u32x4 qf[2][KS], of[2][KS];
+    u32x4 qf[KT][KS], of[KT][KS];
     load_frags(qf, p.q + b * p.sq[0] + h * p.sq[1], p.sq[2], mw, p.M, lane);
     load_frags(of, p.dout + b * p.sdo[0] + h * p.sdo[1], p.sdo[2], mw, p.M, lane);
-    float nl[2], nd[2];
+    float nl[KT], nd[KT];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < KT; ++i) {
       const int row = mw + 16 * i + c16;
       nl[i] = FA_NEG_INF;
       nd[i] = 0.f;
@@ -433,11 +450,11 @@ struct Bwd {
         nd[i] = src[32];
       }
     }
-    floatx4 acc[DT16][2];
+    floatx4 acc[DT16][KT];
 #pragma unroll
     for (int d = 0; d < DT16; ++d)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) acc[d][i] = (floatx4){0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < KT; ++i) acc[d][i] = (floatx4){0.f, 0.f, 0.f, 0.f};
     const uint32_t lds = lds_address(smem);
     const uint32_t ro = row_off(lane), to = tr_off(lane);
     const int n_end = p.causal && m0 + BLOCK < p.N ? m0 + BLOCK : p.N;
@@ -445,27 +462,28 @@ struct Bwd {
     const int first = part * share, tiles = first >= all ? first : (all - first < share ? all : first + share);
     const uint16_t* kb = p.k + b * p.sk[0] + hk * p.sk[1];
     const uint16_t* vb = p.v + b * p.sv[0] + hk * p.sv[1];
-    const Loader lk(p.sk[2], wave, lane), lv(p.sv[2], wave, lane);
     auto load = [&](int t) {
-      const uint32_t dst = lds + (uint32_t)((t & 1) * STAGEB);
-      lk.load(kb + t * (T * p.sk[2]), p.N - t * T, dst, wave);
-      lv.load(vb + t * (T * p.sv[2]), p.N - t * T, dst + TILEB, wave);
+      const uint32_t dst = lds + (uint32_t)((t % STAGES) * STAGEB);
+      const int left = t < tiles ? p.N - t * T : 0;
+      load_tile(kb + t * (T * p.sk[2]), p.sk[2], left, dst, wave, lane);
+      load_tile(vb + t * (T * p.sv[2]), p.sv[2], left, dst + TILEB, wave, lane);
     };
-    if (first < tiles) load(first);
-    for (int t = first; t < tiles; ++t) {
-      wait_vm_lds_barrier<0>();
-      if (t + 1 < tiles) load(t + 1);
-      const char* ks_ = smem + (t & 1) * STAGEB;
+    if (first < tiles)
+      for (int i = 0; i < STAGES - 1; ++i) load(first + i);
+    auto step = [&](int t, auto edge_tile) {
+      constexpr bool EDGE = decltype(edge_tile)::value;
+      wait_vm_lds_barrier<(STAGES - 2) * 2 * NB>();
+      load(t + STAGES - 1);
+      const char* ks_ = smem + (t % STAGES) * STAGEB;
       const char* vs_ = ks_ + TILEB;
       const int n0 = t * T;
-      if (p.causal && n0 > mw + 31) continue;
-      const bool edge = (p.causal && n0 + T - 1 > mw) || n0 + T > p.N;
-      u32x4 sb[2];
+      if (EDGE && p.causal && n0 > mw + OWN - 1) return;
+      u32x4 sb[KT];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        floatx4 s[2], dp[2];
+        floatx4 s[KT], dp[KT];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < KT; ++j) {
           s[j] = (floatx4){0.f, 0.f, 0.f, 0.f};
           dp[j] = (floatx4){nd[j], nd[j], nd[j], nd[j]};
         }
@@ -474,22 +492,22 @@ struct Bwd {
           const u32x4 a = frag(ks_ + i * 16 * ROWB, ro ^ (ks << 6));
           const u32x4 v = frag(vs_ + i * 16 * ROWB, ro ^ (ks << 6));
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
+          for (int j = 0; j < KT; ++j) {
             s[j] = N_::mfma16(a, qf[j][ks], s[j]);
             dp[j] = N_::mfma16(v, of[j][ks], dp[j]);
           }
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < KT; ++j) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float e = fast_exp2(fmaf(p.c, s[j][r], nl[j]));
-            float d = BwdTraits<Tag>::kScaled ? e * (dp[j][r] * sc) : e * dp[j][r];
-            if (edge) {
+            float x = fmaf(p.c, s[j][r], nl[j]);
+            if (EDGE) {
               const int key = n0 + 16 * i + 4 * g + r;
-              if (key >= p.N || (p.causal && key > mw + 16 * j + c16)) d = 0.f;
+              if (key >= p.N || (p.causal && key > mw + 16 * j + c16)) x = FA_NEG_INF;
             }
-            dp[j][r] = d;
+            const float e = fast_exp2(x);
+            dp[j][r] = BwdTraits<Tag>::kScaled ? e * (dp[j][r] * sc) : e * dp[j][r];
           }
           sb[j][2 * i] = N_::pack2(dp[j][0], dp[j][1]);
           sb[j][2 * i + 1] = N_::pack2(dp[j][2], dp[j][3]);
@@ -499,12 +517,18 @@ struct Bwd {
       for (int d = 0; d < DT16; ++d) {
         const u32x4 kt = tfrag(ks_, to ^ (d << 5));
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[d][j] = N_::mfma16(kt, sb[j], acc[d][j]);
+        for (int j = 0; j < KT; ++j) acc[d][j] = N_::mfma16(kt, sb[j], acc[d][j]);
       }
-    }
+    };
+    // whole tiles before the block's first row, then those on the diagonal or past the last key
+    const int whole = p.causal && m0 < p.N ? m0 / T : p.N / T;
+    int t = first;
+    for (; t < tiles && t < whole; ++t) step(t, std::false_type{});
+    for (; t < tiles; ++t) step(t, std::true_type{});
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     const float f = p.scale * unscale * BwdTraits<Tag>::kPUnscale;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < KT; ++j) {
       const int row = mw + 16 * j + c16;
       if (row >= p.M) continue;
       if (p.q_splits > 1) {
@@ -525,14 +549,14 @@ struct Bwd {
 
 // dK/dV blocks first (they are the longer ones), then dQ blocks, in one grid: small problems fill more of
 // the chip, large ones drain together.
-template <typename Tag, int D>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void fa_bwd_kernel(BwdParams p) {
-  __shared__ __align__(1024) char smem[Bwd<Tag, D>::SMEM];
+template <typename Tag, int D, int KT, int PER_CU>
+__global__ __launch_bounds__(256, PER_CU) void fa_bwd_kernel(BwdParams p) {
+  __shared__ __align__(1024) char smem[Bwd<Tag, D, KT>::SMEM];
   const int id = blockIdx.x;
   if (id < p.kv_total)
-    Bwd<Tag, D>::dkdv(p, smem, xcd_remap(id, p.kv_total));
+    Bwd<Tag, D, KT>::dkdv(p, smem, xcd_remap(id, p.kv_total));
   else
-    Bwd<Tag, D>::dq(p, smem, xcd_remap(id - p.kv_total, p.q_total));
+    Bwd<Tag, D, KT>::dq(p, smem, xcd_remap(id - p.kv_total, p.q_total));
 }
 
 // Sums of the splits' partial gradients, in split order: a thread takes four channels of one row.
@@ -570,14 +594,17 @@ __global__ __launch_bounds__(256) void fa_bwd_reduce_kernel(BwdParams p) {
   *reinterpret_cast<u32x2*>(out) = (u32x2){DT<Tag>::pack2(sum[0], sum[1]), DT<Tag>::pack2(sum[2], sum[3])};
 }
 
-#define FA_BWD_ENTRY(TAG, DTYPE, D) \
-  {DTYPE, D, (const void*)&fa_bwd_prep_kernel<TAG, D>, (const void*)&fa_bwd_kernel<TAG, D>, \
-   (const void*)&fa_bwd_reduce_kernel<TAG, D>, Bwd<TAG, D>::BLOCK, kPrepRows}
+#define FA_BWD_ENTRY(TAG, DTYPE, D, KT, PER_CU)                                                          \
+  {DTYPE, D, (const void*)&fa_bwd_prep_kernel<TAG, D>, (const void*)&fa_bwd_kernel<TAG, D, KT, PER_CU>, \
+   (const void*)&fa_bwd_reduce_kernel<TAG, D>, Bwd<TAG, D, KT>::BLOCK, kPrepRows, PER_CU}
 
 static const BwdKernelEntry kBwdEntries[] = {
-    FA_BWD_ENTRY(f16_t, FA_DTYPE_F16, 64),   FA_BWD_ENTRY(f16_t, FA_DTYPE_F16, 128),
-    FA_BWD_ENTRY(f16_t, FA_DTYPE_F16, 256),  FA_BWD_ENTRY(bf16_t, FA_DTYPE_BF16, 64),
-    FA_BWD_ENTRY(bf16_t, FA_DTYPE_BF16, 128), FA_BWD_ENTRY(bf16_t, FA_DTYPE_BF16, 256),
+    FA_BWD_ENTRY(f16_t, FA_DTYPE_F16, 64, 2, 2),
+    FA_BWD_ENTRY(f16_t, FA_DTYPE_F16, 128, 2, 2),
+    FA_BWD_ENTRY(f16_t, FA_DTYPE_F16, 256, 2, 1),
+    FA_BWD_ENTRY(bf16_t, FA_DTYPE_BF16, 64, 2, 2),
+    FA_BWD_ENTRY(bf16_t, FA_DTYPE_BF16, 128, 2, 2),
+    FA_BWD_ENTRY(bf16_t, FA_DTYPE_BF16, 256, 2, 1),
 };
 
 const BwdKernelEntry* fa_bwd_registry(int* count) {

@@ -113,6 +113,7 @@ struct BwdKernelEntry {
   const void* reduce;
   int32_t block;      // keys (dK/dV) and query rows (dQ) of a workgroup
   int32_t prep_rows;  // rows of a row-term block
+  int32_t per_cu;     // workgroups that a CU holds
 };
 
 const BwdKernelEntry* fa_bwd_registry(int* count);
