@@ -161,10 +161,12 @@ struct Bwd {
   static constexpr int ROWB = 2 * D;         // bytes of an LDS row
   static constexpr int CPR = D / 8;          // 16-byte chunks of a row
   static constexpr int TILEB = T * ROWB;
-  static constexpr int STAGEB = 2 * TILEB + 256;  // two tiles and a group of row terms
-  // A ring of four stages: a tile's loads are issued three steps before its use.
-  static constexpr int STAGES = 4;
-  static constexpr int SMEM = STAGES * STAGEB;
+  // A ring of stages of two tiles each, then the stages' groups of row terms. A tile's loads are issued STAGES - 1
+  // steps before its use; two stages measured 3% (D <= 128) and 7% (D = 256) faster than three or four.
+  static constexpr int STAGES = 2;
+  static constexpr int STAGEB = 2 * TILEB;
+  static constexpr int TERMS = STAGES * STAGEB;
+  static constexpr int SMEM = TERMS + STAGES * 256;
   static constexpr int NB = TILEB / 1024 / WAVES;  // LDS-DMA instructions of a wave per tile
 
   // LDS rows are unpadded (LDS-DMA writes 1 KiB blocks); chunk c of row r lies at c ^ swz(r). The LDS serves 256
@@ -174,36 +176,62 @@ struct Bwd {
   __device__ static inline int swz(int r) {
     return D == 64 ? (r & 6) : (r & 7) << 1;
   }
-  typedef DT<Tag> N_;
-
-  // A tile of 32 rows (`base`: its first row, `left`: rows from there to the matrix's end, past which zeros are
-  // read) into LDS. The lanes' offsets are worked out anew for every tile: held across the loop they
-  // are spilled (D = 128 has no register free), and a reload from scratch stalls the loads behind it.
-  __device__ static inline void load_tile(const uint16_t* base, int64_t stride, int left, uint32_t lds, int wave, int lane) {
-    constexpr int RPB = 1024 / ROWB;  // rows of a 1 KiB block
-    const uint32_t pitch = (uint32_t)stride * 2u;
-    const u32x4 rsrc = make_rsrc(base, left <= 0 ? 0u : (uint32_t)((left < T ? left : T) - 1) * pitch + (uint32_t)ROWB);
-    asm volatile("" : "+v"(lane));
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const uint32_t row = (wave + i * WAVES) * RPB + lane / CPR;
-      const uint32_t off = row * pitch + (((lane % CPR) ^ swz(row)) * 16u);
-      buffer_load16_to_lds<0, true>(rsrc, off, lds + (uint32_t)(wave + i * WAVES) * 1024u);
+  typedef DT<Tag> E;
+  __device__ static inline uint32_t pack2(float x, float y) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    if constexpr (BwdTraits<Tag>::kScaled) {
+      typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+      return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){x, y}, h2));
+    } else {
+      return E::pack2(x, y);
     }
+  }
+
+  // Tiles of 32 rows of one head, in order, into LDS; rows past the head's last read as zeros.
+  struct Stream {
+    const uint16_t* at;  // the next tile's first row
+    uint32_t pitch;      // bytes of a row
+    __device__ inline void init(const uint16_t* base, int64_t stride) {
+      at = base;
+      pitch = (uint32_t)stride * 2u;
+    }
+    __device__ inline void next() { at = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(at) + T * pitch); }
+    // `left`: rows from the tile's first to the head's end (none when <= 0).
+    __device__ inline void load(int left, uint32_t lds, int wave, uint32_t row, uint32_t chunk) const {
+      constexpr int RPB = 1024 / ROWB;  // rows of a 1 KiB block
+      const int rows = left < T ? left : T;
+      const u32x4 rsrc = make_rsrc(at, rows <= 0 ? 0u : (uint32_t)(rows - 1) * pitch + (uint32_t)ROWB);
+      const uint32_t off = (row & 31u) * (pitch & 0xffffffu);  // 24-bit product
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const uint32_t step = (uint32_t)(i * WAVES * RPB);
+        buffer_load16_to_lds(rsrc, off + step * pitch + ((chunk ^ swz(row + step)) * 16u),
+                             lds + (uint32_t)(wave + i * WAVES) * 1024u);
+      }
+    }
+  };
+  // The two tiles of a stage. A lane's place in the wave's first 1 KiB block is worked out anew for every stage: held
+  // across the loop it is spilled (D = 128 has no register free), and a reload from scratch stalls the loads behind it.
+  __device__ static inline void load_stage(const Stream& a, const Stream& b, int left, uint32_t lds, int wave, int lane) {
+    asm volatile("" : "+v"(lane));
+    const uint32_t row = (uint32_t)wave * (1024 / ROWB) + (uint32_t)lane / CPR, chunk = (uint32_t)lane % CPR;
+    a.load(left, lds, wave, row, chunk);
+    b.load(left, lds + TILEB, wave, row, chunk);
   }
 
   // The 32 rows' two terms (256 bytes). Every wave loads them, so that all have the same loads in flight.
   __device__ static inline void load_terms(const float* nd, bool live, uint32_t lds, int lane) {
     const u32x4 rsrc = make_rsrc(nd, live ? 256 : 0);
     const uint32_t dst = __builtin_amdgcn_readfirstlane(lds);
-    asm volatile("s_nop 4\n\ts_mov_b32 m0, %1\n\tbuffer_load_dword %0, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %1\n\tbuffer_load_dword %0, %2, 0 offen lds"
                  :
                  : "v"((uint32_t)lane * 4u), "s"(dst), "s"(rsrc)
                  : "memory", "m0");
   }
 
   // Byte offset in a tile of a lane's row fragment (row lane & 15, channels 8 (lane >> 4) ..): step ks is at
-  // off ^ (ks << 6), row tile i at + i * 16 * ROWB.
+  // off ^ (ks << 6), row tile i at + i * 16 * ROWB. Stages are whole multiples of a row, so the exclusive or may
+  // come after the stage's offset is added: one address per stage is held, not one per step.
   __device__ static inline uint32_t row_off(int lane) {
     const int r = lane & 15, g = lane >> 4;
     return (uint32_t)(r * ROWB + ((g ^ swz(r)) << 4));
@@ -214,12 +242,12 @@ struct Bwd {
     const int L = lane & 15, r = 4 * (lane >> 4) + (L >> 2);
     return (uint32_t)(r * ROWB + ((((L & 3) >> 1) ^ swz(r)) << 4) + ((L & 1) << 3));
   }
-  __device__ static inline u32x4 frag(const char* tile, uint32_t off) {
-    return *reinterpret_cast<const u32x4*>(tile + off);
+  __device__ static inline u32x4 frag(const char* smem, uint32_t off, int tile) {
+    return *reinterpret_cast<const u32x4*>(smem + off + tile);
   }
-  __device__ static inline u32x4 tfrag(const char* tile, uint32_t off) {
-    const u32x2 a = lds_read_tr16(reinterpret_cast<const uint16_t*>(tile + off));
-    const u32x2 b = lds_read_tr16(reinterpret_cast<const uint16_t*>(tile + off + 16 * ROWB));
+  __device__ static inline u32x4 tfrag(const char* smem, uint32_t off, int tile) {
+    const u32x2 a = lds_read_tr16(reinterpret_cast<const uint16_t*>(smem + off + tile));
+    const u32x2 b = lds_read_tr16(reinterpret_cast<const uint16_t*>(smem + off + tile + 16 * ROWB));
     return (u32x4){a[0], a[1], b[0], b[1]};
   }
 
@@ -308,22 +336,30 @@ struct Bwd {
     const int h0 = total > 0 ? uniform(first / per_head) : 0, ht0 = qt0 + first - h0 * per_head;
 
     const int hq = hk * p.group + h0;
-    const uint16_t* qh = p.q + b * p.sq[0] + hq * p.sq[1];  // the next load's head
-    const uint16_t* oh = p.dout + b * p.sdo[0] + hq * p.sdo[1];
-    const float* nh = p.nd + ((int64_t)b * p.H + hq) * p.row_groups * 64;
-    int lt = ht0;  // and its tile
+    Stream sq, so;  // at the next load's tile
+    sq.init(p.q + b * p.sq[0] + hq * p.sq[1] + ht0 * (T * p.sq[2]), p.sq[2]);
+    so.init(p.dout + b * p.sdo[0] + hq * p.sdo[1] + ht0 * (T * p.sdo[2]), p.sdo[2]);
+    const float* nh = p.nd + (((int64_t)b * p.H + hq) * p.row_groups + ht0) * 64;
+    // from a head's end to the next head's first tile
+    const int64_t skip_q = p.sq[1] - (int64_t)(per_head * T) * p.sq[2], skip_o = p.sdo[1] - (int64_t)(per_head * T) * p.sdo[2];
+    const int skip_n = (p.row_groups - per_head) * 64;
+    int left = p.M - ht0 * T, ahead = total;  // rows of the head, tiles of the split that are still to be loaded
     // Behind the last step the loads go on with nothing in range: the waits count on a fixed number in flight.
-    auto load_next = [&](int step) {
+    auto load_next = [&](uint32_t step) {
       const uint32_t dst = lds + (uint32_t)((step % STAGES) * STAGEB);
-      const int left = step < total ? p.M - lt * T : 0;
-      load_tile(qh + lt * (T * p.sq[2]), p.sq[2], left, dst, wave, lane);
-      load_tile(oh + lt * (T * p.sdo[2]), p.sdo[2], left, dst + TILEB, wave, lane);
-      load_terms(nh + (int64_t)lt * 64, left > 0, dst + 2 * TILEB, lane);
-      if (step < total && ++lt == qt_all) {
-        lt = qt0;
-        qh += p.sq[1];
-        oh += p.sdo[1];
-        nh += (int64_t)p.row_groups * 64;
+      const int rows = ahead > 0 ? left : 0;
+      load_stage(sq, so, rows, dst, wave, lane);
+      load_terms(nh, rows > 0, lds + (uint32_t)(TERMS + (step % STAGES) * 256), lane);
+      --ahead;
+      left -= T;
+      sq.next();
+      so.next();
+      nh += 64;
+      if (left <= 0) {
+        left = p.M - qt0 * T;
+        sq.at += skip_q;
+        so.at += skip_o;
+        nh += skip_n;
       }
     };
     if (total > 0)
@@ -333,9 +369,8 @@ struct Bwd {
       constexpr bool EDGE = decltype(edge_tile)::value;
       wait_vm_lds_barrier<(STAGES - 2) * (2 * NB + 1)>();
       load_next(it + STAGES - 1);
-      const char* qs = smem + (it % STAGES) * STAGEB;
-      const char* os = qs + TILEB;
-      const float* nd = reinterpret_cast<const float*>(qs + 2 * TILEB);
+      const uint32_t rows = ro + ((uint32_t)it % STAGES) * STAGEB, cols = to + ((uint32_t)it % STAGES) * STAGEB;
+      const float* nd = reinterpret_cast<const float*>(smem + TERMS + ((uint32_t)it % STAGES) * 256);
       const int q0 = ct * T;
       ++it;
       ++ct;
@@ -353,12 +388,12 @@ struct Bwd {
         }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          const u32x4 a = frag(qs + i * 16 * ROWB, ro ^ (ks << 6));
-          const u32x4 o = frag(os + i * 16 * ROWB, ro ^ (ks << 6));
+          const u32x4 a = frag(smem, rows ^ (ks << 6), i * 16 * ROWB);
+          const u32x4 o = frag(smem, rows ^ (ks << 6), i * 16 * ROWB + TILEB);
 #pragma unroll
           for (int j = 0; j < KT; ++j) {
-            s[j] = N_::mfma16(a, kf[j][ks], s[j]);
-            dp[j] = N_::mfma16(o, vf[j][ks], dp[j]);
+            s[j] = E::mfma16(a, kf[j][ks], s[j]);
+            dp[j] = E::mfma16(o, vf[j][ks], dp[j]);
           }
         }
 #pragma unroll
@@ -370,22 +405,25 @@ struct Bwd {
             s[j][r] = fast_exp2(x);
             dp[j][r] = BwdTraits<Tag>::kScaled ? s[j][r] * (dp[j][r] * sc) : s[j][r] * dp[j][r];
           }
-          pb[j][2 * i] = N_::pack2(s[j][0], s[j][1]);
-          pb[j][2 * i + 1] = N_::pack2(s[j][2], s[j][3]);
-          sb[j][2 * i] = N_::pack2(dp[j][0], dp[j][1]);
-          sb[j][2 * i + 1] = N_::pack2(dp[j][2], dp[j][3]);
+          pb[j][2 * i] = pack2(s[j][0], s[j][1]);
+          pb[j][2 * i + 1] = pack2(s[j][2], s[j][3]);
+          sb[j][2 * i] = pack2(dp[j][0], dp[j][1]);
+          sb[j][2 * i + 1] = pack2(dp[j][2], dp[j][3]);
         }
       }
+      // a wave in its second products goes before one in its softmax (the two share a SIMD): 6% at D = 256
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int d = 0; d < DT16; ++d) {
-        const u32x4 ot = tfrag(os, to ^ (d << 5));
-        const u32x4 qt = tfrag(qs, to ^ (d << 5));
+        const u32x4 ot = tfrag(smem, cols ^ (d << 5), TILEB);
+        const u32x4 qt = tfrag(smem, cols ^ (d << 5), 0);
 #pragma unroll
         for (int j = 0; j < KT; ++j) {
-          dv[d][j] = N_::mfma16(ot, pb[j], dv[d][j]);
-          dk[d][j] = N_::mfma16(qt, sb[j], dk[d][j]);
+          dv[d][j] = E::mfma16(ot, pb[j], dv[d][j]);
+          dk[d][j] = E::mfma16(qt, sb[j], dk[d][j]);
         }
       }
+      __builtin_amdgcn_s_setprio(0);
     };
     // head by head: first the tiles on the diagonal, then those that all the block's keys precede
     while (it < total) {
@@ -415,8 +453,8 @@ struct Bwd {
 #pragma unroll
       for (int d = 0; d < DT16; ++d) {
         const floatx4 a = dk[d][j] * fk, v = dv[d][j] * fv;
-        *reinterpret_cast<u32x2*>(ok + 16 * d) = (u32x2){N_::pack2(a[0], a[1]), N_::pack2(a[2], a[3])};
-        *reinterpret_cast<u32x2*>(ov + 16 * d) = (u32x2){N_::pack2(v[0], v[1]), N_::pack2(v[2], v[3])};
+        *reinterpret_cast<u32x2*>(ok + 16 * d) = (u32x2){pack2(a[0], a[1]), pack2(a[2], a[3])};
+        *reinterpret_cast<u32x2*>(ov + 16 * d) = (u32x2){pack2(v[0], v[1]), pack2(v[2], v[3])};
       }
     }
   }
@@ -460,13 +498,17 @@ struct Bwd {
     const int n_end = p.causal && m0 + BLOCK < p.N ? m0 + BLOCK : p.N;
     const int all = (n_end + T - 1) / T, share = (all + p.q_splits - 1) / p.q_splits;
     const int first = part * share, tiles = first >= all ? first : (all - first < share ? all : first + share);
-    const uint16_t* kb = p.k + b * p.sk[0] + hk * p.sk[1];
-    const uint16_t* vb = p.v + b * p.sv[0] + hk * p.sv[1];
-    auto load = [&](int t) {
+    Stream sk, sv;
+    sk.init(p.k + b * p.sk[0] + hk * p.sk[1] + first * (T * p.sk[2]), p.sk[2]);
+    sv.init(p.v + b * p.sv[0] + hk * p.sv[1] + first * (T * p.sv[2]), p.sv[2]);
+    // rows that are still to be loaded: past the split's last tile none are
+    int left = (tiles * T < p.N ? tiles * T : p.N) - first * T;
+    auto load = [&](uint32_t t) {
       const uint32_t dst = lds + (uint32_t)((t % STAGES) * STAGEB);
-      const int left = t < tiles ? p.N - t * T : 0;
-      load_tile(kb + t * (T * p.sk[2]), p.sk[2], left, dst, wave, lane);
-      load_tile(vb + t * (T * p.sv[2]), p.sv[2], left, dst + TILEB, wave, lane);
+      load_stage(sk, sv, left, dst, wave, lane);
+      left -= T;
+      sk.next();
+      sv.next();
     };
     if (first < tiles)
       for (int i = 0; i < STAGES - 1; ++i) load(first + i);
@@ -474,8 +516,7 @@ struct Bwd {
       constexpr bool EDGE = decltype(edge_tile)::value;
       wait_vm_lds_barrier<(STAGES - 2) * 2 * NB>();
       load(t + STAGES - 1);
-      const char* ks_ = smem + (t % STAGES) * STAGEB;
-      const char* vs_ = ks_ + TILEB;
+      const uint32_t rows = ro + ((uint32_t)t % STAGES) * STAGEB, cols = to + ((uint32_t)t % STAGES) * STAGEB;
       const int n0 = t * T;
       if (EDGE && p.causal && n0 > mw + OWN - 1) return;
       u32x4 sb[KT];
@@ -489,12 +530,12 @@ struct Bwd {
         }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          const u32x4 a = frag(ks_ + i * 16 * ROWB, ro ^ (ks << 6));
-          const u32x4 v = frag(vs_ + i * 16 * ROWB, ro ^ (ks << 6));
+          const u32x4 a = frag(smem, rows ^ (ks << 6), i * 16 * ROWB);
+          const u32x4 v = frag(smem, rows ^ (ks << 6), i * 16 * ROWB + TILEB);
 #pragma unroll
           for (int j = 0; j < KT; ++j) {
-            s[j] = N_::mfma16(a, qf[j][ks], s[j]);
-            dp[j] = N_::mfma16(v, of[j][ks], dp[j]);
+            s[j] = E::mfma16(a, qf[j][ks], s[j]);
+            dp[j] = E::mfma16(v, of[j][ks], dp[j]);
           }
         }
 #pragma unroll
@@ -509,16 +550,18 @@ struct Bwd {
             const float e = fast_exp2(x);
             dp[j][r] = BwdTraits<Tag>::kScaled ? e * (dp[j][r] * sc) : e * dp[j][r];
           }
-          sb[j][2 * i] = N_::pack2(dp[j][0], dp[j][1]);
-          sb[j][2 * i + 1] = N_::pack2(dp[j][2], dp[j][3]);
+          sb[j][2 * i] = pack2(dp[j][0], dp[j][1]);
+          sb[j][2 * i + 1] = pack2(dp[j][2], dp[j][3]);
         }
       }
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int d = 0; d < DT16; ++d) {
-        const u32x4 kt = tfrag(ks_, to ^ (d << 5));
+        const u32x4 kt = tfrag(smem, cols ^ (d << 5), 0);
 #pragma unroll
-        for (int j = 0; j < KT; ++j) acc[d][j] = N_::mfma16(kt, sb[j], acc[d][j]);
+        for (int j = 0; j < KT; ++j) acc[d][j] = E::mfma16(kt, sb[j], acc[d][j]);
       }
+      __builtin_amdgcn_s_setprio(0);
     };
     // whole tiles before the block's first row, then those on the diagonal or past the last key
     const int whole = p.causal && m0 < p.N ? m0 / T : p.N / T;
@@ -541,7 +584,7 @@ struct Bwd {
 #pragma unroll
       for (int d = 0; d < DT16; ++d) {
         const floatx4 a = acc[d][j] * f;
-        *reinterpret_cast<u32x2*>(out + 16 * d) = (u32x2){N_::pack2(a[0], a[1]), N_::pack2(a[2], a[3])};
+        *reinterpret_cast<u32x2*>(out + 16 * d) = (u32x2){pack2(a[0], a[1]), pack2(a[2], a[3])};
       }
     }
   }
