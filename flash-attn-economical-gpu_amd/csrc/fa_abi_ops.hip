@@ -125,6 +125,20 @@ int check_cache(const kv4_cache* c) {
   return FA_OK;
 }
 
+// Which attention kernel takes a kv head's query rows: up to 32 the waves of a workgroup share them (and the
+// cache is read once); more go 64 or 128 to a workgroup.
+struct Kv4Kind {
+  int kind;
+  int64_t row_blocks;
+};
+Kv4Kind kv4_kind(const fa::Kv4KernelEntry* e, int64_t rows) {
+  Kv4Kind k;
+  k.kind = rows <= 16 ? 0 : (rows <= 32 ? 1 : 2);
+  const int64_t block = k.kind == 2 ? 64 * e->chunk_tiles : 16 << k.kind;
+  k.row_blocks = (rows + block - 1) / block;
+  return k;
+}
+
 }  // namespace
 
 extern "C" {
@@ -274,6 +288,17 @@ int64_t kv4_attend_workspace_bytes(int32_t B, int32_t H, int32_t M, int32_t D, i
   return align256(rows * D * 4) + rows * 8;
 }
 
+int32_t kv4_attend_splits(int32_t B, int32_t H, int32_t H_kv, int32_t M, int32_t D, int32_t capacity) {
+  const fa::Kv4KernelEntry* e = find_kv4(FA_DTYPE_F16, D);  // alike for both types
+  if (e == nullptr || B <= 0 || H_kv <= 0 || H < H_kv || M <= 0 || capacity <= 0) return 1;
+  const Kv4Kind k = kv4_kind(e, (int64_t)M * (H / H_kv));
+  const int64_t blocks = (int64_t)B * H_kv * k.row_blocks, room = 256LL * e->per_cu[k.kind];
+  // as many as the chip (256 CUs) holds at once, none with less than 256 keys of a full cache
+  int64_t splits = room / blocks;
+  if (splits > capacity / 256) splits = capacity / 256;
+  return splits < 1 ? 1 : (int32_t)(splits > 4096 ? 4096 : splits);
+}
+
 int kv4_attend(const kv4_attend_args* a, void* stream) {
   if (a == nullptr) return fail(FA_EINVAL, "null argument block");
   const kv4_cache* c = &a->cache;
@@ -324,17 +349,18 @@ int kv4_attend(const kv4_attend_args* a, void* stream) {
   p.causal = a->causal ? 1 : 0;
   p.splits = a->splits;
   p.c = a->sm_scale * 1.4426950408889634f;
-  // up to 32 rows the waves of a workgroup share them (and the cache is read once); more rows go 64 or 128
-  // to a workgroup
-  const int kind = rows <= 16 ? 0 : (rows <= 32 ? 1 : 2);
-  const int64_t block_rows = kind == 2 ? 64 * e->chunk_tiles : 16 << kind;
-  p.row_blocks = (int32_t)((rows + block_rows - 1) / block_rows);
-  p.min_tiles = 8;
-  const int64_t blocks = (int64_t)p.row_blocks * a->splits * c->H_kv * c->B;
-  if ((code = launch(e->attend[kind], blocks, 1, 256, &p, stream, "cache attention")) != FA_OK) return code;
+  const Kv4Kind k = kv4_kind(e, rows);
+  p.row_blocks = (int32_t)k.row_blocks;
+  const int64_t slots = (int64_t)c->B * a->splits;
+  const int64_t blocks = k.row_blocks * slots * c->H_kv;
+  if (slots > 0x7fffffffLL) return fail(FA_EINVAL, "too many splits (%lld)", (long long)slots);
+  p.slots = (int32_t)slots;
+  if ((code = launch(e->attend[k.kind], blocks, 1, 256, &p, stream, "cache attention")) != FA_OK) return code;
   if (a->splits > 1) {
-    const int64_t merge = ((int64_t)c->B * a->H * a->M + 3) / 4;
-    if ((code = launch(e->merge, merge, 1, 256, &p, stream, "cache merge")) != FA_OK) return code;
+    const int64_t all = (int64_t)c->B * a->H * a->M;
+    const bool wide = a->splits > 8;
+    if ((code = launch(e->merge[wide ? 0 : 1], wide ? all : (all + 3) / 4, 1, 256, &p, stream, "cache merge")) != FA_OK)
+      return code;
   }
   return ok();
 }

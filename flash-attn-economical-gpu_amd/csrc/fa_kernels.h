@@ -145,12 +145,14 @@ struct Kv4AttendParams {
   const uint8_t* v_scales;
   const int32_t* start;
   const int32_t* count;  // nullable: all rows
-  float* ws_o;           // splits > 1: unnormalised partial sums [splits][B * H * M][D]
-  float* ws_ml;          // splits > 1: their row maximum (log2 units) and sum [splits][B * H * M][2]
+  float* ws_o;           // splits > 1: unnormalised partial sums [slots][H][M][D]
+  float* ws_ml;          // splits > 1: their row maximum (log2 units) and sum [slots][H][M][2]
   int64_t sq[3], so[3], sl[3];
   int64_t code_stride[2], scale_stride[2];
   int32_t B, H, Hkv, M, group, capacity;
-  int32_t causal, splits, min_tiles, row_blocks;
+  int32_t causal, splits;
+  int32_t slots;  // splits that all sequences may have together: B * splits
+  int32_t row_blocks;
   float c;  // scale * log2(e)
 };
 
@@ -158,8 +160,9 @@ struct Kv4KernelEntry {
   int32_t dtype;
   int32_t D;
   const void* append;
-  const void* merge;
+  const void* merge[2];   // a workgroup per row, a wave per row
   const void* attend[3];  // 16 rows shared by a workgroup's waves, 32 rows shared, own rows per wave
+  int32_t per_cu[3];      // workgroups of each that a CU holds
   int32_t chunk_tiles;    // 16-row tiles per wave of the last
 };
 

@@ -129,12 +129,78 @@ __device__ inline int visible_keys(const int32_t* start, const int32_t* count, i
   return end <= 0 ? 0 : (end > capacity ? capacity : (int)end);
 }
 
-// 32-key tiles of a split, the same for all splits of a sequence: at least kMinTiles, so short sequences in a
-// large cache use few splits.
-__device__ inline int tiles_per_split(int keys, int splits, int min_tiles) {
-  const int tiles = (keys + 31) / 32;
-  const int even = (tiles + splits - 1) / splits;
-  return even > min_tiles ? even : min_tiles;
+// How the sequences' 32-key tiles are cut into splits: `per` tiles each, the fewest (but kMinTiles) that make at
+// most B * splits splits of all sequences together, so that sequences of unequal lengths keep the workgroups
+// equally long, and no more of them than the chip was said to hold: 800 where 768 fit took twice the time of
+// 752. A split has a slot: sequence b's are those from its predecessors' number on. Each wave works this out
+// from the lengths (64 sequences at a time, one to a lane).
+constexpr int kMinTiles = 8;
+
+struct Split {
+  int b, index;     // sequence, and which of its splits (b < 0: a slot that no split has)
+  int first, used;  // the sequence's first slot and number of splits
+  int per;          // tiles of a split
+};
+
+// The split of a slot (slot >= 0), or of sequence b (slot < 0: only first, used and per are set).
+__device__ inline Split find_split(const Kv4AttendParams& p, int slot, int b) {
+  Split s;
+  if (p.splits == 1) {
+    s.b = slot;
+    s.index = 0;
+    s.first = slot;
+    s.used = 1;
+    s.per = 0x7fffff;
+    return s;
+  }
+  const int lane = threadIdx.x & 63;
+  int64_t all = 0;
+  int tiles = 0;
+  for (int c = 0; c < p.B; c += 64) {
+    tiles = c + lane < p.B ? (visible_keys(p.start, p.count, c + lane, p.M, p.capacity) + 31) / 32 : 0;
+    uint32_t sum = (uint32_t)tiles;  // of 64 sequences of under 2^26 tiles each
+    for (int k = 1; k < 64 && k < p.B; k *= 2) sum += (uint32_t)__shfl_xor((int)sum, k, 64);
+    all += (uint32_t)__builtin_amdgcn_readfirstlane((int)sum);
+  }
+  const int64_t most = (int64_t)p.B * p.splits;
+  int64_t per = (all + most - 1) / most;
+  if (per < kMinTiles) per = kMinTiles;
+  const int64_t safe = (all + most - p.B - 1) / (most - p.B);  // sum of ceil(t / per) < all / per + B
+  if (p.B > 64) {
+    per = per > safe ? per : safe;
+  } else {
+    while (per < safe) {  // a sixteenth longer at a time
+      int n = (tiles + (int)per - 1) / (int)per;
+      for (int k = 1; k < p.B; k *= 2) n += __shfl_xor(n, k, 64);
+      if (__builtin_amdgcn_readfirstlane(n) <= most) break;
+      per += (per + 15) / 16;
+    }
+  }
+  s.per = (int)per;
+  s.b = -1;
+  s.index = s.first = s.used = 0;
+  int base = 0;
+  for (int c = 0; c < p.B; c += 64) {
+    if (p.B > 64) tiles = c + lane < p.B ? (visible_keys(p.start, p.count, c + lane, p.M, p.capacity) + 31) / 32 : 0;
+    const int n = (tiles + s.per - 1) / s.per;
+    int end = n;  // of the lane's splits
+    for (int k = 1; k < 64 && k < p.B; k *= 2) {
+      const int o = __shfl_up(end, k, 64);
+      if (lane >= k) end += o;
+    }
+    end += base;
+    const uint64_t hit = __ballot(slot >= 0 ? slot < end : c + lane == b);
+    if (hit != 0) {
+      const int who = __builtin_ctzll(hit);
+      s.b = c + who;
+      s.used = __builtin_amdgcn_readlane(n, who);
+      s.first = __builtin_amdgcn_readlane(end, who) - s.used;
+      s.index = slot - s.first;
+      return s;
+    }
+    base = __builtin_amdgcn_readlane(end, 63);  // another 64 sequences follow, so all steps were made
+  }
+  return s;
 }
 
 // Attention over the cache. A wave holds 16 R query rows (columns of every product) and walks 32-key tiles:
@@ -153,13 +219,14 @@ struct Kv4Attend {
   static constexpr int SB = D / 32;   // scale bytes of a row
   static constexpr int CB = D / 2;    // code bytes of a row
   static constexpr int KW = D / 32;   // dwords of K codes per lane and key
+  static constexpr int VS = D == 64 ? 4 : 8;  // dwords of V scales per lane and tile
   typedef DT<Tag> E;
 
   struct Tile {  // one lane's share of a 32-key tile, as stored
     uint32_t k[2][KW];
     uint32_t ks[2];
     uint32_t v[8][CPL >= 8 ? CPL / 8 : 1];
-    uint32_t vs[8];
+    uint32_t vs[VS];
   };
 
   // Keys of a lane's k-slots in the second product: slot i is key 4 g + (i & 3) + 16 (i >> 2).
@@ -187,8 +254,30 @@ struct Kv4Attend {
 #pragma unroll
         for (int w = 0; w < CPL / 8; ++w) t.v[i][w] = reinterpret_cast<const uint32_t*>(src)[w];
       }
-      t.vs[i] = vsc[key * SB + r * CPL / 32];
+      if constexpr (D == 256) t.vs[i] = vsc[key * SB + r * CPL / 32];
     }
+    if constexpr (D != 256) {  // all scales of four neighbouring keys in one load; scale() takes the lane's block
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint8_t* src = vsc + (int64_t)(key0 + 4 * g + 16 * i) * SB;
+        if constexpr (D == 64) {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(src);
+          t.vs[2 * i] = x[0];
+          t.vs[2 * i + 1] = x[1];
+        } else {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(src);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) t.vs[4 * i + j] = x[j];
+        }
+      }
+    }
+  }
+  // V's scale of the lane's i-th key
+  __device__ static inline float v_scale(const Tile& t, int i, int lane) {
+    const uint32_t blk = (uint32_t)(lane & 15) * CPL / 32;
+    if constexpr (D == 256) return scale_of(t.vs[i]);
+    if constexpr (D == 128) return scale_of((t.vs[i] >> (8 * blk)) & 255u);
+    return scale_of((t.vs[i / 2] >> (8 * blk + 16 * (i & 1))) & 255u);
   }
 
   struct State {
@@ -247,21 +336,24 @@ struct Kv4Attend {
       pb[rt] = (u32x4){E::pack2(x[0][rt][0], x[0][rt][1]), E::pack2(x[0][rt][2], x[0][rt][3]),
                        E::pack2(x[1][rt][0], x[1][rt][1]), E::pack2(x[1][rt][2], x[1][rt][3])};
     }
-    if constexpr (EDGE) {  // rows behind the last key may hold anything, NaN too: they read as zeros
+    float vs[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 8; ++i) {
+      vs[i] = v_scale(t, i, lane);
+      if constexpr (EDGE) {  // rows behind the last key may hold anything, NaN too: they read as zeros
         if (key0 + 4 * g + (i & 3) + 16 * (i >> 2) >= keys) {
-          t.vs[i] = 127;
+          vs[i] = 1.f;
 #pragma unroll
           for (int w = 0; w < (CPL >= 8 ? CPL / 8 : 1); ++w) t.v[i][w] = 0;
         }
+      }
     }
     // channels 2 j and 2 j + 1 of the lane's CPL: byte j of a key's codes
     auto pair = [&](auto jc) {
       constexpr int j = decltype(jc)::value;
       uint32_t w[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = Fp4<Tag>::template decode<j % 4>(t.v[i][j / 4], scale_of(t.vs[i]));
+      for (int i = 0; i < 8; ++i) w[i] = Fp4<Tag>::template decode<j % 4>(t.v[i][j / 4], vs[i]);
       u32x4 even, odd;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -285,27 +377,27 @@ struct Kv4Attend {
     }
   }
 
-  // A lane's 4 CPL = D / 4 channels of row rt: channels (D / 4) g .. in order.
-  __device__ static inline void store_row(const Kv4AttendParams& p, int b, int hk, int split, int r, const float* o,
-                                          float m, float l, int g) {
+  // N channels N at .. of row r, whose maximum and sum are m and l.
+  template <int N>
+  __device__ static inline void store_row(const Kv4AttendParams& p, int b, int hk, int slot, int r, const float (&o)[N],
+                                          float m, float l, int at) {
     const int i = r / p.group, h = hk * p.group + r % p.group;
     if (p.splits > 1) {
-      const int64_t row = ((int64_t)b * p.H + h) * p.M + i;
-      const int64_t w = (int64_t)split * p.B * p.H * p.M + row;
-      float* dst = p.ws_o + w * D + g * (D / 4);
+      const int64_t w = ((int64_t)slot * p.H + h) * p.M + i;
+      float* dst = p.ws_o + w * D + at * N;
 #pragma unroll
-      for (int j = 0; j < D / 4; j += 4) *reinterpret_cast<floatx4*>(dst + j) = (floatx4){o[j], o[j + 1], o[j + 2], o[j + 3]};
-      if (g == 0) {
+      for (int j = 0; j < N; j += 4) *reinterpret_cast<floatx4*>(dst + j) = (floatx4){o[j], o[j + 1], o[j + 2], o[j + 3]};
+      if (at == 0) {
         p.ws_ml[2 * w] = m * p.c;
         p.ws_ml[2 * w + 1] = l;
       }
     } else {
       const float inv = l > 0.f ? 1.f / l : 0.f;
-      uint16_t* dst = p.o + b * p.so[0] + h * p.so[1] + i * p.so[2] + g * (D / 4);
+      uint16_t* dst = p.o + b * p.so[0] + h * p.so[1] + i * p.so[2] + at * N;
 #pragma unroll
-      for (int j = 0; j < D / 4; j += 4)
+      for (int j = 0; j < N; j += 4)
         *reinterpret_cast<u32x2*>(dst + j) = (u32x2){E::pack2(o[j] * inv, o[j + 1] * inv), E::pack2(o[j + 2] * inv, o[j + 3] * inv)};
-      if (g == 0 && p.lse != nullptr)
+      if (at == 0 && p.lse != nullptr)
         p.lse[b * p.sl[0] + h * p.sl[1] + i * p.sl[2]] =
             l > 0.f ? (m * p.c + __builtin_amdgcn_logf(l) - Fp4<Tag>::kPBias) * 0.6931471805599453f : FA_NEG_INF;
     }
@@ -315,17 +407,16 @@ struct Kv4Attend {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g = lane >> 4;
     int id = xcd_remap(blockIdx.x, gridDim.x);
-    // splits innermost: a sequence's neighbours run together; row blocks of one split share its tiles in L2
+    // row blocks innermost: those of one split share its tiles in L2
     const int rb = id % p.row_blocks;
     id /= p.row_blocks;
-    const int split = id % p.splits;
-    id /= p.splits;
-    const int hk = id % p.Hkv, b = id / p.Hkv;
+    const int slot = id % p.slots, hk = id / p.slots;
+    const Split part = find_split(p, slot, 0);
+    const int b = __builtin_amdgcn_readfirstlane(part.b);
+    if (b < 0) return;
     const int rows = p.M * p.group;
     const int row0 = (SHARED ? rb : rb * WAVES + wave) * 16 * R;
     const int keys = visible_keys(p.start, p.count, b, p.M, p.capacity);
-    const int per = tiles_per_split(keys, p.splits, p.min_tiles);
-    if (split > 0 && split * per >= (keys + 31) / 32) return;  // behind the last key: the merge does not read it
     const int count = p.count != nullptr ? p.count[b] : p.M;
     const int64_t start = p.start[b];
 
@@ -364,58 +455,65 @@ struct Kv4Attend {
       least = wave_top / p.group < count && row0 + 16 * R <= rows ? (int)low : 0;
     }
     const int tiles = (wave_see + 31) / 32;
-    int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+    const int per = __builtin_amdgcn_readfirstlane(part.per);
+    int t0 = __builtin_amdgcn_readfirstlane(part.index) * per, t1 = t0 + per < tiles ? t0 + per : tiles;
     const uint8_t* kc = p.k_codes + b * p.code_stride[0] + hk * p.code_stride[1];
     const uint8_t* vc = p.v_codes + b * p.code_stride[0] + hk * p.code_stride[1];
     const uint8_t* ks = p.k_scales + b * p.scale_stride[0] + hk * p.scale_stride[1];
     const uint8_t* vs = p.v_scales + b * p.scale_stride[0] + hk * p.scale_stride[1];
     const int stride = SHARED ? WAVES : 1;
     if (SHARED) t0 += wave;
-    Tile now, next;
-    if (t0 < t1) load(now, kc, ks, vc, vs, t0 * 32, lane);
-    for (int t = t0; t < t1; t += stride) {
-      if (t + stride < t1) load(next, kc, ks, vc, vs, (t + stride) * 32, lane);
-      if (t * 32 + 32 <= least) step<false>(s, qf, now, t * 32, see, keys, p.c, lane);
-      else step<true>(s, qf, now, t * 32, see, keys, p.c, lane);
-      now = next;
+    // two tiles in flight
+    Tile even, odd;
+    auto fetch = [&](Tile& x, int t) {
+      if (t < t1) load(x, kc, ks, vc, vs, t * 32, lane);
+    };
+    auto use = [&](Tile& x, int t) {
+      if (t * 32 + 32 <= least) step<false>(s, qf, x, t * 32, see, keys, p.c, lane);
+      else step<true>(s, qf, x, t * 32, see, keys, p.c, lane);
+      fetch(x, t + 2 * stride);
+    };
+    fetch(even, t0);
+    fetch(odd, t0 + stride);
+    for (int t = t0; t < t1; t += 2 * stride) {
+      use(even, t);
+      if (t + stride < t1) use(odd, t + stride);
     }
     if constexpr (SHARED) {
-      // the waves' sums meet in LDS; wave w finishes rows 4 w .. 4 w + 3 of each 16
+      // the waves' sums meet in LDS; wave w finishes rows 4 w .. 4 w + 3 of each 16, 16 lanes to a row
       constexpr int ROW = D + 4;
 #pragma unroll
       for (int rt = 0; rt < R; ++rt) {
-        float l = s.l[rt];
-        l = xquad_sum(l);
+        const float l = xquad_sum(s.l[rt]);
         float* dst = smem + (wave * 16 + c16) * ROW;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-          for (int d = 0; d < CPL; ++d) dst[(4 * g + r) * CPL + d] = s.o[d][rt][r];
+          for (int d = 0; d < CPL; d += 4)
+            *reinterpret_cast<floatx4*>(dst + (4 * g + r) * CPL + d) =
+                (floatx4){s.o[d][rt][r], s.o[d + 1][rt][r], s.o[d + 2][rt][r], s.o[d + 3][rt][r]};
         if (g == 0) {
           dst[D] = s.m[rt];
           dst[D + 1] = l;
         }
         __syncthreads();
-        const int row = 4 * wave + (c16 & 3);
-        if (c16 < 4) {
-          float m = FA_NEG_INF;
+        const int row = 4 * wave + g;
+        float m = FA_NEG_INF;
 #pragma unroll
-          for (int w = 0; w < WAVES; ++w) m = fmaxf(m, smem[(w * 16 + row) * ROW + D]);
-          float sum = 0.f, o[D / 4];
+        for (int w = 0; w < WAVES; ++w) m = fmaxf(m, smem[(w * 16 + row) * ROW + D]);
+        float sum = 0.f, o[CPL];
 #pragma unroll
-          for (int j = 0; j < D / 4; ++j) o[j] = 0.f;
+        for (int j = 0; j < CPL; ++j) o[j] = 0.f;
 #pragma unroll
-          for (int w = 0; w < WAVES; ++w) {
-            const float* src = smem + (w * 16 + row) * ROW;
-            const float mw = src[D];
-            const float f = mw == FA_NEG_INF && m == FA_NEG_INF ? 1.f : fast_exp2((mw - m) * p.c);
-            sum += f * src[D + 1];
+        for (int w = 0; w < WAVES; ++w) {
+          const float* src = smem + (w * 16 + row) * ROW;
+          const float f = m == FA_NEG_INF ? 1.f : fast_exp2((src[D] - m) * p.c);
+          sum += f * src[D + 1];
 #pragma unroll
-            for (int j = 0; j < D / 4; ++j) o[j] = fmaf(f, src[g * (D / 4) + j], o[j]);
-          }
-          const int r = row0 + 16 * rt + row;
-          if (r < rows) store_row(p, b, hk, split, r, o, m, sum, g);
+          for (int j = 0; j < CPL; ++j) o[j] = fmaf(f, src[c16 * CPL + j], o[j]);
         }
+        const int r = row0 + 16 * rt + row;
+        if (r < rows) store_row<CPL>(p, b, hk, slot, r, o, m, sum, c16);
         __syncthreads();
       }
     } else {
@@ -428,61 +526,102 @@ struct Kv4Attend {
 #pragma unroll
           for (int d = 0; d < CPL; ++d) o[r * CPL + d] = s.o[d][rt][r];
         const int r = row0 + 16 * rt + c16;
-        if (r < rows) store_row(p, b, hk, split, r, o, s.m[rt], l, g);
+        if (r < rows) store_row<D / 4>(p, b, hk, slot, r, o, s.m[rt], l, g);
       }
     }
   }
 };
 
+// Waves per SIMD: what the registers of two tiles in flight, Q and O allow.
+template <int D, int R>
+constexpr int attend_waves() {
+  return D == 64 ? (R == 1 ? 4 : 3) : (D == 128 ? (R == 1 ? 3 : 2) : (R == 1 ? 2 : 1));
+}
 template <typename Tag, int D, int R, bool SHARED>
-__global__ __launch_bounds__(256) void kv4_attend_kernel(Kv4AttendParams p) {
+__global__ __launch_bounds__(256, (attend_waves<D, R>())) void kv4_attend_kernel(Kv4AttendParams p) {
   __shared__ float smem[SHARED ? 4 * 16 * (D + 4) : 1];
   Kv4Attend<Tag, D, R, SHARED>::run(p, smem);
 }
 
-// Joins the splits of a row (one wave): weights exp2(m_s - m) of the unnormalised partial sums.
-template <typename Tag, int D>
+// Joins the splits of a row: weights exp2(m_s - m) of the unnormalised partial sums. WPR waves take a row, four
+// where rows are few and splits many (single tokens), one where it is the other way round. D / 4 lanes read one
+// split's row, so a wave has 256 / D of them in flight at once, times the unrolling.
+template <typename Tag, int D, int WPR>
 __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttendParams p) {
-  constexpr int PL = D / 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t rows = (int64_t)p.B * p.H * p.M;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
+  constexpr int LPS = D / 4, AT_ONCE = WPR * 64 / LPS;
+  __shared__ floatx4 part_o[WPR][LPS];
+  __shared__ float part_ml[WPR][2];
+  const int lane = threadIdx.x & 63, wave = WPR == 4 ? threadIdx.x >> 6 : 0;
+  const int64_t row = WPR == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (WPR == 1 && row >= (int64_t)p.B * p.H * p.M) return;
   const int i = (int)(row % p.M);
   const int64_t bh = row / p.M;
   const int h = (int)(bh % p.H), b = (int)(bh / p.H);
-  const int keys = visible_keys(p.start, p.count, b, p.M, p.capacity);
-  const int tiles = (keys + 31) / 32;
-  const int per = tiles_per_split(keys, p.splits, p.min_tiles);
-  const int used = (tiles + per - 1) / per;
-  float m = FA_NEG_INF;
-  for (int s = lane; s < used; s += 64) m = fmaxf(m, p.ws_ml[2 * (s * rows + row)]);
+  const Split part = find_split(p, -1, b);
+  const int64_t stride = (int64_t)p.H * p.M;  // rows of a slot
+  const int64_t at = part.first * stride + (int64_t)h * p.M + i;
+  const int mine = wave * (64 / LPS) + lane / LPS, c4 = lane % LPS;
+  float m = FA_NEG_INF, sum = 0.f;
+  floatx4 o = (floatx4){0.f, 0.f, 0.f, 0.f};
+  for (int s = mine; s < part.used; s += AT_ONCE) m = fmaxf(m, p.ws_ml[2 * (at + s * stride)]);
+  const float base = m == FA_NEG_INF ? 0.f : m;
+#pragma unroll 4
+  for (int s = mine; s < part.used; s += AT_ONCE) {
+    const int64_t w = at + s * stride;
+    const float f = fast_exp2(p.ws_ml[2 * w] - base);
+    const floatx4 x = *reinterpret_cast<const floatx4*>(p.ws_o + w * D + 4 * c4);
+    sum = fmaf(f, p.ws_ml[2 * w + 1], sum);
 #pragma unroll
-  for (int k = 32; k >= 1; k /= 2) m = fmaxf(m, __shfl_xor(m, k, 64));
-  float sum = 0.f, o[PL];
-#pragma unroll
-  for (int j = 0; j < PL; ++j) o[j] = 0.f;
-  for (int s = 0; s < used; ++s) {
-    const float ms = p.ws_ml[2 * (s * rows + row)];
-    const float f = ms == FA_NEG_INF && m == FA_NEG_INF ? 1.f : fast_exp2(ms - m);
-    sum = fmaf(f, p.ws_ml[2 * (s * rows + row) + 1], sum);
-    const float* src = p.ws_o + (s * rows + row) * D + lane * PL;
-#pragma unroll
-    for (int j = 0; j < PL; ++j) o[j] = fmaf(f, src[j], o[j]);
+    for (int j = 0; j < 4; ++j) o[j] = fmaf(f, x[j], o[j]);
   }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  uint16_t* dst = p.o + b * p.so[0] + h * p.so[1] + i * p.so[2] + lane * PL;
 #pragma unroll
-  for (int j = 0; j < PL; ++j) dst[j] = DT<Tag>::from_float(o[j] * inv);
-  if (lane == 0 && p.lse != nullptr)
+  for (int k = LPS; k < 64; k *= 2) {  // the wave's lane groups
+    const float mo = __shfl_xor(m, k, 64), so = __shfl_xor(sum, k, 64);
+    const float top = fmaxf(m, mo), ref = top == FA_NEG_INF ? 0.f : top;
+    const float f = fast_exp2(m - ref), fo = fast_exp2(mo - ref);
+    sum = f * sum + fo * so;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = f * o[j] + fo * __shfl_xor(o[j], k, 64);
+    m = top;
+  }
+  if constexpr (WPR > 1) {
+    if (lane < LPS) part_o[wave][c4] = o;
+    if (lane == 0) {
+      part_ml[wave][0] = m;
+      part_ml[wave][1] = sum;
+    }
+    __syncthreads();
+    if (threadIdx.x >= LPS) return;
+    float top = FA_NEG_INF;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) top = fmaxf(top, part_ml[w][0]);
+    const float ref = top == FA_NEG_INF ? 0.f : top;
+    sum = 0.f;
+    o = (floatx4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) {
+      const float f = fast_exp2(part_ml[w][0] - ref);
+      sum = fmaf(f, part_ml[w][1], sum);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = fmaf(f, part_o[w][c4][j], o[j]);
+    }
+    m = top;
+  }
+  if (lane >= LPS) return;
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  *reinterpret_cast<u32x2*>(p.o + b * p.so[0] + h * p.so[1] + i * p.so[2] + 4 * c4) =
+      (u32x2){DT<Tag>::pack2(o[0] * inv, o[1] * inv), DT<Tag>::pack2(o[2] * inv, o[3] * inv)};
+  if (c4 == 0 && p.lse != nullptr)
     p.lse[b * p.sl[0] + h * p.sl[1] + i * p.sl[2]] =
         sum > 0.f ? (m + __builtin_amdgcn_logf(sum) - Fp4<Tag>::kPBias) * 0.6931471805599453f : FA_NEG_INF;
 }
 
 #define KV4_ENTRY(TAG, DTYPE, D)                                                                                   \
-  {DTYPE, D, (const void*)&kv4_append_kernel<TAG>, (const void*)&kv4_merge_kernel<TAG, D>,                         \
+  {DTYPE, D, (const void*)&kv4_append_kernel<TAG>,                                                                 \
+   {(const void*)&kv4_merge_kernel<TAG, D, 4>, (const void*)&kv4_merge_kernel<TAG, D, 1>},                         \
    {(const void*)&kv4_attend_kernel<TAG, D, 1, true>, (const void*)&kv4_attend_kernel<TAG, D, 2, true>,            \
-    (const void*)&kv4_attend_kernel<TAG, D, (D == 256 ? 1 : 2), false>}, D == 256 ? 1 : 2}
+    (const void*)&kv4_attend_kernel<TAG, D, (D == 256 ? 1 : 2), false>},                                           \
+   {attend_waves<D, 1>(), attend_waves<D, 2>(), attend_waves<D, (D == 256 ? 1 : 2)>()}, D == 256 ? 1 : 2}
 
 static const Kv4KernelEntry kKv4Entries[] = {
     KV4_ENTRY(f16_t, FA_DTYPE_F16, 64),   KV4_ENTRY(f16_t, FA_DTYPE_F16, 128),   KV4_ENTRY(f16_t, FA_DTYPE_F16, 256),

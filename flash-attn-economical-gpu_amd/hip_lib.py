@@ -224,6 +224,7 @@ SIGNATURES = {
     "kv4_append": (ctypes.c_int, [ctypes.POINTER(Kv4AppendArgs), ctypes.c_void_p]),
     "kv4_attend": (ctypes.c_int, [ctypes.POINTER(Kv4AttendArgs), ctypes.c_void_p]),
     "kv4_attend_workspace_bytes": (ctypes.c_int64, [ctypes.c_int32] * 5),
+    "kv4_attend_splits": (ctypes.c_int32, [ctypes.c_int32] * 6),
 }
 
 

@@ -35,12 +35,9 @@ def _positions(t: torch.Tensor | None, name: str, B: int, device: torch.device) 
 
 @functools.lru_cache(maxsize=4096)
 def choose_splits(B: int, H: int, H_kv: int, M: int, D: int, capacity: int) -> int:
-    """Workgroups that share one sequence's keys: enough for two workgroups on each of 256 CUs, none with less
+    """Parts that a sequence's keys are cut into on average: as many workgroups as the chip holds, none with less
     than 256 keys of a full cache."""
-    rows = M * (H // H_kv)
-    row_blocks = -(-rows // (32 if rows <= 32 else (64 if D == 256 else 128)))
-    blocks = max(1, B * H_kv * row_blocks)
-    return max(1, min(-(-512 // blocks), capacity // 256))
+    return int(hip_lib.load().kv4_attend_splits(B, H, H_kv, M, D, capacity))
 
 
 class Kv4Cache:

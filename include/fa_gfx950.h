@@ -318,8 +318,10 @@ int kv4_append(const kv4_append_args* args, void* stream);
 /* Attention of q [B, H, M, D] over the cache. Row i < count[b] (all M without a count) of sequence b stands at
  * position start[b] + i and sees the cached rows up to and including it (causal), or all
  * start[b] + count[b] (otherwise), never past the capacity. Rows that see nothing, and rows at or behind
- * count[b], are zeros with lse = -inf. lse (nullable): fp32 [B, H, M]. splits > 1 splits each sequence's keys over that
- * many workgroups, with a workspace of kv4_attend_workspace_bytes() and a second launch that joins them. */
+ * count[b], are zeros with lse = -inf. lse (nullable): fp32 [B, H, M]. splits > 1 cuts the
+ * sequences' keys into that many parts on average (longer sequences get more), with a workspace of
+ * kv4_attend_workspace_bytes() and a second launch that joins them; kv4_attend_splits() is the number that
+ * fills the chip. */
 typedef struct {
   kv4_cache cache;
   const void* q;
@@ -340,6 +342,7 @@ typedef struct {
 
 int kv4_attend(const kv4_attend_args* args, void* stream);
 int64_t kv4_attend_workspace_bytes(int32_t B, int32_t H, int32_t M, int32_t D, int32_t splits);
+int32_t kv4_attend_splits(int32_t B, int32_t H, int32_t H_kv, int32_t M, int32_t D, int32_t capacity);
 
 #ifdef __cplusplus
 }
