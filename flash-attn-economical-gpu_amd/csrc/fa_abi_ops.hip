@@ -126,7 +126,7 @@ int check_cache(const kv4_cache* c) {
 }
 
 // Which attention kernel takes a kv head's query rows: up to 32 the waves of a workgroup share them (and the
-// cache is read once); more go 64 or 128 to a workgroup.
+// cache is read once); more go chunk_rows to a workgroup.
 struct Kv4Kind {
   int kind;
   int64_t row_blocks;
@@ -134,7 +134,7 @@ struct Kv4Kind {
 Kv4Kind kv4_kind(const fa::Kv4KernelEntry* e, int64_t rows) {
   Kv4Kind k;
   k.kind = rows <= 16 ? 0 : (rows <= 32 ? 1 : 2);
-  const int64_t block = k.kind == 2 ? 64 * e->chunk_tiles : 16 << k.kind;
+  const int64_t block = k.kind == 2 ? e->chunk_rows : 16 << k.kind;
   k.row_blocks = (rows + block - 1) / block;
   return k;
 }
@@ -314,7 +314,8 @@ int kv4_attend(const kv4_attend_args* a, void* stream) {
   if ((code = check_tensor("o", a->o, a->o_stride, c->D, 4)) != FA_OK) return code;
   if (a->start == nullptr) return fail(FA_EINVAL, "null start pointer");
   const int64_t rows = (int64_t)a->M * (a->H / c->H_kv);
-  if (rows > 0x7fffffffLL - 256) return fail(FA_EINVAL, "too many query rows (%lld per kv head)", (long long)rows);
+  if (rows * c->H_kv > (0x7fffffffLL - 256) / c->B) return fail(FA_EINVAL, "too many query rows (%lld per kv head)",
+                                                                  (long long)rows);
   const fa::Kv4KernelEntry* e = find_kv4(c->dtype, c->D);
   if (e == nullptr) return fail(FA_ENOTSUP, "4-bit cache kernels for dtype=%d D=%d are not built", c->dtype, c->D);
   fa::Kv4AttendParams p;
@@ -359,7 +360,8 @@ int kv4_attend(const kv4_attend_args* a, void* stream) {
   if (a->splits > 1) {
     const int64_t all = (int64_t)c->B * a->H * a->M;
     const bool wide = a->splits > 8;
-    if ((code = launch(e->merge[wide ? 0 : 1], wide ? all : (all + 3) / 4, 1, 256, &p, stream, "cache merge")) != FA_OK)
+    const int64_t few = (all + 3) / 4 < 2048 ? (all + 3) / 4 : 2048;  // eight workgroups to a CU, a few rows to a wave
+    if ((code = launch(e->merge[wide ? 0 : 1], wide ? all : few, 1, 256, &p, stream, "cache merge")) != FA_OK)
       return code;
   }
   return ok();

@@ -151,15 +151,18 @@ __global__ __launch_bounds__(256) void fa_bwd_prep_kernel(BwdParams p) {
 }
 
 template <typename Tag, int D, int KT>
-struct Bwd {
+struct Bwd : LdsRows<D> {
+  using L = LdsRows<D>;
+  using L::frag;
+  using L::tfrag;
+  using L::swz;
   static constexpr int WAVES = 4;
   static constexpr int T = 32;                   // rows of a tile passing through LDS
   static constexpr int OWN = 16 * KT;            // rows owned per wave
   static constexpr int BLOCK = WAVES * OWN;      // rows owned per workgroup
   static constexpr int KS = D / 32;          // k = 32 steps over D
   static constexpr int DT16 = D / 16;        // 16-wide tiles over D
-  static constexpr int ROWB = 2 * D;         // bytes of an LDS row
-  static constexpr int CPR = D / 8;          // 16-byte chunks of a row
+  static constexpr int ROWB = L::ROWB, CPR = L::CPR;
   static constexpr int TILEB = T * ROWB;
   // A ring of stages of two tiles each, then the stages' groups of row terms. A tile's loads are issued STAGES - 1
   // steps before its use; two stages measured 3% (D <= 128) and 7% (D = 256) faster than three or four.
@@ -169,13 +172,6 @@ struct Bwd {
   static constexpr int SMEM = TERMS + STAGES * 256;
   static constexpr int NB = TILEB / 1024 / WAVES;  // LDS-DMA instructions of a wave per tile
 
-  // LDS rows are unpadded (LDS-DMA writes 1 KiB blocks); chunk c of row r lies at c ^ swz(r). The LDS serves 256
-  // bytes a cycle: 16 lanes of a row-fragment read (one chunk of 16 rows) and 32 lanes of a transposing read
-  // (an even chunk and the next, of 8 rows). Both fall on different banks when rows 0 .. 7 differ in the chunk
-  // pair and r, r + 8 in the place within it (D = 64, two rows to 256 bytes: rows 0, 2, 4, 6).
-  __device__ static inline int swz(int r) {
-    return D == 64 ? (r & 6) : (r & 7) << 1;
-  }
   typedef DT<Tag> E;
   __device__ static inline uint32_t pack2(float x, float y) {
     typedef float f2 __attribute__((ext_vector_type(2)));
@@ -227,28 +223,6 @@ struct Bwd {
                  :
                  : "v"((uint32_t)lane * 4u), "s"(dst), "s"(rsrc)
                  : "memory", "m0");
-  }
-
-  // Byte offset in a tile of a lane's row fragment (row lane & 15, channels 8 (lane >> 4) ..): step ks is at
-  // off ^ (ks << 6), row tile i at + i * 16 * ROWB. Stages are whole multiples of a row, so the exclusive or may
-  // come after the stage's offset is added: one address per stage is held, not one per step.
-  __device__ static inline uint32_t row_off(int lane) {
-    const int r = lane & 15, g = lane >> 4;
-    return (uint32_t)(r * ROWB + ((g ^ swz(r)) << 4));
-  }
-  // Byte offset of a lane's transposing read (rows 4 (lane >> 4) .. + 3, its 4 of 16 columns): columns
-  // 16 dt .. are at off ^ (dt << 5), row tile i at + i * 16 * ROWB.
-  __device__ static inline uint32_t tr_off(int lane) {
-    const int L = lane & 15, r = 4 * (lane >> 4) + (L >> 2);
-    return (uint32_t)(r * ROWB + ((((L & 3) >> 1) ^ swz(r)) << 4) + ((L & 1) << 3));
-  }
-  __device__ static inline u32x4 frag(const char* smem, uint32_t off, int tile) {
-    return *reinterpret_cast<const u32x4*>(smem + off + tile);
-  }
-  __device__ static inline u32x4 tfrag(const char* smem, uint32_t off, int tile) {
-    const u32x2 a = lds_read_tr16(reinterpret_cast<const uint16_t*>(smem + off + tile));
-    const u32x2 b = lds_read_tr16(reinterpret_cast<const uint16_t*>(smem + off + tile + 16 * ROWB));
-    return (u32x4){a[0], a[1], b[0], b[1]};
   }
 
   // The owned rows' fragments straight from memory, zeros past `rows`.
@@ -326,7 +300,7 @@ struct Bwd {
       for (int i = 0; i < KT; ++i) dk[d][i] = dv[d][i] = (floatx4){0.f, 0.f, 0.f, 0.f};
 
     const uint32_t lds = lds_address(smem);
-    const uint32_t ro = row_off(lane), to = tr_off(lane);
+    const uint32_t ro = L::row_off(lane), to = L::tr_off(lane);
     const int qt_all = (p.M + T - 1) / T;
     const int qt0 = p.causal ? k0 / T : 0;  // rows above the block's first key see none of its keys
     const int per_head = qt_all > qt0 ? qt_all - qt0 : 0;
@@ -494,7 +468,7 @@ struct Bwd {
 #pragma unroll
       for (int i = 0; i < KT; ++i) acc[d][i] = (floatx4){0.f, 0.f, 0.f, 0.f};
     const uint32_t lds = lds_address(smem);
-    const uint32_t ro = row_off(lane), to = tr_off(lane);
+    const uint32_t ro = L::row_off(lane), to = L::tr_off(lane);
     const int n_end = p.causal && m0 + BLOCK < p.N ? m0 + BLOCK : p.N;
     const int all = (n_end + T - 1) / T, share = (all + p.q_splits - 1) / p.q_splits;
     const int first = part * share, tiles = first >= all ? first : (all - first < share ? all : first + share);

@@ -225,6 +225,40 @@ __device__ inline uint32_t lds_address(const void* shared_array) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)shared_array;
 }
 
+// Tiles of rows of D 16-bit values in LDS, unpadded: chunk c (16 bytes) of row r lies at c ^ swz(r). The LDS serves
+// 256 bytes a cycle: 16 lanes of a row-fragment read (lanes 0 .. 3, 12 .. 15 and, with the next chunk, the rows
+// 4 .. 11 of the next 16 lanes) and 32 lanes of a transposing read (an even chunk and the next, of 8 rows). Both
+// fall on different banks when rows 0 .. 7 differ in the chunk pair and r, r + 8 are alike (D = 64, two rows to 256
+// bytes: rows 0, 2, 4, 6 differ). Counted: no bank conflicts.
+template <int D>
+struct LdsRows {
+  static constexpr int ROWB = 2 * D;  // bytes of a row
+  static constexpr int CPR = D / 8;   // 16-byte chunks of a row
+  __device__ static inline int swz(int r) { return D == 64 ? (r & 6) : (r & 7) << 1; }
+  // Byte offset in a tile of a lane's row fragment (row lane & 15, channels 8 (lane >> 4) ..): step ks is at
+  // off ^ (ks << 6), row tile i at + i * 16 * ROWB. Stages are whole multiples of a row, so the exclusive or may
+  // come after the stage's offset is added: one address per stage is held, not one per step.
+  __device__ static inline uint32_t row_off(int lane) {
+    const int r = lane & 15, g = lane >> 4;
+    return (uint32_t)(r * ROWB + ((g ^ swz(r)) << 4));
+  }
+  // Byte offset of a lane's transposing read (rows 4 (lane >> 4) .. + 3, its 4 of 16 columns): columns
+  // 16 dt .. are at off ^ (dt << 5), row tile i at + i * 16 * ROWB.
+  __device__ static inline uint32_t tr_off(int lane) {
+    const int L = lane & 15, r = 4 * (lane >> 4) + (L >> 2);
+    return (uint32_t)(r * ROWB + ((((L & 3) >> 1) ^ swz(r)) << 4) + ((L & 1) << 3));
+  }
+  __device__ static inline u32x4 frag(const char* smem, uint32_t off, int tile) {
+    return *reinterpret_cast<const u32x4*>(smem + off + tile);
+  }
+  // The operand of 32 rows: rows 4 g .. + 3 of the tile, then of its next 16 rows.
+  __device__ static inline u32x4 tfrag(const char* smem, uint32_t off, int tile) {
+    const u32x2 a = lds_read_tr16(reinterpret_cast<const uint16_t*>(smem + off + tile));
+    const u32x2 b = lds_read_tr16(reinterpret_cast<const uint16_t*>(smem + off + tile + 16 * ROWB));
+    return (u32x4){a[0], a[1], b[0], b[1]};
+  }
+};
+
 // Wait until at most N vector-memory operations of this wave are outstanding and all its LDS
 // operations are done, then barrier. Unlike __syncthreads() this does not wait for every
 // outstanding load: LDS-DMA loads issued for later steps stay in flight across the barrier.

@@ -161,9 +161,9 @@ struct Kv4KernelEntry {
   int32_t D;
   const void* append;
   const void* merge[2];   // a workgroup per row, a wave per row
-  const void* attend[3];  // 16 rows shared by a workgroup's waves, 32 rows shared, own rows per wave
+  const void* attend[3];  // 16 rows shared by a workgroup's waves, 32 rows shared, chunks of a prompt
   int32_t per_cu[3];      // workgroups of each that a CU holds
-  int32_t chunk_tiles;    // 16-row tiles per wave of the last
+  int32_t chunk_rows;     // query rows of a workgroup of the last
 };
 
 const Kv4KernelEntry* kv4_registry(int* count);

@@ -209,9 +209,8 @@ __device__ inline Split find_split(const Kv4AttendParams& p, int slot, int b) {
 //                   regroups them by channel with byte permutes; P^T is S^T's accumulator as it stands
 // so nothing passes through LDS but the waves' sums at the end. Query rows are (position, head of the group):
 // row r is head r % group at position r / group, and a workgroup's rows share its kv head's cache.
-//   SHARED: the four waves hold the same rows and take turns at the tiles (single tokens, short drafts)
-//   else:   each wave holds its own rows (chunks of a prompt)
-template <typename Tag, int D, int R, bool SHARED>
+// The four waves hold the same rows (single tokens, short drafts) and take turns at the tiles.
+template <typename Tag, int D, int R>
 struct Kv4Attend {
   static constexpr int WAVES = 4;
   static constexpr int KS = D / 32;   // k = 32 steps over D
@@ -415,7 +414,7 @@ struct Kv4Attend {
     const int b = __builtin_amdgcn_readfirstlane(part.b);
     if (b < 0) return;
     const int rows = p.M * p.group;
-    const int row0 = (SHARED ? rb : rb * WAVES + wave) * 16 * R;
+    const int row0 = rb * 16 * R;
     const int keys = visible_keys(p.start, p.count, b, p.M, p.capacity);
     const int count = p.count != nullptr ? p.count[b] : p.M;
     const int64_t start = p.start[b];
@@ -461,8 +460,7 @@ struct Kv4Attend {
     const uint8_t* vc = p.v_codes + b * p.code_stride[0] + hk * p.code_stride[1];
     const uint8_t* ks = p.k_scales + b * p.scale_stride[0] + hk * p.scale_stride[1];
     const uint8_t* vs = p.v_scales + b * p.scale_stride[0] + hk * p.scale_stride[1];
-    const int stride = SHARED ? WAVES : 1;
-    if (SHARED) t0 += wave;
+    t0 += wave;
     // two tiles in flight
     Tile even, odd;
     auto fetch = [&](Tile& x, int t) {
@@ -471,63 +469,49 @@ struct Kv4Attend {
     auto use = [&](Tile& x, int t) {
       if (t * 32 + 32 <= least) step<false>(s, qf, x, t * 32, see, keys, p.c, lane);
       else step<true>(s, qf, x, t * 32, see, keys, p.c, lane);
-      fetch(x, t + 2 * stride);
+      fetch(x, t + 2 * WAVES);
     };
     fetch(even, t0);
-    fetch(odd, t0 + stride);
-    for (int t = t0; t < t1; t += 2 * stride) {
+    fetch(odd, t0 + WAVES);
+    for (int t = t0; t < t1; t += 2 * WAVES) {
       use(even, t);
-      if (t + stride < t1) use(odd, t + stride);
+      if (t + WAVES < t1) use(odd, t + WAVES);
     }
-    if constexpr (SHARED) {
-      // the waves' sums meet in LDS; wave w finishes rows 4 w .. 4 w + 3 of each 16, 16 lanes to a row
-      constexpr int ROW = D + 4;
+    // the waves' sums meet in LDS; wave w finishes rows 4 w .. 4 w + 3 of each 16, 16 lanes to a row
+    constexpr int ROW = D + 4;
 #pragma unroll
-      for (int rt = 0; rt < R; ++rt) {
-        const float l = xquad_sum(s.l[rt]);
-        float* dst = smem + (wave * 16 + c16) * ROW;
+    for (int rt = 0; rt < R; ++rt) {
+      const float l = xquad_sum(s.l[rt]);
+      float* dst = smem + (wave * 16 + c16) * ROW;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-          for (int d = 0; d < CPL; d += 4)
-            *reinterpret_cast<floatx4*>(dst + (4 * g + r) * CPL + d) =
-                (floatx4){s.o[d][rt][r], s.o[d + 1][rt][r], s.o[d + 2][rt][r], s.o[d + 3][rt][r]};
-        if (g == 0) {
-          dst[D] = s.m[rt];
-          dst[D + 1] = l;
-        }
-        __syncthreads();
-        const int row = 4 * wave + g;
-        float m = FA_NEG_INF;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) m = fmaxf(m, smem[(w * 16 + row) * ROW + D]);
-        float sum = 0.f, o[CPL];
-#pragma unroll
-        for (int j = 0; j < CPL; ++j) o[j] = 0.f;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-          const float* src = smem + (w * 16 + row) * ROW;
-          const float f = m == FA_NEG_INF ? 1.f : fast_exp2((src[D] - m) * p.c);
-          sum += f * src[D + 1];
-#pragma unroll
-          for (int j = 0; j < CPL; ++j) o[j] = fmaf(f, src[c16 * CPL + j], o[j]);
-        }
-        const int r = row0 + 16 * rt + row;
-        if (r < rows) store_row<CPL>(p, b, hk, slot, r, o, m, sum, c16);
-        __syncthreads();
+        for (int d = 0; d < CPL; d += 4)
+          *reinterpret_cast<floatx4*>(dst + (4 * g + r) * CPL + d) =
+              (floatx4){s.o[d][rt][r], s.o[d + 1][rt][r], s.o[d + 2][rt][r], s.o[d + 3][rt][r]};
+      if (g == 0) {
+        dst[D] = s.m[rt];
+        dst[D + 1] = l;
       }
-    } else {
+      __syncthreads();
+      const int row = 4 * wave + g;
+      float m = FA_NEG_INF;
 #pragma unroll
-      for (int rt = 0; rt < R; ++rt) {
-        const float l = xquad_sum(s.l[rt]);
-        float o[D / 4];
+      for (int w = 0; w < WAVES; ++w) m = fmaxf(m, smem[(w * 16 + row) * ROW + D]);
+      float sum = 0.f, o[CPL];
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+      for (int j = 0; j < CPL; ++j) o[j] = 0.f;
 #pragma unroll
-          for (int d = 0; d < CPL; ++d) o[r * CPL + d] = s.o[d][rt][r];
-        const int r = row0 + 16 * rt + c16;
-        if (r < rows) store_row<D / 4>(p, b, hk, slot, r, o, s.m[rt], l, g);
+      for (int w = 0; w < WAVES; ++w) {
+        const float* src = smem + (w * 16 + row) * ROW;
+        const float f = m == FA_NEG_INF ? 1.f : fast_exp2((src[D] - m) * p.c);
+        sum += f * src[D + 1];
+#pragma unroll
+        for (int j = 0; j < CPL; ++j) o[j] = fmaf(f, src[c16 * CPL + j], o[j]);
       }
+      const int r = row0 + 16 * rt + row;
+      if (r < rows) store_row<CPL>(p, b, hk, slot, r, o, m, sum, c16);
+      __syncthreads();
     }
   }
 };
@@ -537,10 +521,232 @@ template <int D, int R>
 constexpr int attend_waves() {
   return D == 64 ? (R == 1 ? 4 : 3) : (D == 128 ? (R == 1 ? 3 : 2) : (R == 1 ? 2 : 1));
 }
-template <typename Tag, int D, int R, bool SHARED>
+template <typename Tag, int D, int R>
 __global__ __launch_bounds__(256, (attend_waves<D, R>())) void kv4_attend_kernel(Kv4AttendParams p) {
-  __shared__ float smem[SHARED ? 4 * 16 * (D + 4) : 1];
-  Kv4Attend<Tag, D, R, SHARED>::run(p, smem);
+  __shared__ __align__(16) float smem[4 * 16 * (D + 4)];
+  Kv4Attend<Tag, D, R>::run(p, smem);
+}
+
+// Chunks of a prompt: more than 32 query rows to a kv head. Here the conversion would cost each wave more than its
+// products if it did it for itself (455 TFLOP/s at 32 rows a wave), so the workgroup's four waves, of 32 rows each,
+// share it: a tile's codes are loaded a tile ahead, 32 channels of a row to a thread, converted once into 16-bit
+// rows in LDS (two stages, one barrier a tile), and both products read their fragments there, V's by the
+// transposing read. S^T = K Q^T and O^T = V^T P^T as above.
+template <typename Tag, int D>
+struct Kv4Chunk {
+  using L = LdsRows<D>;
+  typedef DT<Tag> E;
+  static constexpr int WAVES = 4, QT = D == 256 ? 1 : 2;  // 16-row tiles of queries per wave
+  static constexpr int T = D == 256 ? 32 : 64;  // keys of a tile
+  static constexpr int KT = T / 16, KS = D / 32, DT16 = D / 16, SB = D / 32;
+  static constexpr int BLOCK = WAVES * QT * 16;
+  static constexpr int TILEB = T * L::ROWB, STAGEB = 2 * TILEB;
+  static constexpr int SMEM = 2 * STAGEB;
+  static constexpr int UNITS = T * SB;              // 32-channel units of one matrix' tile
+  static constexpr int PER = 2 * UNITS / (WAVES * 64);  // units per thread: one (D = 64: K or V), else one of each
+  static_assert(PER == 1 || PER == 2, "units");
+
+  struct Codes {
+    u32x4 c[PER];
+    uint32_t e[PER];
+  };
+
+  __device__ static void run(const Kv4AttendParams& p, char* smem) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c16 = lane & 15, g = lane >> 4;
+    int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int rb = id % p.row_blocks;
+    id /= p.row_blocks;
+    const int slot = id % p.slots, hk = id / p.slots;
+    const Split part = find_split(p, slot, 0);
+    const int b = __builtin_amdgcn_readfirstlane(part.b);
+    if (b < 0) return;
+    const int rows = p.M * p.group, row0 = rb * BLOCK + wave * QT * 16;
+    const int keys = visible_keys(p.start, p.count, b, p.M, p.capacity);
+    const int count = p.count != nullptr ? p.count[b] : p.M;
+    const int64_t start = p.start[b];
+    auto seen = [&](int row) {  // keys that a live row sees
+      const int64_t e = p.causal ? start + row / p.group + 1 : keys;
+      return (int)(e < 0 ? 0 : (e > keys ? keys : e));
+    };
+    auto last_live = [&](int first, int n) {  // the last of n rows that exists
+      return first + n <= rows ? first + n - 1 : rows - 1;
+    };
+    const int block_see = seen(last_live(rb * BLOCK, BLOCK));
+    const int wave_see = row0 < rows ? seen(last_live(row0, QT * 16)) : 0;
+    const bool whole = row0 + QT * 16 <= rows && (row0 + QT * 16 - 1) / p.group < count;
+    const int least = whole ? seen(row0) : 0;  // keys that every row of the wave sees
+
+    int see[QT];
+    u32x4 qf[QT][KS];
+#pragma unroll
+    for (int j = 0; j < QT; ++j) {
+      const int r = row0 + 16 * j + c16, i = r / p.group;
+      const bool live = r < rows && i < count;
+      see[j] = live ? seen(r) : 0;
+      const uint16_t* q = p.q + b * p.sq[0] + (int64_t)(hk * p.group + (live ? r % p.group : 0)) * p.sq[1] +
+                          (int64_t)(live ? i : 0) * p.sq[2] + 8 * g;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        qf[j][k] = (u32x4){0, 0, 0, 0};
+        if (live) qf[j][k] = *reinterpret_cast<const u32x4*>(q + 32 * k);
+      }
+    }
+    floatx4 o[DT16][QT];
+    float m[QT], l[QT];
+#pragma unroll
+    for (int j = 0; j < QT; ++j) {
+      m[j] = FA_NEG_INF;
+      l[j] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DT16; ++d) o[d][j] = (floatx4){0.f, 0.f, 0.f, 0.f};
+    }
+
+    // the split's keys, in tiles of T (its share is in tiles of 32)
+    const int64_t per = (int64_t)__builtin_amdgcn_readfirstlane(part.per) * 32;
+    const int64_t k_first = __builtin_amdgcn_readfirstlane(part.index) * per;
+    const int k_end = (int)(k_first + per < block_see ? k_first + per : block_see);
+#pragma unroll
+    for (int j = 0; j < QT; ++j) see[j] = see[j] < k_end ? see[j] : k_end;  // the next split may begin inside a tile
+    const uint8_t* kc = p.k_codes + b * p.code_stride[0] + hk * p.code_stride[1];
+    const uint8_t* vc = p.v_codes + b * p.code_stride[0] + hk * p.code_stride[1];
+    const uint8_t* ksc = p.k_scales + b * p.scale_stride[0] + hk * p.scale_stride[1];
+    const uint8_t* vsc = p.v_scales + b * p.scale_stride[0] + hk * p.scale_stride[1];
+    // thread's unit u of the tile at key0: rows are dense, so units are too. Past the last visible key nothing is read,
+    // and what stands there is zero: rows behind a sequence may hold anything.
+    auto fetch = [&](Codes& x, int64_t key0) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const bool is_v = PER == 1 ? tid >= UNITS : i == 1;
+        const int u = PER == 1 ? tid % UNITS : tid;
+        x.c[i] = (u32x4){0, 0, 0, 0};
+        x.e[i] = 127;
+        if (key0 + u / SB < keys) {
+          const int64_t at = key0 * SB + u;
+          x.c[i] = *reinterpret_cast<const u32x4*>((is_v ? vc : kc) + at * 16);
+          x.e[i] = (is_v ? vsc : ksc)[at];
+        }
+      }
+    };
+    auto convert = [&](const Codes& x, char* stage) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const bool is_v = PER == 1 ? tid >= UNITS : i == 1;
+        const int u = PER == 1 ? tid % UNITS : tid;
+        const int row = u / SB, blk = u % SB;
+        char* dst = stage + (is_v ? TILEB : 0) + row * L::ROWB;
+        const float scale = scale_of(x.e[i]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          *reinterpret_cast<u32x4*>(dst + (((4 * blk + c) ^ L::swz(row)) << 4)) = decode8<Tag>(x.c[i][c], scale);
+      }
+    };
+    const uint32_t ro = L::row_off(lane), to = L::tr_off(lane);
+    auto step = [&](int key0, uint32_t stage, auto edge_tile) {
+      constexpr bool EDGE = decltype(edge_tile)::value;
+      const uint32_t rowb = ro + stage, colb = to + stage;
+      floatx4 x[KT][QT];
+#pragma unroll
+      for (int i = 0; i < KT; ++i) {
+#pragma unroll
+        for (int j = 0; j < QT; ++j) x[i][j] = (floatx4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const u32x4 a = L::frag(smem, rowb ^ (k << 6), i * 16 * L::ROWB);
+#pragma unroll
+          for (int j = 0; j < QT; ++j) x[i][j] = E::mfma16(a, qf[j][k], x[i][j]);
+        }
+      }
+      u32x4 pb[KT / 2][QT];
+#pragma unroll
+      for (int j = 0; j < QT; ++j) {
+        float top = FA_NEG_INF;
+#pragma unroll
+        for (int i = 0; i < KT; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (EDGE && key0 + 16 * i + 4 * g + r >= see[j]) x[i][j][r] = FA_NEG_INF;
+            top = fmaxf(top, x[i][j][r]);
+          }
+        const float m_new = fmaxf(m[j], xquad_max(top));
+        if (__any(m_new > m[j])) {
+          const float base = m_new == FA_NEG_INF ? 0.f : m_new;
+          const float f = fast_exp2((m[j] - base) * p.c);
+          l[j] *= f;
+#pragma unroll
+          for (int d = 0; d < DT16; ++d) o[d][j] *= f;
+          m[j] = m_new;
+        }
+        const float off = Fp4<Tag>::kPBias - (m[j] == FA_NEG_INF ? 0.f : m[j] * p.c);
+#pragma unroll
+        for (int i = 0; i < KT; ++i) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            x[i][j][r] = fast_exp2(fmaf(x[i][j][r], p.c, off));
+            l[j] += x[i][j][r];
+          }
+          pb[i / 2][j][2 * (i & 1)] = E::pack2(x[i][j][0], x[i][j][1]);
+          pb[i / 2][j][2 * (i & 1) + 1] = E::pack2(x[i][j][2], x[i][j][3]);
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < DT16; ++d)
+#pragma unroll
+        for (int i = 0; i < KT / 2; ++i) {
+          const u32x4 v = L::tfrag(smem, colb ^ (d << 5), TILEB + i * 32 * L::ROWB);
+#pragma unroll
+          for (int j = 0; j < QT; ++j) o[d][j] = E::mfma16(v, pb[i][j], o[d][j]);
+        }
+    };
+    Codes next;
+    if (k_first < k_end) fetch(next, k_first);
+    uint32_t stage = 0;
+    // tiles that every row of the wave sees whole, then those on the diagonal or at the end: every wave makes the
+    // same number of passes in all, for the barriers
+    auto pass = [&](int64_t key0, auto edge_tile) {
+      convert(next, smem + stage);
+      if (key0 + T < k_end) fetch(next, key0 + T);
+      wait_vm_lds_barrier<63>();  // LDS writes only: the codes just asked for stay in flight
+      if (key0 < wave_see) step((int)key0, stage, edge_tile);
+      stage ^= STAGEB;
+    };
+    int64_t key0 = k_first;
+    for (; key0 + T <= k_end && key0 + T <= least; key0 += T) pass(key0, std::false_type{});
+    for (; key0 < k_end; key0 += T) pass(key0, std::true_type{});
+
+#pragma unroll
+    for (int j = 0; j < QT; ++j) {
+      const float sum = xquad_sum(l[j]);
+      const int r = row0 + 16 * j + c16;
+      if (r >= rows) continue;
+      const int i = r / p.group, h = hk * p.group + r % p.group;
+      if (p.splits > 1) {
+        const int64_t w = ((int64_t)slot * p.H + h) * p.M + i;
+#pragma unroll
+        for (int d = 0; d < DT16; ++d) *reinterpret_cast<floatx4*>(p.ws_o + w * D + 16 * d + 4 * g) = o[d][j];
+        if (g == 0) {
+          p.ws_ml[2 * w] = m[j] * p.c;
+          p.ws_ml[2 * w + 1] = sum;
+        }
+      } else {
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        uint16_t* dst = p.o + b * p.so[0] + h * p.so[1] + i * p.so[2] + 4 * g;
+#pragma unroll
+        for (int d = 0; d < DT16; ++d)
+          *reinterpret_cast<u32x2*>(dst + 16 * d) =
+              (u32x2){E::pack2(o[d][j][0] * inv, o[d][j][1] * inv), E::pack2(o[d][j][2] * inv, o[d][j][3] * inv)};
+        if (g == 0 && p.lse != nullptr)
+          p.lse[b * p.sl[0] + h * p.sl[1] + i * p.sl[2]] =
+              sum > 0.f ? (m[j] * p.c + __builtin_amdgcn_logf(sum) - Fp4<Tag>::kPBias) * 0.6931471805599453f : FA_NEG_INF;
+      }
+    }
+  }
+};
+
+template <typename Tag, int D>
+__global__ __launch_bounds__(256, 2) void kv4_chunk_kernel(Kv4AttendParams p) {
+  __shared__ __align__(1024) char smem[Kv4Chunk<Tag, D>::SMEM];
+  Kv4Chunk<Tag, D>::run(p, smem);
 }
 
 // Joins the splits of a row: weights exp2(m_s - m) of the unnormalised partial sums. WPR waves take a row, four
@@ -552,76 +758,80 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttendParams p) {
   __shared__ floatx4 part_o[WPR][LPS];
   __shared__ float part_ml[WPR][2];
   const int lane = threadIdx.x & 63, wave = WPR == 4 ? threadIdx.x >> 6 : 0;
-  const int64_t row = WPR == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (WPR == 1 && row >= (int64_t)p.B * p.H * p.M) return;
-  const int i = (int)(row % p.M);
-  const int64_t bh = row / p.M;
-  const int h = (int)(bh % p.H), b = (int)(bh / p.H);
-  const Split part = find_split(p, -1, b);
-  const int64_t stride = (int64_t)p.H * p.M;  // rows of a slot
-  const int64_t at = part.first * stride + (int64_t)h * p.M + i;
-  const int mine = wave * (64 / LPS) + lane / LPS, c4 = lane % LPS;
-  float m = FA_NEG_INF, sum = 0.f;
-  floatx4 o = (floatx4){0.f, 0.f, 0.f, 0.f};
-  for (int s = mine; s < part.used; s += AT_ONCE) m = fmaxf(m, p.ws_ml[2 * (at + s * stride)]);
-  const float base = m == FA_NEG_INF ? 0.f : m;
+  const uint32_t rows = (uint32_t)p.B * p.H * p.M;
+  const uint32_t first = WPR == 4 ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 6);
+  Split part;
+  int of = -1;  // the sequence that `part` is of
+  // a workgroup per row, or so many waves that each takes a few rows
+  for (uint32_t row = __builtin_amdgcn_readfirstlane(first); row < rows; row += WPR == 4 ? rows : gridDim.x * 4) {
+    const uint32_t bh = row / (uint32_t)p.M;
+    const int i = (int)(row % (uint32_t)p.M), h = (int)(bh % (uint32_t)p.H), b = (int)(bh / (uint32_t)p.H);
+    if (b != of) part = find_split(p, -1, of = b);
+    const int64_t stride = (int64_t)p.H * p.M;  // rows of a slot
+    const int64_t at = part.first * stride + (int64_t)h * p.M + i;
+    const int mine = wave * (64 / LPS) + lane / LPS, c4 = lane % LPS;
+    float m = FA_NEG_INF, sum = 0.f;
+    floatx4 o = (floatx4){0.f, 0.f, 0.f, 0.f};
+    for (int s = mine; s < part.used; s += AT_ONCE) m = fmaxf(m, p.ws_ml[2 * (at + s * stride)]);
+    const float base = m == FA_NEG_INF ? 0.f : m;
 #pragma unroll 4
-  for (int s = mine; s < part.used; s += AT_ONCE) {
-    const int64_t w = at + s * stride;
-    const float f = fast_exp2(p.ws_ml[2 * w] - base);
-    const floatx4 x = *reinterpret_cast<const floatx4*>(p.ws_o + w * D + 4 * c4);
-    sum = fmaf(f, p.ws_ml[2 * w + 1], sum);
+    for (int s = mine; s < part.used; s += AT_ONCE) {
+      const int64_t w = at + s * stride;
+      const float f = fast_exp2(p.ws_ml[2 * w] - base);
+      const floatx4 x = *reinterpret_cast<const floatx4*>(p.ws_o + w * D + 4 * c4);
+      sum = fmaf(f, p.ws_ml[2 * w + 1], sum);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = fmaf(f, x[j], o[j]);
-  }
-#pragma unroll
-  for (int k = LPS; k < 64; k *= 2) {  // the wave's lane groups
-    const float mo = __shfl_xor(m, k, 64), so = __shfl_xor(sum, k, 64);
-    const float top = fmaxf(m, mo), ref = top == FA_NEG_INF ? 0.f : top;
-    const float f = fast_exp2(m - ref), fo = fast_exp2(mo - ref);
-    sum = f * sum + fo * so;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = f * o[j] + fo * __shfl_xor(o[j], k, 64);
-    m = top;
-  }
-  if constexpr (WPR > 1) {
-    if (lane < LPS) part_o[wave][c4] = o;
-    if (lane == 0) {
-      part_ml[wave][0] = m;
-      part_ml[wave][1] = sum;
+      for (int j = 0; j < 4; ++j) o[j] = fmaf(f, x[j], o[j]);
     }
-    __syncthreads();
-    if (threadIdx.x >= LPS) return;
-    float top = FA_NEG_INF;
 #pragma unroll
-    for (int w = 0; w < WPR; ++w) top = fmaxf(top, part_ml[w][0]);
-    const float ref = top == FA_NEG_INF ? 0.f : top;
-    sum = 0.f;
-    o = (floatx4){0.f, 0.f, 0.f, 0.f};
+    for (int k = LPS; k < 64; k *= 2) {  // the wave's lane groups
+      const float mo = __shfl_xor(m, k, 64), so = __shfl_xor(sum, k, 64);
+      const float top = fmaxf(m, mo), ref = top == FA_NEG_INF ? 0.f : top;
+      const float f = fast_exp2(m - ref), fo = fast_exp2(mo - ref);
+      sum = f * sum + fo * so;
 #pragma unroll
-    for (int w = 0; w < WPR; ++w) {
-      const float f = fast_exp2(part_ml[w][0] - ref);
-      sum = fmaf(f, part_ml[w][1], sum);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = fmaf(f, part_o[w][c4][j], o[j]);
+      for (int j = 0; j < 4; ++j) o[j] = f * o[j] + fo * __shfl_xor(o[j], k, 64);
+      m = top;
     }
-    m = top;
+    if constexpr (WPR > 1) {
+      if (lane < LPS) part_o[wave][c4] = o;
+      if (lane == 0) {
+        part_ml[wave][0] = m;
+        part_ml[wave][1] = sum;
+      }
+      __syncthreads();
+      if (threadIdx.x >= LPS) return;  // WPR = 4 has one row
+      float top = FA_NEG_INF;
+#pragma unroll
+      for (int w = 0; w < WPR; ++w) top = fmaxf(top, part_ml[w][0]);
+      const float ref = top == FA_NEG_INF ? 0.f : top;
+      sum = 0.f;
+      o = (floatx4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < WPR; ++w) {
+        const float f = fast_exp2(part_ml[w][0] - ref);
+        sum = fmaf(f, part_ml[w][1], sum);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = fmaf(f, part_o[w][c4][j], o[j]);
+      }
+      m = top;
+    }
+    if (lane >= LPS) continue;
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    *reinterpret_cast<u32x2*>(p.o + b * p.so[0] + h * p.so[1] + i * p.so[2] + 4 * c4) =
+        (u32x2){DT<Tag>::pack2(o[0] * inv, o[1] * inv), DT<Tag>::pack2(o[2] * inv, o[3] * inv)};
+    if (c4 == 0 && p.lse != nullptr)
+      p.lse[b * p.sl[0] + h * p.sl[1] + i * p.sl[2]] =
+          sum > 0.f ? (m + __builtin_amdgcn_logf(sum) - Fp4<Tag>::kPBias) * 0.6931471805599453f : FA_NEG_INF;
   }
-  if (lane >= LPS) return;
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  *reinterpret_cast<u32x2*>(p.o + b * p.so[0] + h * p.so[1] + i * p.so[2] + 4 * c4) =
-      (u32x2){DT<Tag>::pack2(o[0] * inv, o[1] * inv), DT<Tag>::pack2(o[2] * inv, o[3] * inv)};
-  if (c4 == 0 && p.lse != nullptr)
-    p.lse[b * p.sl[0] + h * p.sl[1] + i * p.sl[2]] =
-        sum > 0.f ? (m + __builtin_amdgcn_logf(sum) - Fp4<Tag>::kPBias) * 0.6931471805599453f : FA_NEG_INF;
 }
 
 #define KV4_ENTRY(TAG, DTYPE, D)                                                                                   \
   {DTYPE, D, (const void*)&kv4_append_kernel<TAG>,                                                                 \
    {(const void*)&kv4_merge_kernel<TAG, D, 4>, (const void*)&kv4_merge_kernel<TAG, D, 1>},                         \
-   {(const void*)&kv4_attend_kernel<TAG, D, 1, true>, (const void*)&kv4_attend_kernel<TAG, D, 2, true>,            \
-    (const void*)&kv4_attend_kernel<TAG, D, (D == 256 ? 1 : 2), false>},                                           \
-   {attend_waves<D, 1>(), attend_waves<D, 2>(), attend_waves<D, (D == 256 ? 1 : 2)>()}, D == 256 ? 1 : 2}
+   {(const void*)&kv4_attend_kernel<TAG, D, 1>, (const void*)&kv4_attend_kernel<TAG, D, 2>,            \
+    (const void*)&kv4_chunk_kernel<TAG, D>},                                                                        \
+   {attend_waves<D, 1>(), attend_waves<D, 2>(), 2}, Kv4Chunk<TAG, D>::BLOCK}
 
 static const Kv4KernelEntry kKv4Entries[] = {
     KV4_ENTRY(f16_t, FA_DTYPE_F16, 64),   KV4_ENTRY(f16_t, FA_DTYPE_F16, 128),   KV4_ENTRY(f16_t, FA_DTYPE_F16, 256),
