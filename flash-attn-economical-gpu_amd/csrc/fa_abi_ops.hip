@@ -359,9 +359,9 @@ int kv4_attend(const kv4_attend_args* a, void* stream) {
   if ((code = launch(e->attend[k.kind], blocks, 1, 256, &p, stream, "cache attention")) != FA_OK) return code;
   if (a->splits > 1) {
     const int64_t all = (int64_t)c->B * a->H * a->M;
-    const bool wide = a->splits > 8;
+    const int how = a->splits > 32 ? 2 : (a->splits > 8 ? 1 : 0);
     const int64_t few = (all + 3) / 4 < 2048 ? (all + 3) / 4 : 2048;  // eight workgroups to a CU, a few rows to a wave
-    if ((code = launch(e->merge[wide ? 0 : 1], wide ? all : few, 1, 256, &p, stream, "cache merge")) != FA_OK)
+    if ((code = launch(e->merge[how], how > 0 ? all : few, 1, how == 2 ? 1024 : 256, &p, stream, "cache merge")) != FA_OK)
       return code;
   }
   return ok();

@@ -160,7 +160,7 @@ struct Kv4KernelEntry {
   int32_t dtype;
   int32_t D;
   const void* append;
-  const void* merge[2];   // a workgroup per row, a wave per row
+  const void* merge[3];   // one, four and sixteen waves to a row
   const void* attend[3];  // 16 rows shared by a workgroup's waves, 32 rows shared, chunks of a prompt
   int32_t per_cu[3];      // workgroups of each that a CU holds
   int32_t chunk_rows;     // query rows of a workgroup of the last

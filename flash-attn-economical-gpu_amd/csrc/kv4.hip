@@ -749,21 +749,21 @@ __global__ __launch_bounds__(256, 2) void kv4_chunk_kernel(Kv4AttendParams p) {
   Kv4Chunk<Tag, D>::run(p, smem);
 }
 
-// Joins the splits of a row: weights exp2(m_s - m) of the unnormalised partial sums. WPR waves take a row, four
-// where rows are few and splits many (single tokens), one where it is the other way round. D / 4 lanes read one
+// Joins the splits of a row: weights exp2(m_s - m) of the unnormalised partial sums. WPR waves take a row: one
+// where rows are many and splits few, four or sixteen the other way round (single tokens over long caches). D / 4 lanes read one
 // split's row, so a wave has 256 / D of them in flight at once, times the unrolling.
 template <typename Tag, int D, int WPR>
-__global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttendParams p) {
+__global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void kv4_merge_kernel(Kv4AttendParams p) {
   constexpr int LPS = D / 4, AT_ONCE = WPR * 64 / LPS;
   __shared__ floatx4 part_o[WPR][LPS];
   __shared__ float part_ml[WPR][2];
-  const int lane = threadIdx.x & 63, wave = WPR == 4 ? threadIdx.x >> 6 : 0;
+  const int lane = threadIdx.x & 63, wave = WPR > 1 ? threadIdx.x >> 6 : 0;
   const uint32_t rows = (uint32_t)p.B * p.H * p.M;
-  const uint32_t first = WPR == 4 ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 6);
+  const uint32_t first = WPR > 1 ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 6);
   Split part;
   int of = -1;  // the sequence that `part` is of
   // a workgroup per row, or so many waves that each takes a few rows
-  for (uint32_t row = __builtin_amdgcn_readfirstlane(first); row < rows; row += WPR == 4 ? rows : gridDim.x * 4) {
+  for (uint32_t row = __builtin_amdgcn_readfirstlane(first); row < rows; row += WPR > 1 ? rows : gridDim.x * 4) {
     const uint32_t bh = row / (uint32_t)p.M;
     const int i = (int)(row % (uint32_t)p.M), h = (int)(bh % (uint32_t)p.H), b = (int)(bh / (uint32_t)p.H);
     if (b != of) part = find_split(p, -1, of = b);
@@ -800,7 +800,7 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttendParams p) {
         part_ml[wave][1] = sum;
       }
       __syncthreads();
-      if (threadIdx.x >= LPS) return;  // WPR = 4 has one row
+      if (threadIdx.x >= LPS) return;  // there is no other row
       float top = FA_NEG_INF;
 #pragma unroll
       for (int w = 0; w < WPR; ++w) top = fmaxf(top, part_ml[w][0]);
@@ -828,7 +828,8 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttendParams p) {
 
 #define KV4_ENTRY(TAG, DTYPE, D)                                                                                   \
   {DTYPE, D, (const void*)&kv4_append_kernel<TAG>,                                                                 \
-   {(const void*)&kv4_merge_kernel<TAG, D, 4>, (const void*)&kv4_merge_kernel<TAG, D, 1>},                         \
+   {(const void*)&kv4_merge_kernel<TAG, D, 1>, (const void*)&kv4_merge_kernel<TAG, D, 4>,                         \
+    (const void*)&kv4_merge_kernel<TAG, D, 16>},                         \
    {(const void*)&kv4_attend_kernel<TAG, D, 1>, (const void*)&kv4_attend_kernel<TAG, D, 2>,            \
     (const void*)&kv4_chunk_kernel<TAG, D>},                                                                        \
    {attend_waves<D, 1>(), attend_waves<D, 2>(), 2}, Kv4Chunk<TAG, D>::BLOCK}
