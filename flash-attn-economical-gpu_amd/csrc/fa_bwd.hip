@@ -62,68 +62,88 @@ __global__ __launch_bounds__(256) void fa_bwd_prep_kernel(BwdParams p) {
   constexpr int RPP = 256 / LPR;      // rows per pass
   const int t = threadIdx.x, part = t % LPR, r0 = t / LPR;
   __shared__ float red[8];
-  const int qblocks = p.prep_blocks;
-  const int64_t nq = (int64_t)p.B * p.H * qblocks;
-  const int64_t id = blockIdx.x;
+  const uint32_t qblocks = p.prep_blocks, nq = (uint32_t)p.B * p.H * qblocks, id = blockIdx.x;
+  constexpr int NP = kPrepRows / RPP < 4 ? kPrepRows / RPP : 4;  // passes whose loads are issued together
   float top = 0.f, topd = 0.f;
   if (id < nq) {
-    const int64_t bh = id / qblocks;
-    const int blk = (int)(id % qblocks);
-    const int b = (int)(bh / p.H), h = (int)(bh % p.H);
-    for (int i = r0; i < kPrepRows; i += RPP) {
-      const int row = blk * kPrepRows + i;
-      float dot = 0.f, sq = 0.f;
-      if (row < p.M) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(p.o + b * p.so[0] + h * p.so[1] + row * p.so[2] + part * 8);
-        const u32x4 y = *reinterpret_cast<const u32x4*>(p.dout + b * p.sdo[0] + h * p.sdo[1] + row * p.sdo[2] + part * 8);
+    const uint32_t bh = id / qblocks;
+    const int blk = (int)(id % qblocks), b = (int)(bh / (uint32_t)p.H), h = (int)(bh % (uint32_t)p.H);
+    const uint16_t* ob = p.o + b * p.so[0] + h * p.so[1] + part * 8;
+    const uint16_t* gb = p.dout + b * p.sdo[0] + h * p.sdo[1] + part * 8;
+#pragma unroll 1
+    for (int at = r0; at < kPrepRows; at += NP * RPP) {
+      u32x4 x[NP], y[NP];
+      float lse[NP], dlse[NP];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float y0 = DT<Tag>::to_float((uint16_t)y[j]), y1 = DT<Tag>::to_float((uint16_t)(y[j] >> 16));
-          dot += DT<Tag>::to_float((uint16_t)x[j]) * y0;
-          dot += DT<Tag>::to_float((uint16_t)(x[j] >> 16)) * y1;
-          sq += y0 * y0;
-          sq += y1 * y1;
+      for (int i = 0; i < NP; ++i) {
+        const int row = blk * kPrepRows + at + i * RPP;
+        x[i] = y[i] = (u32x4){0, 0, 0, 0};
+        lse[i] = FA_NEG_INF;
+        dlse[i] = 0.f;
+        if (row < p.M) {
+          if (part == 0) {
+            lse[i] = p.lse[b * p.sl[0] + h * p.sl[1] + row * p.sl[2]];
+            if (p.dlse != nullptr) dlse[i] = p.dlse[b * p.sdl[0] + h * p.sdl[1] + row * p.sdl[2]];
+          }
+          x[i] = *reinterpret_cast<const u32x4*>(ob + row * p.so[2]);
+          y[i] = *reinterpret_cast<const u32x4*>(gb + row * p.sdo[2]);
         }
       }
 #pragma unroll
-      for (int s = 1; s < LPR; s *= 2) {
-        dot += __shfl_xor(dot, s, 64);
-        sq += __shfl_xor(sq, s, 64);
-      }
-      float nl = FA_NEG_INF;
-      if (row < p.M) {
-        const float lse = p.lse[b * p.sl[0] + h * p.sl[1] + row * p.sl[2]];
-        if (p.dlse != nullptr) dot -= p.dlse[b * p.sdl[0] + h * p.sdl[1] + row * p.sdl[2]];
-        nl = lse == FA_NEG_INF ? FA_NEG_INF : BwdTraits<Tag>::kPBias - lse * 1.4426950408889634f;
-      }
-      if (part == 0) {
-        float* nd = p.nd + nd_index(p, bh, row);
-        nd[0] = nl;
-        nd[32] = -dot;
-      }
-      if ((__float_as_uint(sq) & 0x7fffffffu) < 0x7f800000u) top = fmaxf(top, sq);
-      if ((__float_as_uint(dot) & 0x7fffffffu) < 0x7f800000u) topd = fmaxf(topd, fabsf(dot));
-    }
-  } else {
-    const int64_t v = id - nq;
-    const int64_t bh = v / p.vblocks;
-    const int blk = (int)(v % p.vblocks);
-    const int b = (int)(bh / p.Hkv), h = (int)(bh % p.Hkv);
-    for (int i = r0; i < kPrepRows; i += RPP) {
-      const int row = blk * kPrepRows + i;
-      float sq = 0.f;
-      if (row < p.N) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(p.v + b * p.sv[0] + h * p.sv[1] + row * p.sv[2] + part * 8);
+      for (int i = 0; i < NP; ++i) {
+        const int row = blk * kPrepRows + at + i * RPP;
+        float dot = 0.f, sq = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float x0 = DT<Tag>::to_float((uint16_t)x[j]), x1 = DT<Tag>::to_float((uint16_t)(x[j] >> 16));
+          const float y0 = DT<Tag>::to_float((uint16_t)y[i][j]), y1 = DT<Tag>::to_float((uint16_t)(y[i][j] >> 16));
+          dot += DT<Tag>::to_float((uint16_t)x[i][j]) * y0;
+          dot += DT<Tag>::to_float((uint16_t)(x[i][j] >> 16)) * y1;
+          if constexpr (BwdTraits<Tag>::kScaled) {
+            sq += y0 * y0;
+            sq += y1 * y1;
+          }
+        }
+#pragma unroll
+        for (int s = 1; s < LPR; s *= 2) {
+          dot += __shfl_xor(dot, s, 64);
+          if constexpr (BwdTraits<Tag>::kScaled) sq += __shfl_xor(sq, s, 64);
+        }
+        if (part == 0) {
+          dot -= dlse[i];
+          float* nd = p.nd + nd_index(p, bh, row);
+          nd[0] = lse[i] == FA_NEG_INF ? FA_NEG_INF : BwdTraits<Tag>::kPBias - lse[i] * 1.4426950408889634f;
+          nd[32] = -dot;
+        }
+        if ((__float_as_uint(sq) & 0x7fffffffu) < 0x7f800000u) top = fmaxf(top, sq);
+        if ((__float_as_uint(dot) & 0x7fffffffu) < 0x7f800000u) topd = fmaxf(topd, fabsf(dot));
+      }
+    }
+  } else {
+    const uint32_t v = id - nq, bh = v / (uint32_t)p.vblocks;
+    const int blk = (int)(v % (uint32_t)p.vblocks), b = (int)(bh / (uint32_t)p.Hkv), h = (int)(bh % (uint32_t)p.Hkv);
+    const uint16_t* vb = p.v + b * p.sv[0] + h * p.sv[1] + part * 8;
+#pragma unroll 1
+    for (int at = r0; at < kPrepRows; at += NP * RPP) {
+      u32x4 x[NP];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int row = blk * kPrepRows + at + i * RPP;
+        x[i] = (u32x4){0, 0, 0, 0};
+        if (row < p.N) x[i] = *reinterpret_cast<const u32x4*>(vb + row * p.sv[2]);
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        float sq = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x0 = DT<Tag>::to_float((uint16_t)x[i][j]), x1 = DT<Tag>::to_float((uint16_t)(x[i][j] >> 16));
           sq += x0 * x0;
           sq += x1 * x1;
         }
-      }
 #pragma unroll
-      for (int s = 1; s < LPR; s *= 2) sq += __shfl_xor(sq, s, 64);
-      if ((__float_as_uint(sq) & 0x7fffffffu) < 0x7f800000u) top = fmaxf(top, sq);
+        for (int s = 1; s < LPR; s *= 2) sq += __shfl_xor(sq, s, 64);
+        if ((__float_as_uint(sq) & 0x7fffffffu) < 0x7f800000u) top = fmaxf(top, sq);
+      }
     }
   }
   if constexpr (BwdTraits<Tag>::kScaled) {
@@ -142,9 +162,9 @@ __global__ __launch_bounds__(256) void fa_bwd_prep_kernel(BwdParams p) {
       const float d = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
       if (id < nq) {
         p.bound[id] = a;
-        p.bound[nq + id] = d;
+        p.bound[(int64_t)nq + id] = d;
       } else {
-        p.bound[2 * nq + (id - nq)] = a;
+        p.bound[(int64_t)nq + id] = a;
       }
     }
   }
