@@ -584,16 +584,27 @@ struct Bwd : LdsRows<D> {
   }
 };
 
-// dK/dV blocks first (they are the longer ones), then dQ blocks, in one grid: small problems fill more of
-// the chip, large ones drain together.
+// dK/dV blocks first (they are the longer ones), then dQ blocks, in one grid, each kind in runs that keep a head's
+// blocks on one XCD. Grids small enough to be split alternate the two kinds in proportion instead: the working
+// set fits the L2 either way, and blocks of unlike lengths run side by side (bf16 B1 12/2 heads N4096 D128 causal
+// 298 -> 272 us; large grids lose 3 to 5% by it, for L2 misses).
 template <typename Tag, int D, int KT, int PER_CU>
 __global__ __launch_bounds__(256, PER_CU) void fa_bwd_kernel(BwdParams p) {
   __shared__ __align__(1024) char smem[Bwd<Tag, D, KT>::SMEM];
-  const int id = blockIdx.x;
-  if (id < p.kv_total)
-    Bwd<Tag, D, KT>::dkdv(p, smem, xcd_remap(id, p.kv_total));
+  const uint32_t id = blockIdx.x;
+  bool is_kv = id < (uint32_t)p.kv_total;
+  int block = is_kv ? xcd_remap(id, p.kv_total) : xcd_remap(id - p.kv_total, p.q_total);
+  if (p.kv_splits * p.q_splits > 1 && p.kv_total % 8 == 0 && p.q_total % 8 == 0) {
+    const uint32_t kv = (uint32_t)p.kv_total / 8, q = (uint32_t)p.q_total / 8, xcd = id % 8, slot = id / 8;
+    const uint32_t before = (uint32_t)((uint64_t)slot * kv / (kv + q));  // dK/dV blocks of the XCD ahead of this slot
+    is_kv = (uint32_t)((uint64_t)(slot + 1) * kv / (kv + q)) > before;
+    block = is_kv ? xcd * kv + before : xcd * q + (slot - before);
+  }
+  block = __builtin_amdgcn_readfirstlane(block);
+  if (is_kv)
+    Bwd<Tag, D, KT>::dkdv(p, smem, block);
   else
-    Bwd<Tag, D, KT>::dq(p, smem, xcd_remap(id - p.kv_total, p.q_total));
+    Bwd<Tag, D, KT>::dq(p, smem, block);
 }
 
 // Sums of the splits' partial gradients, in split order: a thread takes four channels of one row.
