@@ -375,25 +375,33 @@ def sdpa_kv4(query: torch.Tensor, cache: kv4.Kv4Cache, start: torch.Tensor, *, c
     see nothing come out as zeros, their lse as -inf. H is a multiple of the cache's heads. M = 1 is a decode
     step, a few rows a draft being checked, many a chunk of a prompt. start and count are int32 [B] on the GPU;
     nothing synchronises, and the call can be captured into a HIP graph. The result has `sdpa`'s layout."""
-    if query.dim() != 4:
-        raise ValueError(f"query must be 4-D [batch, heads, seq, head_dim], got {tuple(query.shape)}")
+    key = ("kv4", cache._form, _form(query), kv4._form(start), None if count is None else kv4._form(count), bool(is_causal),
+           None if scale is None else float(scale), bool(return_lse))
+    plan = _plans.get(key)
+    checked = plan is not None and not query.data_ptr() & 15
+    if not checked:
+        if query.dim() != 4:
+            raise ValueError(f"query must be 4-D [batch, heads, seq, head_dim], got {tuple(query.shape)}")
+        B, H, M, D = query.shape
+        if B != cache.batch or D != cache.head_dim or H < 1 or H % cache.kv_heads:
+            raise ValueError(f"query {tuple(query.shape)} does not fit a cache of {cache.batch} sequences, {cache.kv_heads} "
+                             f"heads of {cache.head_dim}")
+        if query.dtype != cache.dtype or query.device != cache.device:
+            raise ValueError(f"query is {query.dtype} on {query.device}, the cache {cache.dtype} on {cache.device}")
+        start, count = cache.positions(start, count)
+        query = hip_lib.operand(query, "query")
     B, H, M, D = query.shape
-    if B != cache.batch or D != cache.head_dim or H < 1 or H % cache.kv_heads:
-        raise ValueError(f"query {tuple(query.shape)} does not fit a cache of {cache.batch} sequences, {cache.kv_heads} "
-                         f"heads of {cache.head_dim}")
-    if query.dtype != cache.dtype or query.device != cache.device:
-        raise ValueError(f"query is {query.dtype} on {query.device}, the cache {cache.dtype} on {cache.device}")
-    if start is None:
-        raise ValueError("start is required")
-    start, count = (kv4._positions(t, name, B, cache.device) for name, t in (("start", start), ("count", count)))
-    query = hip_lib.operand(query, "query")
     o = torch.empty_strided((B, H, M, D), (max(M, 1) * H * D, D, H * D, 1), device=query.device, dtype=query.dtype)
     lse = torch.empty(B, H, M, device=query.device, dtype=torch.float32) if return_lse else None
-    splits = kv4.choose_splits(B, H, cache.kv_heads, M, D, cache.capacity)
-    need = hip_lib.kv4_attend_workspace_bytes(B, H, M, D, splits)
-    workspace = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
-    hip_lib.kv4_attend(cache._args, query, o, lse, workspace, start, count, sm_scale=D ** -0.5 if scale is None else scale,
-                       causal=is_causal, splits=splits)
+    if not checked:
+        splits = kv4.choose_splits(B, H, cache.kv_heads, M, D, cache.capacity)
+        plan = (hip_lib.kv4_attend_plan(query, o, lse, sm_scale=D ** -0.5 if scale is None else scale, causal=is_causal,
+                                        splits=splits),
+                hip_lib.kv4_attend_workspace_bytes(B, H, M, D, splits))
+        if key[2:5] == (_form(query), kv4._form(start), None if count is None else kv4._form(count)):
+            _keep_plan(key, plan)  # nothing had to be copied: calls of this form take the short way
+    workspace = torch.empty(plan[1], dtype=torch.uint8, device=query.device) if plan[1] else None
+    hip_lib.kv4_attend_planned(plan[0], cache._args, query, o, lse, workspace, start, count)
     return (o, lse) if return_lse else o
 
 

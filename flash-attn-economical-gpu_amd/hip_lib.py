@@ -558,7 +558,7 @@ def _launch(fn, args, device: torch.device, what: str) -> None:
     """One C entry on the tensors' device and its current stream."""
     index = device.index
     if index == torch.cuda.current_device():
-        code = fn(ctypes.byref(args), _stream_ptr(device))
+        code = fn(ctypes.byref(args), _raw_stream(index) if _raw_stream is not None else _stream_ptr(device))
     else:
         with torch.cuda.device(index):
             code = fn(ctypes.byref(args), _stream_ptr(device))
@@ -621,37 +621,51 @@ def kv4_attend_workspace_bytes(B: int, H: int, M: int, D: int, splits: int) -> i
     return int(load().kv4_attend_workspace_bytes(B, H, M, D, splits))
 
 
-def kv4_append(cache: Kv4CacheArgs, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, count: torch.Tensor | None,
-               k_values: torch.Tensor | None, v_values: torch.Tensor | None) -> None:
-    """Append rows to a 4-bit cache on the current stream; the caller has matched the tensors to the cache."""
+def kv4_append_plan(k: torch.Tensor, v: torch.Tensor, k_values: torch.Tensor | None, v_values: torch.Tensor | None) -> bytes:
+    """kv4_append's argument block for these tensors' shapes and strides (no address in it is used)."""
     args = Kv4AppendArgs()
+    args.k_stride, args.v_stride = _strides4_of(k), _strides4_of(v)
+    if k_values is not None:
+        args.k_values_stride, args.v_values_stride = _strides4_of(k_values), _strides4_of(v_values)
+    args.rows = k.shape[2]
+    return bytes(args)
+
+
+def kv4_append_planned(plan: bytes, cache: Kv4CacheArgs, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor,
+                       count: torch.Tensor | None, k_values: torch.Tensor | None, v_values: torch.Tensor | None) -> None:
+    """Append rows to a 4-bit cache on the current stream; the caller has matched the tensors to cache and plan."""
+    args = Kv4AppendArgs.from_buffer_copy(plan)
     args.cache = cache
     args.k, args.v, args.start = k.data_ptr(), v.data_ptr(), start.data_ptr()
     if count is not None:
         args.count = count.data_ptr()
-    args.k_stride, args.v_stride = _strides4_of(k), _strides4_of(v)
     if k_values is not None:
         args.k_values, args.v_values = k_values.data_ptr(), v_values.data_ptr()
-        args.k_values_stride, args.v_values_stride = _strides4_of(k_values), _strides4_of(v_values)
-    args.rows = k.shape[2]
     _launch(load().kv4_append, args, k.device, "kv4_append")
 
 
-def kv4_attend(cache: Kv4CacheArgs, q: torch.Tensor, o: torch.Tensor, lse: torch.Tensor | None,
-               workspace: torch.Tensor | None, start: torch.Tensor, count: torch.Tensor | None, *, sm_scale: float,
-               causal: bool, splits: int) -> None:
-    """Attention over a 4-bit cache on the current stream; the caller has matched the tensors to the cache."""
+def kv4_attend_plan(q: torch.Tensor, o: torch.Tensor, lse: torch.Tensor | None, *, sm_scale: float, causal: bool,
+                    splits: int) -> bytes:
+    """kv4_attend's argument block for these tensors' shapes and strides (no address in it is used)."""
     args = Kv4AttendArgs()
+    if lse is not None:
+        args.lse_stride = (ctypes.c_int64 * 3)(*lse.stride())
+    args.q_stride, args.o_stride = _strides4_of(q), _strides4_of(o)
+    args.H, args.M = q.shape[1], q.shape[2]
+    args.sm_scale, args.causal, args.splits = float(sm_scale), int(bool(causal)), int(splits)
+    return bytes(args)
+
+
+def kv4_attend_planned(plan: bytes, cache: Kv4CacheArgs, q: torch.Tensor, o: torch.Tensor, lse: torch.Tensor | None,
+                       workspace: torch.Tensor | None, start: torch.Tensor, count: torch.Tensor | None) -> None:
+    """Attention over a 4-bit cache on the current stream; the caller has matched the tensors to cache and plan."""
+    args = Kv4AttendArgs.from_buffer_copy(plan)
     args.cache = cache
     args.q, args.o, args.start = q.data_ptr(), o.data_ptr(), start.data_ptr()
     if count is not None:
         args.count = count.data_ptr()
     if lse is not None:
         args.lse = lse.data_ptr()
-        args.lse_stride = (ctypes.c_int64 * 3)(*lse.stride())
     if workspace is not None:
         args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.numel()
-    args.q_stride, args.o_stride = _strides4_of(q), _strides4_of(o)
-    args.H, args.M = q.shape[1], q.shape[2]
-    args.sm_scale, args.causal, args.splits = float(sm_scale), int(bool(causal)), int(splits)
     _launch(load().kv4_attend, args, q.device, "kv4_attend")

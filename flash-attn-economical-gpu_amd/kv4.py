@@ -24,13 +24,21 @@ import hip_lib
 BLOCK = 32  # channels that share a scale
 
 
-def _positions(t: torch.Tensor | None, name: str, B: int, device: torch.device) -> torch.Tensor | None:
-    if t is None:
-        return None
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or tuple(t.shape) != (B,) or t.device != device:
-        got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
-        raise ValueError(f"{name} must be an int32 tensor [{B}] on {device}, got {got}")
-    return t.contiguous()
+# Argument blocks by the values they depend on (shapes, strides, types, devices, flags): the checks and filling a
+# block field by field are most of a call's host time, which single-token calls would wait for. No tensor or
+# address is kept.
+_plans: dict[tuple, object] = {}
+_MAX_PLANS = 4096
+
+
+def keep_plan(key: tuple, plan) -> None:
+    if len(_plans) >= _MAX_PLANS:
+        _plans.clear()
+    _plans[key] = plan
+
+
+def _form(t) -> tuple:
+    return (t.shape, t.stride(), t.dtype, t.device) if isinstance(t, torch.Tensor) else (type(t),)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -65,6 +73,7 @@ class Kv4Cache:
         c.scale_stride = (ctypes.c_int64 * 2)(*full[1].stride()[:2])
         c.B, c.H_kv, c.D, c.dtype = batch, kv_heads, head_dim, hip_lib.dtype_code(dtype)
         c.rows, c.capacity = rows, capacity
+        self._form = (batch, kv_heads, capacity, head_dim, dtype, self.device)
 
     # The buffers, [batch, kv heads, capacity, bytes] (two codes to a byte, channel 2i in the low half of byte
     # i; scale byte e stands for 2^(e - 127), 255 for NaN). They may be written in place, not replaced.
@@ -93,19 +102,42 @@ class Kv4Cache:
         start[b] + t. Rows outside the capacity are dropped; what is not written stays as it is. With
         return_values, returns what the rows now stand for (zeros in rows that were not written), in k's type,
         for a layer that goes on with the values its later steps will see."""
+        key = (self._form, _form(k), _form(v), _form(start), None if count is None else _form(count), bool(return_values))
+        plan = _plans.get(key)
+        if plan is None or (k.data_ptr() | v.data_ptr()) & 15:
+            k, v, start, count = self._append_operands(k, v, start, count)
+            values = (torch.empty_like(k), torch.empty_like(v)) if return_values else (None, None)
+            plan = hip_lib.kv4_append_plan(k, v, *values)
+            if key == (self._form, _form(k), _form(v), _form(start), None if count is None else _form(count),
+                       bool(return_values)):  # nothing had to be copied: calls of this form take the short way
+                keep_plan(key, plan)
+        else:
+            values = (torch.empty_like(k), torch.empty_like(v)) if return_values else (None, None)
+        hip_lib.kv4_append_planned(plan, self._args, k, v, start, count, *values)
+        return values if return_values else None
+
+    def _append_operands(self, k, v, start, count):
+        """append's arguments, checked, and copied where the kernels cannot read them as they lie."""
         shape = (self.batch, self.kv_heads, k.shape[2] if k.dim() == 4 else -1, self.head_dim)
         for name, t in (("k", k), ("v", v)):
             if tuple(t.shape) != shape or t.dtype != self.dtype or t.device != self.device:
                 raise ValueError(f"{name} must be {self.dtype} [{self.batch}, {self.kv_heads}, rows, {self.head_dim}] on "
                                  f"{self.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-        start = _positions(start, "start", self.batch, self.device)
-        count = _positions(count, "count", self.batch, self.device)
-        if start is None:
-            raise ValueError("start is required")
-        k, v = hip_lib.operand(k, "k"), hip_lib.operand(v, "v")
-        values = (torch.empty_like(k), torch.empty_like(v)) if return_values else (None, None)
-        hip_lib.kv4_append(self._args, k, v, start, count, *values)
-        return values if return_values else None
+        start, count = self.positions(start, count)
+        return hip_lib.operand(k, "k"), hip_lib.operand(v, "v"), start, count
+
+    def positions(self, start: torch.Tensor, count: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor | None]:
+        """start and count as the kernels read them; ValueError if they are anything but int32 [batch] here."""
+        out = []
+        for name, t in (("start", start), ("count", count)):
+            if t is None and name == "count":
+                out.append(None)
+                continue
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or tuple(t.shape) != (self.batch,) or t.device != self.device:
+                got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+                raise ValueError(f"{name} must be an int32 tensor [{self.batch}] on {self.device}, got {got}")
+            out.append(t.contiguous())
+        return out[0], out[1]
 
 
 __all__ = ["BLOCK", "Kv4Cache", "choose_splits"]

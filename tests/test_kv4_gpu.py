@@ -211,6 +211,7 @@ def test_any_number_of_splits(gpu, monkeypatch, splits, M):
     q = _rand(41, B, H, M, D, dtype=BF16).cuda()
     starts = [capacity - M, 700]
     monkeypatch.setattr(kv4, "choose_splits", lambda *a: splits)
+    monkeypatch.setattr(flash_atten, "_plans", {})
     o, lse = flash_atten.sdpa_kv4(q, cache, _i32(*starts), scale=0.2, return_lse=True)
     _check(o, lse, *_attention(q, *_held(cache), starts, [M] * B, True, 0.2, BF16), (splits, M))
 
