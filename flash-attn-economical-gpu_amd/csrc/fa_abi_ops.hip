@@ -52,7 +52,8 @@ int check_tensor(const char* name, const void* ptr, const int64_t* stride, int D
 }
 
 int check_scale(float scale) {
-  if (!std::isfinite(scale) || scale <= 0.f) return fail(FA_EINVAL, "sm_scale must be positive and finite, got %g", (double)scale);
+  if (!std::isfinite(scale * 1.4426950408889634f) || scale <= 0.f)
+    return fail(FA_EINVAL, "sm_scale must be positive and finite, got %g", (double)scale);
   return FA_OK;
 }
 
@@ -113,6 +114,8 @@ int check_cache(const kv4_cache* c) {
   if (code != FA_OK) return code;
   if (c->B < 0 || c->H_kv <= 0 || c->capacity < 0)
     return fail(FA_EINVAL, "invalid cache sizes B=%d H_kv=%d capacity=%d", c->B, c->H_kv, c->capacity);
+  if (c->capacity > KV4_MAX_CAPACITY)
+    return fail(FA_ENOTSUP, "cache capacity %d is beyond %d", c->capacity, KV4_MAX_CAPACITY);
   if (c->rows % 32 || c->rows < c->capacity)
     return fail(FA_EINVAL, "cache rows=%d must be a multiple of 32 and at least the capacity %d", c->rows, c->capacity);
   if (c->B == 0 || c->capacity == 0) return FA_OK;

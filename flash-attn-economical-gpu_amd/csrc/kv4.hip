@@ -391,14 +391,14 @@ struct Kv4Attend {
         p.ws_ml[2 * w + 1] = l;
       }
     } else {
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
       uint16_t* dst = p.o + b * p.so[0] + h * p.so[1] + i * p.so[2] + at * N;
 #pragma unroll
       for (int j = 0; j < N; j += 4)
         *reinterpret_cast<u32x2*>(dst + j) = (u32x2){E::pack2(o[j] * inv, o[j + 1] * inv), E::pack2(o[j + 2] * inv, o[j + 3] * inv)};
       if (at == 0 && p.lse != nullptr)
         p.lse[b * p.sl[0] + h * p.sl[1] + i * p.sl[2]] =
-            l > 0.f ? (m * p.c + __builtin_amdgcn_logf(l) - Fp4<Tag>::kPBias) * 0.6931471805599453f : FA_NEG_INF;
+            l == 0.f ? FA_NEG_INF : (m * p.c + __builtin_amdgcn_logf(l) - Fp4<Tag>::kPBias) * 0.6931471805599453f;
     }
   }
 
@@ -729,7 +729,7 @@ struct Kv4Chunk {
           p.ws_ml[2 * w + 1] = sum;
         }
       } else {
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
         uint16_t* dst = p.o + b * p.so[0] + h * p.so[1] + i * p.so[2] + 4 * g;
 #pragma unroll
         for (int d = 0; d < DT16; ++d)
@@ -737,7 +737,7 @@ struct Kv4Chunk {
               (u32x2){E::pack2(o[d][j][0] * inv, o[d][j][1] * inv), E::pack2(o[d][j][2] * inv, o[d][j][3] * inv)};
         if (g == 0 && p.lse != nullptr)
           p.lse[b * p.sl[0] + h * p.sl[1] + i * p.sl[2]] =
-              sum > 0.f ? (m[j] * p.c + __builtin_amdgcn_logf(sum) - Fp4<Tag>::kPBias) * 0.6931471805599453f : FA_NEG_INF;
+              sum == 0.f ? FA_NEG_INF : (m[j] * p.c + __builtin_amdgcn_logf(sum) - Fp4<Tag>::kPBias) * 0.6931471805599453f;
       }
     }
   }
@@ -817,12 +817,12 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void kv4_merge_kernel(Kv4At
       m = top;
     }
     if (lane >= LPS) continue;
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     *reinterpret_cast<u32x2*>(p.o + b * p.so[0] + h * p.so[1] + i * p.so[2] + 4 * c4) =
         (u32x2){DT<Tag>::pack2(o[0] * inv, o[1] * inv), DT<Tag>::pack2(o[2] * inv, o[3] * inv)};
     if (c4 == 0 && p.lse != nullptr)
       p.lse[b * p.sl[0] + h * p.sl[1] + i * p.sl[2]] =
-          sum > 0.f ? (m + __builtin_amdgcn_logf(sum) - Fp4<Tag>::kPBias) * 0.6931471805599453f : FA_NEG_INF;
+          sum == 0.f ? FA_NEG_INF : (m + __builtin_amdgcn_logf(sum) - Fp4<Tag>::kPBias) * 0.6931471805599453f;
   }
 }
 

@@ -4,7 +4,8 @@ variant (split-KV + LSE merge, GQA heads packed per kv head).
 Decode reads every K/V element once and does ~2 FLOP per element per query head, so the bound is
 HBM bandwidth: algorithmic bytes = |K| + |V| + |Q| + |O| (+ the fp32 split partials the merge pass
 reads back, reported separately), peak 8 TB/s. torch's scaled_dot_product_attention (its default
-ROCm backend, GQA via enable_gqa) on the same inputs is timed beside it.
+ROCm backend, GQA via enable_gqa) on the same inputs is timed beside it, and the same step over a 4-bit cache
+(`kv4.Kv4Cache`, 17/64 of the bytes) that holds the same keys and values.
 
 Usage: python decode_bench.py [--json out.json]
 """
@@ -19,6 +20,7 @@ import torch
 import torch.nn.functional as F
 
 import flash_atten
+import kv4
 
 HBM_PEAK_GBS = 8000.0
 
@@ -94,6 +96,11 @@ def run_case(label, B, H, Hkv, M, N, D, dtype, seed: int = 0) -> dict:
     ms_graph, out_graph = _time_graph(ours)
     graph_diff = (out_graph.float() - out.float()).abs().max().item()
     ms_torch = _time(lambda: F.scaled_dot_product_attention(q, k, v, scale=D ** -0.5, enable_gqa=True))
+    cache = kv4.Kv4Cache(B, Hkv, N, D, dtype=dtype, device=dev)
+    cache.append(k, v, torch.zeros(B, dtype=torch.int32, device=dev))
+    start = torch.full((B,), N - M, dtype=torch.int32, device=dev)
+    ms_kv4, out_kv4 = _time_graph(lambda: flash_atten.sdpa_kv4(q, cache, start, is_causal=False))
+    kv4_rel = ((out_kv4.float() - ref.float()).norm() / ref.float().norm()).item()
     elt = q.element_size()
     kv_bytes = 2 * B * Hkv * N * D * elt
     io_bytes = kv_bytes + 2 * B * H * M * D * elt
@@ -105,12 +112,16 @@ def run_case(label, B, H, Hkv, M, N, D, dtype, seed: int = 0) -> dict:
         "hbm_frac": round(io_bytes / ms / 1e6 / HBM_PEAK_GBS, 4), "TFLOPs": round(flops / ms / 1e9, 1),
         "ms_graph": round(ms_graph, 4), "GBs_graph": round(io_bytes / ms_graph / 1e6, 1),
         "hbm_frac_graph": round(io_bytes / ms_graph / 1e6 / HBM_PEAK_GBS, 4), "graph_vs_eager_max_abs": graph_diff,
-        "max_abs_vs_torch": err,
+        "max_abs_vs_torch": err, "ms_kv4_graph": round(ms_kv4, 4), "kv4_speedup_graph": round(ms_graph / ms_kv4, 2),
+        "kv4_GBs_graph": round((cache.nbytes() + 2 * B * H * M * D * elt) / ms_kv4 / 1e6, 1),
+        "kv4_rel_diff": round(kv4_rel, 4),
     }
     print(f"[decode] {label}: {ms:.4f} ms = {row['GBs']:.0f} GB/s ({100 * row['hbm_frac']:.1f}% of 8 TB/s); "
           f"graph replay {ms_graph:.4f} ms = {row['GBs_graph']:.0f} GB/s ({100 * row['hbm_frac_graph']:.1f}%); "
-          f"torch SDPA {ms_torch:.4f} ms ({row['speedup_vs_torch']:.2f}x), max|diff|={err:.2e}", flush=True)
-    del q, k, v, out, ref, out_graph
+          f"torch SDPA {ms_torch:.4f} ms ({row['speedup_vs_torch']:.2f}x), max|diff|={err:.2e}; "
+          f"4-bit cache {ms_kv4:.4f} ms ({row['kv4_speedup_graph']:.2f}x the graph replay, {row['kv4_GBs_graph']:.0f} GB/s)",
+          flush=True)
+    del q, k, v, out, ref, out_graph, cache, out_kv4
     torch.cuda.empty_cache()
     return row
 

@@ -310,7 +310,7 @@ def attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: to
     operand's layout. Repeated calls give the same bits; nothing synchronises, and the call can be captured
     into a HIP graph."""
     do, q, k, v, o = (hip_lib.operand(t, name) for name, t in (("do", do), ("q", q), ("k", k), ("v", v), ("o", o)))
-    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    dq, dk, dv = hip_lib.dense_like(q), hip_lib.dense_like(k), hip_lib.dense_like(v)
     key = ("backward", _form(do), _form(q), _form(k), _form(v), _form(o), _form(lse),
            None if dlse is None else _form(dlse), bool(causal), None if sm_scale is None else float(sm_scale))
     plan = _plans.get(key)
@@ -339,7 +339,8 @@ class _Attention(torch.autograd.Function):
             plan = (hip_lib.fwd_plan(q, k, v, o, lse, sm_scale=D ** -0.5 if sm_scale is None else sm_scale, causal=causal,
                                      variant=hip_lib.FA_VARIANT_OPT, tile=tile.to_c()),)
             _keep_plan(key, plan)
-        hip_lib.fa_fwd_planned(plan[0], q, k, v, o, lse, None, q.device.index)
+        with torch.cuda.device(q.device):
+            hip_lib.fa_fwd_planned(plan[0], q, k, v, o, lse, None, q.device.index)
         ctx.save_for_backward(q, k, v, o, lse)
         ctx.causal, ctx.sm_scale = causal, sm_scale
         ctx.set_materialize_grads(False)
@@ -361,7 +362,15 @@ def differentiable_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
                              sm_scale: float | None = None, return_lse: bool = False):
     """Attention for training: the optimized forward, whose result takes part in autograd (both o and, with
     return_lse, the log-sum-exp). q [B, H, M, D] and k/v [B, H_kv, N, D] are read through their strides; o is a
-    [B, H, M, D] view of memory laid out [B, M, H, D], as from `sdpa`. First derivatives only."""
+    [B, H, M, D] view of memory laid out [B, M, H, D], as from `sdpa`. First derivatives only. A training step
+    that is captured into a HIP graph uses `attention(..., return_lse=True)` and `attention_backward`: this function
+    refuses a capture with gradients."""
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad) and q.is_cuda
+            and torch.cuda.is_current_stream_capturing()):
+        # autograd waits for the streams of leaves that an eager graph has used; inside a capture that wait can end
+        # the process, and whether such a graph lives cannot be seen from here
+        raise RuntimeError("differentiable_attention is not captured into a HIP graph: capture attention(..., "
+                           "return_lse=True) and attention_backward")
     o, lse = _Attention.apply(q, k, v, bool(causal), None if sm_scale is None else float(sm_scale))
     return (o, lse) if return_lse else o
 

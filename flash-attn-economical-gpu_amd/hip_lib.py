@@ -547,6 +547,12 @@ def operand(t: torch.Tensor, name: str) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def dense_like(t: torch.Tensor) -> torch.Tensor:
+    """An empty tensor of t's shape, in t's order of dimensions where that leaves D innermost."""
+    out = torch.empty_like(t)
+    return out if out.stride(3) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _strides4_of(t: torch.Tensor):
     """Strides with those of dimensions of size 1, which are never used, replaced by valid ones."""
     B, H, S, D = t.shape

@@ -22,6 +22,7 @@ import torch
 import hip_lib
 
 BLOCK = 32  # channels that share a scale
+MAX_CAPACITY = 1 << 30  # KV4_MAX_CAPACITY in include/fa_gfx950.h
 
 
 # Argument blocks by the values they depend on (shapes, strides, types, devices, flags): the checks and filling a
@@ -58,6 +59,8 @@ class Kv4Cache:
             raise hip_lib.FaUnsupportedError(f"head dim {head_dim} is not built (64, 128, 256)")
         if batch < 0 or kv_heads < 1 or capacity < 1:
             raise ValueError(f"invalid cache sizes batch={batch} kv_heads={kv_heads} capacity={capacity}")
+        if capacity > MAX_CAPACITY:
+            raise hip_lib.FaUnsupportedError(f"capacity {capacity} is beyond {MAX_CAPACITY}")
         device = torch.device(device)
         if device.type != "cuda":
             raise ValueError(f"a 4-bit cache lives on a GPU, got device {device}")
@@ -106,13 +109,13 @@ class Kv4Cache:
         plan = _plans.get(key)
         if plan is None or (k.data_ptr() | v.data_ptr()) & 15:
             k, v, start, count = self._append_operands(k, v, start, count)
-            values = (torch.empty_like(k), torch.empty_like(v)) if return_values else (None, None)
+            values = (hip_lib.dense_like(k), hip_lib.dense_like(v)) if return_values else (None, None)
             plan = hip_lib.kv4_append_plan(k, v, *values)
             if key == (self._form, _form(k), _form(v), _form(start), None if count is None else _form(count),
                        bool(return_values)):  # nothing had to be copied: calls of this form take the short way
                 keep_plan(key, plan)
         else:
-            values = (torch.empty_like(k), torch.empty_like(v)) if return_values else (None, None)
+            values = (hip_lib.dense_like(k), hip_lib.dense_like(v)) if return_values else (None, None)
         hip_lib.kv4_append_planned(plan, self._args, k, v, start, count, *values)
         return values if return_values else None
 
@@ -140,4 +143,4 @@ class Kv4Cache:
         return out[0], out[1]
 
 
-__all__ = ["BLOCK", "Kv4Cache", "choose_splits"]
+__all__ = ["BLOCK", "MAX_CAPACITY", "Kv4Cache", "choose_splits"]

@@ -282,7 +282,8 @@ int64_t fa_bwd_workspace_bytes(int32_t B, int32_t H, int32_t H_kv, int32_t M, in
  * bytes, one for 32 channels: e stands for 2^(e - 127), 255 for a block that is NaN throughout. Rows of one
  * (batch, kv head) are dense; batch and head strides are in bytes, multiples of 16, alike for keys and values.
  * `rows` rows are allocated (a multiple of 32: whole tiles are read, whatever the rows behind a sequence
- * hold), `capacity` of them may be used. dtype is the type of the rows that go in and of the queries. */
+ * hold), `capacity` of them may be used, KV4_MAX_CAPACITY at most. dtype is the type of the rows that go in and of the queries. */
+#define KV4_MAX_CAPACITY (1 << 30)
 typedef struct {
   uint8_t* k_codes;
   uint8_t* k_scales;

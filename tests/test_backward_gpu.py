@@ -247,6 +247,41 @@ def test_graph_replays_and_streams(gpu):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_expanded_operands(gpu):
+    """Heads, batches and rows with stride zero, sizes of one with any stride, a lse seen through strides."""
+    B, H, M, N, D = 2, 3, 40, 50, 64
+    q = _rand(110, 1, 1, M, D, dtype=F16).expand(B, H, M, D)
+    k = _rand(111, 1, 1, N, D, dtype=F16).expand(B, 1, N, D)
+    v = _rand(112, B, 1, 1, D, dtype=F16).expand(B, 1, N, D)
+    do = _rand(113, 1, H, 1, D, dtype=F16).expand(B, H, M, D)
+    o, lse = _forward(q, k, v, True)
+    lse2 = torch.empty(M, H, B, device="cuda").permute(2, 1, 0).copy_(lse)
+    grads = flash_atten.attention_backward(do, q, k, v, o, lse2, causal=True)
+    _check(grads, *_reference(do, q, k, v, o, lse, True, D ** -0.5), "expanded")
+    one = [t[:, :, :1] for t in (do, q, k, v, o)]
+    grads = flash_atten.attention_backward(*one, lse[:, :, :1], causal=True)  # one row, one key: P as the lse says
+    _check(grads, *_reference(*one, lse[:, :, :1], True, D ** -0.5), "one row")
+
+
+def test_capture_of_the_differentiable_form_is_refused(gpu):
+    q, k, v, _ = _inputs(120, 1, 2, 2, 32, 32, 64, F16)
+    flash_atten.differentiable_attention(q, k, v)
+    q.requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="capture attention"):
+        with torch.cuda.graph(graph):
+            flash_atten.differentiable_attention(q, k, v)
+    with torch.no_grad():  # without gradients there is nothing to refuse
+        want = flash_atten.differentiable_attention(q, k, v)
+        held = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(held):
+            o = flash_atten.differentiable_attention(q, k, v)
+    for _ in range(2):
+        held.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want)
+
+
 def test_long_causal_and_many_heads(gpu):
     """A longer call against 32-bit formulas per head: relative error of the whole gradient. P and dS are each
     rounded once, and the result: independent errors of at most u each, so under 3 u of the norm."""

@@ -230,8 +230,9 @@ def test_large_and_not_finite_scores(gpu):
         d = (o.double().cpu() - want[0]).abs()
         assert (d <= 1.01 * want[2]).all()
         cache.k_scales[0, 0, 100, 0] = 255
-        bad = flash_atten.sdpa_kv4(q, cache, _i32(capacity - 1))
+        bad, bad_lse = flash_atten.sdpa_kv4(q, cache, _i32(capacity - 1), return_lse=True)
         assert torch.isnan(bad[0, :2]).all() and torch.equal(bad[0, 2:], o[0, 2:])
+        assert torch.isnan(bad_lse[0, :2]).all() and torch.equal(bad_lse[0, 2:], lse[0, 2:])
 
 
 def test_decode_loop_eager_and_captured(gpu):
@@ -303,6 +304,30 @@ def test_training_and_serving_together(gpu):
     assert float((served - same).abs().max()) <= 4 * 2.0 ** -8 * float(vv.abs().max())
     # a code is off by at most an eighth of its value or half its smallest step: within a quarter of the norm
     assert float((served - full).float().norm() / full.float().norm()) <= 0.25
+
+
+def test_far_rows(gpu):
+    """Offsets past 32 bits: 70 million cached rows of one head are 4.5 GB of codes. The keys are zeros but for the
+    last 64, whose scores of about 40 outweigh all others together by e^20: the output is the softmax over those."""
+    capacity, D, n = 70_000_000, 128, 64
+    cache = kv4.Kv4Cache(1, 1, capacity, D, dtype=BF16)
+    q = torch.zeros(1, 2, 1, D, dtype=BF16, device="cuda")
+    q[..., :32] = 2.0
+    k = torch.zeros(1, 1, n, D, dtype=BF16, device="cuda")
+    k[..., :32] = 7.0  # 2 * 6 * 32 / sqrt(128) = 33.9 as cached
+    k[..., 32] = torch.linspace(-1, 1, n, device="cuda")
+    v = _rand(90, 1, 1, n, D, dtype=BF16).cuda()
+    start = _i32(capacity - n)
+    cache.append(k, v, start)
+    for M in (1, 40):
+        qq = q.expand(1, 2, M, D)
+        o = flash_atten.sdpa_kv4(qq, cache, _i32(capacity - M), is_causal=False, scale=0.1)
+        kk, vv = (_decode(s[:, :, -n:].cpu(), c[:, :, -n:].cpu()) for s, c in ((cache.k_scales, cache.k_codes), (cache.v_scales, cache.v_codes)))
+        score = 0.1 * (q.double().cpu()[0, :, 0] @ kk[0, 0].T)
+        assert float(score.min()) - math.log(capacity) > 16  # so the rest weighs under e^-16 of the sum
+        want = torch.softmax(score, -1) @ vv[0, 0]
+        bound = (2 * 2.0 ** -9 + math.exp(-16)) * vv.abs().amax() + 2.0 ** -9 * want.abs()
+        assert ((o[0].double().cpu() - want[:, None]).abs() <= bound[:, None]).all(), M
 
 
 def test_side_stream_and_alignment(gpu):

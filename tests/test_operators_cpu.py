@@ -55,6 +55,7 @@ def _bwd(**over):
     ({"D": 96}, hip_lib.FA_ENOTSUP, "head dim"), ({"dtype": 2}, hip_lib.FA_ENOTSUP, "dtype"),
     ({"H": 3}, hip_lib.FA_EINVAL, "multiple of kv heads"), ({"M": -1}, hip_lib.FA_EINVAL, "invalid sizes"),
     ({"sm_scale": 0.0}, hip_lib.FA_EINVAL, "sm_scale"), ({"sm_scale": float("inf")}, hip_lib.FA_EINVAL, "sm_scale"),
+    ({"sm_scale": 3e38}, hip_lib.FA_EINVAL, "sm_scale"),
     ({"q": None}, hip_lib.FA_EINVAL, "null q"), ({"dv": None}, hip_lib.FA_EINVAL, "null dv"),
     ({"lse": None}, hip_lib.FA_EINVAL, "null lse"), ({"k": 264}, hip_lib.FA_EINVAL, "k must be 16-byte aligned"),
     ({"v_stride": _i64(8192, 4096, 64, 2)}, hip_lib.FA_EINVAL, "head-dim stride of v"),
@@ -115,7 +116,8 @@ def _attend(cache=None, **over):
 CACHE_REFUSALS = [
     ({"D": 32}, hip_lib.FA_ENOTSUP, "head dim"), ({"dtype": 5}, hip_lib.FA_ENOTSUP, "dtype"),
     ({"H_kv": 0}, hip_lib.FA_EINVAL, "invalid cache sizes"), ({"rows": 50}, hip_lib.FA_EINVAL, "multiple of 32"),
-    ({"capacity": 65}, hip_lib.FA_EINVAL, "at least the capacity"), ({"v_scales": None}, hip_lib.FA_EINVAL, "null cache"),
+    ({"capacity": 65}, hip_lib.FA_EINVAL, "at least the capacity"),
+    ({"capacity": (1 << 30) + 1, "rows": (1 << 30) + 32}, hip_lib.FA_ENOTSUP, "is beyond"), ({"v_scales": None}, hip_lib.FA_EINVAL, "null cache"),
     ({"k_codes": 264}, hip_lib.FA_EINVAL, "16-byte aligned"), ({"code_stride": _i64(4096, 2040)}, hip_lib.FA_EINVAL, "multiples of 16"),
 ]
 
@@ -161,6 +163,8 @@ def test_python_refusals_without_a_gpu():
         kv4.Kv4Cache(1, 1, 8, 96, dtype=torch.float16)
     with pytest.raises(hip_lib.FaUnsupportedError):
         kv4.Kv4Cache(1, 1, 8, 64, dtype=torch.float32)
+    with pytest.raises(hip_lib.FaUnsupportedError, match="is beyond"):
+        kv4.Kv4Cache(1, 1, (1 << 30) + 1, 64, dtype=torch.float16)
     with pytest.raises(ValueError, match="invalid cache sizes"):
         kv4.Kv4Cache(1, 1, 0, 64, dtype=torch.float16)
 
