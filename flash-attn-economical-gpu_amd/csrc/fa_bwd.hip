@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256) void fa_bwd_prep_kernel(BwdParams p) {
   const int t = threadIdx.x, part = t % LPR, r0 = t / LPR;
   __shared__ float red[8];
   const uint32_t qblocks = p.prep_blocks, nq = (uint32_t)p.B * p.H * qblocks, id = blockIdx.x;
-  constexpr int NP = kPrepRows / RPP < 4 ? kPrepRows / RPP : 4;  // passes whose loads are issued together
+  constexpr int NP = 2;  // passes whose loads are issued together (four take a third longer: fewer waves fit)
   float top = 0.f, topd = 0.f;
   if (id < nq) {
     const uint32_t bh = id / qblocks;
