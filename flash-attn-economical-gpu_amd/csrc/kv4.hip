@@ -689,6 +689,7 @@ struct Kv4Chunk {
           pb[i / 2][j][2 * (i & 1) + 1] = E::pack2(x[i][j][2], x[i][j][3]);
         }
       }
+      __builtin_amdgcn_s_setprio(1);  // before a neighbour's softmax: 2 to 5%
 #pragma unroll
       for (int d = 0; d < DT16; ++d)
 #pragma unroll
@@ -697,6 +698,7 @@ struct Kv4Chunk {
 #pragma unroll
           for (int j = 0; j < QT; ++j) o[d][j] = E::mfma16(v, pb[i][j], o[d][j]);
         }
+      __builtin_amdgcn_s_setprio(0);
     };
     Codes next;
     if (k_first < k_end) fetch(next, k_first);
