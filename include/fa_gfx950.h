@@ -1,10 +1,10 @@
 /*
- * fa_gfx950.h -- C ABI of libfa_gfx950.so, the MI355X (gfx950 / CDNA4) FlashAttention-forward
- * and fp16 GEMM library.
+ * fa_gfx950.h -- C ABI of libfa_gfx950.so, the MI355X (gfx950 / CDNA4) library of FlashAttention forward and
+ * backward, the fp16 GEMM, and a 4-bit key/value cache with attention over it.
  *
  * Every entry point is plain C: pointers, fixed-width integers and floats, no HIP or torch types.
- * Device pointers come from the caller (PyTorch allocates every buffer, including the split-KV
- * workspace); the library never allocates or frees device memory. `stream` is a hipStream_t
+ * Device pointers come from the caller (PyTorch allocates every buffer, workspaces
+ * included); the library never allocates or frees device memory. `stream` is a hipStream_t
  * passed as void* (the caller's current stream); no entry point synchronises the host.
  *
  * Return value of every int-returning entry point: FA_OK (0) or one of the FA_E* codes below;
