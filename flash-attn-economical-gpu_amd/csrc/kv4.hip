@@ -137,6 +137,9 @@ __device__ inline int visible_keys(const int32_t* start, const int32_t* count, i
 // 752. A split has a slot: sequence b's are those from its predecessors' number on. Each wave works this out
 // from the lengths (64 sequences at a time, one to a lane).
 constexpr int kMinTiles = 8;
+constexpr int kAllTiles = KV4_MAX_CAPACITY / 32;  // of the largest cache: the share where nothing is split
+static_assert(KV4_MAX_CAPACITY % 32 == 0 && (uint64_t)kAllTiles * 64 <= 0xffffffffu,
+              "64 sequences of whole tiles are summed in 32 bits");
 
 struct Split {
   int b, index;     // sequence, and which of its splits (b < 0: a slot that no split has)
@@ -152,7 +155,7 @@ __device__ inline Split find_split(const Kv4AttendParams& p, int slot, int b) {
     s.index = 0;
     s.first = slot;
     s.used = 1;
-    s.per = 0x7fffff;
+    s.per = kAllTiles;
     return s;
   }
   const int lane = threadIdx.x & 63;
@@ -160,7 +163,7 @@ __device__ inline Split find_split(const Kv4AttendParams& p, int slot, int b) {
   int tiles = 0;
   for (int c = 0; c < p.B; c += 64) {
     tiles = c + lane < p.B ? (visible_keys(p.start, p.count, c + lane, p.M, p.capacity) + 31) / 32 : 0;
-    uint32_t sum = (uint32_t)tiles;  // of 64 sequences of under 2^26 tiles each
+    uint32_t sum = (uint32_t)tiles;  // of 64 sequences of at most 2^25 tiles each
     for (int k = 1; k < 64 && k < p.B; k *= 2) sum += (uint32_t)__shfl_xor((int)sum, k, 64);
     all += (uint32_t)__builtin_amdgcn_readfirstlane((int)sum);
   }
