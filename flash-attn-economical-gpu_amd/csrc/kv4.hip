@@ -49,6 +49,18 @@ struct Fp4<bf16_t> {
   }
 };
 
+// The larger of two scores, NaN if one is: one instruction, where fmaxf has to quiet each operand first.
+__device__ inline float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// Of a row's scores, over the four lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ inline float row_max(float x) {
+  uint32_t u = __float_as_uint(x);
+  const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  u = __float_as_uint(larger(__uint_as_float(h[0]), __uint_as_float(h[1])));
+  const auto q = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return larger(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+
 __device__ inline float scale_of(uint32_t e) { return __uint_as_float(e << 23); }
 
 // Eight codes (a dword) to eight 16-bit values.
@@ -320,10 +332,10 @@ struct Kv4Attend {
           for (int r = 0; r < 4; ++r)
             if (key0 + 16 * i + 4 * g + r >= see[rt]) x[i][rt][r] = FA_NEG_INF;
       }
-      float top = fmaxf(fmaxf(fmaxf(x[0][rt][0], x[0][rt][1]), fmaxf(x[0][rt][2], x[0][rt][3])),
-                        fmaxf(fmaxf(x[1][rt][0], x[1][rt][1]), fmaxf(x[1][rt][2], x[1][rt][3])));
-      top = xquad_max(top);
-      const float m_new = fmaxf(s.m[rt], top);
+      // a NaN score makes the row NaN: through P, whether or not the maximum moves
+      const float top = larger(larger(larger(x[0][rt][0], x[0][rt][1]), larger(x[0][rt][2], x[0][rt][3])),
+                               larger(larger(x[1][rt][0], x[1][rt][1]), larger(x[1][rt][2], x[1][rt][3])));
+      const float m_new = larger(s.m[rt], row_max(top));
       if (__any(m_new > s.m[rt])) {
         const float base = m_new == FA_NEG_INF ? 0.f : m_new;
         const float f = fast_exp2((s.m[rt] - base) * c);
@@ -469,6 +481,8 @@ struct Kv4Attend {
     const uint8_t* ks = p.k_scales + b * p.scale_stride[0] + hk * p.scale_stride[1];
     const uint8_t* vs = p.v_scales + b * p.scale_stride[0] + hk * p.scale_stride[1];
     t0 += wave;
+    // in vector registers: with scalar branches the allocator spills a hundred bytes inside the loop
+    asm volatile("" : "+v"(t1), "+v"(least));
     // two tiles in flight
     Tile even, odd;
     auto fetch = [&](Tile& x, int t) {
@@ -656,6 +670,16 @@ struct Kv4Chunk {
     auto step = [&](int key0, uint32_t stage, auto edge_tile) {
       constexpr bool EDGE = decltype(edge_tile)::value;
       const uint32_t rowb = ro + stage, colb = to + stage;
+      // D = 64: all of K's fragments (32 registers) are asked for before the first product. Left to the compiler they came
+      // one by one, each waited for: 214 against 205 us (512 rows over 16k keys, 28/4 heads).
+      u32x4 ahead[KT][KS];
+      if constexpr (D == 64) {
+#pragma unroll
+        for (int i = 0; i < KT; ++i)
+#pragma unroll
+          for (int k = 0; k < KS; ++k) ahead[i][k] = L::frag(smem, rowb ^ (k << 6), i * 16 * L::ROWB);
+        __builtin_amdgcn_sched_barrier(0);
+      }
       floatx4 x[KT][QT];
 #pragma unroll
       for (int i = 0; i < KT; ++i) {
@@ -663,7 +687,7 @@ struct Kv4Chunk {
         for (int j = 0; j < QT; ++j) x[i][j] = (floatx4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          const u32x4 a = L::frag(smem, rowb ^ (k << 6), i * 16 * L::ROWB);
+          const u32x4 a = D == 64 ? ahead[i][k] : L::frag(smem, rowb ^ (k << 6), i * 16 * L::ROWB);
 #pragma unroll
           for (int j = 0; j < QT; ++j) x[i][j] = E::mfma16(a, qf[j][k], x[i][j]);
         }
@@ -677,9 +701,9 @@ struct Kv4Chunk {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             if (EDGE && key0 + 16 * i + 4 * g + r >= see[j]) x[i][j][r] = FA_NEG_INF;
-            top = fmaxf(top, x[i][j][r]);
+            top = larger(top, x[i][j][r]);
           }
-        const float m_new = fmaxf(m[j], xquad_max(top));
+        const float m_new = larger(m[j], row_max(top));
         if (__any(m_new > m[j])) {
           const float base = m_new == FA_NEG_INF ? 0.f : m_new;
           const float f = fast_exp2((m[j] - base) * p.c);
