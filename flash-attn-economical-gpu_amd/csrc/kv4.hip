@@ -304,10 +304,49 @@ struct Kv4Attend {
     float m[R], l[R];
   };
 
-  // One tile: keys [key0, key0 + 32), of which row rt sees those below see[rt] (a lane's own row).
+  // The n-th key's values, of the blocks marked in `bad` only, times P: a product of its own, whose result only the
+  // rows that see the key take.
+  __device__ static inline void add_alone(State& s, const Tile& t, const float (&vs)[8], const u32x4 (&pb)[R], uint32_t bad,
+                                          int n, int key0, const int (&see)[R], int lane) {
+    const int slot = (n & 3) + 4 * (n >> 4);
+    const bool mine = lane >> 4 == ((n >> 2) & 3) && (bad >> slot & 1u) != 0;
+    if (!__any(mine)) return;
+    uint32_t code[CPL >= 8 ? CPL / 8 : 1] = {};
+    float scale = 1.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i == slot) {
+        scale = vs[i];
+#pragma unroll
+        for (int w = 0; w < (CPL >= 8 ? CPL / 8 : 1); ++w) code[w] = t.v[i][w];
+      }
+    auto pair = [&](auto jc) {
+      constexpr int j = decltype(jc)::value;
+      const uint32_t x = mine ? Fp4<Tag>::template decode<j % 4>(code[j / 4], scale) : 0u;
+      u32x4 even, odd;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        even[i] = i == slot / 2 ? (x & 0xffffu) << (16 * (slot & 1)) : 0u;
+        odd[i] = i == slot / 2 ? (x >> 16) << (16 * (slot & 1)) : 0u;
+      }
+#pragma unroll
+      for (int rt = 0; rt < R; ++rt) {
+        const floatx4 zero = (floatx4){0.f, 0.f, 0.f, 0.f};
+        const floatx4 a = E::mfma16(even, pb[rt], zero), b = E::mfma16(odd, pb[rt], zero);
+        if (key0 + n < see[rt]) {
+          s.o[2 * j][rt] += a;
+          s.o[2 * j + 1][rt] += b;
+        }
+      }
+    };
+    for_each<CPL / 2>(pair);
+  }
+
+  // One tile: keys [key0, key0 + 32), of which row rt sees those below see[rt] (a lane's own row). `unseen`: a row
+  // before count does not see all of the sequence's keys among them.
   template <bool EDGE>
   __device__ static inline void step(State& s, const u32x4 (&qf)[R][KS], Tile& t, int key0, const int (&see)[R],
-                                     int keys, float c, int lane) {
+                                     int keys, bool unseen, float c, int lane) {
     const int g = lane >> 4;
     floatx4 x[2][R];
 #pragma unroll
@@ -367,6 +406,26 @@ struct Kv4Attend {
         }
       }
     }
+    if constexpr (EDGE) {
+      // A block that is NaN, or whose scale takes it past the type, would be 0 x NaN to the rows that do not see it.
+      // Such blocks (rare) leave the tile's product and are added key by key.
+      uint32_t bad = 0;
+      if (unseen) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) bad |= (vs[i] > scale_of(Fp4<Tag>::kCeil) ? 1u : 0u) << i;
+      }
+      if (__builtin_expect(__any(bad != 0), 0)) {
+#pragma unroll 1
+        for (int n = 0; n < 32; ++n) add_alone(s, t, vs, pb, bad, n, key0, see, lane);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (bad >> i & 1u) {
+            vs[i] = 1.f;
+#pragma unroll
+            for (int w = 0; w < (CPL >= 8 ? CPL / 8 : 1); ++w) t.v[i][w] = 0;
+          }
+      }
+    }
     // channels 2 j and 2 j + 1 of the lane's CPL: byte j of a key's codes
     auto pair = [&](auto jc) {
       constexpr int j = decltype(jc)::value;
@@ -396,7 +455,8 @@ struct Kv4Attend {
     }
   }
 
-  // N channels N at .. of row r, whose maximum and sum are m and l.
+  // N channels N at .. of row r, whose maximum and sum are m and l. A row that saw no key (l = 0) is zeros, whatever its
+  // products with values that are no numbers left in o.
   template <int N>
   __device__ static inline void store_row(const Kv4AttendParams& p, int b, int hk, int slot, int r, const float (&o)[N],
                                           float m, float l, int at) {
@@ -405,17 +465,18 @@ struct Kv4Attend {
       const int64_t w = ((int64_t)slot * p.H + h) * p.M + i;
       float* dst = p.ws_o + w * D + at * N;
 #pragma unroll
-      for (int j = 0; j < N; j += 4) *reinterpret_cast<floatx4*>(dst + j) = (floatx4){o[j], o[j + 1], o[j + 2], o[j + 3]};
+      for (int j = 0; j < N; j += 4)
+        *reinterpret_cast<floatx4*>(dst + j) = l == 0.f ? (floatx4){0.f, 0.f, 0.f, 0.f} : (floatx4){o[j], o[j + 1], o[j + 2], o[j + 3]};
       if (at == 0) {
         p.ws_ml[2 * w] = m * p.c;
         p.ws_ml[2 * w + 1] = l;
       }
     } else {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = 1.f / l;
       uint16_t* dst = p.o + b * p.so[0] + h * p.so[1] + i * p.so[2] + at * N;
 #pragma unroll
       for (int j = 0; j < N; j += 4)
-        *reinterpret_cast<u32x2*>(dst + j) = (u32x2){E::pack2(o[j] * inv, o[j + 1] * inv), E::pack2(o[j + 2] * inv, o[j + 3] * inv)};
+        *reinterpret_cast<u32x2*>(dst + j) = l == 0.f ? (u32x2){0u, 0u} : (u32x2){E::pack2(o[j] * inv, o[j + 1] * inv), E::pack2(o[j + 2] * inv, o[j + 3] * inv)};
       if (at == 0 && p.lse != nullptr)
         p.lse[b * p.sl[0] + h * p.sl[1] + i * p.sl[2]] =
             l == 0.f ? FA_NEG_INF : (m * p.c + __builtin_amdgcn_logf(l) - Fp4<Tag>::kPBias) * 0.6931471805599453f;
@@ -448,7 +509,8 @@ struct Kv4Attend {
       const int64_t e = p.causal ? start + wave_top / p.group + 1 : keys;
       wave_see = (int)(e < 0 ? 0 : (e > keys ? keys : e));
     }
-    int least = wave_see;  // keys that every row of the wave sees
+    int least = wave_see;   // keys that every row of the wave sees
+    int live_least = 0x7fffffff;  // and those that every row before count sees
 #pragma unroll
     for (int rt = 0; rt < R; ++rt) {
       const int r = row0 + 16 * rt + c16;
@@ -472,6 +534,7 @@ struct Kv4Attend {
       const int64_t e = p.causal ? start + row0 / p.group + 1 : keys;
       const int64_t low = e < 0 ? 0 : (e > keys ? keys : e);
       least = wave_top / p.group < count && row0 + 16 * R <= rows ? (int)low : 0;
+      if (row0 / p.group < count) live_least = (int)low;
     }
     const int tiles = (wave_see + 31) / 32;
     const int per = __builtin_amdgcn_readfirstlane(part.per);
@@ -489,8 +552,8 @@ struct Kv4Attend {
       if (t < t1) load(x, kc, ks, vc, vs, t * 32, lane);
     };
     auto use = [&](Tile& x, int t) {
-      if (t * 32 + 32 <= least) step<false>(s, qf, x, t * 32, see, keys, p.c, lane);
-      else step<true>(s, qf, x, t * 32, see, keys, p.c, lane);
+      if (t * 32 + 32 <= least) step<false>(s, qf, x, t * 32, see, keys, false, p.c, lane);
+      else step<true>(s, qf, x, t * 32, see, keys, (t * 32 + 32 < keys ? t * 32 + 32 : keys) > live_least, p.c, lane);
       fetch(x, t + 2 * WAVES);
     };
     fetch(even, t0);
@@ -598,9 +661,9 @@ struct Kv4Chunk {
       return first + n <= rows ? first + n - 1 : rows - 1;
     };
     const int block_see = seen(last_live(rb * BLOCK, BLOCK));
-    const int wave_see = row0 < rows ? seen(last_live(row0, QT * 16)) : 0;
+    const int wave_see = __builtin_amdgcn_readfirstlane(row0 < rows ? seen(last_live(row0, QT * 16)) : 0);
     const bool whole = row0 + QT * 16 <= rows && (row0 + QT * 16 - 1) / p.group < count;
-    const int least = whole ? seen(row0) : 0;  // keys that every row of the wave sees
+    const int least = __builtin_amdgcn_readfirstlane(whole ? seen(row0) : 0);  // keys that every row of the wave sees
 
     int see[QT];
     u32x4 qf[QT][KS];
@@ -630,9 +693,12 @@ struct Kv4Chunk {
     // the split's keys, in tiles of T (its share is in tiles of 32)
     const int64_t per = (int64_t)__builtin_amdgcn_readfirstlane(part.per) * 32;
     const int64_t k_first = __builtin_amdgcn_readfirstlane(part.index) * per;
-    const int k_end = (int)(k_first + per < block_see ? k_first + per : block_see);
+    const int k_end = __builtin_amdgcn_readfirstlane((int)(k_first + per < block_see ? k_first + per : block_see));
 #pragma unroll
     for (int j = 0; j < QT; ++j) see[j] = see[j] < k_end ? see[j] : k_end;  // the next split may begin inside a tile
+    // of the split's keys, those that every row before count sees
+    const int live_least = __builtin_amdgcn_readfirstlane(
+        row0 < rows && row0 / p.group < count ? (seen(row0) < k_end ? seen(row0) : k_end) : 0x7fffffff);
     const uint8_t* kc = p.k_codes + b * p.code_stride[0] + hk * p.code_stride[1];
     const uint8_t* vc = p.v_codes + b * p.code_stride[0] + hk * p.code_stride[1];
     const uint8_t* ksc = p.k_scales + b * p.scale_stride[0] + hk * p.scale_stride[1];
@@ -653,13 +719,13 @@ struct Kv4Chunk {
         }
       }
     };
-    auto convert = [&](const Codes& x, char* stage) {
+    auto convert = [&](const Codes& x, uint32_t stage) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const bool is_v = PER == 1 ? tid >= UNITS : i == 1;
         const int u = PER == 1 ? tid % UNITS : tid;
         const int row = u / SB, blk = u % SB;
-        char* dst = stage + (is_v ? TILEB : 0) + row * L::ROWB;
+        char* dst = smem + stage + (is_v ? TILEB : 0) + row * L::ROWB;
         const float scale = scale_of(x.e[i]);
 #pragma unroll
         for (int c = 0; c < 4; ++c)
@@ -670,6 +736,20 @@ struct Kv4Chunk {
     auto step = [&](int key0, uint32_t stage, auto edge_tile) {
       constexpr bool EDGE = decltype(edge_tile)::value;
       const uint32_t rowb = ro + stage, colb = to + stage;
+      // A block that is NaN or past the type would be 0 x NaN to the rows that do not see it: keys that have one (rare)
+      // are left out of the tile's product and added one by one, to the rows that see them. Looked for in the few
+      // tiles that a row before count does not see whole.
+      uint64_t alone = 0;  // keys of the tile
+      if (EDGE && (key0 + T < keys ? key0 + T : keys) > live_least) {
+        bool bad = false;
+        if (lane < T && key0 + lane < keys) {
+          typedef uint8_t scales_t __attribute__((ext_vector_type(SB)));
+          const scales_t e = *reinterpret_cast<const scales_t*>(vsc + (int64_t)(key0 + lane) * SB);
+#pragma unroll
+          for (int n = 0; n < SB; ++n) bad |= e[n] > Fp4<Tag>::kCeil;
+        }
+        alone = __ballot(bad);
+      }
       // D = 64: all of K's fragments (32 registers) are asked for before the first product. Left to the compiler they came
       // one by one, each waited for: 214 against 205 us (512 rows over 16k keys, 28/4 heads).
       u32x4 ahead[KT][KS];
@@ -724,16 +804,53 @@ struct Kv4Chunk {
           pb[i / 2][j][2 * (i & 1) + 1] = E::pack2(x[i][j][2], x[i][j][3]);
         }
       }
+      // a lane's keys of an operand that are in `set`: 4 g .. + 3 (dwords 0, 1), then 16 further (dwords 2, 3)
+      auto lanes_of = [&](uint32_t set) {
+        const uint32_t x = set >> (4 * g);
+        u32x4 m;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const uint32_t two = x >> (16 * (n / 2) + 2 * (n & 1));
+          m[n] = (two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
+        }
+        return m;
+      };
       __builtin_amdgcn_s_setprio(1);  // before a neighbour's softmax: 2 to 5%
 #pragma unroll
       for (int d = 0; d < DT16; ++d)
 #pragma unroll
         for (int i = 0; i < KT / 2; ++i) {
-          const u32x4 v = L::tfrag(smem, colb ^ (d << 5), TILEB + i * 32 * L::ROWB);
+          u32x4 v = L::tfrag(smem, colb ^ (d << 5), TILEB + i * 32 * L::ROWB);
+          if (EDGE && alone != 0) v &= ~lanes_of((uint32_t)(alone >> (32 * i)));
 #pragma unroll
           for (int j = 0; j < QT; ++j) o[d][j] = E::mfma16(v, pb[i][j], o[d][j]);
         }
       __builtin_amdgcn_s_setprio(0);
+      if constexpr (EDGE) {
+#pragma unroll 1
+        for (; alone != 0; alone &= alone - 1) {
+          const int key = __builtin_ctzll(alone), i = key / 32;
+          const u32x4 one = lanes_of(1u << (key & 31));
+          uint32_t cols = colb + (uint32_t)(i * 32 * L::ROWB);
+          asm volatile("" : "+v"(cols));  // addresses worked out here, not held through the loops
+#pragma unroll
+          for (int j = 0; j < QT; ++j) {
+            u32x4 w;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const uint32_t low = pb[0][j][n], high = pb[KT / 2 - 1][j][n];
+              w[n] = i != 0 ? high : low;
+            }
+#pragma unroll
+            for (int d = 0; d < DT16; ++d) {
+              __builtin_amdgcn_sched_barrier(0);  // nor reads ahead
+              const u32x4 v = L::tfrag(smem, cols ^ (d << 5), TILEB) & one;
+              const floatx4 x = E::mfma16(v, w, (floatx4){0.f, 0.f, 0.f, 0.f});
+              if (key0 + key < see[j]) o[d][j] += x;
+            }
+          }
+        }
+      }
     };
     Codes next;
     if (k_first < k_end) fetch(next, k_first);
@@ -741,7 +858,7 @@ struct Kv4Chunk {
     // tiles that every row of the wave sees whole, then those on the diagonal or at the end: every wave makes the
     // same number of passes in all, for the barriers
     auto pass = [&](int64_t key0, auto edge_tile) {
-      convert(next, smem + stage);
+      convert(next, stage);
       if (key0 + T < k_end) fetch(next, key0 + T);
       wait_vm_lds_barrier<63>();  // LDS writes only: the codes just asked for stay in flight
       if (key0 < wave_see) step((int)key0, stage, edge_tile);
@@ -760,17 +877,18 @@ struct Kv4Chunk {
       if (p.splits > 1) {
         const int64_t w = ((int64_t)slot * p.H + h) * p.M + i;
 #pragma unroll
-        for (int d = 0; d < DT16; ++d) *reinterpret_cast<floatx4*>(p.ws_o + w * D + 16 * d + 4 * g) = o[d][j];
+        for (int d = 0; d < DT16; ++d)  // a row that saw no key is zeros, whatever values that are no numbers left in o
+          *reinterpret_cast<floatx4*>(p.ws_o + w * D + 16 * d + 4 * g) = sum == 0.f ? (floatx4){0.f, 0.f, 0.f, 0.f} : o[d][j];
         if (g == 0) {
           p.ws_ml[2 * w] = m[j] * p.c;
           p.ws_ml[2 * w + 1] = sum;
         }
       } else {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const float inv = 1.f / sum;
         uint16_t* dst = p.o + b * p.so[0] + h * p.so[1] + i * p.so[2] + 4 * g;
 #pragma unroll
         for (int d = 0; d < DT16; ++d)
-          *reinterpret_cast<u32x2*>(dst + 16 * d) =
+          *reinterpret_cast<u32x2*>(dst + 16 * d) = sum == 0.f ? (u32x2){0u, 0u} :
               (u32x2){E::pack2(o[d][j][0] * inv, o[d][j][1] * inv), E::pack2(o[d][j][2] * inv, o[d][j][3] * inv)};
         if (g == 0 && p.lse != nullptr)
           p.lse[b * p.sl[0] + h * p.sl[1] + i * p.sl[2]] =
@@ -781,7 +899,7 @@ struct Kv4Chunk {
 };
 
 template <typename Tag, int D>
-__global__ __launch_bounds__(256, 2) void kv4_chunk_kernel(Kv4AttendParams p) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv4_chunk_kernel(Kv4AttendParams p) {
   __shared__ __align__(1024) char smem[Kv4Chunk<Tag, D>::SMEM];
   Kv4Chunk<Tag, D>::run(p, smem);
 }

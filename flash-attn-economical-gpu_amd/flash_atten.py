@@ -381,7 +381,7 @@ def sdpa_kv4(query: torch.Tensor, cache: kv4.Kv4Cache, start: torch.Tensor, *, c
 
     Row i of sequence b stands at position start[b] + i and sees the cached tokens up to and including it
     (is_causal), or all start[b] + count[b] of them. Rows i >= count[b] (none without a count) and rows that
-    see nothing come out as zeros, their lse as -inf. H is a multiple of the cache's heads. M = 1 is a decode
+    see nothing come out as zeros, their lse as -inf; a NaN in the cache reaches the rows that see it and no other. H is a multiple of the cache's heads. M = 1 is a decode
     step, a few rows a draft being checked, many a chunk of a prompt. start and count are int32 [B] on the GPU;
     nothing synchronises, and the call can be captured into a HIP graph. The result has `sdpa`'s layout."""
     key = ("kv4", cache._form, _form(query), kv4._form(start), None if count is None else kv4._form(count), bool(is_causal),

@@ -319,7 +319,8 @@ int kv4_append(const kv4_append_args* args, void* stream);
 /* Attention of q [B, H, M, D] over the cache. Row i < count[b] (all M without a count) of sequence b stands at
  * position start[b] + i and sees the cached rows up to and including it (causal), or all
  * start[b] + count[b] (otherwise), never past the capacity. Rows that see nothing, and rows at or behind
- * count[b], are zeros with lse = -inf. lse (nullable): fp32 [B, H, M]. splits > 1 cuts the
+ * count[b], are zeros with lse = -inf. A NaN block of a cached row (or one that its scale byte takes past the type)
+ * reaches the rows that see it and no other. lse (nullable): fp32 [B, H, M]. splits > 1 cuts the
  * sequences' keys into that many parts on average (longer sequences get more), with a workspace of
  * kv4_attend_workspace_bytes() and a second launch that joins them; kv4_attend_splits() is the number that
  * fills the chip. */

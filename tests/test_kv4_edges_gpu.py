@@ -1,4 +1,5 @@
-"""The 4-bit cache at its edges: the largest unsplit passes.
+"""The 4-bit cache at its edges: the largest unsplit passes, value blocks that are no numbers in places that a row
+does not see.
 
 Tolerances are those of the other tests of the cache (its `_attention`): the cached values are exact, P and the
 result are rounded to the type once each."""
@@ -11,7 +12,7 @@ import torch
 
 import flash_atten
 import kv4
-from test_kv4_gpu import BF16, _decode, _i32, _rand
+from test_kv4_gpu import BF16, F16, _decode, _filled, _i32, _rand
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +48,61 @@ def test_unsplit_pass_over_more_than_2_28_keys(gpu, monkeypatch):
         # the 64 weights' sum, and e^-16 of it
         top = torch.logsumexp(score, -1)
         assert ((lse[0].double().cpu() - top[:, None]).abs() <= 2e-5 + 2.0 ** -22 * top[:, None] + math.exp(-16)).all(), M
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("H,M", [(2, 5), (10, 5), (14, 40)], ids=["16rows", "32rows", "chunk"])
+def test_values_that_are_no_numbers_reach_only_rows_that_see_them(gpu, monkeypatch, H, M, dtype, D, splits):
+    """A NaN block of values (and of keys) at a drafted token: the rows before it, and the rows at or behind count,
+    come out bit for bit as without it; the rows from it on are NaN in that block's channels, and in no other
+    for the values. So does a block whose scale byte, one that append never writes, takes its values past the type."""
+    B, Hk, capacity = 2, 2, 1200
+    starts, counts = [1100, 517], [M, M - 1]
+    _force_splits(monkeypatch, splits)
+    cache = _filled(200 + D + M, B, Hk, capacity, D, dtype)
+    q = _rand(201, B, H, M, D, dtype=dtype).cuda()
+    start, count = _i32(*starts), _i32(*counts)
+    call = lambda: flash_atten.sdpa_kv4(q, cache, start, count=count, return_lse=True)  # noqa: E731
+    clean, clean_lse = call()
+    assert torch.isfinite(clean).all()
+    g = H // Hk
+    for row in (M - 2, M // 2, 1):  # the draft's row whose token is bad
+        for b in range(B):
+            at = starts[b] + row
+            for block in (0, D // 32 - 1):
+                channels = slice(32 * block, 32 * block + 32)
+                saved = cache.v_scales[b, 1, at, block].clone(), cache.v_codes[b, 1, at].clone()
+                cache.v_scales[b, 1, at, block] = 255
+                o, lse = call()
+                assert torch.equal(o[:, :g], clean[:, :g]) and torch.equal(lse, clean_lse)
+                assert torch.equal(o[1 - b], clean[1 - b])
+                assert torch.equal(o[b, g:, :row], clean[b, g:, :row]), (row, b, block)
+                seen = o[b, g:, row:counts[b]]
+                assert torch.isnan(seen[..., channels]).all()
+                others = torch.ones(D, dtype=torch.bool)
+                others[channels] = False
+                # the same sums, perhaps in another order: P |V| in fp32, then one rounding each
+                d = (seen[..., others].double() - clean[b, g:, row:counts[b]][..., others].double()).abs()
+                assert (d <= torch.finfo(dtype).eps * (clean[b, g:, row:counts[b]][..., others].double().abs() + 2.0 ** -10)).all()
+                assert torch.equal(o[b, :, counts[b]:], clean[b, :, counts[b]:]) and not o[b, :, counts[b]:].any()
+                # past the type's range: 4 * 2^23 or 4 * 2^127
+                cache.v_scales[b, 1, at, block] = 150 if dtype == F16 else 254
+                cache.v_codes[b, 1, at] = 0x66
+                o, _ = call()
+                assert torch.equal(o[b, g:, :row], clean[b, g:, :row]), (row, b, block)
+                assert not o[b, :, counts[b]:].any()
+                cache.v_scales[b, 1, at, block], cache.v_codes[b, 1, at] = saved
+            saved = cache.k_scales[b, 1, at, 0].clone()
+            cache.k_scales[b, 1, at, 0] = 255
+            o, lse = call()
+            assert torch.equal(o[b, g:, :row], clean[b, g:, :row]) and torch.equal(lse[b, g:, :row], clean_lse[b, g:, :row])
+            assert torch.isnan(o[b, g:, row:counts[b]]).all() and torch.isnan(lse[b, g:, row:counts[b]]).all()
+            assert not o[b, :, counts[b]:].any() and torch.isinf(lse[b, :, counts[b]:]).all()
+            cache.k_scales[b, 1, at, 0] = saved
+    # a NaN block that every live row sees: rows at or behind count are zeros all the same
+    cache.v_scales[1, 0, 100, 0] = 255
+    o, lse = call()
+    assert torch.isnan(o[1, :g, :counts[1], :32]).all() and not o[1, :, counts[1]:].any()
+    assert torch.equal(o[0], clean[0]) and torch.equal(o[1, g:], clean[1, g:]) and torch.equal(lse, clean_lse)
