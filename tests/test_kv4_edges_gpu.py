@@ -1,5 +1,5 @@
 """The 4-bit cache at its edges: the largest unsplit passes, value blocks that are no numbers in places that a row
-does not see.
+does not see, more than 64 sequences to a call, every merge at every head dimension.
 
 Tolerances are those of the other tests of the cache (its `_attention`): the cached values are exact, P and the
 result are rounded to the type once each."""
@@ -12,7 +12,7 @@ import torch
 
 import flash_atten
 import kv4
-from test_kv4_gpu import BF16, F16, _decode, _filled, _i32, _rand
+from test_kv4_gpu import BF16, F16, _attention, _check, _decode, _filled, _held, _i32, _rand
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +106,39 @@ def test_values_that_are_no_numbers_reach_only_rows_that_see_them(gpu, monkeypat
     o, lse = call()
     assert torch.isnan(o[1, :g, :counts[1], :32]).all() and not o[1, :, counts[1]:].any()
     assert torch.equal(o[0], clean[0]) and torch.equal(o[1, g:], clean[1, g:]) and torch.equal(lse, clean_lse)
+
+
+@pytest.mark.parametrize("B", [65, 130])
+@pytest.mark.parametrize("M,H", [(1, 4), (12, 4)], ids=["token", "chunk"])
+@pytest.mark.parametrize("splits", [2, 7, 40])
+def test_more_than_64_sequences(gpu, monkeypatch, B, M, H, splits):
+    """The split of a slot is looked up 64 sequences at a time: ragged lengths, with empty sequences first, last,
+    and on both sides of a group's border."""
+    capacity, D = 1500, 64
+    starts = [(37 * b * b + 11) % (capacity - M) for b in range(B)]
+    counts = [M] * B
+    for b in (0, 63, 64, B - 1):
+        counts[b] = 0
+    counts[1] = max(1, M // 2)
+    starts[2], starts[5] = -5, capacity - 1
+    _force_splits(monkeypatch, splits)
+    cache = _filled(300 + B, B, 1, capacity, D, F16)
+    q = _rand(301, B, H, M, D, dtype=F16).cuda()
+    print(f"[kv4] B={B} M={M} splits={splits}", flush=True)
+    o, lse = flash_atten.sdpa_kv4(q, cache, _i32(*starts), count=_i32(*counts), return_lse=True)
+    _check(o, lse, *_attention(q, *_held(cache), starts, counts, True, D ** -0.5, F16), (B, M, splits))
+
+
+@pytest.mark.parametrize("D", [64, 256])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("splits", [2, 12, 50])
+@pytest.mark.parametrize("M", [1, 6, 40])
+def test_every_merge(gpu, monkeypatch, D, dtype, splits, M):
+    """One, four and sixteen waves to a row, at the head dimensions beside 128."""
+    B, H, Hk, capacity = 2, 8, 2, 13000
+    cache = _filled(400 + D, B, Hk, capacity, D, dtype)
+    q = _rand(401, B, H, M, D, dtype=dtype).cuda()
+    starts = [capacity - M, 4321]
+    _force_splits(monkeypatch, splits)
+    o, lse = flash_atten.sdpa_kv4(q, cache, _i32(*starts), scale=0.1, return_lse=True)
+    _check(o, lse, *_attention(q, *_held(cache), starts, [M] * B, True, 0.1, dtype), (D, splits, M))
