@@ -31,7 +31,9 @@
 // fp16 range. P and dS enter the second products as 16-bit values. With fp16, P of long rows and dS of small
 // gradients would fall under 2^-14 and lose bits, so P is scaled by 2^15 (in the exponent's offset, free)
 // and dS by a power of two from a bound on |dP - delta| (row norms of dO and V, |delta|) that puts it under
-// 2^15; the sums are scaled back in fp32. bf16 has fp32's range and takes neither.
+// 2^15; the sums are scaled back in fp32. In dQ blocks a lane's products are all of one row, and the power is the
+// row's own; in dK/dV blocks it is that of the largest row which the block's keys meet, and a row 2^k smaller keeps its
+// bits down to weights of 2^(k - 29). bf16 has fp32's range and takes neither.
 #include <type_traits>
 
 #include "fa_common.h"
@@ -272,38 +274,49 @@ struct Bwd : LdsRows<D> {
     }
   }
 
-  // Power of two that brings |dP - delta| under 1 (fp16), from the bounds of this kv head's rows.
-  __device__ static inline int scale_exponent(const BwdParams& p, int b, int hk, float* red) {
+  // The largest of a term over the workgroup; `red` is LDS of the workgroup, free again on return.
+  template <int N>
+  __device__ static inline void block_max(float (&x)[N], float* red) {
     const int t = threadIdx.x;
-    const int64_t nq = (int64_t)p.B * p.H * p.prep_blocks;
-    const int64_t first = ((int64_t)b * p.H + (int64_t)hk * p.group) * p.prep_blocks;
-    const int count = p.group * p.prep_blocks;
-    float o2 = 0.f, dl = 0.f, v2 = 0.f;
-    for (int i = t; i < count; i += WAVES * 64) {
-      o2 = fmaxf(o2, p.bound[first + i]);
-      dl = fmaxf(dl, p.bound[nq + first + i]);
-    }
-    const float* vb = p.bound + 2 * nq + ((int64_t)b * p.Hkv + hk) * p.vblocks;
-    for (int i = t; i < p.vblocks; i += WAVES * 64) v2 = fmaxf(v2, vb[i]);
 #pragma unroll
-    for (int s = 32; s >= 1; s /= 2) {
-      o2 = fmaxf(o2, __shfl_xor(o2, s, 64));
-      dl = fmaxf(dl, __shfl_xor(dl, s, 64));
-      v2 = fmaxf(v2, __shfl_xor(v2, s, 64));
-    }
-    if (t % 64 == 0) {
-      red[t / 64] = o2;
-      red[4 + t / 64] = dl;
-      red[8 + t / 64] = v2;
+    for (int n = 0; n < N; ++n) {
+#pragma unroll
+      for (int s = 32; s >= 1; s /= 2) x[n] = fmaxf(x[n], __shfl_xor(x[n], s, 64));
+      if (t % 64 == 0) red[4 * n + t / 64] = x[n];
     }
     __syncthreads();
-    o2 = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    dl = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
-    v2 = fmaxf(fmaxf(red[8], red[9]), fmaxf(red[10], red[11]));
+#pragma unroll
+    for (int n = 0; n < N; ++n) x[n] = fmaxf(fmaxf(red[4 * n], red[4 * n + 1]), fmaxf(red[4 * n + 2], red[4 * n + 3]));
     __syncthreads();
-    const float bound = sqrtf(o2) * sqrtf(v2) + dl;
-    const int e = (int)(__float_as_uint(bound) >> 23) - 126;  // 2^e > bound
-    return uniform(e < -100 ? -100 : (e > 100 ? 100 : e));
+  }
+  // Largest |V row|^2 of the kv head's first `rows` rows.
+  __device__ static inline float v_bound(const BwdParams& p, int b, int hk, int rows) {
+    const float* vb = p.bound + 2 * (int64_t)p.B * p.H * p.prep_blocks + ((int64_t)b * p.Hkv + hk) * p.vblocks;
+    const int n = (rows + kPrepRows - 1) / kPrepRows;
+    float v2 = 0.f;
+    for (int i = threadIdx.x; i < n; i += WAVES * 64) v2 = fmaxf(v2, vb[i]);
+    return v2;
+  }
+  // Power of two above |dP - delta| <= |dO| |V| + |delta|.
+  __device__ static inline int exponent_above(float o2, float v2, float delta) {
+    const float bound = sqrtf(o2) * sqrtf(v2) + delta;
+    const int e = (int)(__float_as_uint(bound) >> 23) - 126;
+    return e < -100 ? -100 : (e > 100 ? 100 : e);
+  }
+  // That of the rows which the keys from k0 on meet: of all query heads of the kv head, under a causal mask from row k0 on.
+  __device__ static inline int scale_exponent(const BwdParams& p, int b, int hk, int k0, float* red) {
+    const int64_t nq = (int64_t)p.B * p.H * p.prep_blocks;
+    const int skip = p.causal ? k0 / kPrepRows : 0;
+    float x[3] = {0.f, 0.f, v_bound(p, b, hk, p.N)};
+    for (int h = 0; h < p.group; ++h) {
+      const float* ob = p.bound + ((int64_t)b * p.H + (int64_t)hk * p.group + h) * p.prep_blocks;
+      for (int i = skip + (int)threadIdx.x; i < p.prep_blocks; i += WAVES * 64) {
+        x[0] = fmaxf(x[0], ob[i]);
+        x[1] = fmaxf(x[1], ob[nq + i]);
+      }
+    }
+    block_max(x, red);
+    return uniform(exponent_above(x[0], x[2], x[1]));
   }
   __device__ static inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
   __device__ static inline float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
@@ -318,7 +331,7 @@ struct Bwd : LdsRows<D> {
     const int k0 = nb * BLOCK, kw = k0 + OWN * wave;  // first key of the block, of the wave
     float sc = 1.f, unscale = 1.f;
     if constexpr (BwdTraits<Tag>::kScaled) {
-      const int e = scale_exponent(p, b, hk, reinterpret_cast<float*>(smem));
+      const int e = scale_exponent(p, b, hk, k0, reinterpret_cast<float*>(smem));
       sc = pow2(-e);
       unscale = pow2(e);
     }
@@ -439,11 +452,14 @@ struct Bwd : LdsRows<D> {
       for (int n = total - it < qt_all - ct ? total - it : qt_all - ct; n > 0; --n) step(std::false_type{});
       ct = qt0;
     }
+    int key0 = threadIdx.x & 15;  // worked out anew: held through the loops it costs D = 256 a spilled fragment
+    asm volatile("" : "+v"(key0));
+    key0 += kw;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may reach LDS after the workgroup's end
     const float fk = p.scale * unscale * BwdTraits<Tag>::kPUnscale, fv = BwdTraits<Tag>::kPUnscale;
 #pragma unroll
     for (int j = 0; j < KT; ++j) {
-      const int key = kw + 16 * j + c16;
+      const int key = key0 + 16 * j;
       if (key >= p.N) continue;
       if (p.kv_splits > 1) {
         const int64_t w = ((int64_t)(part * p.B + b) * p.Hkv + hk) * p.N + key;
@@ -473,11 +489,11 @@ struct Bwd : LdsRows<D> {
     const int mb = uniform(p.causal ? p.mblocks - 1 - at : at);  // causal: the block with the most keys first
     const int b = uniform(bh / p.H), h = uniform(bh % p.H), hk = uniform(h / p.group);
     const int m0 = mb * BLOCK, mw = m0 + OWN * wave;
-    float sc = 1.f, unscale = 1.f;
+    const int n_end = p.causal && m0 + BLOCK < p.N ? m0 + BLOCK : p.N;
+    float v2[1] = {0.f};
     if constexpr (BwdTraits<Tag>::kScaled) {
-      const int e = scale_exponent(p, b, hk, reinterpret_cast<float*>(smem));
-      sc = pow2(-e);
-      unscale = pow2(e);
+      v2[0] = v_bound(p, b, hk, n_end);
+      block_max(v2, reinterpret_cast<float*>(smem));
     }
     u32x4 qf[KT][KS], of[KT][KS];
     load_frags(qf, p.q + b * p.sq[0] + h * p.sq[1], p.sq[2], mw, p.M, lane);
@@ -494,6 +510,23 @@ struct Bwd : LdsRows<D> {
         nd[i] = src[32];
       }
     }
+    // a lane's products are all of its own row: the row's own scale
+    float sc[KT];
+    if constexpr (BwdTraits<Tag>::kScaled) {
+#pragma unroll
+      for (int i = 0; i < KT; ++i) {
+        float o2 = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float a = E::to_float((uint16_t)of[i][ks][j]), c = E::to_float((uint16_t)(of[i][ks][j] >> 16));
+            o2 += a * a;
+            o2 += c * c;
+          }
+        sc[i] = pow2(-exponent_above(xquad_sum(o2), v2[0], fabsf(nd[i])));
+      }
+    }
     floatx4 acc[DT16][KT];
 #pragma unroll
     for (int d = 0; d < DT16; ++d)
@@ -501,7 +534,6 @@ struct Bwd : LdsRows<D> {
       for (int i = 0; i < KT; ++i) acc[d][i] = (floatx4){0.f, 0.f, 0.f, 0.f};
     const uint32_t lds = lds_address(smem);
     const uint32_t ro = L::row_off(lane), to = L::tr_off(lane);
-    const int n_end = p.causal && m0 + BLOCK < p.N ? m0 + BLOCK : p.N;
     const int all = (n_end + T - 1) / T, share = (all + p.q_splits - 1) / p.q_splits;
     const int first = part * share, tiles = first >= all ? first : (all - first < share ? all : first + share);
     Stream sk, sv;
@@ -554,7 +586,7 @@ struct Bwd : LdsRows<D> {
               if (key >= p.N || (p.causal && key > mw + 16 * j + c16)) x = FA_NEG_INF;
             }
             const float e = fast_exp2(x);
-            dp[j][r] = BwdTraits<Tag>::kScaled ? e * (dp[j][r] * sc) : e * dp[j][r];
+            dp[j][r] = BwdTraits<Tag>::kScaled ? e * (dp[j][r] * sc[j]) : e * dp[j][r];
           }
           sb[j][2 * i] = pack2(dp[j][0], dp[j][1]);
           sb[j][2 * i + 1] = pack2(dp[j][2], dp[j][3]);
@@ -575,11 +607,11 @@ struct Bwd : LdsRows<D> {
     for (; t < tiles && t < whole; ++t) step(t, std::false_type{});
     for (; t < tiles; ++t) step(t, std::true_type{});
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const float f = p.scale * unscale * BwdTraits<Tag>::kPUnscale;
 #pragma unroll
     for (int j = 0; j < KT; ++j) {
       const int row = mw + 16 * j + c16;
       if (row >= p.M) continue;
+      const float f = p.scale * (BwdTraits<Tag>::kScaled ? BwdTraits<Tag>::kPUnscale / sc[j] : 1.f);
       if (p.q_splits > 1) {
         const int64_t w = ((int64_t)(part * p.B + b) * p.H + h) * p.M + row;
 #pragma unroll
