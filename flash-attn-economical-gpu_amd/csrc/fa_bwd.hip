@@ -123,13 +123,14 @@ __global__ __launch_bounds__(256) void fa_bwd_prep_kernel(BwdParams p) {
           if constexpr (BwdTraits<Tag>::kScaled) sq += __shfl_xor(sq, s, 64);
         }
         if (part == 0) {
-          dot -= dlse[i];
+          const bool live = lse[i] != FA_NEG_INF;  // a row without P takes nothing from its O, dlse and bounds
+          dot = live ? dot - dlse[i] : 0.f;
           float* nd = p.nd + nd_index(p, bh, row);
-          nd[0] = lse[i] == FA_NEG_INF ? FA_NEG_INF : BwdTraits<Tag>::kPBias - lse[i] * 1.4426950408889634f;
+          nd[0] = live ? BwdTraits<Tag>::kPBias - lse[i] * 1.4426950408889634f : FA_NEG_INF;
           nd[32] = -dot;
+          if (live && (__float_as_uint(sq) & 0x7fffffffu) < 0x7f800000u) top = fmaxf(top, sq);
+          if ((__float_as_uint(dot) & 0x7fffffffu) < 0x7f800000u) topd = fmaxf(topd, fabsf(dot));
         }
-        if ((__float_as_uint(sq) & 0x7fffffffu) < 0x7f800000u) top = fmaxf(top, sq);
-        if ((__float_as_uint(dot) & 0x7fffffffu) < 0x7f800000u) topd = fmaxf(topd, fabsf(dot));
       }
     }
   } else {
@@ -297,11 +298,12 @@ struct Bwd : LdsRows<D> {
     for (int i = threadIdx.x; i < n; i += WAVES * 64) v2 = fmaxf(v2, vb[i]);
     return v2;
   }
-  // Power of two above |dP - delta| <= |dO| |V| + |delta|.
+  // Power of two above |dP - delta| <= |dO| |V| + |delta|. Not under 2^-60, which scales no product of fp16 numbers past
+  // fp32 (rows without keys are not in the bounds), and under which no gradient is an fp16 number.
   __device__ static inline int exponent_above(float o2, float v2, float delta) {
     const float bound = sqrtf(o2) * sqrtf(v2) + delta;
     const int e = (int)(__float_as_uint(bound) >> 23) - 126;
-    return e < -100 ? -100 : (e > 100 ? 100 : e);
+    return e < -60 ? -60 : (e > 100 ? 100 : e);
   }
   // That of the rows which the keys from k0 on meet: of all query heads of the kv head, under a causal mask from row k0 on.
   __device__ static inline int scale_exponent(const BwdParams& p, int b, int hk, int k0, float* red) {

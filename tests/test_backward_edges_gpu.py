@@ -1,15 +1,17 @@
 """Attention's backward pass where rows' gradients differ in size by many powers of two: fp16 keeps the small rows'
-bits beside the large ones'.
+bits beside the large ones'; and rows without keys, which take no part.
 
 Tolerances are those of the other tests of the backward (its `_reference`), but the absolute error of dS is taken
 from the rows that share its scale: a row's own for dq, the rows from the key block's first on for causal dk."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
 import flash_atten
-from test_backward_gpu import E32, F16, _forward, _rand
+from test_backward_gpu import BF16, E32, F16, _check, _forward, _inputs, _rand, _reference
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +83,27 @@ def test_causal_keys_behind_large_rows(gpu, H, Hk, N):
     assert float((d / bound).max()) <= 1.01, float((d / bound)[:, :, 128:].max())
     err = d[:, :, 128:].norm() / want[:, :, 128:].norm()
     assert float(err) <= 3 * 2.0 ** -11 + 2.0 ** -25 * want[:, :, 128:].numel() ** 0.5 / float(want[:, :, 128:].norm())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("causal", [False, True])
+def test_rows_without_keys_take_no_part(gpu, dtype, causal):
+    """Rows whose lse is -inf, with NaN in their O, infinities in their dlse and a large dO: zero dq, and the others'
+    gradients are what they are without those rows."""
+    B, H, Hk, M, N, D = 1, 2, 1, 70, 50, 128
+    q, k, v, do = _inputs(320, B, H, Hk, M, N, D, dtype)
+    o, lse = _forward(q, k, v, causal)
+    dlse = _rand(325, B, H, M, dtype=torch.float32, sigma=0.1)
+    dead = torch.zeros(M, dtype=torch.bool)
+    dead[5:40] = dead[M - 1] = True
+    clean_do, clean_o, clean_dlse = do.clone(), o.clone(), dlse.clone()
+    for t in (clean_do, clean_o, clean_dlse):
+        t[:, :, dead.cuda()] = 0
+    lse[:, :, dead.cuda()] = -math.inf
+    do[:, :, dead.cuda()] = 1e4
+    o[:, :, dead.cuda()] = math.nan
+    dlse[:, :, dead.cuda()] = math.inf
+    grads = flash_atten.attention_backward(do, q, k, v, o, lse, causal=causal, dlse=dlse)
+    assert not grads[0][:, :, dead.cuda()].any()
+    want, bound = _reference(clean_do, q, k, v, clean_o, lse, causal, D ** -0.5, clean_dlse)
+    _check(grads, want, bound, (dtype, causal))
