@@ -325,6 +325,14 @@ def attention_backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: to
     return dq, dk, dv
 
 
+def _refuse_capture() -> None:
+    # autograd waits for the streams of leaves that an eager graph has used; inside a capture that wait can end
+    # the process, and whether such a graph lives cannot be seen from here
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("differentiable_attention is not captured into a HIP graph: capture attention(..., "
+                           "return_lse=True) and attention_backward")
+
+
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, causal, sm_scale):
@@ -349,6 +357,7 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do, dlse):
+        _refuse_capture()
         q, k, v, o, lse = ctx.saved_tensors
         if do is None:
             if dlse is None:
@@ -364,13 +373,9 @@ def differentiable_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     return_lse, the log-sum-exp). q [B, H, M, D] and k/v [B, H_kv, N, D] are read through their strides; o is a
     [B, H, M, D] view of memory laid out [B, M, H, D], as from `sdpa`. First derivatives only. A training step
     that is captured into a HIP graph uses `attention(..., return_lse=True)` and `attention_backward`: this function
-    refuses a capture with gradients."""
-    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad) and q.is_cuda
-            and torch.cuda.is_current_stream_capturing()):
-        # autograd waits for the streams of leaves that an eager graph has used; inside a capture that wait can end
-        # the process, and whether such a graph lives cannot be seen from here
-        raise RuntimeError("differentiable_attention is not captured into a HIP graph: capture attention(..., "
-                           "return_lse=True) and attention_backward")
+    refuses a capture with gradients, and so does the backward of a result that was made outside of one."""
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad) and q.is_cuda:
+        _refuse_capture()
     o, lse = _Attention.apply(q, k, v, bool(causal), None if sm_scale is None else float(sm_scale))
     return (o, lse) if return_lse else o
 

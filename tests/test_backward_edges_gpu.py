@@ -107,3 +107,26 @@ def test_rows_without_keys_take_no_part(gpu, dtype, causal):
     assert not grads[0][:, :, dead.cuda()].any()
     want, bound = _reference(clean_do, q, k, v, clean_o, lse, causal, D ** -0.5, clean_dlse)
     _check(grads, want, bound, (dtype, causal))
+
+
+def test_capture_of_an_eager_result_s_backward_is_refused(gpu):
+    """The forward ran eagerly on a side stream; its backward inside a capture on that stream raises before it
+    launches anything, and works again afterwards."""
+    q, k, v, do = _inputs(330, 1, 2, 2, 32, 32, 64, F16)
+    q.requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        o = flash_atten.differentiable_attention(q, k, v)
+    torch.cuda.synchronize()
+    print("[backward] captured", flush=True)
+    with pytest.raises(RuntimeError, match="capture attention"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+            torch.autograd.grad(o, q, do, retain_graph=True)
+    torch.cuda.synchronize()
+    print("[backward] eager", flush=True)
+    with torch.cuda.stream(side):
+        (dq,) = torch.autograd.grad(o, q, do)
+    torch.cuda.synchronize()
+    want = flash_atten.attention_backward(do, q.detach(), k, v, *_forward(q.detach(), k, v, False))[0]
+    assert torch.equal(dq, want)
