@@ -61,8 +61,14 @@ void copy3(int64_t* dst, const int64_t* src) { std::memcpy(dst, src, 3 * sizeof(
 
 int64_t align256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
+// HIP takes less than 2^32 threads along a dimension. Every entry asks before its first launch.
+int check_grid(int64_t blocks, int threads, const char* what) {
+  if (blocks > 0xffffffffLL / threads)
+    return fail(FA_EINVAL, "%s grid too large (%lld workgroups of %d)", what, (long long)blocks, threads);
+  return FA_OK;
+}
+
 int launch(const void* fn, int64_t blocks, int64_t y, int threads, void* params, void* stream, const char* what) {
-  if (blocks > 0x7fffffffLL) return fail(FA_EINVAL, "%s grid too large (%lld workgroups)", what, (long long)blocks);
   void* args[] = {params};
   const hipError_t err = hipLaunchKernel(fn, dim3((unsigned)blocks, (unsigned)y), dim3((unsigned)threads), args, 0,
                                          static_cast<hipStream_t>(stream));
@@ -233,10 +239,13 @@ int fa_bwd(const fa_bwd_args* a, void* stream) {
   p.kv_total = (int32_t)kv_total;
   p.q_total = (int32_t)q_total;
   const int64_t prep = (int64_t)a->B * a->H * p.prep_blocks + (int64_t)a->B * a->H_kv * p.vblocks;
-  if (prep > 0 && (code = launch(e->prep, prep, 1, 256, &p, stream, "row-term")) != FA_OK) return code;
-  if ((code = launch(e->main, kv_total + q_total, 1, 256, &p, stream, "backward")) != FA_OK) return code;
   const int64_t sums = ((s.kv_splits > 1 ? 2 * (int64_t)a->B * a->H_kv * a->N : 0) +
                         (s.q_splits > 1 ? (int64_t)a->B * a->H * a->M : 0)) * (a->D / 4);
+  if ((code = check_grid(prep, 256, "row-term")) != FA_OK || (code = check_grid(kv_total + q_total, 256, "backward")) != FA_OK ||
+      (code = check_grid((sums + 255) / 256, 256, "gradient sum")) != FA_OK)
+    return code;
+  if (prep > 0 && (code = launch(e->prep, prep, 1, 256, &p, stream, "row-term")) != FA_OK) return code;
+  if ((code = launch(e->main, kv_total + q_total, 1, 256, &p, stream, "backward")) != FA_OK) return code;
   if (sums > 0 && (code = launch(e->reduce, (sums + 255) / 256, 1, 256, &p, stream, "gradient sum")) != FA_OK) return code;
   return ok();
 }
@@ -281,6 +290,7 @@ int kv4_append(const kv4_append_args* a, void* stream) {
   }
   p.B = c->B; p.Hkv = c->H_kv; p.D = c->D; p.rows = a->rows; p.capacity = c->capacity;
   const int64_t threads = (int64_t)c->B * c->H_kv * a->rows * (c->D / 8);
+  if ((code = check_grid((threads + 255) / 256, 256, "cache append")) != FA_OK) return code;
   if ((code = launch(e->append, (threads + 255) / 256, 2, 256, &p, stream, "cache append")) != FA_OK) return code;
   return ok();
 }
@@ -359,14 +369,15 @@ int kv4_attend(const kv4_attend_args* a, void* stream) {
   const int64_t blocks = k.row_blocks * slots * c->H_kv;
   if (slots > 0x7fffffffLL) return fail(FA_EINVAL, "too many splits (%lld)", (long long)slots);
   p.slots = (int32_t)slots;
+  const int64_t all = (int64_t)c->B * a->H * a->M;
+  const int how = a->splits > 32 ? 2 : (a->splits > 8 ? 1 : 0);
+  const int64_t few = (all + 3) / 4 < 2048 ? (all + 3) / 4 : 2048;  // eight workgroups to a CU, a few rows to a wave
+  const int64_t joins = a->splits > 1 ? (how > 0 ? all : few) : 0;
+  const int joiners = how == 2 ? 1024 : 256;
+  if ((code = check_grid(blocks, 256, "cache attention")) != FA_OK || (code = check_grid(joins, joiners, "cache merge")) != FA_OK)
+    return code;
   if ((code = launch(e->attend[k.kind], blocks, 1, 256, &p, stream, "cache attention")) != FA_OK) return code;
-  if (a->splits > 1) {
-    const int64_t all = (int64_t)c->B * a->H * a->M;
-    const int how = a->splits > 32 ? 2 : (a->splits > 8 ? 1 : 0);
-    const int64_t few = (all + 3) / 4 < 2048 ? (all + 3) / 4 : 2048;  // eight workgroups to a CU, a few rows to a wave
-    if ((code = launch(e->merge[how], how > 0 ? all : few, 1, how == 2 ? 1024 : 256, &p, stream, "cache merge")) != FA_OK)
-      return code;
-  }
+  if (joins > 0 && (code = launch(e->merge[how], joins, 1, joiners, &p, stream, "cache merge")) != FA_OK) return code;
   return ok();
 }
 
