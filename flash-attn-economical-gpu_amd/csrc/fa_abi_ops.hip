@@ -86,7 +86,8 @@ struct BwdSizes {
 
 // How many workgroups share a block's steps. A step is a 32-row tile against a block: four products for dK/dV,
 // three for dQ. The chip (256 CUs) holds `slots` workgroups; a block that is longer than an even share of all
-// work (and than kMinWork, below which the sums' extra pass costs more than it gives) is split to that.
+// work (and than kMinWork, below which the sums' extra pass costs more than it gives) is split to that. One number of
+// parts for all blocks of a kind, from the longest: under a causal mask the shorter blocks' parts are shorter.
 BwdSizes bwd_sizes(const fa::BwdKernelEntry* e, int64_t B, int64_t H, int64_t Hkv, int64_t M, int64_t N, int64_t D,
                    bool causal) {
   constexpr int64_t kMinWork = 32;

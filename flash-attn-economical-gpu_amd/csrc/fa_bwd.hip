@@ -19,12 +19,13 @@
 //
 // What bounds it. Per 32 x 32 step a wave makes 64 (dK/dV) or 48 (dQ) MFMAs of 16 cycles at D = 128 against 93 or 100
 // vector instructions, 16 of them exponentials, and every Q, dO, K or V fragment read from LDS feeds two MFMAs:
-// 128 bytes of LDS a cycle and CU at the full matrix rate. fp16 B4 H32 D128 N8192 takes 13.3 ms: 827 TFLOP/s of
-// the five products, 1158 of the seven executed, where an 8192-cube product of normal numbers reaches 1129 on the
-// same card; the matrix pipes are busy 59% of cycles, waves wait 30% of theirs. bf16 D256 N2048: 920 executed
-// (the 512 registers of one wave per SIMD leave nothing to run beside its waits). Short sequences pay for each
-// workgroup's own operands and gradients (a quarter of the time at N2048 causal, 588 us), few heads for the
-// partial sums (bf16 B1 12/2 heads N4096 causal, 243 us).
+// 128 bytes of LDS a cycle and CU at the full matrix rate. fp16 B4 H32 D128 N8192 takes 13.4 to 13.9 ms by card: 790 to
+// 820 TFLOP/s of the five products, 1105 to 1150 of the seven executed, where an 8192-cube product reaches 1345 once the
+// clock is up. The matrix rate is not the bound: the matrix pipes are busy 59% of cycles, waves wait 29% of theirs for a
+// counter or barrier and 34% to issue. bf16 D256 N2048: 918 executed, pipes busy 39% (one wave per SIMD: nothing covers its
+// softmax and its own LDS reads). Short sequences pay for each workgroup's own operands and gradients (a quarter of the
+// time at N2048 causal, 580 to 605 us), few heads for the partial sums and for parts of unequal length: causal blocks
+// have from all tiles to one block's, and all are cut into as many parts as the longest (bf16 B1 12/2 heads N4096, 241 us).
 // Tried and slower: 64 rows per wave at D = 128 (half the LDS reads, but one wave per SIMD: 17.0 against 13.5 ms),
 // three and four ring stages, reads scheduled ahead by hand, heavy and light causal blocks in pairs.
 //
@@ -654,7 +655,7 @@ __global__ __launch_bounds__(256, PER_CU) void fa_bwd_kernel(BwdParams p) {
 }
 
 // Sums of the splits' partial gradients, in split order: a thread takes four channels of one row. Bound by memory:
-// nine partials of 2 x 4 MB in 15 us (bf16 B1 12/2 heads N4096).
+// ten partials of 2 x 4 MB in 15 us (bf16 B1 12/2 heads N4096 causal).
 template <typename Tag, int D>
 __global__ __launch_bounds__(256) void fa_bwd_reduce_kernel(BwdParams p) {
   const int64_t kv_rows = p.kv_splits > 1 ? (int64_t)p.B * p.Hkv * p.N : 0;

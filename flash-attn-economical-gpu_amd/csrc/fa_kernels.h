@@ -113,7 +113,7 @@ struct BwdKernelEntry {
   const void* reduce;
   int32_t block;      // keys (dK/dV) and query rows (dQ) of a workgroup
   int32_t prep_rows;  // rows of a row-term block
-  int32_t per_cu;     // workgroups that a CU holds
+  int32_t per_cu;     // workgroups that the split rule counts on per CU (at D = 64 three fit where two are counted)
 };
 
 const BwdKernelEntry* fa_bwd_registry(int* count);
@@ -162,7 +162,7 @@ struct Kv4KernelEntry {
   const void* append;
   const void* merge[3];   // one, four and sixteen waves to a row
   const void* attend[3];  // 16 rows shared by a workgroup's waves, 32 rows shared, chunks of a prompt
-  int32_t per_cu[3];      // workgroups of each that a CU holds
+  int32_t per_cu[3];      // workgroups of each that the split rule counts on per CU (chunks at D = 64: three fit)
   int32_t chunk_rows;     // query rows of a workgroup of the last
 };
 

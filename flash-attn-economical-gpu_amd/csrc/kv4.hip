@@ -75,7 +75,7 @@ __device__ inline u32x4 decode8(uint32_t codes, float scale) {
 // where a power below would clip 7 to 6 or a power above spend the top codes. Scale choice and conversion use
 // integer compares and exact scalings only, so the result does not depend on the arithmetic of the host that
 // checks it. Bound by memory (2 bytes in and 17/32 out per channel, 2 more with the values): 4 prompts of 2-4k tokens,
-// 8 heads of 128, values returned, 136 MB in 29 us (4.7 TB/s, what a large copy reaches); one token for 32
+// 8 heads of 128, values returned, 136 MB in 26 us (5.3 TB/s; a copy of 4 GiB reaches 4.7); one token for 32
 // sequences 4 us, a launch.
 template <typename Tag>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendParams p) {
@@ -227,7 +227,7 @@ __device__ inline Split find_split(const Kv4AttendParams& p, int slot, int b) {
 // so nothing passes through LDS but the waves' sums at the end. About 170 vector instructions a wave and tile at
 // D = 128, 100 of them conversion, take some 40% of the vector slots at the rate memory delivers; two tiles in flight per wave and two to four waves per SIMD cover the
 // latency. 8 sequences of 16-32k tokens, 8 heads of 128: 223 MB in 46 us (4.8 TB/s) and 6 us for the join; one
-// sequence of 8k: 7.6 + 5 us, launch and dependent-load latencies. Query rows are (position, head of the group):
+// sequence of 8k: 7.2 + 5 us, launch and dependent-load latencies. Query rows are (position, head of the group):
 // row r is head r % group at position r / group, and a workgroup's rows share its kv head's cache.
 // The four waves hold the same rows (single tokens, short drafts) and take turns at the tiles.
 template <typename Tag, int D, int R>
@@ -617,9 +617,10 @@ __global__ __launch_bounds__(256, (attend_waves<D, R>())) void kv4_attend_kernel
 // share it: a tile's codes are loaded a tile ahead, 32 channels of a row to a thread, converted once into 16-bit
 // rows in LDS (two stages, one barrier a tile), and both products read their fragments there, V's by the
 // transposing read. S^T = K Q^T and O^T = V^T P^T as above. Bound by the softmax's vector work beside the MFMAs (216
-// vector instructions, 32 of them exponentials, to 64 MFMAs a wave and tile at D = 128): 960 TFLOP/s where the grid
-// fills the chip (1024 rows over 32k keys, 32/8 heads), 620 with 392 workgroups of 512 (509 and 382 rows over 16k and
-// 12k, 28/4 heads). 32-key tiles at D = 128 and converting a tile ahead were 5 to 7% slower.
+// vector instructions, 32 of them exponentials, to 64 MFMAs a wave and tile at D = 128): 970 TFLOP/s where the grid
+// fills the chip (1024 rows over 32k keys, 32/8 heads), 610 with 448 workgroups for 512 places (509 and 382 rows over 16k
+// and 12k, 28/4 heads). 56 of those 448 hold no row before count: their zeros are right, but they walk the keys for
+// nothing, and rows behind count cost as much as rows before it. 32-key tiles at D = 128 and converting a tile ahead were 5 to 7% slower.
 template <typename Tag, int D>
 struct Kv4Chunk {
   using L = LdsRows<D>;
