@@ -243,7 +243,9 @@ int fa_device_limits(int32_t device, fa_device_limits_t* out);
  * strides as in fa_fwd_args (row strides at least D and at most 2^22 elements); dout is the gradient of o,
  * dlse (nullable) that of lse. dq has q's shape, dk and dv k's: a kv head's gradients are summed over its
  * query heads. Causal is top-left as in the forward. A row whose lse is -inf (no keys) has zero gradients and adds
- * nothing to the others', whatever its o and dlse hold; its q and dout are read, and have to be finite.
+ * nothing to the others', whatever its o and dlse hold; its q and dout are read, and have to be finite. Under a
+ * causal mask an infinity or NaN in a key or row may reach, as in the forward, rows and keys that the mask keeps from
+ * it inside their 32 x 32 tile on the diagonal, and none beyond.
  * workspace: fa_bwd_workspace_bytes(), 256-byte aligned; nothing in it is kept between calls. Results do not
  * depend on the order in which the GPU runs the work. No counterpart in the reference. */
 typedef struct {

@@ -1,5 +1,5 @@
 """Attention's backward pass where rows' gradients differ in size by many powers of two: fp16 keeps the small rows'
-bits beside the large ones'; and rows without keys, which take no part.
+bits beside the large ones'; rows without keys, which take no part; captures; numbers that are not finite.
 
 Tolerances are those of the other tests of the backward (its `_reference`), but the absolute error of dS is taken
 from the rows that share its scale: a row's own for dq, the rows from the key block's first on for causal dk."""
@@ -130,3 +130,24 @@ def test_capture_of_an_eager_result_s_backward_is_refused(gpu):
     torch.cuda.synchronize()
     want = flash_atten.attention_backward(do, q.detach(), k, v, *_forward(q.detach(), k, v, False))[0]
     assert torch.equal(dq, want)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_causal_numbers_stay_in_their_tile(gpu, D, bad):
+    """Causal: what is not finite in key 50 reaches no row before 32, and in row 50's gradient no key from 64 on, bit for
+    bit (tiles of 32)."""
+    B, H, M = 1, 2, 200
+    q, k, v, do = _inputs(340 + D, B, H, H, M, M, D, BF16)
+    o, lse = _forward(q, k, v, True)
+    clean = flash_atten.attention_backward(do, q, k, v, o, lse, causal=True)
+    for t in (k, v):
+        held = t[:, :, 50].clone()
+        t[:, :, 50] = bad
+        dq = flash_atten.attention_backward(do, q, k, v, o, lse, causal=True)[0]
+        assert torch.equal(dq[:, :, :32], clean[0][:, :, :32])
+        assert not torch.isfinite(dq[:, :, 50:]).any()
+        t[:, :, 50] = held
+    do[:, :, 50] = bad
+    _, dk, dv = flash_atten.attention_backward(do, q, k, v, o, lse, causal=True)
+    assert torch.equal(dk[:, :, 64:], clean[1][:, :, 64:]) and torch.equal(dv[:, :, 64:], clean[2][:, :, 64:])
