@@ -2,7 +2,7 @@
 
 Usage: python build_lib.py [--jobs N]
 
-Each csrc/*.hip file is compiled to an object in _build/ (in parallel), then linked into
+Each *.hip file under csrc/ is compiled to an object in _build/ (in parallel), then linked into
 libfa_gfx950.so next to this file. The compiler's kernel-resource-usage remarks are parsed into
 kernel_resources.json (VGPR/AGPR/SGPR counts, LDS bytes, scratch, occupancy per kernel symbol), which
 the tuner's resource filter and the resource report read on hosts without a GPU. Each file is also
@@ -44,7 +44,7 @@ HIPCC_FLAGS = [
 # The forward and GEMM kernels make no NaN of finite operands (masked scores are -inf, kept: infinities stay
 # honoured): without the promise to honour NaN, fmaxf needs no operand canonicalisation and v_max3 applies
 # directly to MFMA results. What they do with a NaN operand is pinned by the tests, not by the language. Everything
-# else keeps the promise: NaN is part of the 4-bit cache's format, its kernels and the backward's choose by values
+# else keeps the promise: NaN is part of the caches' formats, their kernels and the backward's choose by values
 # that may be NaN, and the host code refuses NaN arguments.
 NAN_FREE = {"fa_fwd", "fa_fwd16", "gemm"}
 NAN_FREE_FLAGS = ["-fno-honor-nans", "-mno-amdgpu-ieee"]
@@ -227,7 +227,7 @@ def _compile_resource_table(resources: dict[str, dict[str, object]]) -> Path:
 
 def build(jobs: int | None = None, verbose: bool = True) -> Path:
     BUILD.mkdir(exist_ok=True)
-    sources = sorted(CSRC.glob("*.hip"))
+    sources = sorted(CSRC.rglob("*.hip"))
     if not sources:
         raise RuntimeError(f"no HIP sources under {CSRC}")
     jobs = jobs or min(len(sources), max(1, min(16, os.cpu_count() or 1)))

@@ -168,6 +168,92 @@ struct Kv4KernelEntry {
 
 const Kv4KernelEntry* kv4_registry(int* count);
 
+// The paged 8-bit cache (kv8.hip, kv8_pages.hip). Strides of it are in bytes. The page layout is that of kv8_cache in
+// include/fa_gfx950.h.
+struct Kv8Pages {
+  uint8_t* data;  // of one layer (append, attention), or of all
+  int32_t* table;
+  int32_t* refs;
+  int64_t layer_stride, page_stride;
+  int64_t scales_at;    // bytes of a page's codes
+  int32_t pages, columns;
+  int32_t blocks_log2;  // 32-token blocks of a page
+};
+
+struct Kv8AppendParams {
+  Kv8Pages cache;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* k_values;  // nullable (both): what the appended rows now stand for
+  uint16_t* v_values;
+  const int32_t* start;
+  const int32_t* count;  // nullable: all rows
+  int64_t sk[3], sv[3], skv[3], svv[3];
+  int32_t B, Hkv, rows, capacity;
+  int32_t blocks;  // blocks that `rows` tokens may lie in
+};
+
+struct Kv8AttendParams {
+  Kv8Pages cache;
+  const uint16_t* q;
+  uint16_t* o;
+  float* lse;  // nullable
+  const int32_t* start;
+  const int32_t* count;  // nullable: all rows
+  float* ws_o;           // splits > 1: unnormalised partial sums [slots][H][M][D]
+  float* ws_ml;          // splits > 1: their row maximum (log2 units) and sum [slots][H][M][2]
+  int64_t sq[3], so[3], sl[3];
+  int32_t B, H, Hkv, M, group, capacity;
+  int32_t causal, splits;
+  int32_t slots;  // splits that all sequences may have together: B * splits
+  int32_t row_blocks;
+  float c;  // scale * log2(e)
+};
+
+struct Kv8KernelEntry {
+  int32_t dtype;
+  int32_t D;
+  const void* append;
+  const void* merge[3];   // one, four and sixteen waves to a row
+  const void* attend[3];  // 16 rows shared by a workgroup's waves, 32 rows shared, chunks of a prompt
+  int32_t per_cu[3];      // workgroups of each that the split rule counts on per CU
+  int32_t chunk_rows;     // query rows of a workgroup of the last
+};
+
+const Kv8KernelEntry* kv8_registry(int* count);
+
+struct Kv8PageParams {
+  Kv8Pages cache;
+  const int32_t* a;      // start, parent or length
+  const int32_t* count;  // nullable: all rows
+  int32_t* result;       // missing or used pages
+  int32_t* plan;         // workspace: number of copies, pages in use
+  int32_t* source;       // workspace: pages to be copied, and where to
+  int32_t* target;
+  int32_t* mark;         // workspace, by page: last sharer and number of sharers (reserve), new page (compact)
+  int32_t* wants;        // workspace, by item (reserve)
+  int32_t B, rows, capacity, layers;
+  int32_t span;            // entries that `rows` tokens may lie in
+  int32_t columns_each;    // columns of the table that a workgroup takes (fork)
+  int32_t slices;          // parts of a page that are copied by themselves
+  int64_t slice_bytes, page_bytes;
+};
+
+// Kernels of the page operations, and the threads of a workgroup of each.
+struct Kv8PageKernels {
+  const void* reserve;
+  const void* fork;
+  const void* truncate;
+  const void* compact;
+  const void* copy;  // of what reserve planned
+  const void* move;  // of what compact planned
+  int32_t plan_threads, threads;
+};
+
+constexpr int kForkEntries = 16384;  // entries of the table that a workgroup of fork holds in LDS (KV8_MAX_FORK)
+
+Kv8PageKernels kv8_page_kernels();
+
 // The last error of the calling thread (fa_last_error), shared by the files that implement the C ABI.
 int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int ok();

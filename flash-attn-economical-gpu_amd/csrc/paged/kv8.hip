@@ -1,0 +1,987 @@
+// Paged 8-bit key/value cache for gfx950: append of new rows, and attention over the cache.
+//
+// Format. 32 consecutive tokens of a kv head are a block: one scale byte e, standing for 2^(e - 127), and an e4m3
+// code for each channel. gfx950 converts such codes to fp16 or bf16, scale included, two to an instruction
+// (v_cvt_scalef32_pk_*_fp8), so the products stay 16-bit MFMAs on exact values. A floating code keeps its relative
+// step whatever the scale, so one power of two for 32 rows costs nothing until a channel lies 2^14 below the block's
+// largest value. Blocks never cross a page, and a tile of the attention kernels is one or two whole blocks.
+#include <type_traits>
+
+#include "../fa_common.h"
+#include "../fa_kernels.h"
+#include "../kv_split.h"
+#include "../../../include/fa_gfx950.h"
+
+namespace fa {
+
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef short shortx2 __attribute__((ext_vector_type(2)));
+typedef unsigned short ushortx2 __attribute__((ext_vector_type(2)));
+
+template <typename Tag>
+struct Fp8;
+template <>
+struct Fp8<f16_t> {
+  // Range of scale bytes: the smallest and largest values, 2^-9 and 448 times 2^(e - 127), are numbers of the type.
+  static constexpr uint32_t kFloor = 112, kCeil = 134;
+  static constexpr uint32_t kInfBits = 0x7c00u;
+  static constexpr uint32_t kMaxBits = 0x7b00u;  // 448 * 2^7
+  template <bool HIGH>
+  __device__ static inline shortx2 encode(shortx2 old, uint32_t pair, float scale) {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(old, __builtin_bit_cast(half2_t, pair), scale, HIGH);
+  }
+  template <bool HIGH>
+  __device__ static inline uint32_t decode(uint32_t codes, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, HIGH));
+  }
+};
+template <>
+struct Fp8<bf16_t> {
+  static constexpr uint32_t kFloor = 10, kCeil = 246;
+  static constexpr uint32_t kInfBits = 0x7f80u;
+  static constexpr uint32_t kMaxBits = 0x7f60u;  // 448 * 2^119
+  template <bool HIGH>
+  __device__ static inline shortx2 encode(shortx2 old, uint32_t pair, float scale) {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(old, __builtin_bit_cast(bf16x2_t, pair), scale, HIGH);
+  }
+  template <bool HIGH>
+  __device__ static inline uint32_t decode(uint32_t codes, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, HIGH));
+  }
+};
+
+// Scale of a cached byte: one past the largest that append writes would make infinities of codes.
+template <typename Tag>
+__device__ inline float block_scale(uint32_t e) {
+  return scale_of(e < Fp8<Tag>::kCeil ? e : Fp8<Tag>::kCeil);
+}
+
+// Four codes (a dword) to 16-bit values, two to a dword.
+template <typename Tag>
+__device__ inline u32x2 decode4(uint32_t codes, float scale) {
+  return (u32x2){Fp8<Tag>::template decode<false>(codes, scale), Fp8<Tag>::template decode<true>(codes, scale)};
+}
+// Eight codes (two dwords): an MFMA operand.
+template <typename Tag>
+__device__ inline u32x4 decode8(uint32_t low, uint32_t high, float scale) {
+  const u32x2 a = decode4<Tag>(low, scale), b = decode4<Tag>(high, scale);
+  return (u32x4){a[0], a[1], b[0], b[1]};
+}
+template <typename Tag>
+__device__ inline uint32_t encode4(uint32_t a, uint32_t b, float scale) {
+  shortx2 x = (shortx2){0, 0};
+  x = Fp8<Tag>::template encode<false>(x, a, scale);
+  x = Fp8<Tag>::template encode<true>(x, b, scale);
+  return __builtin_bit_cast(uint32_t, x);
+}
+// Does one of a dword's four codes stand for NaN?
+__device__ inline bool has_nan(uint32_t codes) {
+  return (((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+}
+
+__device__ inline uint32_t wave_max(uint32_t x) {
+#pragma unroll
+  for (int s = 1; s < 64; s *= 2) {
+    const uint32_t o = __shfl_xor(x, s, 64);
+    x = x > o ? x : o;
+  }
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
+// The page of a sequence's column, or -1. `column` lies inside the table.
+__device__ inline int page_at(const Kv8Pages& c, int b, int64_t column) {
+  const int page = c.table[(int64_t)b * c.columns + column];
+  return (uint32_t)page < (uint32_t)c.pages ? page : -1;
+}
+
+// Append: a wave takes a block, 16 channels of a row to a lane and step: the tokens that the block holds already, the
+// new rows, zeros behind them. The largest finite magnitude of all gives the scale (integer compares: any host that
+// follows the definition gets the same bytes), and the block is written whole, so what it holds depends on its tokens
+// only, not on rows that were drafted in vain or on what the page held before.
+template <typename Tag, int D>
+__global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendParams p) {
+  typedef Fp8<Tag> F;
+  constexpr int UPR = D / 16, PER = 32 * UPR / 64;
+  const int lane = threadIdx.x & 63;
+  int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (id >= (int64_t)p.B * p.blocks * p.Hkv) return;
+  const bool is_v = blockIdx.y != 0;
+  const int h = (int)(id % p.Hkv);  // consecutive rows of a projection output [B, S, H, D] are its heads
+  id /= p.Hkv;
+  const int blk = (int)(id % p.blocks), b = (int)(id / p.blocks);
+  const int64_t start = p.start[b];
+  int n = p.count != nullptr ? p.count[b] : p.rows;
+  n = n < 0 ? 0 : (n > p.rows ? p.rows : n);
+  const int64_t at = ((start >> 5) + blk) * 32;  // the block's first token
+  if (at >= start + p.rows) return;
+  const int64_t low = start > 0 ? start : 0;
+  const int64_t high = start + n < p.capacity ? start + n : p.capacity;
+  // rows [r0, r1) of the block are new
+  const int r0 = (int)(low - at < 0 ? 0 : (low - at > 32 ? 32 : low - at));
+  const int r1 = (int)(high - at < 0 ? 0 : (high - at > 32 ? 32 : high - at));
+  const Kv8Pages& c = p.cache;
+  int page = -1;
+  if (r1 > r0) {
+    page = page_at(c, b, at >> (5 + c.blocks_log2));
+    if (page >= 0 && c.refs[page] != 1) page = -1;
+  }
+  uint16_t* out = is_v ? p.v_values : p.k_values;
+  if (page < 0 && out == nullptr) return;
+  const int64_t* st = is_v ? p.sv : p.sk;
+  const uint16_t* src = (is_v ? p.v : p.k) + b * st[0] + h * st[1];
+  const int sub = (int)(at >> 5) & ((1 << c.blocks_log2) - 1);
+  uint8_t* base = c.data + page * c.page_stride;
+  uint8_t* codes = base + (((int64_t)(2 * h + is_v) << c.blocks_log2) + sub) * (32 * D);
+  uint8_t* scale_byte = base + c.scales_at + 2 * (((int64_t)h << c.blocks_log2) + sub) + is_v;
+  u32x4 x[PER][2];
+  uint32_t e = 0;
+  if (page >= 0) {
+    const float old = block_scale<Tag>(*scale_byte);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int u = lane + 64 * i, row = u / UPR, part = u % UPR;
+      x[i][0] = x[i][1] = (u32x4){0, 0, 0, 0};
+      if (row >= r0 && row < r1) {
+        const uint16_t* from = src + (at + row - start) * st[2] + part * 16;
+        x[i][0] = reinterpret_cast<const u32x4*>(from)[0];
+        x[i][1] = reinterpret_cast<const u32x4*>(from)[1];
+      } else if (row < r0) {
+        const u32x4 held = *reinterpret_cast<const u32x4*>(codes + row * D + part * 16);
+        x[i][0] = decode8<Tag>(held[0], held[1], old);
+        x[i][1] = decode8<Tag>(held[2], held[3], old);
+      }
+    }
+    // the largest magnitude, two channels at a time; magnitudes of a type compare as whole numbers
+    ushortx2 both = (ushortx2){0, 0};
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        both = __builtin_elementwise_max(both, __builtin_bit_cast(ushortx2, x[i][j / 4][j % 4] & 0x7fff7fffu));
+    uint32_t top = wave_max(both[0] > both[1] ? both[0] : both[1]);
+    bool rare = top > F::kMaxBits;
+    if (rare) {
+      top = 0;  // of the finite ones; the others, and values past the largest code's, are looked for below
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const uint32_t a = (x[i][j / 8][j % 8 / 2] >> (16 * (j & 1))) & 0x7fffu;
+          top = a < F::kInfBits && a > top ? a : top;
+        }
+      top = wave_max(top);
+    }
+    const int power = (int)((__float_as_uint(DT<Tag>::to_float((uint16_t)top)) + 0x1fffffu) >> 23) - 8;
+    e = power < (int)F::kFloor ? F::kFloor : (power > (int)F::kCeil ? F::kCeil : (uint32_t)power);
+    const float scale = scale_of(e);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      u32x4 nan = (u32x4){0, 0, 0, 0};
+      if (rare) {  // NaN for what is not finite; values past the largest code's become that
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int sh = 16 * (j & 1);
+          const uint32_t word = x[i][j / 8][j % 8 / 2], a = (word >> sh) & 0x7fffu;
+          uint32_t to = a > F::kMaxBits ? (a >= F::kInfBits ? 0u : F::kMaxBits) : a;
+          if (a < F::kInfBits) to |= (word >> sh) & 0x8000u;
+          if (a >= F::kInfBits) nan[j / 4] |= 0x7fu << (8 * (j % 4));
+          x[i][j / 8][j % 8 / 2] = (word & ~(0xffffu << sh)) | (to << sh);
+        }
+      }
+      const int u = lane + 64 * i;
+      u32x4 held;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        held[j] = encode4<Tag>(x[i][j / 2][2 * (j & 1)], x[i][j / 2][2 * (j & 1) + 1], scale) | nan[j];
+      *reinterpret_cast<u32x4*>(codes + (int64_t)u * 16) = held;
+      if (out != nullptr) {
+        x[i][0] = decode8<Tag>(held[0], held[1], scale);
+        x[i][1] = decode8<Tag>(held[2], held[3], scale);
+      }
+    }
+    if (lane == 0) *scale_byte = (uint8_t)e;
+  }
+  if (out == nullptr) return;
+  const int64_t* so = is_v ? p.svv : p.skv;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int u = lane + 64 * i, row = u / UPR, part = u % UPR;
+    const int64_t t = at + row - start;
+    if (t < 0 || t >= p.rows) continue;
+    const bool written = page >= 0 && row >= r0 && row < r1;
+    u32x4* to = reinterpret_cast<u32x4*>(out + b * so[0] + h * so[1] + t * so[2] + part * 16);
+    to[0] = written ? x[i][0] : (u32x4){0, 0, 0, 0};
+    to[1] = written ? x[i][1] : (u32x4){0, 0, 0, 0};
+  }
+}
+
+// The rows that a group of query rows sees. Query rows are (position, head of the group): row r is head r % group at
+// position r / group, and a workgroup's rows share its kv head's cache.
+struct Rows {
+  int rows, live;  // rows of the kv head, and those before count
+  int keys;        // of the sequence
+  int group;
+  int64_t start;
+  bool causal;
+  __device__ inline Rows(const Kv8AttendParams& p, int b) {
+    const int n = p.count != nullptr ? p.count[b] : p.M;
+    rows = p.M * p.group;
+    live = (n < 0 ? 0 : (n > p.M ? p.M : n)) * p.group;
+    keys = visible_keys(p.start, p.count, b, p.M, p.capacity);
+    group = p.group;
+    start = p.start[b];
+    causal = p.causal != 0;
+  }
+  // keys that row r sees, if it is live
+  __device__ inline int sees(int r) const {
+    const int64_t e = causal ? start + r / group + 1 : keys;
+    return (int)(e < 0 ? 0 : (e > keys ? keys : e));
+  }
+  // most keys that one of the live rows in [r, r + n) sees, and the fewest (0 if one of them is not live)
+  __device__ inline int most(int r, int n) const { return r >= live ? 0 : sees(r + n <= live ? r + n - 1 : live - 1); }
+  __device__ inline int least(int r, int n) const { return r + n <= live ? sees(r) : 0; }
+  // fewest that a live row sees
+  __device__ inline int live_least(int r) const { return r < live ? sees(r) : 0x7fffffff; }
+};
+
+template <int N, int J = 0, typename Fn>
+__device__ inline void for_each(Fn& f) {
+  if constexpr (J < N) {
+    f(std::integral_constant<int, J>{});
+    for_each<N, J + 1>(f);
+  }
+}
+
+// Attention over the cache, up to 32 query rows to a kv head. A wave holds 16 R query rows (columns of every product)
+// and walks 32-key tiles, which are blocks:
+//   S^T = K Q^T     A = K rows: lane (key, 16 of each 64 channels) reads its channels and converts them in place
+//   O^T += V^T P^T  A = V^T: lane (channels, 8 keys) reads the keys' codes of its D / 16 channels, converts, and
+//                   regroups them by channel with byte permutes; P^T is S^T's accumulator as it stands
+// so nothing passes through LDS but the waves' sums at the end. A lane keeps the table entries of its wave's next 64
+// tiles, so that a page number costs no load in the loop; a tile without a page is passed over.
+// The four waves hold the same rows and take turns at the tiles. A wave has one tile's registers: the next tile's keys are
+// asked for when the scores stand, its values when the second product does, so that half a tile or more is in flight.
+template <typename Tag, int D, int R>
+struct Kv8Attend {
+  static constexpr int WAVES = 4;
+  static constexpr int KS = D / 32;   // k = 32 steps over D
+  static constexpr int CPL = D / 16;  // channels of V per lane
+  static constexpr int KW = D / 16;   // dwords of K codes per lane and key
+  static constexpr int VW = CPL / 4;  // dwords of V codes per lane and key
+  typedef DT<Tag> E;
+  typedef Fp8<Tag> F;
+
+  // One lane's share of a block, as stored.
+  typedef uint32_t Keys[2][KW];
+  typedef uint32_t Values[8][VW];
+
+  __device__ static inline void load_keys(Keys& k, const uint8_t* from, int lane) {
+    from += (uint32_t)((lane & 15) * D + 16 * (lane >> 4));
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(from + 16 * i * D + 64 * j);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) k[i][4 * j + w] = x[w];
+      }
+  }
+  // Keys of a lane's k-slots in the second product: slot i is key 4 g + (i & 3) + 16 (i >> 2).
+  __device__ static inline void load_values(Values& v, const uint8_t* from, int lane) {
+    from += (uint32_t)(4 * (lane >> 4) * D + (lane & 15) * CPL);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint8_t* at = from + ((i & 3) + 16 * (i >> 2)) * D;
+      if constexpr (VW == 1) {
+        v[i][0] = *reinterpret_cast<const uint32_t*>(at);
+      } else {
+        typedef uint32_t words_t __attribute__((ext_vector_type(VW)));
+        const words_t x = *reinterpret_cast<const words_t*>(at);
+#pragma unroll
+        for (int w = 0; w < VW; ++w) v[i][w] = x[w];
+      }
+    }
+  }
+
+  struct State {
+    floatx4 o[CPL][R];
+    float m[R], l[R];
+  };
+
+  // The n-th key's values times P, if it is marked in `bad`: a product of its own, whose result only the rows that see
+  // the key take.
+  __device__ static inline void add_alone(State& s, const Values& v, float scale, const u32x4 (&pb)[R], uint32_t bad, int n,
+                                          int key0, const int (&see)[R], int lane) {
+    const int slot = (n & 3) + 4 * (n >> 4);
+    const bool mine = lane >> 4 == ((n >> 2) & 3) && (bad >> slot & 1u) != 0;
+    if (!__any(mine)) return;
+    uint32_t code[VW] = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i == slot) {
+#pragma unroll
+        for (int w = 0; w < VW; ++w) code[w] = v[i][w];
+      }
+    auto pair = [&](auto jc) {
+      constexpr int j = decltype(jc)::value;
+      const uint32_t x = mine ? F::template decode<(j & 1) != 0>(code[j / 2], scale) : 0u;
+      u32x4 even, odd;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        even[i] = i == slot / 2 ? (x & 0xffffu) << (16 * (slot & 1)) : 0u;
+        odd[i] = i == slot / 2 ? (x >> 16) << (16 * (slot & 1)) : 0u;
+      }
+#pragma unroll
+      for (int rt = 0; rt < R; ++rt) {
+        const floatx4 zero = (floatx4){0.f, 0.f, 0.f, 0.f};
+        const floatx4 a = E::mfma16(even, pb[rt], zero), b = E::mfma16(odd, pb[rt], zero);
+        if (key0 + n < see[rt]) {
+          s.o[2 * j][rt] += a;
+          s.o[2 * j + 1][rt] += b;
+        }
+      }
+    };
+    for_each<CPL / 2>(pair);
+  }
+
+  // One tile: keys [key0, key0 + 32), of which row rt sees those below see[rt] (a lane's own row). e: its scale bytes.
+  // `edge`: a row does not see all of them; `unseen`: a live row does not see all of the sequence's keys among them.
+  // next_keys() and next_values() ask for the next tile's codes as soon as this one's have been used. (One body with
+  // branches for the edge: with a body of its own for whole tiles the registers of both are held, and 60 spilled.)
+  template <typename NextKeys, typename NextValues>
+  __device__ static inline void step(State& s, const u32x4 (&qf)[R][KS], const Keys& kc, Values& vc, uint32_t e, int key0,
+                                     const int (&see)[R], int keys, bool edge, bool unseen, float c, int lane,
+                                     NextKeys&& next_keys, NextValues&& next_values) {
+    const int g = lane >> 4;
+    const float ks = block_scale<Tag>(e & 255u), vs = block_scale<Tag>(e >> 8);
+    floatx4 x[2][R];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int rt = 0; rt < R; ++rt) x[i][rt] = (floatx4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const u32x4 a = decode8<Tag>(kc[i][2 * k], kc[i][2 * k + 1], ks);
+#pragma unroll
+        for (int rt = 0; rt < R; ++rt) x[i][rt] = E::mfma16(a, qf[rt][k], x[i][rt]);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    next_keys();
+    __builtin_amdgcn_sched_barrier(0);
+    u32x4 pb[R];
+#pragma unroll
+    for (int rt = 0; rt < R; ++rt) {
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (key0 + 16 * i + 4 * g + r >= see[rt]) x[i][rt][r] = FA_NEG_INF;
+      }
+      // a NaN score makes the row NaN: through P, whether or not the maximum moves
+      const float top = larger(larger(larger(x[0][rt][0], x[0][rt][1]), larger(x[0][rt][2], x[0][rt][3])),
+                               larger(larger(x[1][rt][0], x[1][rt][1]), larger(x[1][rt][2], x[1][rt][3])));
+      const float m_new = larger(s.m[rt], row_max(top));
+      if (__any(m_new > s.m[rt])) {
+        const float base = m_new == FA_NEG_INF ? 0.f : m_new;
+        const float f = fast_exp2((s.m[rt] - base) * c);
+        s.l[rt] *= f;
+#pragma unroll
+        for (int d = 0; d < CPL; ++d) s.o[d][rt] *= f;
+        s.m[rt] = m_new;
+      }
+      const float base = s.m[rt] == FA_NEG_INF ? 0.f : s.m[rt];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[i][rt][r] = fast_exp2(fmaf(x[i][rt][r] - base, c, weight_bias<Tag>()));
+          s.l[rt] += x[i][rt][r];
+        }
+      pb[rt] = (u32x4){E::pack2(x[0][rt][0], x[0][rt][1]), E::pack2(x[0][rt][2], x[0][rt][3]),
+                       E::pack2(x[1][rt][0], x[1][rt][1]), E::pack2(x[1][rt][2], x[1][rt][3])};
+    }
+    if (edge) {
+      // Rows behind the last key may hold anything, NaN too: they read as zeros. A NaN would be 0 x NaN to the rows
+      // that do not see its key: keys that have one (rare) leave the tile's product and are added one by one.
+      uint32_t bad = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool behind = key0 + 4 * g + (i & 3) + 16 * (i >> 2) >= keys;
+        bool nan = false;
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          if (behind) vc[i][w] = 0;
+          nan |= has_nan(vc[i][w]);
+        }
+        bad |= (nan ? 1u : 0u) << i;
+      }
+      if (!unseen) bad = 0;
+      if (__builtin_expect(__any(bad != 0), 0)) {
+#pragma unroll 1
+        for (int n = 0; n < 32; ++n) add_alone(s, vc, vs, pb, bad, n, key0, see, lane);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (bad >> i & 1u) {
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vc[i][w] = 0;
+          }
+      }
+    }
+    // channels 2 j and 2 j + 1 of the lane's CPL
+    auto pair = [&](auto jc) {
+      constexpr int j = decltype(jc)::value;
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = F::template decode<(j & 1) != 0>(vc[i][j / 2], vs);
+      u32x4 even, odd;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        even[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
+        odd[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
+      }
+#pragma unroll
+      for (int rt = 0; rt < R; ++rt) {
+        s.o[2 * j][rt] = E::mfma16(even, pb[rt], s.o[2 * j][rt]);
+        s.o[2 * j + 1][rt] = E::mfma16(odd, pb[rt], s.o[2 * j + 1][rt]);
+      }
+    };
+    for_each<CPL / 2>(pair);
+    __builtin_amdgcn_sched_barrier(0);
+    next_values();
+  }
+
+  // N channels N at .. of row r, whose maximum and sum are m and l. A row that saw no key (l = 0) is zeros, whatever its
+  // products with values that are no numbers left in o.
+  template <int N>
+  __device__ static inline void store_row(const Kv8AttendParams& p, int b, int hk, int slot, int r, const float (&o)[N],
+                                          float m, float l, int at) {
+    const int i = r / p.group, h = hk * p.group + r % p.group;
+    if (p.splits > 1) {
+      const int64_t w = ((int64_t)slot * p.H + h) * p.M + i;
+      float* dst = p.ws_o + w * D + at * N;
+#pragma unroll
+      for (int j = 0; j < N; j += 4)
+        *reinterpret_cast<floatx4*>(dst + j) =
+            l == 0.f ? (floatx4){0.f, 0.f, 0.f, 0.f} : (floatx4){o[j], o[j + 1], o[j + 2], o[j + 3]};
+      if (at == 0) {
+        p.ws_ml[2 * w] = m * p.c;
+        p.ws_ml[2 * w + 1] = l;
+      }
+    } else {
+      const float inv = 1.f / l;
+      uint16_t* dst = p.o + b * p.so[0] + h * p.so[1] + i * p.so[2] + at * N;
+#pragma unroll
+      for (int j = 0; j < N; j += 4)
+        *reinterpret_cast<u32x2*>(dst + j) = l == 0.f ? (u32x2){0u, 0u}
+                                                      : (u32x2){E::pack2(o[j] * inv, o[j + 1] * inv),
+                                                                E::pack2(o[j + 2] * inv, o[j + 3] * inv)};
+      if (at == 0 && p.lse != nullptr)
+        p.lse[b * p.sl[0] + h * p.sl[1] + i * p.sl[2]] =
+            l == 0.f ? FA_NEG_INF : (m * p.c + __builtin_amdgcn_logf(l) - weight_bias<Tag>()) * 0.6931471805599453f;
+    }
+  }
+
+  __device__ static void run(const Kv8AttendParams& p, float* smem) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c16 = lane & 15, g = lane >> 4;
+    int id = xcd_remap(blockIdx.x, gridDim.x);
+    // row blocks innermost: those of one split share its tiles in L2
+    const int rb = id % p.row_blocks;
+    id /= p.row_blocks;
+    const int slot = id % p.slots, hk = id / p.slots;
+    const Split part = find_split(p, slot, 0);
+    const int b = __builtin_amdgcn_readfirstlane(part.b);
+    if (b < 0) return;
+    const Rows q_rows(p, b);
+    const int row0 = rb * 16 * R, keys = q_rows.keys;
+
+    int see[R];  // keys that the lane's row sees
+    u32x4 qf[R][KS];
+    State s;
+#pragma unroll
+    for (int rt = 0; rt < R; ++rt) {
+      const int r = row0 + 16 * rt + c16;
+      const bool live = r < q_rows.live;
+      see[rt] = live ? q_rows.sees(r) : 0;
+      const uint16_t* q = p.q + b * p.sq[0] + (int64_t)(hk * p.group + (live ? r % p.group : 0)) * p.sq[1] +
+                          (int64_t)(live ? r / p.group : 0) * p.sq[2] + g * 16;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        qf[rt][k] = (u32x4){0, 0, 0, 0};
+        if (live) qf[rt][k] = *reinterpret_cast<const u32x4*>(q + 64 * (k / 2) + 8 * (k & 1));
+      }
+      s.m[rt] = FA_NEG_INF;
+      s.l[rt] = 0.f;
+#pragma unroll
+      for (int d = 0; d < CPL; ++d) s.o[d][rt] = (floatx4){0.f, 0.f, 0.f, 0.f};
+    }
+    const int least = __builtin_amdgcn_readfirstlane(q_rows.least(row0, 16 * R));
+    const int live_least = __builtin_amdgcn_readfirstlane(q_rows.live_least(row0));
+    const int tiles = (__builtin_amdgcn_readfirstlane(q_rows.most(row0, 16 * R)) + 31) / 32;
+    const int per = __builtin_amdgcn_readfirstlane(part.per);
+    const int64_t first = (int64_t)__builtin_amdgcn_readfirstlane(part.index) * per;
+    const int t1 = (int)(first + per < tiles ? first + per : tiles);
+    const Kv8Pages& pg = p.cache;
+    const int64_t half = (int64_t)(32 * D) << pg.blocks_log2;  // bytes of a page's keys of a head
+    const uint8_t* data = pg.data + 2 * hk * half;
+    const uint8_t* scales = pg.data + pg.scales_at + 2 * ((int64_t)hk << pg.blocks_log2);
+    const int* table = pg.table + (int64_t)b * pg.columns;
+    const int t0 = first < t1 ? (int)first + wave : t1;
+    int entries = -1;  // of the wave's next 64 tiles, one to a lane
+    int used = 0;      // tiles that were asked for
+    struct Place {
+      const uint8_t* keys;
+      const uint8_t* scales;
+      bool there;
+    };
+    auto locate = [&](int t) {
+      Place x = {nullptr, nullptr, false};
+      if (t >= t1) return x;
+      if ((used & 63) == 0) {
+        const int64_t mine = t + (int64_t)lane * WAVES;
+        entries = mine < t1 ? table[mine >> pg.blocks_log2] : -1;
+      }
+      const int page = __builtin_amdgcn_readlane(entries, used & 63);
+      ++used;
+      x.there = (uint32_t)page < (uint32_t)pg.pages;
+      const int sub = t & ((1 << pg.blocks_log2) - 1);
+      x.keys = data + page * pg.page_stride + sub * (32 * D);
+      x.scales = scales + page * pg.page_stride + 2 * sub;
+      return x;
+    };
+    Keys kc;
+    Values vc;
+    uint32_t e = 0, e_next = 0;
+    Place next = locate(t0);
+    auto next_keys = [&]() {
+      if (!next.there) return;
+      load_keys(kc, next.keys, lane);
+      e_next = *reinterpret_cast<const uint16_t*>(next.scales);
+    };
+    auto next_values = [&]() {
+      if (next.there) load_values(vc, next.keys + half, lane);
+    };
+    next_keys();
+    next_values();
+    for (int t = t0; t < t1; t += WAVES) {
+      const bool there = next.there;
+      e = e_next;
+      next = locate(t + WAVES);
+      if (!there) {
+        next_keys();
+        next_values();
+      } else {
+        step(s, qf, kc, vc, e, t * 32, see, keys, t * 32 + 32 > least,
+             (t * 32 + 32 < keys ? t * 32 + 32 : keys) > live_least, p.c, lane, next_keys, next_values);
+      }
+    }
+    // the waves' sums meet in LDS; wave w finishes rows 4 w .. 4 w + 3 of each 16, 16 lanes to a row
+    constexpr int ROW = D + 4;
+#pragma unroll
+    for (int rt = 0; rt < R; ++rt) {
+      const float l = xquad_sum(s.l[rt]);
+      float* dst = smem + (wave * 16 + c16) * ROW;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int d = 0; d < CPL; d += 4)
+          *reinterpret_cast<floatx4*>(dst + (4 * g + r) * CPL + d) =
+              (floatx4){s.o[d][rt][r], s.o[d + 1][rt][r], s.o[d + 2][rt][r], s.o[d + 3][rt][r]};
+      if (g == 0) {
+        dst[D] = s.m[rt];
+        dst[D + 1] = l;
+      }
+      __syncthreads();
+      const int row = 4 * wave + g;
+      float m = FA_NEG_INF;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) m = fmaxf(m, smem[(w * 16 + row) * ROW + D]);
+      float sum = 0.f, o[CPL];
+#pragma unroll
+      for (int j = 0; j < CPL; ++j) o[j] = 0.f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        const float* src = smem + (w * 16 + row) * ROW;
+        const float f = m == FA_NEG_INF ? 1.f : fast_exp2((src[D] - m) * p.c);
+        sum += f * src[D + 1];
+#pragma unroll
+        for (int j = 0; j < CPL; ++j) o[j] = fmaf(f, src[c16 * CPL + j], o[j]);
+      }
+      const int r = row0 + 16 * rt + row;
+      if (r < q_rows.rows) store_row<CPL>(p, b, hk, slot, r, o, m, sum, c16);
+      __syncthreads();
+    }
+  }
+};
+
+// Waves per SIMD: what the registers of a tile, Q and O allow.
+template <int D, int R>
+constexpr int attend8_waves() {
+  return D == 64 ? (R == 1 ? 5 : 4) : (D == 128 ? (R == 1 ? 4 : 2) : (R == 1 ? 2 : 1));
+}
+template <typename Tag, int D, int R>
+__global__ __launch_bounds__(256, (attend8_waves<D, R>())) void kv8_attend_kernel(Kv8AttendParams p) {
+  __shared__ __align__(16) float smem[4 * 16 * (D + 4)];
+  Kv8Attend<Tag, D, R>::run(p, smem);
+}
+
+// Chunks of a prompt: more than 32 query rows to a kv head. The workgroup's four waves, of 32 rows each, share the
+// conversion: a tile's codes are loaded a tile ahead, 16 channels of a row to a thread and step, converted once into
+// 16-bit rows in LDS (two stages, one barrier a tile), and both products read their fragments there, V's by the
+// transposing read. S^T = K Q^T and O^T = V^T P^T as above.
+template <typename Tag, int D>
+struct Kv8Chunk {
+  using L = LdsRows<D>;
+  typedef DT<Tag> E;
+  typedef Fp8<Tag> F;
+  static constexpr int WAVES = 4, QT = D == 256 ? 1 : 2;  // 16-row tiles of queries per wave
+  static constexpr int T = D == 256 ? 32 : 64;  // keys of a tile
+  static constexpr int NB = T / 32;             // its blocks
+  static constexpr int KT = T / 16, KS = D / 32, DT16 = D / 16, UPR = D / 16;
+  static constexpr int BLOCK = WAVES * QT * 16;
+  static constexpr int TILEB = T * L::ROWB, STAGEB = 2 * TILEB;
+  static constexpr int SMEM = 2 * STAGEB;
+  static constexpr int PER = T * UPR / 256;  // 16-channel units of K, and of V, per thread
+  static_assert(PER * 256 == T * UPR, "units");
+
+  struct Codes {
+    u32x4 k[PER], v[PER];
+    uint32_t e[PER];  // scale bytes of the unit's block
+    bool there[NB];
+  };
+
+  // block of the tile that a wave's i-th unit lies in
+  __device__ static inline int block_of(int i, int wave) { return D == 128 ? i : (D == 64 ? wave >> 1 : 0); }
+
+  // flags: words with a bit for each key of the tile whose values hold a NaN, for three tiles in turn
+  __device__ static void run(const Kv8AttendParams& p, char* smem, uint32_t (*flags)[2]) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c16 = lane & 15, g = lane >> 4;
+    int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int rb = id % p.row_blocks;
+    id /= p.row_blocks;
+    const int slot = id % p.slots, hk = id / p.slots;
+    const Split part = find_split(p, slot, 0);
+    const int b = __builtin_amdgcn_readfirstlane(part.b);
+    if (b < 0) return;
+    if (tid < 6) flags[tid / 2][tid % 2] = 0;
+    __syncthreads();
+    const Rows q_rows(p, b);
+    const int row0 = rb * BLOCK + wave * QT * 16, keys = q_rows.keys;
+    const int block_see = __builtin_amdgcn_readfirstlane(q_rows.most(rb * BLOCK, BLOCK));
+    const int wave_see = __builtin_amdgcn_readfirstlane(q_rows.most(row0, QT * 16));
+    const int least = __builtin_amdgcn_readfirstlane(q_rows.least(row0, QT * 16));
+    const int block_least = __builtin_amdgcn_readfirstlane(q_rows.live_least(rb * BLOCK));
+
+    int see[QT];
+    u32x4 qf[QT][KS];
+#pragma unroll
+    for (int j = 0; j < QT; ++j) {
+      const int r = row0 + 16 * j + c16;
+      const bool live = r < q_rows.live;
+      see[j] = live ? q_rows.sees(r) : 0;
+      const uint16_t* q = p.q + b * p.sq[0] + (int64_t)(hk * p.group + (live ? r % p.group : 0)) * p.sq[1] +
+                          (int64_t)(live ? r / p.group : 0) * p.sq[2] + 8 * g;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        qf[j][k] = (u32x4){0, 0, 0, 0};
+        if (live) qf[j][k] = *reinterpret_cast<const u32x4*>(q + 32 * k);
+      }
+    }
+    floatx4 o[DT16][QT];
+    float m[QT], l[QT];
+#pragma unroll
+    for (int j = 0; j < QT; ++j) {
+      m[j] = FA_NEG_INF;
+      l[j] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DT16; ++d) o[d][j] = (floatx4){0.f, 0.f, 0.f, 0.f};
+    }
+
+    // the split's keys, in tiles of T (its share is in tiles of 32)
+    const int64_t per = (int64_t)__builtin_amdgcn_readfirstlane(part.per) * 32;
+    const int64_t k_first = __builtin_amdgcn_readfirstlane(part.index) * per;
+    const int k_end = (int)(k_first + per < block_see ? k_first + per : block_see);
+#pragma unroll
+    for (int j = 0; j < QT; ++j) see[j] = see[j] < k_end ? see[j] : k_end;  // the next split may begin inside a tile
+    int live_least = __builtin_amdgcn_readfirstlane(q_rows.live_least(row0));
+    if (live_least < 0x7fffffff && live_least > k_end) live_least = k_end;
+    const Kv8Pages& pg = p.cache;
+    const int64_t half = (int64_t)(32 * D) << pg.blocks_log2;  // bytes of a page's keys of a head
+    const uint8_t* data = pg.data + 2 * hk * half;
+    const uint8_t* scales = pg.data + pg.scales_at + 2 * ((int64_t)hk << pg.blocks_log2);
+    const int* table = pg.table + (int64_t)b * pg.columns;
+    // pages of the tile at key0
+    auto entries = [&](int (&at)[NB], int64_t key0) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const int64_t key = key0 + 32 * n;
+        at[n] = key < k_end ? table[key >> (5 + pg.blocks_log2)] : -1;
+      }
+    };
+    // Past the last visible key nothing is read, and what stands there is zero: rows behind a sequence may hold anything.
+    auto fetch = [&](Codes& x, int64_t key0, const int (&at)[NB]) {
+      int page[NB];
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        page[n] = __builtin_amdgcn_readfirstlane(at[n]);
+        x.there[n] = (uint32_t)page[n] < (uint32_t)pg.pages;
+      }
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int n = block_of(i, wave), row = (tid + 256 * i) / UPR, part16 = tid % UPR;
+        const int at_page = NB == 2 && n ? page[NB - 1] : page[0];
+        const bool here = NB == 2 && n ? x.there[NB - 1] : x.there[0];
+        x.k[i] = x.v[i] = (u32x4){0, 0, 0, 0};
+        x.e[i] = 0x7f7f;
+        if (here) {
+          const int sub = (int)((key0 >> 5) + n) & ((1 << pg.blocks_log2) - 1);
+          const uint8_t* from = data + at_page * pg.page_stride + sub * (32 * D);
+          const uint32_t off = (uint32_t)((row & 31) * D + part16 * 16);
+          if (key0 + row < keys) {
+            x.k[i] = *reinterpret_cast<const u32x4*>(from + off);
+            x.v[i] = *reinterpret_cast<const u32x4*>(from + half + off);
+          }
+          x.e[i] = *reinterpret_cast<const uint16_t*>(scales + at_page * pg.page_stride + 2 * sub);
+        }
+      }
+    };
+    // `mark`: the tile has keys that one of the workgroup's live rows does not see
+    auto convert = [&](const Codes& x, uint32_t stage, int turn, bool mark) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int row = (tid + 256 * i) / UPR, part16 = tid % UPR;
+        char* dst = smem + stage + row * L::ROWB;
+        const uint32_t c0 = (uint32_t)(((2 * part16) ^ L::swz(row)) << 4), c1 = (uint32_t)(((2 * part16 + 1) ^ L::swz(row)) << 4);
+        const float ks = block_scale<Tag>(x.e[i] & 255u), vs = block_scale<Tag>(x.e[i] >> 8);
+        *reinterpret_cast<u32x4*>(dst + c0) = decode8<Tag>(x.k[i][0], x.k[i][1], ks);
+        *reinterpret_cast<u32x4*>(dst + c1) = decode8<Tag>(x.k[i][2], x.k[i][3], ks);
+        *reinterpret_cast<u32x4*>(dst + TILEB + c0) = decode8<Tag>(x.v[i][0], x.v[i][1], vs);
+        *reinterpret_cast<u32x4*>(dst + TILEB + c1) = decode8<Tag>(x.v[i][2], x.v[i][3], vs);
+        if (mark && (has_nan(x.v[i][0]) || has_nan(x.v[i][1]) || has_nan(x.v[i][2]) || has_nan(x.v[i][3])))
+          atomicOr(&flags[turn][row >> 5], 1u << (row & 31));
+      }
+    };
+    const uint32_t ro = L::row_off(lane), to = L::tr_off(lane);
+    auto step = [&](int key0, uint32_t stage, const bool (&there)[NB], int turn, auto edge_tile) {
+      constexpr bool EDGE = decltype(edge_tile)::value;
+      const uint32_t rowb = ro + stage, colb = to + stage;
+      // A NaN would be 0 x NaN to the rows that do not see its key: keys that have one (rare) are left out of the tile's
+      // product and added one by one, to the rows that see them.
+      uint64_t alone = 0;  // keys of the tile
+      if (EDGE && (key0 + T < keys ? key0 + T : keys) > live_least)
+        alone = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)flags[turn][0]) |
+                (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)flags[turn][1]) << 32;
+      // D = 64: all of K's fragments (32 registers) are asked for before the first product.
+      u32x4 ahead[KT][KS];
+      if constexpr (D == 64) {
+#pragma unroll
+        for (int i = 0; i < KT; ++i)
+#pragma unroll
+          for (int k = 0; k < KS; ++k) ahead[i][k] = L::frag(smem, rowb ^ (k << 6), i * 16 * L::ROWB);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      floatx4 x[KT][QT];
+#pragma unroll
+      for (int i = 0; i < KT; ++i) {
+#pragma unroll
+        for (int j = 0; j < QT; ++j) x[i][j] = (floatx4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const u32x4 a = D == 64 ? ahead[i][k] : L::frag(smem, rowb ^ (k << 6), i * 16 * L::ROWB);
+#pragma unroll
+          for (int j = 0; j < QT; ++j) x[i][j] = E::mfma16(a, qf[j][k], x[i][j]);
+        }
+      }
+      u32x4 pb[KT / 2][QT];
+#pragma unroll
+      for (int j = 0; j < QT; ++j) {
+        float top = FA_NEG_INF;
+#pragma unroll
+        for (int i = 0; i < KT; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (EDGE && (key0 + 16 * i + 4 * g + r >= see[j] || !there[i / 2])) x[i][j][r] = FA_NEG_INF;
+            top = larger(top, x[i][j][r]);
+          }
+        const float m_new = larger(m[j], row_max(top));
+        if (__any(m_new > m[j])) {
+          const float base = m_new == FA_NEG_INF ? 0.f : m_new;
+          const float f = fast_exp2((m[j] - base) * p.c);
+          l[j] *= f;
+#pragma unroll
+          for (int d = 0; d < DT16; ++d) o[d][j] *= f;
+          m[j] = m_new;
+        }
+        const float base = m[j] == FA_NEG_INF ? 0.f : m[j];
+        const float off = weight_bias<Tag>() - base * p.c;
+        // One instruction to an argument, where the rounding of m c, which does not cancel, stays small beside the
+        // argument: beyond, the difference is taken first.
+        if (__builtin_expect(__any(fabsf(base * p.c) > 0x1p14f), 0)) {
+#pragma unroll
+          for (int i = 0; i < KT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[i][j][r] = fmaf(x[i][j][r] - base, p.c, weight_bias<Tag>());
+        } else {
+#pragma unroll
+          for (int i = 0; i < KT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[i][j][r] = fmaf(x[i][j][r], p.c, off);
+        }
+#pragma unroll
+        for (int i = 0; i < KT; ++i) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            x[i][j][r] = fast_exp2(x[i][j][r]);
+            l[j] += x[i][j][r];
+          }
+          pb[i / 2][j][2 * (i & 1)] = E::pack2(x[i][j][0], x[i][j][1]);
+          pb[i / 2][j][2 * (i & 1) + 1] = E::pack2(x[i][j][2], x[i][j][3]);
+        }
+      }
+      // a lane's keys of an operand that are in `set`: 4 g .. + 3 (dwords 0, 1), then 16 further (dwords 2, 3)
+      auto lanes_of = [&](uint32_t set) {
+        const uint32_t x = set >> (4 * g);
+        u32x4 m;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const uint32_t two = x >> (16 * (n / 2) + 2 * (n & 1));
+          m[n] = (two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
+        }
+        return m;
+      };
+      __builtin_amdgcn_s_setprio(1);  // before a neighbour's softmax
+#pragma unroll
+      for (int d = 0; d < DT16; ++d)
+#pragma unroll
+        for (int i = 0; i < KT / 2; ++i) {
+          u32x4 v = L::tfrag(smem, colb ^ (d << 5), TILEB + i * 32 * L::ROWB);
+          if (EDGE && alone != 0) v &= ~lanes_of((uint32_t)(alone >> (32 * i)));
+#pragma unroll
+          for (int j = 0; j < QT; ++j) o[d][j] = E::mfma16(v, pb[i][j], o[d][j]);
+        }
+      __builtin_amdgcn_s_setprio(0);
+      if constexpr (EDGE) {
+#pragma unroll 1
+        for (; alone != 0; alone &= alone - 1) {
+          const int key = __builtin_ctzll(alone), i = key / 32;
+          const u32x4 one = lanes_of(1u << (key & 31));
+          uint32_t cols = colb + (uint32_t)(i * 32 * L::ROWB);
+          asm volatile("" : "+v"(cols));  // addresses worked out here, not held through the loops
+#pragma unroll
+          for (int j = 0; j < QT; ++j) {
+            u32x4 w;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const uint32_t low = pb[0][j][n], high = pb[KT / 2 - 1][j][n];
+              w[n] = i != 0 ? high : low;
+            }
+#pragma unroll
+            for (int d = 0; d < DT16; ++d) {
+              __builtin_amdgcn_sched_barrier(0);  // nor reads ahead
+              const u32x4 v = L::tfrag(smem, cols ^ (d << 5), TILEB) & one;
+              const floatx4 x = E::mfma16(v, w, (floatx4){0.f, 0.f, 0.f, 0.f});
+              if (key0 + key < see[j]) o[d][j] += x;
+            }
+          }
+        }
+      }
+    };
+    Codes next;
+    int ahead[NB];
+    entries(ahead, k_first);
+    if (k_first < k_end) fetch(next, k_first, ahead);
+    entries(ahead, k_first + T);
+    uint32_t stage = 0;
+    int turn = 0;
+    // Tiles that every row of the wave sees whole, up to a missing page; then the rest, on the diagonal, at the end or
+    // with pages missing: every wave makes the same number of passes in all, for the barriers.
+    auto pass = [&](int64_t key0, auto edge_tile) {
+      bool there[NB];
+#pragma unroll
+      for (int n = 0; n < NB; ++n) there[n] = next.there[n];
+      convert(next, stage, turn, key0 + T > block_least);
+      if (key0 + T < k_end) fetch(next, key0 + T, ahead);
+      entries(ahead, key0 + 2 * T);
+      const int after = turn == 2 ? 0 : turn + 1;
+      if (tid < 2) flags[after][tid] = 0;  // last read two barriers ago, written again after the next
+      wait_vm_lds_barrier<63>();  // LDS writes only: the codes just asked for stay in flight
+      if (key0 < wave_see) step((int)key0, stage, there, turn, edge_tile);
+      stage ^= STAGEB;
+      turn = after;
+    };
+    auto whole = [&]() {
+      bool all = next.there[0];
+#pragma unroll
+      for (int n = 1; n < NB; ++n) all = all && next.there[n];
+      return all;
+    };
+    int64_t key0 = k_first;
+    for (; key0 + T <= k_end && key0 + T <= least && whole(); key0 += T) pass(key0, std::false_type{});
+    for (; key0 < k_end; key0 += T) pass(key0, std::true_type{});
+
+#pragma unroll
+    for (int j = 0; j < QT; ++j) {
+      const float sum = xquad_sum(l[j]);
+      const int r = row0 + 16 * j + c16;
+      if (r >= q_rows.rows) continue;
+      const int i = r / p.group, h = hk * p.group + r % p.group;
+      if (p.splits > 1) {
+        const int64_t w = ((int64_t)slot * p.H + h) * p.M + i;
+#pragma unroll
+        for (int d = 0; d < DT16; ++d)  // a row that saw no key is zeros, whatever values that are no numbers left in o
+          *reinterpret_cast<floatx4*>(p.ws_o + w * D + 16 * d + 4 * g) = sum == 0.f ? (floatx4){0.f, 0.f, 0.f, 0.f} : o[d][j];
+        if (g == 0) {
+          p.ws_ml[2 * w] = m[j] * p.c;
+          p.ws_ml[2 * w + 1] = sum;
+        }
+      } else {
+        const float inv = 1.f / sum;
+        uint16_t* dst = p.o + b * p.so[0] + h * p.so[1] + i * p.so[2] + 4 * g;
+#pragma unroll
+        for (int d = 0; d < DT16; ++d)
+          *reinterpret_cast<u32x2*>(dst + 16 * d) =
+              sum == 0.f ? (u32x2){0u, 0u}
+                         : (u32x2){E::pack2(o[d][j][0] * inv, o[d][j][1] * inv), E::pack2(o[d][j][2] * inv, o[d][j][3] * inv)};
+        if (g == 0 && p.lse != nullptr)
+          p.lse[b * p.sl[0] + h * p.sl[1] + i * p.sl[2]] =
+              sum == 0.f ? FA_NEG_INF : (m[j] * p.c + __builtin_amdgcn_logf(sum) - weight_bias<Tag>()) * 0.6931471805599453f;
+      }
+    }
+  }
+};
+
+template <typename Tag, int D>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv8_chunk_kernel(Kv8AttendParams p) {
+  __shared__ __align__(1024) char smem[Kv8Chunk<Tag, D>::SMEM];
+  __shared__ uint32_t flags[3][2];
+  Kv8Chunk<Tag, D>::run(p, smem, flags);
+}
+
+template <typename Tag, int D, int WPR>
+__global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void kv8_merge_kernel(Kv8AttendParams p) {
+  merge_splits<Tag, D, WPR>(p);
+}
+
+#define KV8_ENTRY(TAG, DTYPE, D)                                                                            \
+  {DTYPE, D, (const void*)&kv8_append_kernel<TAG, D>,                                                       \
+   {(const void*)&kv8_merge_kernel<TAG, D, 1>, (const void*)&kv8_merge_kernel<TAG, D, 4>,                   \
+    (const void*)&kv8_merge_kernel<TAG, D, 16>},                                                            \
+   {(const void*)&kv8_attend_kernel<TAG, D, 1>, (const void*)&kv8_attend_kernel<TAG, D, 2>,                 \
+    (const void*)&kv8_chunk_kernel<TAG, D>},                                                                \
+   {attend8_waves<D, 1>(), attend8_waves<D, 2>(), 2}, Kv8Chunk<TAG, D>::BLOCK}
+
+static const Kv8KernelEntry kKv8Entries[] = {
+    KV8_ENTRY(f16_t, FA_DTYPE_F16, 64),   KV8_ENTRY(f16_t, FA_DTYPE_F16, 128),   KV8_ENTRY(f16_t, FA_DTYPE_F16, 256),
+    KV8_ENTRY(bf16_t, FA_DTYPE_BF16, 64), KV8_ENTRY(bf16_t, FA_DTYPE_BF16, 128), KV8_ENTRY(bf16_t, FA_DTYPE_BF16, 256),
+};
+
+const Kv8KernelEntry* kv8_registry(int* count) {
+  *count = (int)(sizeof(kKv8Entries) / sizeof(kKv8Entries[0]));
+  return kKv8Entries;
+}
+
+}  // namespace fa

@@ -28,6 +28,7 @@ import torch
 import gfx950_configs as cfgs
 import hip_lib
 import kv4
+import kv8
 from tuner import FlashAttentionLaunchSpec
 
 logger = logging.getLogger(__name__)
@@ -416,6 +417,42 @@ def sdpa_kv4(query: torch.Tensor, cache: kv4.Kv4Cache, start: torch.Tensor, *, c
             _keep_plan(key, plan)  # nothing had to be copied: calls of this form take the short way
     workspace = torch.empty(plan[1], dtype=torch.uint8, device=query.device) if plan[1] else None
     hip_lib.kv4_attend_planned(plan[0], cache._args, query, o, lse, workspace, start, count)
+    return (o, lse) if return_lse else o
+
+
+def sdpa_kv8(query: torch.Tensor, cache: kv8.Kv8Cache, start: torch.Tensor, *, count: torch.Tensor | None = None,
+             layer: int = 0, is_causal: bool = True, scale: float | None = None, return_lse: bool = False):
+    """Attention of new tokens' queries [B, H, M, D] over a layer of a paged 8-bit cache that already holds their keys:
+    `sdpa_kv4`'s rules for rows, lengths, empty rows and NaN, and its layout. Tokens whose page is missing are not seen.
+    start and count are int32 [B] on the GPU; nothing synchronises, and the call can be captured into a HIP graph."""
+    key = (cache._form, _form(query), kv4._form(start), None if count is None else kv4._form(count), layer, bool(is_causal),
+           None if scale is None else float(scale), bool(return_lse))
+    plan = _plans.get(key)
+    checked = plan is not None and not query.data_ptr() & 15
+    if not checked:
+        if query.dim() != 4:
+            raise ValueError(f"query must be 4-D [batch, heads, seq, head_dim], got {tuple(query.shape)}")
+        B, H, M, D = query.shape
+        if B != cache.batch or D != cache.head_dim or H < 1 or H % cache.kv_heads:
+            raise ValueError(f"query {tuple(query.shape)} does not fit a cache of {cache.batch} sequences, {cache.kv_heads} "
+                             f"heads of {cache.head_dim}")
+        if query.dtype != cache.dtype or query.device != cache.device:
+            raise ValueError(f"query is {query.dtype} on {query.device}, the cache {cache.dtype} on {cache.device}")
+        cache._layer(layer)
+        start, count = cache.positions(start, count)
+        query = hip_lib.operand(query, "query")
+    B, H, M, D = query.shape
+    o = torch.empty_strided((B, H, M, D), (max(M, 1) * H * D, D, H * D, 1), device=query.device, dtype=query.dtype)
+    lse = torch.empty(B, H, M, device=query.device, dtype=torch.float32) if return_lse else None
+    if not checked:
+        splits = kv8.choose_splits(B, H, cache.kv_heads, M, D, cache.capacity)
+        plan = (hip_lib.kv8_attend_plan(query, o, lse, sm_scale=D ** -0.5 if scale is None else scale, causal=is_causal,
+                                        splits=splits, layer=layer),
+                hip_lib.kv8_attend_workspace_bytes(B, H, M, D, splits))
+        if key[1:4] == (_form(query), kv4._form(start), None if count is None else kv4._form(count)):
+            _keep_plan(key, plan)  # nothing had to be copied: calls of this form take the short way
+    workspace = torch.empty(plan[1], dtype=torch.uint8, device=query.device) if plan[1] else None
+    hip_lib.kv8_attend_planned(plan[0], cache._args, query, o, lse, workspace, start, count)
     return (o, lse) if return_lse else o
 
 

@@ -18,7 +18,7 @@ import torch
 HERE = Path(__file__).resolve().parent
 LIB_PATH = HERE / "libfa_gfx950.so"
 RESOURCES_PATH = HERE / "kernel_resources.json"
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 FA_OK, FA_EINVAL, FA_ENOTSUP, FA_EHIP, FA_EWORKSPACE = 0, 1, 2, 3, 4
 FA_DTYPE_F16, FA_DTYPE_BF16 = 0, 1
@@ -162,6 +162,64 @@ class Kv4AttendArgs(ctypes.Structure):
     ]
 
 
+class Kv8CacheArgs(ctypes.Structure):
+    _fields_ = [
+        *((name, ctypes.c_void_p) for name in ("data", "table", "refs")),
+        ("layer_stride", ctypes.c_int64),
+        ("page_stride", ctypes.c_int64),
+        *((name, ctypes.c_int32) for name in ("B", "H_kv", "D", "dtype", "page", "pages", "columns", "capacity", "layers")),
+    ]
+
+
+class Kv8AppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", Kv8CacheArgs),
+        *((name, ctypes.c_void_p) for name in ("k", "v", "k_values", "v_values", "start", "count")),
+        ("k_stride", ctypes.c_int64 * 4),
+        ("v_stride", ctypes.c_int64 * 4),
+        ("k_values_stride", ctypes.c_int64 * 4),
+        ("v_values_stride", ctypes.c_int64 * 4),
+        ("rows", ctypes.c_int32),
+        ("layer", ctypes.c_int32),
+    ]
+
+
+class Kv8AttendArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", Kv8CacheArgs),
+        *((name, ctypes.c_void_p) for name in ("q", "o", "lse", "workspace")),
+        ("workspace_bytes", ctypes.c_int64),
+        ("start", ctypes.c_void_p),
+        ("count", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 4),
+        ("o_stride", ctypes.c_int64 * 4),
+        ("lse_stride", ctypes.c_int64 * 3),
+        ("H", ctypes.c_int32),
+        ("M", ctypes.c_int32),
+        ("sm_scale", ctypes.c_float),
+        ("causal", ctypes.c_int32),
+        ("splits", ctypes.c_int32),
+        ("layer", ctypes.c_int32),
+    ]
+
+
+class Kv8ReserveArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", Kv8CacheArgs),
+        *((name, ctypes.c_void_p) for name in ("start", "count", "missing", "workspace")),
+        ("workspace_bytes", ctypes.c_int64),
+        ("rows", ctypes.c_int32),
+    ]
+
+
+class Kv8CompactArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", Kv8CacheArgs),
+        *((name, ctypes.c_void_p) for name in ("used", "workspace")),
+        ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
 # Every symbol include/fa_gfx950.h declares, with its ctypes signature.
 SIGNATURES = {
     "fa_abi_version": (ctypes.c_int, []),
@@ -225,6 +283,17 @@ SIGNATURES = {
     "kv4_attend": (ctypes.c_int, [ctypes.POINTER(Kv4AttendArgs), ctypes.c_void_p]),
     "kv4_attend_workspace_bytes": (ctypes.c_int64, [ctypes.c_int32] * 5),
     "kv4_attend_splits": (ctypes.c_int32, [ctypes.c_int32] * 6),
+    "kv8_page_bytes": (ctypes.c_int64, [ctypes.c_int32] * 3),
+    "kv8_append": (ctypes.c_int, [ctypes.POINTER(Kv8AppendArgs), ctypes.c_void_p]),
+    "kv8_attend": (ctypes.c_int, [ctypes.POINTER(Kv8AttendArgs), ctypes.c_void_p]),
+    "kv8_attend_workspace_bytes": (ctypes.c_int64, [ctypes.c_int32] * 5),
+    "kv8_attend_splits": (ctypes.c_int32, [ctypes.c_int32] * 6),
+    "kv8_reserve": (ctypes.c_int, [ctypes.POINTER(Kv8ReserveArgs), ctypes.c_void_p]),
+    "kv8_reserve_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(Kv8CacheArgs), ctypes.c_int32]),
+    "kv8_fork": (ctypes.c_int, [ctypes.POINTER(Kv8CacheArgs), ctypes.c_void_p, ctypes.c_void_p]),
+    "kv8_truncate": (ctypes.c_int, [ctypes.POINTER(Kv8CacheArgs), ctypes.c_void_p, ctypes.c_void_p]),
+    "kv8_compact": (ctypes.c_int, [ctypes.POINTER(Kv8CompactArgs), ctypes.c_void_p]),
+    "kv8_compact_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(Kv8CacheArgs)]),
 }
 
 
@@ -560,14 +629,14 @@ def _strides4_of(t: torch.Tensor):
     return _I64x4(b if B > 1 else 0, h if H > 1 else 0, r if S > 1 else D, d if D > 1 else 1)
 
 
-def _launch(fn, args, device: torch.device, what: str) -> None:
-    """One C entry on the tensors' device and its current stream."""
+def _launch(fn, args, device: torch.device, what: str, *more) -> None:
+    """One C entry on the tensors' device and its current stream; `more` arguments follow the block."""
     index = device.index
     if index == torch.cuda.current_device():
-        code = fn(ctypes.byref(args), _raw_stream(index) if _raw_stream is not None else _stream_ptr(device))
+        code = fn(ctypes.byref(args), *more, _raw_stream(index) if _raw_stream is not None else _stream_ptr(device))
     else:
         with torch.cuda.device(index):
-            code = fn(ctypes.byref(args), _stream_ptr(device))
+            code = fn(ctypes.byref(args), *more, _stream_ptr(device))
     if code:
         check(code, what)
 
@@ -675,3 +744,100 @@ def kv4_attend_planned(plan: bytes, cache: Kv4CacheArgs, q: torch.Tensor, o: tor
     if workspace is not None:
         args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.numel()
     _launch(load().kv4_attend, args, q.device, "kv4_attend")
+
+
+def kv8_page_bytes(H_kv: int, page: int, D: int) -> int:
+    return int(load().kv8_page_bytes(H_kv, page, D))
+
+
+@functools.lru_cache(maxsize=4096)
+def kv8_attend_workspace_bytes(B: int, H: int, M: int, D: int, splits: int) -> int:
+    return int(load().kv8_attend_workspace_bytes(B, H, M, D, splits))
+
+
+def kv8_append_plan(k: torch.Tensor, v: torch.Tensor, k_values: torch.Tensor | None, v_values: torch.Tensor | None, *,
+                    layer: int) -> bytes:
+    """kv8_append's argument block for these tensors' shapes and strides (no address in it is used)."""
+    args = Kv8AppendArgs()
+    args.k_stride, args.v_stride = _strides4_of(k), _strides4_of(v)
+    if k_values is not None:
+        args.k_values_stride, args.v_values_stride = _strides4_of(k_values), _strides4_of(v_values)
+    args.rows, args.layer = k.shape[2], layer
+    return bytes(args)
+
+
+def kv8_append_planned(plan: bytes, cache: Kv8CacheArgs, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor,
+                       count: torch.Tensor | None, k_values: torch.Tensor | None, v_values: torch.Tensor | None) -> None:
+    """Append rows to a paged cache on the current stream; the caller has matched the tensors to cache and plan."""
+    args = Kv8AppendArgs.from_buffer_copy(plan)
+    args.cache = cache
+    args.k, args.v, args.start = k.data_ptr(), v.data_ptr(), start.data_ptr()
+    if count is not None:
+        args.count = count.data_ptr()
+    if k_values is not None:
+        args.k_values, args.v_values = k_values.data_ptr(), v_values.data_ptr()
+    _launch(load().kv8_append, args, k.device, "kv8_append")
+
+
+def kv8_attend_plan(q: torch.Tensor, o: torch.Tensor, lse: torch.Tensor | None, *, sm_scale: float, causal: bool,
+                    splits: int, layer: int) -> bytes:
+    """kv8_attend's argument block for these tensors' shapes and strides (no address in it is used)."""
+    args = Kv8AttendArgs()
+    if lse is not None:
+        args.lse_stride = (ctypes.c_int64 * 3)(*lse.stride())
+    args.q_stride, args.o_stride = _strides4_of(q), _strides4_of(o)
+    args.H, args.M, args.layer = q.shape[1], q.shape[2], layer
+    args.sm_scale, args.causal, args.splits = float(sm_scale), int(bool(causal)), int(splits)
+    return bytes(args)
+
+
+def kv8_attend_planned(plan: bytes, cache: Kv8CacheArgs, q: torch.Tensor, o: torch.Tensor, lse: torch.Tensor | None,
+                       workspace: torch.Tensor | None, start: torch.Tensor, count: torch.Tensor | None) -> None:
+    """Attention over a paged cache on the current stream; the caller has matched the tensors to cache and plan."""
+    args = Kv8AttendArgs.from_buffer_copy(plan)
+    args.cache = cache
+    args.q, args.o, args.start = q.data_ptr(), o.data_ptr(), start.data_ptr()
+    if count is not None:
+        args.count = count.data_ptr()
+    if lse is not None:
+        args.lse = lse.data_ptr()
+    if workspace is not None:
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    _launch(load().kv8_attend, args, q.device, "kv8_attend")
+
+
+_kv8_workspaces: dict[tuple, int] = {}
+
+
+def kv8_reserve_workspace_bytes(form: tuple, cache: Kv8CacheArgs, rows: int) -> int:
+    """By the cache's form, which its sizes follow from."""
+    need = _kv8_workspaces.get((form, rows))
+    if need is None:
+        if len(_kv8_workspaces) >= 4096:
+            _kv8_workspaces.clear()
+        need = _kv8_workspaces[(form, rows)] = int(load().kv8_reserve_workspace_bytes(ctypes.byref(cache), rows))
+    return need
+
+
+def kv8_compact_workspace_bytes(cache: Kv8CacheArgs) -> int:
+    return int(load().kv8_compact_workspace_bytes(ctypes.byref(cache)))
+
+
+def kv8_reserve(cache: Kv8CacheArgs, start: torch.Tensor, count: torch.Tensor | None, rows: int, missing: torch.Tensor,
+                workspace: torch.Tensor, device: torch.device) -> None:
+    args = Kv8ReserveArgs(cache, start.data_ptr(), None if count is None else count.data_ptr(), missing.data_ptr(),
+                          workspace.data_ptr(), workspace.numel(), rows)
+    _launch(load().kv8_reserve, args, device, "kv8_reserve")
+
+
+def kv8_fork(cache: Kv8CacheArgs, parent: torch.Tensor, device: torch.device) -> None:
+    _launch(load().kv8_fork, cache, device, "kv8_fork", parent.data_ptr())
+
+
+def kv8_truncate(cache: Kv8CacheArgs, length: torch.Tensor, device: torch.device) -> None:
+    _launch(load().kv8_truncate, cache, device, "kv8_truncate", length.data_ptr())
+
+
+def kv8_compact(cache: Kv8CacheArgs, used: torch.Tensor, workspace: torch.Tensor, device: torch.device) -> None:
+    args = Kv8CompactArgs(cache, used.data_ptr(), workspace.data_ptr(), workspace.numel())
+    _launch(load().kv8_compact, args, device, "kv8_compact")

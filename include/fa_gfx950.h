@@ -1,6 +1,6 @@
 /*
  * fa_gfx950.h -- C ABI of libfa_gfx950.so, the MI355X (gfx950 / CDNA4) library of FlashAttention forward and
- * backward, the fp16 GEMM, and a 4-bit key/value cache with attention over it.
+ * backward, the fp16 GEMM, and two key/value caches with attention over them: of 4 bits, and of 8 bits in pages.
  *
  * Every entry point is plain C: pointers, fixed-width integers and floats, no HIP or torch types.
  * Device pointers come from the caller (PyTorch allocates every buffer, workspaces
@@ -20,7 +20,7 @@
  *   fa_kernel_resources                <- Triton compile metadata (shared, n_regs)          tuner.py:341-376
  *   fa_kernel_symbol                   <- the compiled kernel that metadata belongs to      tuner.py:356-357
  *   fa_fwd_noalloc                     (no counterpart: fa_fwd for callers that cannot allocate)
- *   fa_bwd, kv4_append, kv4_attend     (no counterpart: the reference has forward attention only)
+ *   fa_bwd, kv4_*, kv8_*               (no counterpart: the reference has forward attention only)
  */
 #ifndef FA_GFX950_H
 #define FA_GFX950_H
@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define FA_ABI_VERSION 7
+#define FA_ABI_VERSION 8
 
 enum {
   FA_OK = 0,
@@ -348,6 +348,116 @@ typedef struct {
 int kv4_attend(const kv4_attend_args* args, void* stream);
 int64_t kv4_attend_workspace_bytes(int32_t B, int32_t H, int32_t M, int32_t D, int32_t splits);
 int32_t kv4_attend_splits(int32_t B, int32_t H, int32_t H_kv, int32_t M, int32_t D, int32_t capacity);
+
+/* Key/value cache of 8-bit codes in pages. A page holds `page` tokens (32, 64, 128 or 256) of every kv head, in each of
+ * `layers` layers; `data` is [layers][pages] of them, layer_stride and page_stride bytes apart (multiples of 16). A page is
+ *   codes   [H_kv][2][page][D]      keys, then values, one byte a channel: e4m3 (sign, 4 exponent bits, 3 mantissa bits;
+ *                                   largest 448, 127 and 255 are NaN)
+ *   scales  [H_kv][page / 32][2]    keys', then values': byte e stands for 2^(e - 127)
+ * with kv8_page_bytes() bytes in all. A block, 32 tokens of a head, shares a scale, in 112 .. 134 (fp16) or 10 .. 246
+ * (bf16), so that all codes stand for numbers of the type; larger scale bytes are read as the largest.
+ * Token t of sequence b is in page table[b * columns + t / page]; an entry outside [0, pages) is no page. refs[p] is
+ * the number of entries that are p; pages with none are free. The caller keeps table and refs consistent, or leaves
+ * them to kv8_reserve, kv8_fork, kv8_truncate and kv8_compact. `capacity` tokens of a sequence may be used. Calls that
+ * write a cache are ordered by the caller; attention calls on one cache may overlap. */
+#define KV8_MAX_CAPACITY (1 << 30)
+typedef struct {
+  uint8_t* data;
+  int32_t* table;
+  int32_t* refs;
+  int64_t layer_stride;
+  int64_t page_stride;
+  int32_t B, H_kv, D, dtype;
+  int32_t page, pages, columns, capacity, layers;
+} kv8_cache;
+
+int64_t kv8_page_bytes(int32_t H_kv, int32_t page, int32_t D);
+
+/* Rows t < count[b] (all `rows` without a count) of k and v [B, H_kv, rows, D] become tokens start[b] + t of `layer`.
+ * A block that gets tokens is encoded anew from what its tokens before start[b] stand for and the new rows; its tokens
+ * behind the new ones become zeros. Its scale puts the largest finite magnitude in (224, 448] steps; infinities and NaN
+ * become NaN, alone. Rows outside [0, capacity), or in a page that is missing or has other holders (refs other than 1),
+ * are dropped. start and count are int32 [B] in device memory. k_values and v_values (both or neither) receive what the
+ * appended rows now stand for, in k's type, and zeros in rows that were not written. */
+typedef struct {
+  kv8_cache cache;
+  const void* k;
+  const void* v;
+  void* k_values;
+  void* v_values;
+  const int32_t* start;
+  const int32_t* count;
+  int64_t k_stride[4];
+  int64_t v_stride[4];
+  int64_t k_values_stride[4];
+  int64_t v_values_stride[4];
+  int32_t rows, layer;
+} kv8_append_args;
+
+int kv8_append(const kv8_append_args* args, void* stream);
+
+/* Attention of q [B, H, M, D] over the cache: kv4_attend's rules, and tokens whose page is missing are not seen. A NaN
+ * of a cached row reaches the rows that see it and no other. */
+typedef struct {
+  kv8_cache cache;
+  const void* q;
+  void* o;
+  float* lse;
+  void* workspace;
+  int64_t workspace_bytes;
+  const int32_t* start;
+  const int32_t* count;
+  int64_t q_stride[4];
+  int64_t o_stride[4];
+  int64_t lse_stride[3];
+  int32_t H, M;
+  float sm_scale;
+  int32_t causal;
+  int32_t splits, layer;
+} kv8_attend_args;
+
+int kv8_attend(const kv8_attend_args* args, void* stream);
+int64_t kv8_attend_workspace_bytes(int32_t B, int32_t H, int32_t M, int32_t D, int32_t splits);
+int32_t kv8_attend_splits(int32_t B, int32_t H, int32_t H_kv, int32_t M, int32_t D, int32_t capacity);
+
+/* Pages for tokens start[b] .. start[b] + n - 1 inside the capacity, n = min(rows, count[b]) (rows without a count), that
+ * append may write. In order of sequence and token: an entry without a page takes the lowest free page; one whose page
+ * has other holders takes the lowest free page and a copy of all layers of it, but for the last such entry of a page where
+ * all its holders are among them: it keeps the page. Where no page is free any more entries stay as they are.
+ * missing (int32 [1], device memory) receives how many. workspace: kv8_reserve_workspace_bytes(), 16-byte aligned. */
+typedef struct {
+  kv8_cache cache;
+  const int32_t* start;
+  const int32_t* count;
+  int32_t* missing;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t rows;
+} kv8_reserve_args;
+
+int kv8_reserve(const kv8_reserve_args* args, void* stream);
+int64_t kv8_reserve_workspace_bytes(const kv8_cache* cache, int32_t rows);
+
+/* Sequence b takes the page table that sequence parent[b] had before the call (its own entries are given up); a parent
+ * outside [0, B) leaves it empty. No page is copied. KV8_MAX_FORK sequences at most. */
+#define KV8_MAX_FORK 16384
+int kv8_fork(const kv8_cache* cache, const int32_t* parent, void* stream);
+
+/* Entries of pages that hold none of sequence b's first length[b] tokens are given up. */
+int kv8_truncate(const kv8_cache* cache, const int32_t* length, void* stream);
+
+/* The pages in use become the first ones: the k-th used page behind their number moves, with all layers, to the k-th
+ * free one before it. used (int32 [1], device memory) receives their number. workspace: kv8_compact_workspace_bytes(),
+ * 16-byte aligned. */
+typedef struct {
+  kv8_cache cache;
+  int32_t* used;
+  void* workspace;
+  int64_t workspace_bytes;
+} kv8_compact_args;
+
+int kv8_compact(const kv8_compact_args* args, void* stream);
+int64_t kv8_compact_workspace_bytes(const kv8_cache* cache);
 
 #ifdef __cplusplus
 }
