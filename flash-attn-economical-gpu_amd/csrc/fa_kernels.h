@@ -193,6 +193,18 @@ struct Kv8AppendParams {
   int32_t blocks;  // blocks that `rows` tokens may lie in
 };
 
+// n / d by a multiplication: (high half of n * multiplier + n) >> shift, for n < 2^31.
+struct Divisor {
+  uint32_t multiplier;
+  int32_t shift;
+  static Divisor of(int64_t d) {
+    Divisor x = {0, 0};
+    while ((1LL << x.shift) < d) ++x.shift;
+    x.multiplier = (uint32_t)(((1ULL << 32) * (uint64_t)((1LL << x.shift) - d)) / (uint64_t)d + 1);
+    return x;
+  }
+};
+
 struct Kv8AttendParams {
   Kv8Pages cache;
   const uint16_t* q;
@@ -202,11 +214,13 @@ struct Kv8AttendParams {
   const int32_t* count;  // nullable: all rows
   float* ws_o;           // splits > 1: unnormalised partial sums [slots][H][M][D]
   float* ws_ml;          // splits > 1: their row maximum (log2 units) and sum [slots][H][M][2]
+  int32_t* parts;        // chunks, splits > 1: first workgroup and number of parts [Hkv][B][row_blocks][2]
   int64_t sq[3], so[3], sl[3];
   int32_t B, H, Hkv, M, group, capacity;
   int32_t causal, splits;
-  int32_t slots;  // splits that all sequences may have together: B * splits
+  int32_t slots;  // splits that all sequences may have together: B * splits (chunks: heads of all sequences)
   int32_t row_blocks;
+  Divisor by_group, by_blocks, by_slots;
   float c;  // scale * log2(e)
 };
 
@@ -216,8 +230,11 @@ struct Kv8KernelEntry {
   const void* append;
   const void* merge[3];   // one, four and sixteen waves to a row
   const void* attend[3];  // 16 rows shared by a workgroup's waves, 32 rows shared, chunks of a prompt
+  const void* join;       // of the last one's parts
   int32_t per_cu[3];      // workgroups of each that the split rule counts on per CU
-  int32_t chunk_rows;     // query rows of a workgroup of the last
+  int32_t chunk_rows;     // query rows of a workgroup of the last, and its keys at a time
+  int32_t chunk_keys;
+  int32_t join_rows;      // rows of a joining workgroup
 };
 
 const Kv8KernelEntry* kv8_registry(int* count);

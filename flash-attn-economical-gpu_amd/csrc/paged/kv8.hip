@@ -216,12 +216,39 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendParams p) {
   }
 }
 
+// Running softmax of the prompt chunks. A row's weights are 2^(x c - R + bias), R a whole number: the row's largest score,
+// in log2 units, when it was last moved. It is moved when the present one is over kLag further, so that the sums are
+// rescaled a few times in all and not at every new maximum, by exact powers of two. fp16: weights up to 2^(8 + 7.5) fit,
+// and those down to 2^-22 keep all their bits.
+constexpr float kLag = 7.f;
+template <typename Tag>
+__device__ constexpr float lag_bias();
+template <>
+__device__ constexpr float lag_bias<f16_t>() { return 8.f; }
+template <>
+__device__ constexpr float lag_bias<bf16_t>() { return 0.f; }
+// Beyond this R, x c and R c cancel to what their rounding leaves: the difference of the scores is taken first.
+constexpr float kLargeR = 0x1p20f;
+
+// n / d for 0 <= n < 2^31 (the host's numbers in fa_kernels.h): with `shift` = ceil(log2 d), 2^32 + multiplier is
+// 2^(32 + shift) / d rounded up. Every workgroup runs through its set-up once, from a cold instruction cache: there a
+// division by its 35 instructions is 140 bytes of code to fetch, and there were a dozen.
+__device__ inline int divide(int n, const Divisor& d) { return (int)((__umulhi(d.multiplier, (uint32_t)n) + (uint32_t)n) >> d.shift); }
+
+// a / b of whole numbers below 2^53, b > 0.
+__device__ inline int64_t divide(int64_t a, int64_t b) {
+  int64_t q = (int64_t)((double)a / (double)b);
+  if (q * b > a) --q;
+  if ((q + 1) * b <= a) ++q;
+  return q;
+}
+
 // The rows that a group of query rows sees. Query rows are (position, head of the group): row r is head r % group at
 // position r / group, and a workgroup's rows share its kv head's cache.
 struct Rows {
   int rows, live;  // rows of the kv head, and those before count
   int keys;        // of the sequence
-  int group;
+  Divisor by_group;
   int64_t start;
   bool causal;
   __device__ inline Rows(const Kv8AttendParams& p, int b) {
@@ -229,13 +256,13 @@ struct Rows {
     rows = p.M * p.group;
     live = (n < 0 ? 0 : (n > p.M ? p.M : n)) * p.group;
     keys = visible_keys(p.start, p.count, b, p.M, p.capacity);
-    group = p.group;
+    by_group = p.by_group;
     start = p.start[b];
     causal = p.causal != 0;
   }
   // keys that row r sees, if it is live
   __device__ inline int sees(int r) const {
-    const int64_t e = causal ? start + r / group + 1 : keys;
+    const int64_t e = causal ? start + divide(r, by_group) + 1 : keys;
     return (int)(e < 0 ? 0 : (e > keys ? keys : e));
   }
   // most keys that one of the live rows in [r, r + n) sees, and the fewest (0 if one of them is not live)
@@ -243,6 +270,51 @@ struct Rows {
   __device__ inline int least(int r, int n) const { return r + n <= live ? sees(r) : 0; }
   // fewest that a live row sees
   __device__ inline int live_least(int r) const { return r < live ? sees(r) : 0x7fffffff; }
+};
+
+// Where a sequence's blocks of one kv head lie, 64 at a time, one to a lane: page (or -1) and scale bytes. Read a lane at
+// a time, so that neither costs a load in the loops over tiles.
+struct Blocks {
+  const int* table;
+  const uint8_t* data;    // the head's keys in page 0
+  const uint8_t* scales;  // and its scale bytes
+  int64_t page_stride, half;  // bytes of a page; of a head's keys in one
+  int blocks_log2, pages;
+  int page;
+  uint32_t scale;
+
+  template <int D>
+  __device__ inline void init(const Kv8Pages& c, int b, int hk) {
+    half = (int64_t)(32 * D) << c.blocks_log2;
+    table = c.table + (int64_t)b * c.columns;
+    data = c.data + 2 * hk * half;
+    scales = c.data + c.scales_at + 2 * ((int64_t)hk << c.blocks_log2);
+    page_stride = c.page_stride;
+    blocks_log2 = c.blocks_log2;
+    pages = c.pages;
+  }
+  // The lane's block becomes `mine` (none at or behind `end`). The page is waited for here, the scale bytes where they
+  // are first used.
+  __device__ inline void look_up(int64_t mine, int64_t end) {
+    page = -1;
+    if (mine < end) page = table[mine >> blocks_log2];
+    asm volatile("" : "+v"(page));
+    const bool there = (uint32_t)page < (uint32_t)pages;
+    scale = 0;
+    if (there)
+      scale = *reinterpret_cast<const uint16_t*>(scales + page * page_stride + 2 * (mine & ((1 << blocks_log2) - 1)));
+    if (!there) page = -1;
+  }
+  __device__ inline void wait() { asm volatile("" : "+v"(scale)); }
+  __device__ inline int page_of(int lane) const { return __builtin_amdgcn_readlane(page, lane); }
+  __device__ inline uint32_t scale_of(int lane) const { return (uint32_t)__builtin_amdgcn_readlane((int)scale, lane); }
+  // Bytes from `data` to a block's keys, in page 0 where it has no page; in scalar registers.
+  template <int D>
+  __device__ inline int64_t place_of(int page, int64_t block) const {
+    const int64_t at = (page < 0 ? 0 : page) * page_stride + (int)(block & ((1 << blocks_log2) - 1)) * (32 * D);
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)at) |
+                     (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32);
+  }
 };
 
 template <int N, int J = 0, typename Fn>
@@ -259,7 +331,7 @@ __device__ inline void for_each(Fn& f) {
 //   O^T += V^T P^T  A = V^T: lane (channels, 8 keys) reads the keys' codes of its D / 16 channels, converts, and
 //                   regroups them by channel with byte permutes; P^T is S^T's accumulator as it stands
 // so nothing passes through LDS but the waves' sums at the end. A lane keeps the table entries of its wave's next 64
-// tiles, so that a page number costs no load in the loop; a tile without a page is passed over.
+// tiles, so that a page number costs no load in the loop; a tile without a page is one that no row sees.
 // The four waves hold the same rows and take turns at the tiles. A wave has one tile's registers: the next tile's keys are
 // asked for when the scores stand, its values when the second product does, so that half a tile or more is in flight.
 template <typename Tag, int D, int R>
@@ -346,12 +418,12 @@ struct Kv8Attend {
   }
 
   // One tile: keys [key0, key0 + 32), of which row rt sees those below see[rt] (a lane's own row). e: its scale bytes.
-  // `edge`: a row does not see all of them; `unseen`: a live row does not see all of the sequence's keys among them.
+  // there: they have a page (`keys` is 0 otherwise). `edge`: a row does not see all of them; `unseen`: a live row does not see all of the sequence's keys among them.
   // next_keys() and next_values() ask for the next tile's codes as soon as this one's have been used. (One body with
   // branches for the edge: with a body of its own for whole tiles the registers of both are held, and 60 spilled.)
   template <typename NextKeys, typename NextValues>
   __device__ static inline void step(State& s, const u32x4 (&qf)[R][KS], const Keys& kc, Values& vc, uint32_t e, int key0,
-                                     const int (&see)[R], int keys, bool edge, bool unseen, float c, int lane,
+                                     const int (&see)[R], int keys, bool there, bool edge, bool unseen, float c, int lane,
                                      NextKeys&& next_keys, NextValues&& next_values) {
     const int g = lane >> 4;
     const float ks = block_scale<Tag>(e & 255u), vs = block_scale<Tag>(e >> 8);
@@ -378,7 +450,7 @@ struct Kv8Attend {
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (key0 + 16 * i + 4 * g + r >= see[rt]) x[i][rt][r] = FA_NEG_INF;
+            if (key0 + 16 * i + 4 * g + r >= see[rt] || !there) x[i][rt][r] = FA_NEG_INF;
       }
       // a NaN score makes the row NaN: through P, whether or not the maximum moves
       const float top = larger(larger(larger(x[0][rt][0], x[0][rt][1]), larger(x[0][rt][2], x[0][rt][3])),
@@ -458,7 +530,7 @@ struct Kv8Attend {
   template <int N>
   __device__ static inline void store_row(const Kv8AttendParams& p, int b, int hk, int slot, int r, const float (&o)[N],
                                           float m, float l, int at) {
-    const int i = r / p.group, h = hk * p.group + r % p.group;
+    const int i = divide(r, p.by_group), h = hk * p.group + r - i * p.group;
     if (p.splits > 1) {
       const int64_t w = ((int64_t)slot * p.H + h) * p.M + i;
       float* dst = p.ws_o + w * D + at * N;
@@ -487,11 +559,10 @@ struct Kv8Attend {
   __device__ static void run(const Kv8AttendParams& p, float* smem) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g = lane >> 4;
-    int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int id = xcd_remap(blockIdx.x, gridDim.x);
     // row blocks innermost: those of one split share its tiles in L2
-    const int rb = id % p.row_blocks;
-    id /= p.row_blocks;
-    const int slot = id % p.slots, hk = id / p.slots;
+    const int rest = divide(id, p.by_blocks), rb = id - rest * p.row_blocks;
+    const int hk = divide(rest, p.by_slots), slot = rest - hk * p.slots;
     const Split part = find_split(p, slot, 0);
     const int b = __builtin_amdgcn_readfirstlane(part.b);
     if (b < 0) return;
@@ -506,8 +577,8 @@ struct Kv8Attend {
       const int r = row0 + 16 * rt + c16;
       const bool live = r < q_rows.live;
       see[rt] = live ? q_rows.sees(r) : 0;
-      const uint16_t* q = p.q + b * p.sq[0] + (int64_t)(hk * p.group + (live ? r % p.group : 0)) * p.sq[1] +
-                          (int64_t)(live ? r / p.group : 0) * p.sq[2] + g * 16;
+      const int pos = live ? divide(r, p.by_group) : 0, member = live ? r - pos * p.group : 0;
+      const uint16_t* q = p.q + b * p.sq[0] + (int64_t)(hk * p.group + member) * p.sq[1] + pos * p.sq[2] + g * 16;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         qf[rt][k] = (u32x4){0, 0, 0, 0};
@@ -523,58 +594,41 @@ struct Kv8Attend {
     const int tiles = (__builtin_amdgcn_readfirstlane(q_rows.most(row0, 16 * R)) + 31) / 32;
     const int per = __builtin_amdgcn_readfirstlane(part.per);
     const int64_t first = (int64_t)__builtin_amdgcn_readfirstlane(part.index) * per;
-    const int t1 = (int)(first + per < tiles ? first + per : tiles);
-    const Kv8Pages& pg = p.cache;
-    const int64_t half = (int64_t)(32 * D) << pg.blocks_log2;  // bytes of a page's keys of a head
-    const uint8_t* data = pg.data + 2 * hk * half;
-    const uint8_t* scales = pg.data + pg.scales_at + 2 * ((int64_t)hk << pg.blocks_log2);
-    const int* table = pg.table + (int64_t)b * pg.columns;
-    const int t0 = first < t1 ? (int)first + wave : t1;
-    int entries = -1;  // of the wave's next 64 tiles, one to a lane
-    int used = 0;      // tiles that were asked for
-    struct Place {
-      const uint8_t* keys;
-      const uint8_t* scales;
-      bool there;
-    };
-    auto locate = [&](int t) {
-      Place x = {nullptr, nullptr, false};
-      if (t >= t1) return x;
-      if ((used & 63) == 0) {
-        const int64_t mine = t + (int64_t)lane * WAVES;
-        entries = mine < t1 ? table[mine >> pg.blocks_log2] : -1;
-      }
-      const int page = __builtin_amdgcn_readlane(entries, used & 63);
-      ++used;
-      x.there = (uint32_t)page < (uint32_t)pg.pages;
-      const int sub = t & ((1 << pg.blocks_log2) - 1);
-      x.keys = data + page * pg.page_stride + sub * (32 * D);
-      x.scales = scales + page * pg.page_stride + 2 * sub;
-      return x;
-    };
-    Keys kc;
-    Values vc;
-    uint32_t e = 0, e_next = 0;
-    Place next = locate(t0);
-    auto next_keys = [&]() {
-      if (!next.there) return;
-      load_keys(kc, next.keys, lane);
-      e_next = *reinterpret_cast<const uint16_t*>(next.scales);
-    };
-    auto next_values = [&]() {
-      if (next.there) load_values(vc, next.keys + half, lane);
-    };
-    next_keys();
-    next_values();
-    for (int t = t0; t < t1; t += WAVES) {
-      const bool there = next.there;
-      e = e_next;
-      next = locate(t + WAVES);
-      if (!there) {
-        next_keys();
-        next_values();
-      } else {
-        step(s, qf, kc, vc, e, t * 32, see, keys, t * 32 + 32 > least,
+    const int t1 = __builtin_amdgcn_readfirstlane((int)(first + per < tiles ? first + per : tiles));
+    const int t0 = __builtin_amdgcn_readfirstlane(first < t1 ? (int)first + wave : t1);
+    Blocks blocks;  // of the wave's next 64 tiles
+    blocks.init<D>(p.cache, b, hk);
+    if (t0 < t1) blocks.look_up(t0 + (int64_t)lane * WAVES, t1);
+    // Codes are asked for without a condition, so that a wait for one load need not be a wait for all behind it: where
+    // there is no next tile the last one is read again (from L2), where it has no page page 0 is.
+    if (t0 < t1) {
+      int used = 0;  // of the 64
+      int64_t at = 0;
+      bool there = false;  // the next tile has a page
+      auto locate = [&](int t) {
+        if (t >= t1) return;
+        if (used == 64) {
+          blocks.look_up(t + (int64_t)lane * WAVES, t1);
+          blocks.wait();
+          used = 0;
+        }
+        const int page = blocks.page_of(used++);
+        there = page >= 0;
+        at = blocks.place_of<D>(page, t);
+      };
+      Keys kc;
+      Values vc;
+      auto next_keys = [&]() { load_keys(kc, blocks.data + at, lane); };
+      auto next_values = [&]() { load_values(vc, blocks.data + blocks.half + at, lane); };
+      locate(t0);
+      next_keys();
+      next_values();
+      blocks.wait();
+      for (int t = t0; t < t1; t += WAVES) {
+        const bool now = there;
+        const uint32_t scale_bytes = blocks.scale_of(used - 1);
+        locate(t + WAVES);
+        step(s, qf, kc, vc, scale_bytes, t * 32, see, now ? keys : 0, now, t * 32 + 32 > least || !now,
              (t * 32 + 32 < keys ? t * 32 + 32 : keys) > live_least, p.c, lane, next_keys, next_values);
       }
     }
@@ -631,7 +685,10 @@ __global__ __launch_bounds__(256, (attend8_waves<D, R>())) void kv8_attend_kerne
 // Chunks of a prompt: more than 32 query rows to a kv head. The workgroup's four waves, of 32 rows each, share the
 // conversion: a tile's codes are loaded a tile ahead, 16 channels of a row to a thread and step, converted once into
 // 16-bit rows in LDS (two stages, one barrier a tile), and both products read their fragments there, V's by the
-// transposing read. S^T = K Q^T and O^T = V^T P^T as above.
+// transposing read. S^T = K Q^T and O^T = V^T P^T as above. The chip's workgroups take equal shares of all blocks' tiles.
+// Fewest key tiles to a workgroup's share: below, the parts' extra pass costs more than it gives.
+constexpr int kMinShare = 4;
+
 template <typename Tag, int D>
 struct Kv8Chunk {
   using L = LdsRows<D>;
@@ -649,26 +706,109 @@ struct Kv8Chunk {
 
   struct Codes {
     u32x4 k[PER], v[PER];
-    uint32_t e[PER];  // scale bytes of the unit's block
+    uint32_t e[NB];  // scale bytes of the tile's blocks
     bool there[NB];
   };
 
   // block of the tile that a wave's i-th unit lies in
   __device__ static inline int block_of(int i, int wave) { return D == 128 ? i : (D == 64 ? wave >> 1 : 0); }
 
+  // The work of all row blocks, head after head, is a line of key tiles: block rb of sequence b has as many as its rows
+  // see. (One at least: blocks without live rows have zeros to write.) A pair is b * row_blocks + rb.
+  __device__ static inline int tiles_of(const Kv8AttendParams& p, int pair) {
+    const int b = divide(pair, p.by_blocks);
+    const Rows rows(p, b);
+    const int n = (rows.most((pair - b * p.row_blocks) * BLOCK, BLOCK) + T - 1) / T;
+    return n > 0 ? n : 1;
+  }
+  // Tiles of a head's pairs up to the one that holds tile `at` (and that pair), or of all. 64 pairs at a time, one to a
+  // lane; every wave works it out for itself.
+  struct Place {
+    int pair;
+    int64_t before;
+  };
+  __device__ static inline Place find(const Kv8AttendParams& p, int64_t at) {
+    const int lane = threadIdx.x & 63, pairs = p.B * p.row_blocks;
+    int64_t base = 0;
+    for (int c = 0; c < pairs; c += 64) {
+      const int n = c + lane < pairs ? tiles_of(p, c + lane) : 0;  // at most 2^25: 64 of them fit 32 bits
+      int end = n;
+#pragma unroll
+      for (int k = 1; k < 64; k *= 2) {
+        const int o = __shfl_up(end, k, 64);
+        if (lane >= k) end += o;
+      }
+      const uint64_t hit = __ballot(at < base + end);
+      if (hit != 0) {
+        const int who = __builtin_ctzll(hit);
+        return {c + who, base + __builtin_amdgcn_readlane(end - n, who)};
+      }
+      base += __builtin_amdgcn_readlane(end, 63);
+    }
+    return {pairs, base};
+  }
+
+  // One workgroup: a row block (splits = 1; the longest first), or an equal share of the line, whose ends may lie inside
+  // a block: such parts are left in the workspace, the share's first part (which continues a block) in slot 2 id and its
+  // last (which begins one) in slot 2 id + 1.
   // flags: words with a bit for each key of the tile whose values hold a NaN, for three tiles in turn
   __device__ static void run(const Kv8AttendParams& p, char* smem, uint32_t (*flags)[2]) {
+    const int pairs = p.B * p.row_blocks;
+    const bool shared = p.splits > 1;
+    const int id = shared ? xcd_remap(blockIdx.x, gridDim.x) : (int)blockIdx.x;
+    if (threadIdx.x < 6) flags[threadIdx.x / 2][threadIdx.x % 2] = 0;
+    __syncthreads();
+    Turn turn = {0, 0};
+    int hk, pair;
+    int64_t at = 0, end = 1, begun = 0, share = 1;  // on the line; of the pair's tiles
+    if (shared) {
+      const int64_t all = find(p, INT64_MAX).before, line = all * p.Hkv;
+      share = divide(line + gridDim.x - 1, (int64_t)gridDim.x);
+      if (share < kMinShare) share = kMinShare;
+      at = id * share;
+      end = at + share < line ? at + share : line;
+      if (at >= end) return;
+      hk = (int)divide(at, all);
+      const Place place = find(p, at - hk * all);
+      pair = place.pair;
+      begun = at - hk * all - place.before;
+    } else {
+      const int from_last = divide(id, p.by_slots), rest = id - from_last * p.slots;  // slots: heads of all sequences
+      hk = rest % p.Hkv;
+      pair = rest / p.Hkv * p.row_blocks + p.row_blocks - 1 - from_last;
+    }
+    hk = __builtin_amdgcn_readfirstlane(hk);
+    pair = __builtin_amdgcn_readfirstlane(pair);
+    while (at < end) {
+      const int n = __builtin_amdgcn_readfirstlane(tiles_of(p, pair));
+      const int t0 = __builtin_amdgcn_readfirstlane((int)begun);
+      const int t1 = __builtin_amdgcn_readfirstlane((int)(shared && end - at < n - t0 ? t0 + (end - at) : n));
+      const int b = __builtin_amdgcn_readfirstlane(divide(pair, p.by_blocks));
+      part(p, smem, flags, turn, hk, b, pair - b * p.row_blocks, t0, t1, t0 == 0 && t1 == n ? -1 : 2 * id + (t0 == 0));
+      if (shared && t1 == n && threadIdx.x == 0) {  // who has the block's parts: the first workgroup, and how many
+        const int first = (int)divide(at - t0, share);
+        p.parts[2 * (hk * (int64_t)pairs + pair)] = first;
+        p.parts[2 * (hk * (int64_t)pairs + pair) + 1] = id - first + 1;
+      }
+      at += t1 - t0;
+      begun = 0;
+      if (++pair == pairs) {
+        pair = 0;
+        ++hk;
+      }
+    }
+  }
+
+  struct Turn {  // LDS stage and flags' turn: they go on from part to part
+    uint32_t stage;
+    int flag;
+  };
+
+  // Tiles [t0, t1) of row block rb, for one kv head of one sequence. slot: -1, or where the sums are left.
+  __device__ static void part(const Kv8AttendParams& p, char* smem, uint32_t (*flags)[2], Turn& at_turn, int hk, int b, int rb,
+                              int t0, int t1, int slot) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c16 = lane & 15, g = lane >> 4;
-    int id = xcd_remap(blockIdx.x, gridDim.x);
-    const int rb = id % p.row_blocks;
-    id /= p.row_blocks;
-    const int slot = id % p.slots, hk = id / p.slots;
-    const Split part = find_split(p, slot, 0);
-    const int b = __builtin_amdgcn_readfirstlane(part.b);
-    if (b < 0) return;
-    if (tid < 6) flags[tid / 2][tid % 2] = 0;
-    __syncthreads();
     const Rows q_rows(p, b);
     const int row0 = rb * BLOCK + wave * QT * 16, keys = q_rows.keys;
     const int block_see = __builtin_amdgcn_readfirstlane(q_rows.most(rb * BLOCK, BLOCK));
@@ -683,8 +823,8 @@ struct Kv8Chunk {
       const int r = row0 + 16 * j + c16;
       const bool live = r < q_rows.live;
       see[j] = live ? q_rows.sees(r) : 0;
-      const uint16_t* q = p.q + b * p.sq[0] + (int64_t)(hk * p.group + (live ? r % p.group : 0)) * p.sq[1] +
-                          (int64_t)(live ? r / p.group : 0) * p.sq[2] + 8 * g;
+      const int pos = live ? divide(r, p.by_group) : 0, member = live ? r - pos * p.group : 0;
+      const uint16_t* q = p.q + b * p.sq[0] + (int64_t)(hk * p.group + member) * p.sq[1] + pos * p.sq[2] + 8 * g;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         qf[j][k] = (u32x4){0, 0, 0, 0};
@@ -692,71 +832,73 @@ struct Kv8Chunk {
       }
     }
     floatx4 o[DT16][QT];
-    float m[QT], l[QT];
+    float m[QT], l[QT], off[QT];  // row's reference score, sum of weights, bias - R
+    bool large = false;
+    const float lag = kLag / p.c;
 #pragma unroll
     for (int j = 0; j < QT; ++j) {
       m[j] = FA_NEG_INF;
       l[j] = 0.f;
+      off[j] = lag_bias<Tag>();
 #pragma unroll
       for (int d = 0; d < DT16; ++d) o[d][j] = (floatx4){0.f, 0.f, 0.f, 0.f};
     }
 
-    // the split's keys, in tiles of T (its share is in tiles of 32)
-    const int64_t per = (int64_t)__builtin_amdgcn_readfirstlane(part.per) * 32;
-    const int64_t k_first = __builtin_amdgcn_readfirstlane(part.index) * per;
-    const int k_end = (int)(k_first + per < block_see ? k_first + per : block_see);
-#pragma unroll
-    for (int j = 0; j < QT; ++j) see[j] = see[j] < k_end ? see[j] : k_end;  // the next split may begin inside a tile
+    const int64_t k_first = (int64_t)t0 * T;
+    const int k_end = (int)((int64_t)t1 * T < block_see ? (int64_t)t1 * T : block_see);
     int live_least = __builtin_amdgcn_readfirstlane(q_rows.live_least(row0));
     if (live_least < 0x7fffffff && live_least > k_end) live_least = k_end;
-    const Kv8Pages& pg = p.cache;
-    const int64_t half = (int64_t)(32 * D) << pg.blocks_log2;  // bytes of a page's keys of a head
-    const uint8_t* data = pg.data + 2 * hk * half;
-    const uint8_t* scales = pg.data + pg.scales_at + 2 * ((int64_t)hk << pg.blocks_log2);
-    const int* table = pg.table + (int64_t)b * pg.columns;
-    // pages of the tile at key0
-    auto entries = [&](int (&at)[NB], int64_t key0) {
+    Blocks blocks;
+    blocks.init<D>(p.cache, b, hk);
+    const int end = (k_end + 31) / 32;
+    int used = 0;
+    if (k_first < k_end) blocks.look_up(k_first / 32 + lane, end);
+    // Whole blocks are read, from any page where there is none; what is not to be seen is cleared when it is converted.
+    auto fetch = [&](Codes& x, int64_t key0) {
+      if (used == 64) {
+        blocks.look_up(key0 / 32 + lane, end);
+        blocks.wait();
+        used = 0;
+      }
+      const uint8_t* from[NB];
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        const int64_t key = key0 + 32 * n;
-        at[n] = key < k_end ? table[key >> (5 + pg.blocks_log2)] : -1;
+        const int page = blocks.page_of(used + n);
+        x.e[n] = blocks.scale_of(used + n);
+        x.there[n] = page >= 0;
+        from[n] = blocks.data + blocks.place_of<D>(page, key0 / 32 + n);
       }
-    };
-    // Past the last visible key nothing is read, and what stands there is zero: rows behind a sequence may hold anything.
-    auto fetch = [&](Codes& x, int64_t key0, const int (&at)[NB]) {
-      int page[NB];
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        page[n] = __builtin_amdgcn_readfirstlane(at[n]);
-        x.there[n] = (uint32_t)page[n] < (uint32_t)pg.pages;
-      }
+      used += NB;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int n = block_of(i, wave), row = (tid + 256 * i) / UPR, part16 = tid % UPR;
-        const int at_page = NB == 2 && n ? page[NB - 1] : page[0];
-        const bool here = NB == 2 && n ? x.there[NB - 1] : x.there[0];
-        x.k[i] = x.v[i] = (u32x4){0, 0, 0, 0};
-        x.e[i] = 0x7f7f;
-        if (here) {
-          const int sub = (int)((key0 >> 5) + n) & ((1 << pg.blocks_log2) - 1);
-          const uint8_t* from = data + at_page * pg.page_stride + sub * (32 * D);
-          const uint32_t off = (uint32_t)((row & 31) * D + part16 * 16);
-          if (key0 + row < keys) {
-            x.k[i] = *reinterpret_cast<const u32x4*>(from + off);
-            x.v[i] = *reinterpret_cast<const u32x4*>(from + half + off);
-          }
-          x.e[i] = *reinterpret_cast<const uint16_t*>(scales + at_page * pg.page_stride + 2 * sub);
-        }
+        const int n = block_of(i, wave);
+        const uint8_t* at = (NB == 2 && n ? from[NB - 1] : from[0]) + (uint32_t)((tid + 256 * i) / UPR % 32 * D + tid % UPR * 16);
+        x.k[i] = *reinterpret_cast<const u32x4*>(at);
+        x.v[i] = *reinterpret_cast<const u32x4*>(at + blocks.half);
       }
     };
     // `mark`: the tile has keys that one of the workgroup's live rows does not see
-    auto convert = [&](const Codes& x, uint32_t stage, int turn, bool mark) {
+    // Keys behind the last one that any row sees may hold anything, NaN too: their values read as zeros.
+    auto convert = [&](Codes& x, int64_t key0, uint32_t stage, int turn, bool mark) {
+      bool clear = key0 + T > keys;
+#pragma unroll
+      for (int n = 0; n < NB; ++n) clear = clear || !x.there[n];
+      if (clear) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int n = block_of(i, wave);
+          const bool here = NB == 2 && n ? x.there[NB - 1] : x.there[0];
+          if (!here || key0 + (tid + 256 * i) / UPR >= keys) x.v[i] = (u32x4){0, 0, 0, 0};
+        }
+      }
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int row = (tid + 256 * i) / UPR, part16 = tid % UPR;
+        const int n = block_of(i, wave);
+        const uint32_t e = NB == 2 && n ? x.e[NB - 1] : x.e[0];
         char* dst = smem + stage + row * L::ROWB;
         const uint32_t c0 = (uint32_t)(((2 * part16) ^ L::swz(row)) << 4), c1 = (uint32_t)(((2 * part16 + 1) ^ L::swz(row)) << 4);
-        const float ks = block_scale<Tag>(x.e[i] & 255u), vs = block_scale<Tag>(x.e[i] >> 8);
+        const float ks = block_scale<Tag>(e & 255u), vs = block_scale<Tag>(e >> 8);
         *reinterpret_cast<u32x4*>(dst + c0) = decode8<Tag>(x.k[i][0], x.k[i][1], ks);
         *reinterpret_cast<u32x4*>(dst + c1) = decode8<Tag>(x.k[i][2], x.k[i][3], ks);
         *reinterpret_cast<u32x4*>(dst + TILEB + c0) = decode8<Tag>(x.v[i][0], x.v[i][1], vs);
@@ -796,7 +938,8 @@ struct Kv8Chunk {
           for (int j = 0; j < QT; ++j) x[i][j] = E::mfma16(a, qf[j][k], x[i][j]);
         }
       }
-      u32x4 pb[KT / 2][QT];
+      bool move[QT];
+      float tops[QT];
 #pragma unroll
       for (int j = 0; j < QT; ++j) {
         float top = FA_NEG_INF;
@@ -807,41 +950,52 @@ struct Kv8Chunk {
             if (EDGE && (key0 + 16 * i + 4 * g + r >= see[j] || !there[i / 2])) x[i][j][r] = FA_NEG_INF;
             top = larger(top, x[i][j][r]);
           }
-        const float m_new = larger(m[j], row_max(top));
-        if (__any(m_new > m[j])) {
-          const float base = m_new == FA_NEG_INF ? 0.f : m_new;
-          const float f = fast_exp2((m[j] - base) * p.c);
+        tops[j] = row_max(top);
+        move[j] = tops[j] > m[j] + lag;  // a NaN score makes the row NaN through P
+      }
+      if (__any(QT == 2 ? move[0] || move[QT - 1] : move[0])) {
+        bool far = false;
+#pragma unroll
+        for (int j = 0; j < QT; ++j) {
+          // each row by itself: what another row of the wave sees does not change its bits
+          const float to = move[j] ? lag_bias<Tag>() - __builtin_rintf(tops[j] * p.c) : off[j];
+          const float f = m[j] == FA_NEG_INF ? 0.f : (move[j] ? fast_exp2(to - off[j]) : 1.f);
           l[j] *= f;
 #pragma unroll
           for (int d = 0; d < DT16; ++d) o[d][j] *= f;
-          m[j] = m_new;
+          m[j] = move[j] ? tops[j] : m[j];
+          off[j] = to;
+          far |= !(fabsf(to) <= kLargeR);
         }
-        const float base = m[j] == FA_NEG_INF ? 0.f : m[j];
-        const float off = weight_bias<Tag>() - base * p.c;
-        // One instruction to an argument, where the rounding of m c, which does not cancel, stays small beside the
-        // argument: beyond, the difference is taken first.
-        if (__builtin_expect(__any(fabsf(base * p.c) > 0x1p14f), 0)) {
+        large = __any(far);
+      }
+      float add[QT];
+#pragma unroll
+      for (int j = 0; j < QT; ++j) add[j] = off[j];
+      if (__builtin_expect(large, 0)) {
+#pragma unroll
+        for (int j = 0; j < QT; ++j) {
+          const bool far = !(fabsf(off[j]) <= kLargeR);
+          add[j] = far ? lag_bias<Tag>() : off[j];
 #pragma unroll
           for (int i = 0; i < KT; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[i][j][r] = fmaf(x[i][j][r] - base, p.c, weight_bias<Tag>());
-        } else {
-#pragma unroll
-          for (int i = 0; i < KT; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) x[i][j][r] = fmaf(x[i][j][r], p.c, off);
+            for (int n = 0; n < 4; ++n) x[i][j][n] -= far ? m[j] : 0.f;
         }
+      }
+      u32x4 pb[KT / 2][QT];
+#pragma unroll
+      for (int j = 0; j < QT; ++j)
 #pragma unroll
         for (int i = 0; i < KT; ++i) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            x[i][j][r] = fast_exp2(x[i][j][r]);
+            x[i][j][r] = fast_exp2(fmaf(x[i][j][r], p.c, add[j]));
             l[j] += x[i][j][r];
           }
           pb[i / 2][j][2 * (i & 1)] = E::pack2(x[i][j][0], x[i][j][1]);
           pb[i / 2][j][2 * (i & 1) + 1] = E::pack2(x[i][j][2], x[i][j][3]);
         }
-      }
       // a lane's keys of an operand that are in `set`: 4 g .. + 3 (dwords 0, 1), then 16 further (dwords 2, 3)
       auto lanes_of = [&](uint32_t set) {
         const uint32_t x = set >> (4 * g);
@@ -891,21 +1045,17 @@ struct Kv8Chunk {
       }
     };
     Codes next;
-    int ahead[NB];
-    entries(ahead, k_first);
-    if (k_first < k_end) fetch(next, k_first, ahead);
-    entries(ahead, k_first + T);
-    uint32_t stage = 0;
-    int turn = 0;
+    if (k_first < k_end) fetch(next, k_first);
+    uint32_t stage = at_turn.stage;
+    int turn = at_turn.flag;
     // Tiles that every row of the wave sees whole, up to a missing page; then the rest, on the diagonal, at the end or
     // with pages missing: every wave makes the same number of passes in all, for the barriers.
     auto pass = [&](int64_t key0, auto edge_tile) {
       bool there[NB];
 #pragma unroll
       for (int n = 0; n < NB; ++n) there[n] = next.there[n];
-      convert(next, stage, turn, key0 + T > block_least);
-      if (key0 + T < k_end) fetch(next, key0 + T, ahead);
-      entries(ahead, key0 + 2 * T);
+      convert(next, key0, stage, turn, key0 + T > block_least);
+      if (key0 + T < k_end) fetch(next, key0 + T);
       const int after = turn == 2 ? 0 : turn + 1;
       if (tid < 2) flags[after][tid] = 0;  // last read two barriers ago, written again after the next
       wait_vm_lds_barrier<63>();  // LDS writes only: the codes just asked for stay in flight
@@ -922,20 +1072,21 @@ struct Kv8Chunk {
     int64_t key0 = k_first;
     for (; key0 + T <= k_end && key0 + T <= least && whole(); key0 += T) pass(key0, std::false_type{});
     for (; key0 < k_end; key0 += T) pass(key0, std::true_type{});
+    at_turn = {stage, turn};
 
 #pragma unroll
     for (int j = 0; j < QT; ++j) {
       const float sum = xquad_sum(l[j]);
       const int r = row0 + 16 * j + c16;
       if (r >= q_rows.rows) continue;
-      const int i = r / p.group, h = hk * p.group + r % p.group;
-      if (p.splits > 1) {
-        const int64_t w = ((int64_t)slot * p.H + h) * p.M + i;
+      const int i = divide(r, p.by_group), h = hk * p.group + r - i * p.group;
+      if (slot >= 0) {
+        const int64_t w = (int64_t)slot * BLOCK + r - rb * BLOCK;
 #pragma unroll
         for (int d = 0; d < DT16; ++d)  // a row that saw no key is zeros, whatever values that are no numbers left in o
           *reinterpret_cast<floatx4*>(p.ws_o + w * D + 16 * d + 4 * g) = sum == 0.f ? (floatx4){0.f, 0.f, 0.f, 0.f} : o[d][j];
         if (g == 0) {
-          p.ws_ml[2 * w] = m[j] * p.c;
+          p.ws_ml[2 * w] = m[j] == FA_NEG_INF ? FA_NEG_INF : lag_bias<Tag>() - off[j];
           p.ws_ml[2 * w + 1] = sum;
         }
       } else {
@@ -948,11 +1099,66 @@ struct Kv8Chunk {
                          : (u32x2){E::pack2(o[d][j][0] * inv, o[d][j][1] * inv), E::pack2(o[d][j][2] * inv, o[d][j][3] * inv)};
         if (g == 0 && p.lse != nullptr)
           p.lse[b * p.sl[0] + h * p.sl[1] + i * p.sl[2]] =
-              sum == 0.f ? FA_NEG_INF : (m[j] * p.c + __builtin_amdgcn_logf(sum) - weight_bias<Tag>()) * 0.6931471805599453f;
+              sum == 0.f ? FA_NEG_INF : (__builtin_amdgcn_logf(sum) - off[j]) * 0.6931471805599453f;
       }
     }
   }
 };
+
+// Joins the parts of a row block: weights exp2(m_s - m) of the unnormalised sums. A wave takes a row, D / 4 lanes a
+// part's row; a workgroup kJoinRows rows of a block.
+constexpr int kJoinRows = 4;
+template <typename Tag, int D, int BLOCK>
+__device__ inline void join_parts(const Kv8AttendParams& p) {
+  constexpr int LPS = D / 4, AT_ONCE = 64 / LPS, GROUPS = BLOCK / kJoinRows;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int block = (int)(blockIdx.x / GROUPS);  // hk, b, rb
+  const int first = p.parts[2 * (int64_t)block], n = p.parts[2 * (int64_t)block + 1];
+  if (n <= 1) return;
+  const int pair = divide(block, p.by_blocks), rb = block - pair * p.row_blocks, hk = pair / p.B, b = pair % p.B;
+  const int c4 = lane % LPS;
+  for (int k = wave; k < kJoinRows; k += 4) {
+    const int at = (int)(blockIdx.x % GROUPS) * kJoinRows + k, r = rb * BLOCK + at;
+    if (r >= p.M * p.group) return;
+    auto place = [&](int s) { return (int64_t)(s == 0 ? 2 * first + 1 : 2 * (first + s)) * BLOCK + at; };
+    float m = FA_NEG_INF, sum = 0.f;
+    floatx4 o = (floatx4){0.f, 0.f, 0.f, 0.f};
+    for (int s = lane / LPS; s < n; s += AT_ONCE) m = fmaxf(m, p.ws_ml[2 * place(s)]);
+    const float base = m == FA_NEG_INF ? 0.f : m;
+#pragma unroll 2
+    for (int s = lane / LPS; s < n; s += AT_ONCE) {
+      const int64_t w = place(s);
+      const float f = fast_exp2(p.ws_ml[2 * w] - base);
+      const floatx4 x = *reinterpret_cast<const floatx4*>(p.ws_o + w * D + 4 * c4);
+      sum = fmaf(f, p.ws_ml[2 * w + 1], sum);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = fmaf(f, x[j], o[j]);
+    }
+#pragma unroll
+    for (int x = LPS; x < 64; x *= 2) {  // the wave's lane groups
+      const float mo = __shfl_xor(m, x, 64), so = __shfl_xor(sum, x, 64);
+      const float top = fmaxf(m, mo), ref = top == FA_NEG_INF ? 0.f : top;
+      const float f = fast_exp2(m - ref), fo = fast_exp2(mo - ref);
+      sum = f * sum + fo * so;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = f * o[j] + fo * __shfl_xor(o[j], x, 64);
+      m = top;
+    }
+    if (lane >= LPS) continue;
+    const int i = divide(r, p.by_group), h = hk * p.group + r - i * p.group;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    *reinterpret_cast<u32x2*>(p.o + b * p.so[0] + h * p.so[1] + i * p.so[2] + 4 * c4) =
+        (u32x2){DT<Tag>::pack2(o[0] * inv, o[1] * inv), DT<Tag>::pack2(o[2] * inv, o[3] * inv)};
+    if (c4 == 0 && p.lse != nullptr)
+      p.lse[b * p.sl[0] + h * p.sl[1] + i * p.sl[2]] =
+          sum == 0.f ? FA_NEG_INF : (m + __builtin_amdgcn_logf(sum) - lag_bias<Tag>()) * 0.6931471805599453f;
+  }
+}
+
+template <typename Tag, int D>
+__global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttendParams p) {
+  join_parts<Tag, D, Kv8Chunk<Tag, D>::BLOCK>(p);
+}
 
 template <typename Tag, int D>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv8_chunk_kernel(Kv8AttendParams p) {
@@ -972,7 +1178,8 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void kv8_merge_kernel(Kv8At
     (const void*)&kv8_merge_kernel<TAG, D, 16>},                                                            \
    {(const void*)&kv8_attend_kernel<TAG, D, 1>, (const void*)&kv8_attend_kernel<TAG, D, 2>,                 \
     (const void*)&kv8_chunk_kernel<TAG, D>},                                                                \
-   {attend8_waves<D, 1>(), attend8_waves<D, 2>(), 2}, Kv8Chunk<TAG, D>::BLOCK}
+   (const void*)&kv8_join_kernel<TAG, D>,                                                                  \
+   {attend8_waves<D, 1>(), attend8_waves<D, 2>(), D == 64 ? 3 : 2}, Kv8Chunk<TAG, D>::BLOCK, Kv8Chunk<TAG, D>::T, kJoinRows}
 
 static const Kv8KernelEntry kKv8Entries[] = {
     KV8_ENTRY(f16_t, FA_DTYPE_F16, 64),   KV8_ENTRY(f16_t, FA_DTYPE_F16, 128),   KV8_ENTRY(f16_t, FA_DTYPE_F16, 256),

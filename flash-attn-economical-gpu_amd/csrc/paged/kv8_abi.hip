@@ -27,7 +27,7 @@ int64_t codes_bytes(int64_t Hkv, int64_t page, int64_t D) { return 2 * Hkv * pag
 int check_cache(const kv8_cache* c) {
   const int code = check_type(c->dtype, c->D);
   if (code != FA_OK) return code;
-  if (c->B < 0 || c->H_kv <= 0 || c->pages < 0 || c->columns < 0 || c->capacity < 0 || c->layers < 1)
+  if (c->B < 0 || c->H_kv <= 0 || c->pages < 1 || c->columns < 0 || c->capacity < 0 || c->layers < 1)
     return fail(FA_EINVAL, "invalid cache sizes B=%d H_kv=%d pages=%d columns=%d capacity=%d layers=%d", c->B, c->H_kv, c->pages,
                 c->columns, c->capacity, c->layers);
   if (c->page != 32 && c->page != 64 && c->page != 128 && c->page != 256)
@@ -39,7 +39,7 @@ int check_cache(const kv8_cache* c) {
     return fail(FA_EINVAL, "%d columns of %d tokens do not hold the capacity %d", c->columns, c->page, c->capacity);
   if ((int64_t)c->B * c->columns > (1 << 30)) return fail(FA_EINVAL, "page table too large (%d x %d)", c->B, c->columns);
   if (c->B == 0 || c->columns == 0) return FA_OK;
-  if (!c->table || (c->pages > 0 && (!c->data || !c->refs))) return fail(FA_EINVAL, "null cache pointer");
+  if (!c->table || !c->data || !c->refs) return fail(FA_EINVAL, "null cache pointer");
   if (!aligned(c->data, 16) || c->page_stride % 16 || c->layer_stride % 16)
     return fail(FA_EINVAL, "cache data and its strides must be 16-byte aligned");
   if (c->pages > 1 && c->page_stride < kv8_page_bytes(c->H_kv, c->page, c->D))
@@ -80,6 +80,21 @@ Kind kind_of(const fa::Kv8KernelEntry* e, int64_t rows) {
   const int64_t block = k.kind == 2 ? e->chunk_rows : 16 << k.kind;
   k.row_blocks = (rows + block - 1) / block;
   return k;
+}
+
+// Partial sums of the splits: [slots][H][M] rows, or two row blocks of a workgroup (chunks).
+struct AttendWorkspace {
+  int64_t ml_at, parts_at, bytes;
+};
+AttendWorkspace attend_workspace(const fa::Kv8KernelEntry* e, int64_t B, int64_t H, int64_t Hkv, int64_t M, int64_t D,
+                                 int64_t splits) {
+  const Kind k = kind_of(e, M * (H / Hkv));
+  const int64_t rows = k.kind == 2 ? 2 * splits * e->chunk_rows : splits * B * H * M;
+  AttendWorkspace w;
+  w.ml_at = align256(rows * D * 4);
+  w.parts_at = w.bytes = w.ml_at + rows * 8;
+  if (k.kind == 2) w.bytes += 8 * B * Hkv * k.row_blocks;
+  return w;
 }
 
 int check_workspace(const void* workspace, int64_t bytes, int64_t need, const char* what) {
@@ -196,18 +211,24 @@ int kv8_append(const kv8_append_args* a, void* stream) {
   return ok();
 }
 
-int64_t kv8_attend_workspace_bytes(int32_t B, int32_t H, int32_t M, int32_t D, int32_t splits) {
-  if (splits <= 1 || B <= 0 || H <= 0 || M <= 0 || D <= 0) return 0;
-  const int64_t rows = (int64_t)splits * B * H * M;
-  return align256(rows * D * 4) + rows * 8;
+int64_t kv8_attend_workspace_bytes(int32_t B, int32_t H, int32_t H_kv, int32_t M, int32_t D, int32_t splits) {
+  const fa::Kv8KernelEntry* e = find_kv8(FA_DTYPE_F16, D);  // alike for both types
+  if (e == nullptr || splits <= 1 || B <= 0 || H_kv <= 0 || H < H_kv || M <= 0) return 0;
+  return attend_workspace(e, B, H, H_kv, M, D, splits).bytes;
 }
 
 int32_t kv8_attend_splits(int32_t B, int32_t H, int32_t H_kv, int32_t M, int32_t D, int32_t capacity) {
-  const fa::Kv8KernelEntry* e = find_kv8(FA_DTYPE_F16, D);  // alike for both types
+  const fa::Kv8KernelEntry* e = find_kv8(FA_DTYPE_F16, D);
   if (e == nullptr || B <= 0 || H_kv <= 0 || H < H_kv || M <= 0 || capacity <= 0) return 1;
   const Kind k = kind_of(e, (int64_t)M * (H / H_kv));
   const int64_t blocks = (int64_t)B * H_kv * k.row_blocks, room = 256LL * e->per_cu[k.kind];
   // as many as the chip (256 CUs) holds at once, none with less than 256 keys of a full cache
+  if (k.kind == 2) {
+    // twice as many blocks as fit are given out whole, the longest first: nothing is left to join
+    if (blocks >= 2 * room) return 1;
+    const int64_t most = blocks * ((capacity + 255) / 256);
+    return (int32_t)(most < room ? most : room);
+  }
   int64_t splits = room / blocks;
   if (splits > capacity / 256) splits = capacity / 256;
   return splits < 1 ? 1 : (int32_t)(splits > 4096 ? 4096 : splits);
@@ -234,12 +255,13 @@ int kv8_attend(const kv8_attend_args* a, void* stream) {
   if (e == nullptr) return fail(FA_ENOTSUP, "8-bit cache kernels for dtype=%d D=%d are not built", c->dtype, c->D);
   fa::Kv8AttendParams p;
   std::memset(&p, 0, sizeof(p));
-  const int64_t need = kv8_attend_workspace_bytes(c->B, a->H, a->M, c->D, a->splits);
-  if (need > 0) {
-    if ((code = check_workspace(a->workspace, a->workspace_bytes, need, "split")) != FA_OK) return code;
-    p.ws_o = static_cast<float*>(a->workspace);
-    p.ws_ml = reinterpret_cast<float*>(static_cast<char*>(a->workspace) +
-                                       align256((int64_t)a->splits * c->B * a->H * a->M * c->D * 4));
+  if (a->splits > 1) {
+    const AttendWorkspace w = attend_workspace(e, c->B, a->H, c->H_kv, a->M, c->D, a->splits);
+    if ((code = check_workspace(a->workspace, a->workspace_bytes, w.bytes, "split")) != FA_OK) return code;
+    char* ws = static_cast<char*>(a->workspace);
+    p.ws_o = reinterpret_cast<float*>(ws);
+    p.ws_ml = reinterpret_cast<float*>(ws + w.ml_at);
+    p.parts = reinterpret_cast<int32_t*>(ws + w.parts_at);
   }
   p.cache = pages_of(c, a->layer);
   p.q = static_cast<const uint16_t*>(a->q);
@@ -256,10 +278,24 @@ int kv8_attend(const kv8_attend_args* a, void* stream) {
   p.c = a->sm_scale * 1.4426950408889634f;
   const Kind k = kind_of(e, rows);
   p.row_blocks = (int32_t)k.row_blocks;
+  p.by_group = fa::Divisor::of(p.group);
+  p.by_blocks = fa::Divisor::of(k.row_blocks);
+  if (k.kind == 2) {
+    const int64_t all = k.row_blocks * c->B * c->H_kv;
+    p.slots = c->B * c->H_kv;
+    p.by_slots = fa::Divisor::of(p.slots);
+    const int64_t blocks = a->splits > 1 ? a->splits : all, joins = a->splits > 1 ? all * (e->chunk_rows / e->join_rows) : 0;
+    if ((code = check_grid(blocks, 256, "cache attention")) != FA_OK || (code = check_grid(joins, 256, "cache join")) != FA_OK)
+      return code;
+    if ((code = launch(e->attend[2], blocks, 1, 256, &p, stream, "cache attention")) != FA_OK) return code;
+    if (joins > 0 && (code = launch(e->join, joins, 1, 256, &p, stream, "cache join")) != FA_OK) return code;
+    return ok();
+  }
   const int64_t slots = (int64_t)c->B * a->splits;
   const int64_t blocks = k.row_blocks * slots * c->H_kv;
   if (slots > 0x7fffffffLL) return fail(FA_EINVAL, "too many splits (%lld)", (long long)slots);
   p.slots = (int32_t)slots;
+  p.by_slots = fa::Divisor::of(slots);
   const int64_t all = (int64_t)c->B * a->H * a->M;
   const int how = a->splits > 32 ? 2 : (a->splits > 8 ? 1 : 0);
   const int64_t few = (all + 3) / 4 < 2048 ? (all + 3) / 4 : 2048;  // eight workgroups to a CU, a few rows to a wave

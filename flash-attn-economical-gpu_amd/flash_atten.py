@@ -448,7 +448,7 @@ def sdpa_kv8(query: torch.Tensor, cache: kv8.Kv8Cache, start: torch.Tensor, *, c
         splits = kv8.choose_splits(B, H, cache.kv_heads, M, D, cache.capacity)
         plan = (hip_lib.kv8_attend_plan(query, o, lse, sm_scale=D ** -0.5 if scale is None else scale, causal=is_causal,
                                         splits=splits, layer=layer),
-                hip_lib.kv8_attend_workspace_bytes(B, H, M, D, splits))
+                hip_lib.kv8_attend_workspace_bytes(B, H, cache.kv_heads, M, D, splits))
         if key[1:4] == (_form(query), kv4._form(start), None if count is None else kv4._form(count)):
             _keep_plan(key, plan)  # nothing had to be copied: calls of this form take the short way
     workspace = torch.empty(plan[1], dtype=torch.uint8, device=query.device) if plan[1] else None

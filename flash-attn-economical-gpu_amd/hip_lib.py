@@ -286,7 +286,7 @@ SIGNATURES = {
     "kv8_page_bytes": (ctypes.c_int64, [ctypes.c_int32] * 3),
     "kv8_append": (ctypes.c_int, [ctypes.POINTER(Kv8AppendArgs), ctypes.c_void_p]),
     "kv8_attend": (ctypes.c_int, [ctypes.POINTER(Kv8AttendArgs), ctypes.c_void_p]),
-    "kv8_attend_workspace_bytes": (ctypes.c_int64, [ctypes.c_int32] * 5),
+    "kv8_attend_workspace_bytes": (ctypes.c_int64, [ctypes.c_int32] * 6),
     "kv8_attend_splits": (ctypes.c_int32, [ctypes.c_int32] * 6),
     "kv8_reserve": (ctypes.c_int, [ctypes.POINTER(Kv8ReserveArgs), ctypes.c_void_p]),
     "kv8_reserve_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(Kv8CacheArgs), ctypes.c_int32]),
@@ -751,8 +751,8 @@ def kv8_page_bytes(H_kv: int, page: int, D: int) -> int:
 
 
 @functools.lru_cache(maxsize=4096)
-def kv8_attend_workspace_bytes(B: int, H: int, M: int, D: int, splits: int) -> int:
-    return int(load().kv8_attend_workspace_bytes(B, H, M, D, splits))
+def kv8_attend_workspace_bytes(B: int, H: int, H_kv: int, M: int, D: int, splits: int) -> int:
+    return int(load().kv8_attend_workspace_bytes(B, H, H_kv, M, D, splits))
 
 
 def kv8_append_plan(k: torch.Tensor, v: torch.Tensor, k_values: torch.Tensor | None, v_values: torch.Tensor | None, *,

@@ -37,8 +37,8 @@ MAX_FORK = 16384  # KV8_MAX_FORK
 
 @functools.lru_cache(maxsize=4096)
 def choose_splits(B: int, H: int, H_kv: int, M: int, D: int, capacity: int) -> int:
-    """Parts that a sequence's keys are cut into on average: as many workgroups as the chip holds, none with less
-    than 256 keys of a full cache."""
+    """Parts that a sequence's keys are cut into on average (up to 32 query rows to a kv head), or workgroups that share
+    all the work (more rows): as many workgroups as the chip holds, none with less than 256 keys of a full cache."""
     return int(hip_lib.load().kv8_attend_splits(B, H, H_kv, M, D, capacity))
 
 

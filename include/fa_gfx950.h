@@ -397,7 +397,8 @@ typedef struct {
 int kv8_append(const kv8_append_args* args, void* stream);
 
 /* Attention of q [B, H, M, D] over the cache: kv4_attend's rules, and tokens whose page is missing are not seen. A NaN
- * of a cached row reaches the rows that see it and no other. */
+ * of a cached row reaches the rows that see it and no other. splits, with up to 32 query rows to a kv head (M * H /
+ * H_kv): as kv4_attend's; with more, workgroups that share the work of all rows in equal parts (1: whole blocks of rows). */
 typedef struct {
   kv8_cache cache;
   const void* q;
@@ -417,7 +418,7 @@ typedef struct {
 } kv8_attend_args;
 
 int kv8_attend(const kv8_attend_args* args, void* stream);
-int64_t kv8_attend_workspace_bytes(int32_t B, int32_t H, int32_t M, int32_t D, int32_t splits);
+int64_t kv8_attend_workspace_bytes(int32_t B, int32_t H, int32_t H_kv, int32_t M, int32_t D, int32_t splits);
 int32_t kv8_attend_splits(int32_t B, int32_t H, int32_t H_kv, int32_t M, int32_t D, int32_t capacity);
 
 /* Pages for tokens start[b] .. start[b] + n - 1 inside the capacity, n = min(rows, count[b]) (rows without a count), that

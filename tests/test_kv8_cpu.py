@@ -112,7 +112,7 @@ def _compact(cache=None, **over):
 CACHE_REFUSALS = [
     ({"D": 32}, hip_lib.FA_ENOTSUP, "head dim"), ({"dtype": 5}, hip_lib.FA_ENOTSUP, "dtype"),
     ({"H_kv": 0}, hip_lib.FA_EINVAL, "invalid cache sizes"), ({"layers": 0}, hip_lib.FA_EINVAL, "invalid cache sizes"),
-    ({"pages": -1}, hip_lib.FA_EINVAL, "invalid cache sizes"), ({"B": -1}, hip_lib.FA_EINVAL, "invalid cache sizes"),
+    ({"pages": 0}, hip_lib.FA_EINVAL, "invalid cache sizes"), ({"B": -1}, hip_lib.FA_EINVAL, "invalid cache sizes"),
     ({"page": 48}, hip_lib.FA_ENOTSUP, "pages of 48"), ({"capacity": 257}, hip_lib.FA_EINVAL, "do not hold"),
     ({"capacity": (1 << 30) + 1, "columns": 1 << 28}, hip_lib.FA_ENOTSUP, "is beyond"),
     ({"pages": (1 << 30) + 1}, hip_lib.FA_ENOTSUP, "pages are beyond"), ({"H_kv": (1 << 20) + 1}, hip_lib.FA_ENOTSUP, "beyond 2^20"),
@@ -198,8 +198,9 @@ def test_empty_calls_do_nothing():
     assert lib.kv8_append(ctypes.byref(_append(_cache(B=0))), None) == hip_lib.FA_OK
     assert lib.kv8_page_bytes(2, 64, 64) == 2 * 2 * 64 * 64 + 128 and lib.kv8_page_bytes(0, 64, 64) == 0
     assert lib.kv8_page_bytes(64, 256, 128) == 2 * 64 * 256 * 128 + 2 * 64 * 8
-    assert lib.kv8_attend_workspace_bytes(2, 4, 3, 64, 5) == 5 * 24 * (64 * 4 + 8)
-    assert lib.kv8_attend_workspace_bytes(1, 1, 1, 64, 1) == lib.kv8_reserve_workspace_bytes(None, 1) == 0
+    assert lib.kv8_attend_workspace_bytes(2, 4, 2, 3, 64, 5) == 5 * 24 * (64 * 4 + 8)
+    assert lib.kv8_attend_workspace_bytes(2, 4, 2, 300, 64, 5) == 2 * 5 * 128 * (64 * 4 + 8) + 8 * 2 * 2 * 5
+    assert lib.kv8_attend_workspace_bytes(1, 1, 1, 1, 64, 1) == lib.kv8_reserve_workspace_bytes(None, 1) == 0
 
 
 def test_python_refusals_without_a_gpu():
@@ -223,7 +224,8 @@ def test_splits_rule():
     assert kv8.choose_splits(1, 32, 8, 1, 128, 255) == 1
     for B, H, Hk, M, D, cap in ((1, 32, 8, 1, 128, 8192), (1, 12, 2, 4, 128, 100000), (2, 28, 4, 509, 128, 16384), (1, 1, 1, 1, 64, 1 << 20)):
         n = kv8.choose_splits(B, H, Hk, M, D, cap)
-        assert 1 <= n <= max(1, cap // 256) and n <= 4096
+        blocks = B * Hk * -(-M * (H // Hk) // 128) if M * (H // Hk) > 32 else 1
+        assert 1 <= n <= max(1, -(-cap // 256)) * blocks and n <= 4096
 
 
 def test_the_model_follows_the_format():
