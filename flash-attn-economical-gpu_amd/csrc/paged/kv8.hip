@@ -272,19 +272,27 @@ struct Rows {
   __device__ inline int live_least(int r) const { return r < live ? sees(r) : 0x7fffffff; }
 };
 
-// Where a sequence's blocks of one kv head lie, 64 at a time, one to a lane: page (or -1) and scale bytes. Read a lane at
-// a time, so that neither costs a load in the loops over tiles.
+// Where a sequence's blocks of one kv head lie, 64 at a time, one to a lane, and their scales. They are read a lane at a
+// time, ready to be used: in the loops over tiles they cost neither a load nor arithmetic.
+template <typename Tag, int D>
 struct Blocks {
   const int* table;
-  const uint8_t* data;    // the head's keys in page 0
-  const uint8_t* scales;  // and its scale bytes
+  const uint8_t* data;        // the head's keys in page 0
+  const uint8_t* scales;      // and its scale bytes
   int64_t page_stride, half;  // bytes of a page; of a head's keys in one
   int blocks_log2, pages;
-  int page;
-  uint32_t scale;
+  // of the lane's block: bytes from `data` to its keys, in two halves, and its scales. Without a page: page 0, and the
+  // keys' scale is negative.
+  int at[2];
+  float ks, vs;
 
-  template <int D>
-  __device__ inline void init(const Kv8Pages& c, int b, int hk) {
+  struct Place {
+    int64_t at;
+    float ks, vs;
+    bool there;
+  };
+
+  __device__ inline Blocks(const Kv8Pages& c, int b, int hk) {
     half = (int64_t)(32 * D) << c.blocks_log2;
     table = c.table + (int64_t)b * c.columns;
     data = c.data + 2 * hk * half;
@@ -292,29 +300,31 @@ struct Blocks {
     page_stride = c.page_stride;
     blocks_log2 = c.blocks_log2;
     pages = c.pages;
+    at[0] = at[1] = 0;
+    ks = vs = -1.f;
   }
-  // The lane's block becomes `mine` (none at or behind `end`). The page is waited for here, the scale bytes where they
+  // The lane's block becomes `mine` (none at or behind `end`). Where it lies is waited for here, its scales where they
   // are first used.
-  __device__ inline void look_up(int64_t mine, int64_t end) {
-    page = -1;
+  __device__ inline void look_up(int mine, int end) {
+    int page = -1;
     if (mine < end) page = table[mine >> blocks_log2];
     asm volatile("" : "+v"(page));
     const bool there = (uint32_t)page < (uint32_t)pages;
-    scale = 0;
-    if (there)
-      scale = *reinterpret_cast<const uint16_t*>(scales + page * page_stride + 2 * (mine & ((1 << blocks_log2) - 1)));
-    if (!there) page = -1;
+    const int sub = mine & ((1 << blocks_log2) - 1);
+    const int64_t base = there ? page * page_stride : 0, place = base + sub * (32 * D);
+    at[0] = (int)place;
+    at[1] = (int)(place >> 32);
+    const uint32_t e = *reinterpret_cast<const uint16_t*>(scales + base + 2 * sub);
+    ks = there ? block_scale<Tag>(e & 255u) : -1.f;
+    vs = block_scale<Tag>(e >> 8);
   }
-  __device__ inline void wait() { asm volatile("" : "+v"(scale)); }
-  __device__ inline int page_of(int lane) const { return __builtin_amdgcn_readlane(page, lane); }
-  __device__ inline uint32_t scale_of(int lane) const { return (uint32_t)__builtin_amdgcn_readlane((int)scale, lane); }
-  // Bytes from `data` to a block's keys, in page 0 where it has no page; in scalar registers.
-  template <int D>
-  __device__ inline int64_t place_of(int page, int64_t block) const {
-    const int64_t at = (page < 0 ? 0 : page) * page_stride + (int)(block & ((1 << blocks_log2) - 1)) * (32 * D);
-    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)at) |
-                     (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32);
+  __device__ inline void wait() { asm volatile("" : "+v"(ks), "+v"(vs)); }
+  __device__ inline int64_t keys_at(int lane) const {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(at[0], lane) |
+                     (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at[1], lane) << 32);
   }
+  __device__ inline float key_scale(int lane) const { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks), lane)); }
+  __device__ inline float value_scale(int lane) const { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs), lane)); }
 };
 
 template <int N, int J = 0, typename Fn>
@@ -417,16 +427,15 @@ struct Kv8Attend {
     for_each<CPL / 2>(pair);
   }
 
-  // One tile: keys [key0, key0 + 32), of which row rt sees those below see[rt] (a lane's own row). e: its scale bytes.
+  // One tile: keys [key0, key0 + 32), of which row rt sees those below see[rt] (a lane's own row). ks, vs: its scales.
   // there: they have a page (`keys` is 0 otherwise). `edge`: a row does not see all of them; `unseen`: a live row does not see all of the sequence's keys among them.
   // next_keys() and next_values() ask for the next tile's codes as soon as this one's have been used. (One body with
   // branches for the edge: with a body of its own for whole tiles the registers of both are held, and 60 spilled.)
   template <typename NextKeys, typename NextValues>
-  __device__ static inline void step(State& s, const u32x4 (&qf)[R][KS], const Keys& kc, Values& vc, uint32_t e, int key0,
-                                     const int (&see)[R], int keys, bool there, bool edge, bool unseen, float c, int lane,
+  __device__ static inline void step(State& s, const u32x4 (&qf)[R][KS], const Keys& kc, Values& vc, float ks, float vs,
+                                     int key0, const int (&see)[R], int keys, bool there, bool edge, bool unseen, float c, int lane,
                                      NextKeys&& next_keys, NextValues&& next_values) {
     const int g = lane >> 4;
-    const float ks = block_scale<Tag>(e & 255u), vs = block_scale<Tag>(e >> 8);
     floatx4 x[2][R];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -596,39 +605,32 @@ struct Kv8Attend {
     const int64_t first = (int64_t)__builtin_amdgcn_readfirstlane(part.index) * per;
     const int t1 = __builtin_amdgcn_readfirstlane((int)(first + per < tiles ? first + per : tiles));
     const int t0 = __builtin_amdgcn_readfirstlane(first < t1 ? (int)first + wave : t1);
-    Blocks blocks;  // of the wave's next 64 tiles
-    blocks.init<D>(p.cache, b, hk);
-    if (t0 < t1) blocks.look_up(t0 + (int64_t)lane * WAVES, t1);
+    Blocks<Tag, D> blocks(p.cache, b, hk);  // of the wave's next 64 tiles
     // Codes are asked for without a condition, so that a wait for one load need not be a wait for all behind it: where
     // there is no next tile the last one is read again (from L2), where it has no page page 0 is.
     if (t0 < t1) {
+      blocks.look_up(t0 + lane * WAVES, t1);
       int used = 0;  // of the 64
-      int64_t at = 0;
-      bool there = false;  // the next tile has a page
-      auto locate = [&](int t) {
-        if (t >= t1) return;
-        if (used == 64) {
-          blocks.look_up(t + (int64_t)lane * WAVES, t1);
-          blocks.wait();
-          used = 0;
-        }
-        const int page = blocks.page_of(used++);
-        there = page >= 0;
-        at = blocks.place_of<D>(page, t);
-      };
       Keys kc;
       Values vc;
+      int64_t at = blocks.keys_at(0);  // of the next tile's keys
       auto next_keys = [&]() { load_keys(kc, blocks.data + at, lane); };
       auto next_values = [&]() { load_values(vc, blocks.data + blocks.half + at, lane); };
-      locate(t0);
       next_keys();
       next_values();
       blocks.wait();
       for (int t = t0; t < t1; t += WAVES) {
-        const bool now = there;
-        const uint32_t scale_bytes = blocks.scale_of(used - 1);
-        locate(t + WAVES);
-        step(s, qf, kc, vc, scale_bytes, t * 32, see, now ? keys : 0, now, t * 32 + 32 > least || !now,
+        const float ks = blocks.key_scale(used), vs = blocks.value_scale(used);
+        const bool there = ks >= 0.f;
+        if (t + WAVES < t1) {
+          if (++used == 64) {
+            blocks.look_up(t + WAVES + lane * WAVES, t1);
+            blocks.wait();
+            used = 0;
+          }
+          at = blocks.keys_at(used);
+        }
+        step(s, qf, kc, vc, ks, vs, t * 32, see, there ? keys : 0, there, t * 32 + 32 > least || !there,
              (t * 32 + 32 < keys ? t * 32 + 32 : keys) > live_least, p.c, lane, next_keys, next_values);
       }
     }
@@ -706,8 +708,7 @@ struct Kv8Chunk {
 
   struct Codes {
     u32x4 k[PER], v[PER];
-    uint32_t e[NB];  // scale bytes of the tile's blocks
-    bool there[NB];
+    float ks[NB], vs[NB];  // scales of the tile's blocks; ks < 0: it has no page
   };
 
   // block of the tile that a wave's i-th unit lies in
@@ -844,17 +845,16 @@ struct Kv8Chunk {
       for (int d = 0; d < DT16; ++d) o[d][j] = (floatx4){0.f, 0.f, 0.f, 0.f};
     }
 
-    const int64_t k_first = (int64_t)t0 * T;
-    const int k_end = (int)((int64_t)t1 * T < block_see ? (int64_t)t1 * T : block_see);
+    const int k_first = t0 * T;
+    const int k_end = t1 * T < block_see ? t1 * T : block_see;  // t1 * T <= the capacity rounded up, under 2^31
     int live_least = __builtin_amdgcn_readfirstlane(q_rows.live_least(row0));
     if (live_least < 0x7fffffff && live_least > k_end) live_least = k_end;
-    Blocks blocks;
-    blocks.init<D>(p.cache, b, hk);
+    Blocks<Tag, D> blocks(p.cache, b, hk);
     const int end = (k_end + 31) / 32;
     int used = 0;
     if (k_first < k_end) blocks.look_up(k_first / 32 + lane, end);
-    // Whole blocks are read, from any page where there is none; what is not to be seen is cleared when it is converted.
-    auto fetch = [&](Codes& x, int64_t key0) {
+    // Whole blocks are read, from page 0 where there is no page; what is not to be seen is cleared when it is converted.
+    auto fetch = [&](Codes& x, int key0) {
       if (used == 64) {
         blocks.look_up(key0 / 32 + lane, end);
         blocks.wait();
@@ -863,10 +863,9 @@ struct Kv8Chunk {
       const uint8_t* from[NB];
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        const int page = blocks.page_of(used + n);
-        x.e[n] = blocks.scale_of(used + n);
-        x.there[n] = page >= 0;
-        from[n] = blocks.data + blocks.place_of<D>(page, key0 / 32 + n);
+        from[n] = blocks.data + blocks.keys_at(used + n);
+        x.ks[n] = blocks.key_scale(used + n);
+        x.vs[n] = blocks.value_scale(used + n);
       }
       used += NB;
 #pragma unroll
@@ -879,26 +878,25 @@ struct Kv8Chunk {
     };
     // `mark`: the tile has keys that one of the workgroup's live rows does not see
     // Keys behind the last one that any row sees may hold anything, NaN too: their values read as zeros.
-    auto convert = [&](Codes& x, int64_t key0, uint32_t stage, int turn, bool mark) {
+    auto convert = [&](Codes& x, int key0, uint32_t stage, int turn, bool mark) {
       bool clear = key0 + T > keys;
 #pragma unroll
-      for (int n = 0; n < NB; ++n) clear = clear || !x.there[n];
+      for (int n = 0; n < NB; ++n) clear = clear || x.ks[n] < 0.f;
       if (clear) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
           const int n = block_of(i, wave);
-          const bool here = NB == 2 && n ? x.there[NB - 1] : x.there[0];
-          if (!here || key0 + (tid + 256 * i) / UPR >= keys) x.v[i] = (u32x4){0, 0, 0, 0};
+          const bool gone = (NB == 2 && n ? x.ks[NB - 1] : x.ks[0]) < 0.f;
+          if (gone || key0 + (tid + 256 * i) / UPR >= keys) x.v[i] = (u32x4){0, 0, 0, 0};
         }
       }
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int row = (tid + 256 * i) / UPR, part16 = tid % UPR;
         const int n = block_of(i, wave);
-        const uint32_t e = NB == 2 && n ? x.e[NB - 1] : x.e[0];
         char* dst = smem + stage + row * L::ROWB;
         const uint32_t c0 = (uint32_t)(((2 * part16) ^ L::swz(row)) << 4), c1 = (uint32_t)(((2 * part16 + 1) ^ L::swz(row)) << 4);
-        const float ks = block_scale<Tag>(e & 255u), vs = block_scale<Tag>(e >> 8);
+        const float ks = NB == 2 && n ? x.ks[NB - 1] : x.ks[0], vs = NB == 2 && n ? x.vs[NB - 1] : x.vs[0];
         *reinterpret_cast<u32x4*>(dst + c0) = decode8<Tag>(x.k[i][0], x.k[i][1], ks);
         *reinterpret_cast<u32x4*>(dst + c1) = decode8<Tag>(x.k[i][2], x.k[i][3], ks);
         *reinterpret_cast<u32x4*>(dst + TILEB + c0) = decode8<Tag>(x.v[i][0], x.v[i][1], vs);
@@ -1050,26 +1048,26 @@ struct Kv8Chunk {
     int turn = at_turn.flag;
     // Tiles that every row of the wave sees whole, up to a missing page; then the rest, on the diagonal, at the end or
     // with pages missing: every wave makes the same number of passes in all, for the barriers.
-    auto pass = [&](int64_t key0, auto edge_tile) {
+    auto pass = [&](int key0, auto edge_tile) {
       bool there[NB];
 #pragma unroll
-      for (int n = 0; n < NB; ++n) there[n] = next.there[n];
+      for (int n = 0; n < NB; ++n) there[n] = next.ks[n] >= 0.f;
       convert(next, key0, stage, turn, key0 + T > block_least);
       if (key0 + T < k_end) fetch(next, key0 + T);
       const int after = turn == 2 ? 0 : turn + 1;
       if (tid < 2) flags[after][tid] = 0;  // last read two barriers ago, written again after the next
       wait_vm_lds_barrier<63>();  // LDS writes only: the codes just asked for stay in flight
-      if (key0 < wave_see) step((int)key0, stage, there, turn, edge_tile);
+      if (key0 < wave_see) step(key0, stage, there, turn, edge_tile);
       stage ^= STAGEB;
       turn = after;
     };
     auto whole = [&]() {
-      bool all = next.there[0];
+      bool all = next.ks[0] >= 0.f;
 #pragma unroll
-      for (int n = 1; n < NB; ++n) all = all && next.there[n];
+      for (int n = 1; n < NB; ++n) all = all && next.ks[n] >= 0.f;
       return all;
     };
-    int64_t key0 = k_first;
+    int key0 = k_first;
     for (; key0 + T <= k_end && key0 + T <= least && whole(); key0 += T) pass(key0, std::false_type{});
     for (; key0 < k_end; key0 += T) pass(key0, std::true_type{});
     at_turn = {stage, turn};
