@@ -258,7 +258,8 @@ struct Kv8PageParams {
 
 // Kernels of the page operations, and the threads of a workgroup of each.
 struct Kv8PageKernels {
-  const void* reserve;
+  const void* reserve[2];  // items in the workspace; up to held_items of them in registers
+  int32_t held_items;
   const void* fork;
   const void* truncate;
   const void* compact;

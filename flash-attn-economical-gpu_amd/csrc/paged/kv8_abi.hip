@@ -332,7 +332,7 @@ int kv8_reserve(const kv8_reserve_args* a, void* stream) {
   p.span = (int32_t)span;
   const fa::Kv8PageKernels k = fa::kv8_page_kernels();
   const int64_t items = c->B * span;
-  if ((code = launch(k.reserve, 1, 1, k.plan_threads, &p, stream, "page reserve")) != FA_OK) return code;
+  if ((code = launch(k.reserve[items <= k.held_items], 1, 1, k.plan_threads, &p, stream, "page reserve")) != FA_OK) return code;
   if (items > 0 && c->pages > 1 &&
       (code = launch(k.copy, copy_blocks(p, items < c->pages ? items : c->pages), 1, k.threads, &p, stream, "page copy")) != FA_OK)
     return code;

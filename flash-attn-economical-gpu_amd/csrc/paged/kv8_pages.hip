@@ -17,8 +17,10 @@ constexpr int kPlanThreads = 1024, kThreads = 256;
 // Reads and writes of words that other lanes change with atomics: those act in L2, past this CU's cache.
 __device__ inline int load_shared(const int* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ inline void store_shared(int* p, int x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// A barrier behind which they, and what this workgroup has written to its workspace, can be read: all of it has reached
+// L2, of which a workgroup sees one. (A device-wide fence would write L2 back: 2 us each.)
 __device__ inline void sync_shared() {
-  __threadfence();
+  __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
 }
 
@@ -52,21 +54,23 @@ enum { kHeld = 0, kNew = 1, kCopy = 2 };
 
 struct Item {
   int64_t at;  // of the entry in the table
-  int entry;
-  bool active;
+  int entry;   // -1 if nothing is asked of it
+  int kind;
 };
 __device__ inline Item item_of(const Kv8PageParams& p, int i) {
-  const int b = i / p.span, s = i % p.span;
+  const Kv8Pages& c = p.cache;
+  const int b = i / p.span, s = i - b * p.span;
   int n = p.count != nullptr ? p.count[b] : p.rows;
   n = n < 0 ? 0 : (n > p.rows ? p.rows : n);
   const int64_t start = p.a[b];
   const int64_t low = start > 0 ? start : 0, high = start + n < p.capacity ? start + n : p.capacity;
-  const int page_log2 = 5 + p.cache.blocks_log2;
+  const int page_log2 = 5 + c.blocks_log2;
   const int64_t column = (low >> page_log2) + s;
+  const bool active = high > low && column << page_log2 < high;  // so column < columns: high <= capacity
   Item x;
-  x.active = high > low && column << page_log2 < high;  // so column < columns: high <= capacity
-  x.at = (int64_t)b * p.cache.columns + column;
-  x.entry = x.active ? p.cache.table[x.at] : -1;
+  x.at = (int64_t)b * c.columns + column;
+  x.entry = active ? c.table[x.at] : -1;
+  x.kind = !active ? kHeld : (!is_page(c, x.entry) ? kNew : (c.refs[x.entry] > 1 ? kCopy : kHeld));
   return x;
 }
 
@@ -74,47 +78,74 @@ __device__ inline Item item_of(const Kv8PageParams& p, int i) {
 // copied unless it is the last of them and all of them are items: marked by the largest item and the number of items of
 // each page. Then the items that want a page are counted, as many free pages are found from the lowest on, and the k-th
 // item takes the k-th page.
+// HELD: items stay in registers, EACH to a thread, and the pages found in LDS (up to 8192 items); otherwise they are
+// looked up again and kept in the workspace. One decode step of 32 sequences 5 us, the prompts of 32 sequences of 2-4k
+// tokens 7, where the workspace form takes 8 and 18.
+constexpr int kHeldItems = 8;
+template <bool HELD>
 __global__ __launch_bounds__(kPlanThreads) void kv8_reserve_kernel(Kv8PageParams p) {
+  constexpr int EACH = HELD ? kHeldItems : 1;
   __shared__ uint32_t parts[kPlanThreads / 64];
   __shared__ int copies;
+  __shared__ int pages[HELD ? kPlanThreads * EACH : 1];
   const Kv8Pages& c = p.cache;
   const int items = p.B * p.span, each = (items + kPlanThreads - 1) / kPlanThreads;
-  const int i0 = min((int)threadIdx.x * each, items), i1 = min(i0 + each, items);
+  const int i0 = (int)min((int64_t)threadIdx.x * each, (int64_t)items), i1 = min(i0 + each, items);
   int* last = p.mark;
   int* sharers = p.mark + c.pages;
+  Item held[EACH];
+  // f(item, its number) of the thread's items; the kind that f leaves is kept
+  auto for_items = [&](auto f) {
+    if constexpr (HELD) {
+#pragma unroll
+      for (int k = 0; k < EACH; ++k)
+        if (i0 + k < i1) f(held[k], i0 + k);
+    } else {
+      for (int i = i0; i < i1; ++i) {
+        Item x = item_of(p, i);
+        x.kind = p.wants[i];
+        f(x, i);
+        p.wants[i] = x.kind;
+      }
+    }
+  };
   uint32_t wanted = 0;
   bool shared = false;
   if (threadIdx.x == 0) copies = 0;
-#pragma unroll 4
-  for (int i = i0; i < i1; ++i) {
-    const Item x = item_of(p, i);
-    int kind = kHeld;
-    if (x.active) kind = !is_page(c, x.entry) ? kNew : (c.refs[x.entry] > 1 ? kCopy : kHeld);
-    p.wants[i] = kind;
-    wanted += kind == kNew;
-    if (kind == kCopy) {
+  if constexpr (HELD) {
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      held[k] = {0, -1, kHeld};
+      if (i0 + k < i1) held[k] = item_of(p, i0 + k);
+    }
+  } else {
+    for (int i = i0; i < i1; ++i) p.wants[i] = item_of(p, i).kind;
+  }
+  for_items([&](Item& x, int) {
+    wanted += x.kind == kNew;
+    if (x.kind == kCopy) {
       shared = true;
       store_shared(last + x.entry, -1);
       store_shared(sharers + x.entry, 0);
     }
-  }
+  });
   if (__syncthreads_or(shared)) {
     sync_shared();
     if (shared)
-      for (int i = i0; i < i1; ++i)
-        if (p.wants[i] == kCopy) {
-          const int page = item_of(p, i).entry;
-          atomicMax(last + page, i);
-          atomicAdd(sharers + page, 1);
+      for_items([&](Item& x, int i) {
+        if (x.kind == kCopy) {
+          atomicMax(last + x.entry, i);
+          atomicAdd(sharers + x.entry, 1);
         }
+      });
     sync_shared();
     if (shared)
-      for (int i = i0; i < i1; ++i)
-        if (p.wants[i] == kCopy) {
-          const int page = item_of(p, i).entry;
-          if (load_shared(last + page) == i && load_shared(sharers + page) == c.refs[page]) p.wants[i] = kHeld;
+      for_items([&](Item& x, int i) {
+        if (x.kind == kCopy) {
+          if (load_shared(last + x.entry) == i && load_shared(sharers + x.entry) == c.refs[x.entry]) x.kind = kHeld;
           else ++wanted;
         }
+      });
     __syncthreads();  // refs are read above and changed below
   }
   uint32_t total;
@@ -135,23 +166,23 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_reserve_kernel(Kv8PageParams
     }
     uint32_t here;
     uint32_t at = found + prefix_sum((uint32_t)__popc(free), here, parts);
-    for (; free != 0; free &= free - 1, ++at)
-      if (at < total) p.target[at] = (int)first + __builtin_ctz(free);
+    for (; free != 0 && at < total; free &= free - 1, ++at) {
+      const int page = (int)first + __builtin_ctz(free);
+      if constexpr (HELD) pages[at] = page;
+      else p.target[at] = page;
+    }
     found += here;
   }
   const uint32_t given = found < total ? found : total;
-  sync_shared();
-  // p.target[k]: the page of the k-th item that wants one; those that are copies are told again in p.source by pairs
+  sync_shared();  // the k-th item that wants a page takes pages[k]; refs are read above and changed below
   if (wanted != 0)
-    for (int i = i0; i < i1; ++i) {
-      const int kind = p.wants[i];
-      if (kind == kHeld) continue;
+    for_items([&](Item& x, int) {
+      if (x.kind == kHeld) return;
       if (rank < given) {
-        const Item x = item_of(p, i);
-        const int page = p.target[rank];
+        const int page = HELD ? pages[HELD ? rank : 0] : p.target[rank];
         c.table[x.at] = page;
         store_shared(c.refs + page, 1);
-        if (kind == kCopy) {
+        if (x.kind == kCopy) {
           atomicSub(c.refs + x.entry, 1);
           const int k = atomicAdd(&copies, 1);
           p.source[2 * k] = x.entry;
@@ -159,7 +190,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_reserve_kernel(Kv8PageParams
         }
       }
       ++rank;
-    }
+    });
   __syncthreads();
   if (threadIdx.x == 0) {
     p.plan[0] = copies;
@@ -215,14 +246,16 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_compact_kernel(Kv8PageParams
     }
     return used;
   };
-  uint32_t mine = 0, live;
-  for (int64_t base = 0; base < c.pages; base += (int64_t)kPlanThreads * RUN)
-    mine += (uint32_t)__popc(used_of(base + (int)threadIdx.x * RUN));
+  uint32_t mine = 0, live, used_now = 0;
+  for (int64_t base = 0; base < c.pages; base += (int64_t)kPlanThreads * RUN) {
+    used_now = used_of(base + (int)threadIdx.x * RUN);
+    mine += (uint32_t)__popc(used_now);
+  }
   prefix_sum(mine, live, parts);
   uint32_t moved = 0, holes = 0;
   for (int64_t base = 0; base < c.pages; base += (int64_t)kPlanThreads * RUN) {
     const int64_t first = base + (int)threadIdx.x * RUN;
-    const uint32_t used = used_of(first);
+    const uint32_t used = c.pages <= kPlanThreads * RUN ? used_now : used_of(first);  // one step: it is known
     const int inside = first >= c.pages ? 0 : (int)(c.pages - first < RUN ? c.pages - first : RUN);
     const int low = first >= live ? 0 : (int)(live - first < inside ? live - first : inside);  // pages before `live`
     const uint32_t low_bits = (1u << low) - 1, all_bits = (1u << inside) - 1;
@@ -292,7 +325,8 @@ __global__ __launch_bounds__(kThreads) void kv8_move_kernel(Kv8PageParams p) {
 }
 
 Kv8PageKernels kv8_page_kernels() {
-  return {(const void*)&kv8_reserve_kernel,   (const void*)&kv8_fork_kernel,       (const void*)&kv8_truncate_kernel,
+  return {{(const void*)&kv8_reserve_kernel<false>, (const void*)&kv8_reserve_kernel<true>}, kHeldItems * kPlanThreads,
+           (const void*)&kv8_fork_kernel,       (const void*)&kv8_truncate_kernel,
           (const void*)&kv8_compact_kernel,   (const void*)&kv8_move_kernel<false>, (const void*)&kv8_move_kernel<true>,
           kPlanThreads, kThreads};
 }
