@@ -182,9 +182,12 @@ def test_grids_that_hip_does_not_take():
     wide = _cache(B=64, H_kv=1 << 20, page_stride=1 << 40)
     assert lib.kv8_append(ctypes.byref(_append(wide, rows=1 << 10, k_stride=rows, v_stride=rows)), None) == hip_lib.FA_EINVAL
     assert "cache append grid too large" in hip_lib.last_error()
-    many = _attend(_cache(B=64, H_kv=1), H=1, M=1 << 16, splits=33, workspace=256, workspace_bytes=1 << 60)
+    many = _attend(_cache(B=1 << 18, H_kv=1), H=16, M=1, splits=33, workspace=256, workspace_bytes=1 << 60)
     assert lib.kv8_attend(ctypes.byref(many), None) == hip_lib.FA_EINVAL
     assert "cache merge grid too large" in hip_lib.last_error()
+    chunks = _attend(_cache(B=1 << 14, H_kv=1), H=1, M=1 << 12, splits=512, workspace=256, workspace_bytes=1 << 60)
+    assert lib.kv8_attend(ctypes.byref(chunks), None) == hip_lib.FA_EINVAL
+    assert "cache join grid too large" in hip_lib.last_error()
 
 
 def test_empty_calls_do_nothing():
