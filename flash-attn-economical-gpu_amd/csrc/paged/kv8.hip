@@ -673,15 +673,23 @@ struct Kv8Attend {
   }
 };
 
-// Waves per SIMD: what the registers of a tile, Q and O allow.
+// Waves per SIMD: what the registers of a tile, Q and O allow without spilling.
 template <int D, int R>
 constexpr int attend8_waves() {
-  return D == 64 ? (R == 1 ? 5 : 4) : (D == 128 ? (R == 1 ? 4 : 2) : (R == 1 ? 2 : 1));
+  return D == 64 ? (R == 1 ? 5 : 3) : (D == 128 && R == 1 ? 4 : 2);
 }
 template <typename Tag, int D, int R>
 __global__ __launch_bounds__(256, (attend8_waves<D, R>())) void kv8_attend_kernel(Kv8AttendParams p) {
   __shared__ __align__(16) float smem[4 * 16 * (D + 4)];
   Kv8Attend<Tag, D, R>::run(p, smem);
+}
+// The kernel of 32 rows. At D = 256 a tile, Q and O of 32 rows take more registers than a wave has (144 spilled): there
+// workgroups of 16 rows lie next to each other and the second reads the cache from L2. 24 rows against 16k keys, one
+// sequence: 23.3 us against 22.8, 8 sequences 63 against 61; prompts' kernel 48 and 75.
+template <typename Tag, int D>
+constexpr const void* attend_two_tiles() {
+  if constexpr (D == 256) return nullptr;
+  else return (const void*)&kv8_attend_kernel<Tag, D, 2>;
 }
 
 // Chunks of a prompt: more than 32 query rows to a kv head. The workgroup's four waves, of 32 rows each, share the
@@ -1158,8 +1166,14 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttendParams p) {
   join_parts<Tag, D, Kv8Chunk<Tag, D>::BLOCK>(p);
 }
 
+// Workgroups to a CU. At D = 64 the third costs 4 spilled registers, and 1024 rows against 16k keys twice take 207 us
+// where two workgroups take 221.
+template <int D>
+constexpr int chunk8_waves() {
+  return D == 64 ? 3 : 2;
+}
 template <typename Tag, int D>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv8_chunk_kernel(Kv8AttendParams p) {
+__global__ __launch_bounds__(256, (chunk8_waves<D>())) void kv8_chunk_kernel(Kv8AttendParams p) {
   __shared__ __align__(1024) char smem[Kv8Chunk<Tag, D>::SMEM];
   __shared__ uint32_t flags[3][2];
   Kv8Chunk<Tag, D>::run(p, smem, flags);
@@ -1174,10 +1188,10 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void kv8_merge_kernel(Kv8At
   {DTYPE, D, (const void*)&kv8_append_kernel<TAG, D>,                                                       \
    {(const void*)&kv8_merge_kernel<TAG, D, 1>, (const void*)&kv8_merge_kernel<TAG, D, 4>,                   \
     (const void*)&kv8_merge_kernel<TAG, D, 16>},                                                            \
-   {(const void*)&kv8_attend_kernel<TAG, D, 1>, (const void*)&kv8_attend_kernel<TAG, D, 2>,                 \
-    (const void*)&kv8_chunk_kernel<TAG, D>},                                                                \
-   (const void*)&kv8_join_kernel<TAG, D>,                                                                  \
-   {attend8_waves<D, 1>(), attend8_waves<D, 2>(), D == 64 ? 3 : 2}, Kv8Chunk<TAG, D>::BLOCK, Kv8Chunk<TAG, D>::T, kJoinRows}
+   {(const void*)&kv8_attend_kernel<TAG, D, 1>, attend_two_tiles<TAG, D>(), (const void*)&kv8_chunk_kernel<TAG, D>}, \
+   (const void*)&kv8_join_kernel<TAG, D>,                                                                   \
+   {attend8_waves<D, 1>(), attend8_waves<D, 2>(), chunk8_waves<D>()},                                       \
+   Kv8Chunk<TAG, D>::BLOCK, Kv8Chunk<TAG, D>::T, kJoinRows}
 
 static const Kv8KernelEntry kKv8Entries[] = {
     KV8_ENTRY(f16_t, FA_DTYPE_F16, 64),   KV8_ENTRY(f16_t, FA_DTYPE_F16, 128),   KV8_ENTRY(f16_t, FA_DTYPE_F16, 256),

@@ -69,14 +69,14 @@ int check_layer(const kv8_cache* c, int layer) {
 }
 
 // Which attention kernel takes a kv head's query rows: up to 32 the waves of a workgroup share them (and the cache is read
-// once); more go chunk_rows to a workgroup.
+// once, or by two workgroups of 16 rows); more go chunk_rows to a workgroup.
 struct Kind {
   int kind;
   int64_t row_blocks;
 };
 Kind kind_of(const fa::Kv8KernelEntry* e, int64_t rows) {
   Kind k;
-  k.kind = rows <= 16 ? 0 : (rows <= 32 ? 1 : 2);
+  k.kind = rows <= 32 ? (rows <= 16 || e->attend[1] == nullptr ? 0 : 1) : 2;
   const int64_t block = k.kind == 2 ? e->chunk_rows : 16 << k.kind;
   k.row_blocks = (rows + block - 1) / block;
   return k;
