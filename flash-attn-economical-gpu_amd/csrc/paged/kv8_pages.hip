@@ -80,7 +80,7 @@ __device__ inline Item item_of(const Kv8PageParams& p, int i) {
 // item takes the k-th page.
 // HELD: items stay in registers, EACH to a thread, and the pages found in LDS (up to 8192 items); otherwise they are
 // looked up again and kept in the workspace. One decode step of 32 sequences 5 us, the prompts of 32 sequences of 2-4k
-// tokens 7, where the workspace form takes 8 and 18.
+// tokens 9, where the workspace form takes 8 and 18. Bound by five dependent loads and the barriers between them.
 constexpr int kHeldItems = 8;
 template <bool HELD>
 __global__ __launch_bounds__(kPlanThreads) void kv8_reserve_kernel(Kv8PageParams p) {
@@ -198,7 +198,8 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_reserve_kernel(Kv8PageParams
   }
 }
 
-// A workgroup takes some columns of all sequences: every entry is read before one is written.
+// A workgroup takes some columns of all sequences: every entry is read before one is written. 32 sequences of 32 columns
+// 4.3 us: a launch and two loads, one behind the other, then the counts' atomics.
 __global__ __launch_bounds__(kThreads) void kv8_fork_kernel(Kv8PageParams p) {
   __shared__ int old[kForkEntries];
   const Kv8Pages& c = p.cache;
@@ -215,6 +216,7 @@ __global__ __launch_bounds__(kThreads) void kv8_fork_kernel(Kv8PageParams p) {
   }
 }
 
+// Every entry of the table, a lane to each; 32 x 128 of them 2.8 us, a launch.
 __global__ __launch_bounds__(kThreads) void kv8_truncate_kernel(Kv8PageParams p) {
   const Kv8Pages& c = p.cache;
   const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
@@ -228,7 +230,7 @@ __global__ __launch_bounds__(kThreads) void kv8_truncate_kernel(Kv8PageParams p)
 }
 
 // Which pages move where: the k-th used page at or behind the number of used pages goes to the k-th free one before it.
-// p.mark: the new number of each page from there on.
+// p.mark: the new number of each page from there on. 2048 pages: 4.8 us, as reserve.
 __global__ __launch_bounds__(kPlanThreads) void kv8_compact_kernel(Kv8PageParams p) {
   __shared__ uint32_t parts[kPlanThreads / 64];
   const Kv8Pages& c = p.cache;
@@ -288,7 +290,8 @@ __global__ __launch_bounds__(kPlanThreads) void kv8_compact_kernel(Kv8PageParams
 }
 
 // Copies the planned pages, all layers, and (MAP) writes the table's new entries. The host does not know how many there
-// are: workgroups take slices in turn until there is none left.
+// are: workgroups take slices in turn until there is none left. 269 MB read and as much written 90 us right after a call
+// that read them (6.0 TB/s; a large copy has 4.8), 16 pages of 32 layers (67 MB and as much) 26 us, 5.2 TB/s.
 template <bool MAP>
 __global__ __launch_bounds__(kThreads) void kv8_move_kernel(Kv8PageParams p) {
   const Kv8Pages& c = p.cache;
