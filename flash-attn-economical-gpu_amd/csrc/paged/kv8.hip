@@ -229,7 +229,8 @@ template <>
 __device__ constexpr float lag_bias<f16_t>() { return 8.f; }
 template <>
 __device__ constexpr float lag_bias<bf16_t>() { return 0.f; }
-// Beyond this R, x c and R c cancel to what their rounding leaves: the difference of the scores is taken first.
+// Beyond this R, x c and R cancel to what their rounding leaves: the difference of the scores is taken first, from the
+// score that gave R, which is its product with c as it stands (rounded to a whole number it would be another's).
 constexpr float kLargeR = 0x1p20f;
 
 // n / d for 0 <= n < 2^31 (the host's numbers in fa_kernels.h): with `shift` = ceil(log2 d), 2^32 + multiplier is
@@ -853,7 +854,7 @@ struct Kv8Chunk {
     floatx4 o[DT16][QT];
     float m[QT], l[QT], off[QT];  // row's reference score, sum of weights, bias - R
     bool large = false;
-    const float lag = kLag / p.c;
+    const float lag = fminf(kLag / p.c, 0x1.fffffep127f);  // finite, so that any score moves the first maximum
 #pragma unroll
     for (int j = 0; j < QT; ++j) {
       m[j] = FA_NEG_INF;
@@ -974,8 +975,12 @@ struct Kv8Chunk {
 #pragma unroll
         for (int j = 0; j < QT; ++j) {
           // each row by itself: what another row of the wave sees does not change its bits
-          const float to = move[j] ? lag_bias<Tag>() - __builtin_rintf(tops[j] * p.c) : off[j];
-          const float f = m[j] == FA_NEG_INF ? 0.f : (move[j] ? fast_exp2(to - off[j]) : 1.f);
+          float to = lag_bias<Tag>() - tops[j] * p.c;
+          bool still = fabsf(to) <= kLargeR;
+          if (still) to = lag_bias<Tag>() - __builtin_rintf(tops[j] * p.c);
+          still |= fabsf(off[j]) <= kLargeR;  // the old one or the new one lies in reach
+          const float f = m[j] == FA_NEG_INF ? 0.f : (move[j] ? fast_exp2(still ? to - off[j] : (m[j] - tops[j]) * p.c) : 1.f);
+          to = move[j] ? to : off[j];
           l[j] *= f;
 #pragma unroll
           for (int d = 0; d < DT16; ++d) o[d][j] *= f;

@@ -233,6 +233,61 @@ def test_large_scores_and_odd_scale_bytes(gpu):
         assert torch.equal(out[0], out[1]) and torch.equal(out[0], out[2])
 
 
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("M", [1, 40])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+def test_scores_far_from_zero(gpu, monkeypatch, dtype, M, splits):
+    """Scores of 2^21 that differ by a few: softmax is of the differences, whatever the scores themselves are.
+
+    Scores are exact (two channels: 2^11 x 2^10, and 1 x a multiple of 1/2), so are their differences. An exponent is
+    a difference times scale x log2 e, rounded: 2^-24 x 2 x 24 x 1.45 x ln 2 < 2^-18. Where parts are joined, each is
+    known by fl(m c), of about 3 x 2^20: half a step is 1/8, two of them 1/4, a factor of 2^(1/4) at most."""
+    B, H, Hk, capacity, D = 1, 2, 2, 400, 64
+    monkeypatch.setattr(kv8, "choose_splits", lambda *a: splits)
+    monkeypatch.setattr(flash_atten, "_plans", {})
+    cache = kv8.Kv8Cache(B, Hk, capacity, D, dtype=dtype)
+    _deal(cache, [capacity])
+    k, v = torch.zeros(B, Hk, capacity, D), _rand(5, B, Hk, capacity, D, dtype=dtype)
+    k[..., 0] = 2.0 ** 10
+    k[..., 1] = torch.arange(capacity)[None, None] // 64 * 3.5 + torch.arange(capacity)[None, None] % 3  # it keeps growing
+    cache.append(k.to(dtype).cuda(), v.cuda(), _i32(0))
+    q = torch.zeros(B, H, M, D)
+    q[..., 0], q[..., 1] = 2.0 ** 11, 1.0
+    q = q.to(dtype).cuda()
+    for start in (capacity - M, 300, 100):
+        o = flash_atten.sdpa_kv8(q, cache, _i32(start), scale=1.0)
+        model = Model(cache)
+        want, lse, _ = model.attention(q, [start], scale=1.0)
+        keys, values, _ = model.line(0, 0)
+        mass = torch.stack([torch.softmax((q[0, h].double().cpu() @ keys[h].t()).masked_fill(
+            torch.arange(capacity)[None] > start + torch.arange(M)[:, None], -math.inf), -1) @ values[h].abs() for h in range(H)])
+        u = torch.finfo(dtype).eps / 2
+        e = 2 * 2.0 ** -18 + (0.0 if splits == 1 else 2 * (2.0 ** 0.25 - 1))
+        assert ((o[0].double().cpu() - want[0]).abs() <= 1.01 * ((u + e) * mass + u * want[0].abs() + 2.0 ** -24)).all()
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("M", [1, 40])
+def test_a_scale_of_almost_nothing(gpu, monkeypatch, M, splits):
+    """A scale below the smallest normal number: every key weighs the same, the result is the mean of the values (of 400
+    terms at most, summed in fp32; the weights are exact)."""
+    B, H, Hk, capacity, D = 1, 4, 2, 400, 64
+    monkeypatch.setattr(kv8, "choose_splits", lambda *a: splits)
+    monkeypatch.setattr(flash_atten, "_plans", {})
+    cache = kv8.Kv8Cache(B, Hk, capacity, D, dtype=F16)
+    _deal(cache, [capacity])
+    cache.append(*(_rand(i, B, Hk, capacity, D, dtype=F16).cuda() for i in range(2)), _i32(0))
+    q = _rand(2, B, H, M, D, dtype=F16).cuda()
+    o, lse = flash_atten.sdpa_kv8(q, cache, _i32(capacity - M), scale=1e-39, return_lse=True)
+    _, values, _ = Model(cache).line(0, 0)
+    for h in range(H):
+        for i in range(M):
+            v = values[h // 2, :capacity - M + i + 1]
+            mean, u = v.mean(0), 2.0 ** -11
+            assert ((o[0, h, i].double().cpu() - mean).abs() <= u * mean.abs() + 400 * 2.0 ** -24 * v.abs().mean(0) + 2.0 ** -25).all()
+            assert abs(float(lse[0, h, i]) - math.log(len(v))) <= 2e-6
+
+
 def _state(seed, B, capacity, page, pages, layers=1, D=64, Hk=1):
     cache = kv8.Kv8Cache(B, Hk, capacity, D, dtype=BF16, pages=pages, page_size=page, layers=layers)
     g = torch.Generator().manual_seed(seed)
