@@ -24,6 +24,16 @@ const fa::Kv8KernelEntry* find_kv8(int dtype, int D) {
 
 int64_t codes_bytes(int64_t Hkv, int64_t page, int64_t D) { return 2 * Hkv * page * D; }
 
+int check_buffers(const kv8_cache* c) {
+  if (!c->data || !c->refs) return fail(FA_EINVAL, "null cache pointer");
+  if (!aligned(c->data, 16) || c->page_stride % 16 || c->layer_stride % 16)
+    return fail(FA_EINVAL, "cache data and its strides must be 16-byte aligned");
+  if (c->pages > 1 && c->page_stride < kv8_page_bytes(c->H_kv, c->page, c->D))
+    return fail(FA_EINVAL, "page stride %lld is under a page's %lld bytes", (long long)c->page_stride,
+                (long long)kv8_page_bytes(c->H_kv, c->page, c->D));
+  return FA_OK;
+}
+
 int check_cache(const kv8_cache* c) {
   const int code = check_type(c->dtype, c->D);
   if (code != FA_OK) return code;
@@ -38,14 +48,9 @@ int check_cache(const kv8_cache* c) {
   if ((int64_t)c->columns * c->page < c->capacity)
     return fail(FA_EINVAL, "%d columns of %d tokens do not hold the capacity %d", c->columns, c->page, c->capacity);
   if ((int64_t)c->B * c->columns > (1 << 30)) return fail(FA_EINVAL, "page table too large (%d x %d)", c->B, c->columns);
-  if (c->B == 0 || c->columns == 0) return FA_OK;
-  if (!c->table || !c->data || !c->refs) return fail(FA_EINVAL, "null cache pointer");
-  if (!aligned(c->data, 16) || c->page_stride % 16 || c->layer_stride % 16)
-    return fail(FA_EINVAL, "cache data and its strides must be 16-byte aligned");
-  if (c->pages > 1 && c->page_stride < kv8_page_bytes(c->H_kv, c->page, c->D))
-    return fail(FA_EINVAL, "page stride %lld is under a page's %lld bytes", (long long)c->page_stride,
-                (long long)kv8_page_bytes(c->H_kv, c->page, c->D));
-  return FA_OK;
+  if (c->B == 0 || c->columns == 0) return FA_OK;  // no call but compact reads anything
+  if (!c->table) return fail(FA_EINVAL, "null cache pointer");
+  return check_buffers(c);
 }
 
 fa::Kv8Pages pages_of(const kv8_cache* c, int layer) {
@@ -321,7 +326,7 @@ int kv8_reserve(const kv8_reserve_args* a, void* stream) {
   if (a->rows < 0) return fail(FA_EINVAL, "invalid row count %d", a->rows);
   if (a->missing == nullptr) return fail(FA_EINVAL, "null missing pointer");
   const int64_t span = span_of(c, a->rows);
-  if (span > 0 && a->start == nullptr) return fail(FA_EINVAL, "null start pointer");
+  if (c->B * span > 0 && a->start == nullptr) return fail(FA_EINVAL, "null start pointer");
   const PageWorkspace w = reserve_workspace(c, a->rows);
   if ((code = check_workspace(a->workspace, a->workspace_bytes, w.bytes, "reserve")) != FA_OK) return code;
   fa::Kv8PageParams p = page_params(c);
@@ -383,6 +388,7 @@ int kv8_compact(const kv8_compact_args* a, void* stream) {
   const kv8_cache* c = &a->cache;
   int code = check_cache(c);
   if (code != FA_OK) return code;
+  if ((code = check_buffers(c)) != FA_OK) return code;
   if (a->used == nullptr) return fail(FA_EINVAL, "null used pointer");
   const PageWorkspace w = compact_workspace(c);
   if ((code = check_workspace(a->workspace, a->workspace_bytes, w.bytes, "compact")) != FA_OK) return code;

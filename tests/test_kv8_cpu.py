@@ -190,6 +190,13 @@ def test_grids_that_hip_does_not_take():
     assert "cache join grid too large" in hip_lib.last_error()
 
 
+def test_compact_needs_the_counts_without_sequences_too():
+    lib = hip_lib.load()
+    for over in ({"refs": None}, {"data": None}):
+        assert lib.kv8_compact(ctypes.byref(_compact(_cache(B=0, **over))), None) == hip_lib.FA_EINVAL
+        assert "null cache" in hip_lib.last_error()
+
+
 def test_empty_calls_do_nothing():
     lib = hip_lib.load()
     assert lib.kv8_append(None, None) == lib.kv8_attend(None, None) == hip_lib.FA_EINVAL

@@ -358,6 +358,20 @@ def test_the_same_page_twice(gpu):
     model.check(cache)
 
 
+def test_no_sequences(gpu):
+    cache = kv8.Kv8Cache(0, 2, 100, 64, dtype=F16, pages=5, layers=2)
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    kv = torch.zeros(0, 2, 3, 64, dtype=F16, device="cuda")
+    assert cache.reserve(none, 3).tolist() == [0] and cache.reserve(none, 3, count=none).tolist() == [0]
+    got = cache.append(kv, kv, none, return_values=True)
+    assert [t.shape for t in got] == [kv.shape] * 2
+    o, lse = flash_atten.sdpa_kv8(torch.zeros(0, 4, 3, 64, dtype=F16, device="cuda"), cache, none, return_lse=True)
+    assert o.shape == (0, 4, 3, 64) and lse.shape == (0, 4, 3)
+    cache.fork(none)
+    cache.truncate(none)
+    assert cache.compact().tolist() == [0] and cache.refs.tolist() == [0] * 5
+
+
 def test_large_pools_and_tables(gpu):
     """Many steps of each search: 70000 pages, 130 sequences; reserve of 65000 entries, compaction of a pool in use at both
     ends."""
