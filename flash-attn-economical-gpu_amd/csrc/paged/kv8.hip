@@ -722,6 +722,7 @@ struct Kv8Chunk {
   static constexpr int BLOCK = WAVES * QT * 16;
   static constexpr int TILEB = T * L::ROWB, STAGEB = 2 * TILEB;
   static constexpr int SMEM = 2 * STAGEB;
+  static constexpr int kAhead = 4;  // fragments
   static constexpr int PER = T * UPR / 256;  // 16-channel units of K, and of V, per thread
   static_assert(PER * 256 == T * UPR, "units");
 
@@ -934,26 +935,22 @@ struct Kv8Chunk {
       if (EDGE && (key0 + T < keys ? key0 + T : keys) > live_least)
         alone = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)flags[turn][0]) |
                 (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)flags[turn][1]) << 32;
-      // D = 64: all of K's fragments (32 registers) are asked for before the first product.
-      u32x4 ahead[KT][KS];
-      if constexpr (D == 64) {
+      // Fragments are asked for kAhead before their products, in this order: left to itself the compiler asks for each right
+      // before its two products and waits for it, an LDS latency for every 32 cycles of the matrix unit.
+      u32x4 ring[kAhead];
+      auto keys_of = [&](int n) { return L::frag(smem, rowb ^ (n % KS << 6), n / KS * 16 * L::ROWB); };
 #pragma unroll
-        for (int i = 0; i < KT; ++i)
-#pragma unroll
-          for (int k = 0; k < KS; ++k) ahead[i][k] = L::frag(smem, rowb ^ (k << 6), i * 16 * L::ROWB);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      for (int n = 0; n < kAhead; ++n) ring[n] = keys_of(n);
+      __builtin_amdgcn_sched_barrier(0);
       floatx4 x[KT][QT];
 #pragma unroll
-      for (int i = 0; i < KT; ++i) {
+      for (int n = 0; n < KT * KS; ++n) {
+        const int i = n / KS, k = n % KS;
 #pragma unroll
-        for (int j = 0; j < QT; ++j) x[i][j] = (floatx4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const u32x4 a = D == 64 ? ahead[i][k] : L::frag(smem, rowb ^ (k << 6), i * 16 * L::ROWB);
-#pragma unroll
-          for (int j = 0; j < QT; ++j) x[i][j] = E::mfma16(a, qf[j][k], x[i][j]);
-        }
+        for (int j = 0; j < QT; ++j)
+          x[i][j] = E::mfma16(ring[n % kAhead], qf[j][k], k == 0 ? (floatx4){0.f, 0.f, 0.f, 0.f} : x[i][j]);
+        if (n + kAhead < KT * KS) ring[n % kAhead] = keys_of(n + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
       }
       bool move[QT];
       float tops[QT];
@@ -1004,6 +1001,11 @@ struct Kv8Chunk {
             for (int n = 0; n < 4; ++n) x[i][j][n] -= far ? m[j] : 0.f;
         }
       }
+      constexpr int VALUES = DT16 * KT / 2;
+      auto values_of = [&](int n) { return L::tfrag(smem, colb ^ (n / (KT / 2) << 5), TILEB + n % (KT / 2) * 32 * L::ROWB); };
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) ring[n] = values_of(n);
+      __builtin_amdgcn_sched_barrier(0);
       u32x4 pb[KT / 2][QT];
 #pragma unroll
       for (int j = 0; j < QT; ++j)
@@ -1030,14 +1032,15 @@ struct Kv8Chunk {
       };
       __builtin_amdgcn_s_setprio(1);  // before a neighbour's softmax
 #pragma unroll
-      for (int d = 0; d < DT16; ++d)
+      for (int n = 0; n < VALUES; ++n) {
+        const int d = n / (KT / 2), i = n % (KT / 2);
+        u32x4 v = ring[n % kAhead];
+        if (EDGE && alone != 0) v &= ~lanes_of((uint32_t)(alone >> (32 * i)));
 #pragma unroll
-        for (int i = 0; i < KT / 2; ++i) {
-          u32x4 v = L::tfrag(smem, colb ^ (d << 5), TILEB + i * 32 * L::ROWB);
-          if (EDGE && alone != 0) v &= ~lanes_of((uint32_t)(alone >> (32 * i)));
-#pragma unroll
-          for (int j = 0; j < QT; ++j) o[d][j] = E::mfma16(v, pb[i][j], o[d][j]);
-        }
+        for (int j = 0; j < QT; ++j) o[d][j] = E::mfma16(v, pb[i][j], o[d][j]);
+        if (n + kAhead < VALUES) ring[n % kAhead] = values_of(n + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
+      }
       __builtin_amdgcn_s_setprio(0);
       if constexpr (EDGE) {
 #pragma unroll 1
