@@ -703,10 +703,13 @@ constexpr const void* attend_two_tiles() {
 // 16-bit rows in LDS (two stages, one barrier a tile), and both products read their fragments there, V's by the
 // transposing read. S^T = K Q^T and O^T = V^T P^T as above. The chip's workgroups take equal shares of all blocks' tiles,
 // or whole blocks where there are at least two to a place, the longest first: 2 x 32 heads of a first 2048 rows 93 us whole
-// and 167 in shares; 2 x 28 heads of 509 rows against 12-16k keys (not even one to a place) 261 in shares and 598 whole.
-// Products of 1024 rows against 32k keys, 32/8 heads, D = 128 run at 900 TFLOP/s, of a first 2048 rows at 735, D = 64 and
-// 256 at 650. Two waves to a SIMD (registers, LDS) wait for LDS and barriers 40% of their cycles. Eight waves in two groups
-// that take turns at products and softmax gave 847, 650, 508 and 521: their barriers cost more than the overlap gave.
+// and 167 in shares; 2 x 28 heads of 509 rows against 12-16k keys (not even one to a place) 261 in shares and 598 whole (both
+// before fragments were asked for ahead: 88 and 245 since).
+// Products of 1024 rows against 32k keys, 32/8 heads, D = 128 run at 1000 TFLOP/s, of a first 2048 rows at 775, D = 64 at
+// 690 and D = 256 at 755. Bound by two waves to a SIMD (registers, LDS): matrix unit, vector unit and LDS are busy about
+// half of the time each, and overlap as far as two waves let them. Eight waves in two groups that take turns at products
+// and softmax were 5 to 25% slower than four (without fragments ahead), their barriers cost more than the overlap gave.
+// Sums of the rounded weights by the matrix unit gave 1 to 5% and an lse of 16-bit weights: the sums stay in the vector unit.
 // Fewest key tiles to a workgroup's share: below, the parts' extra pass costs more than it gives.
 constexpr int kMinShare = 4;
 
@@ -722,7 +725,9 @@ struct Kv8Chunk {
   static constexpr int BLOCK = WAVES * QT * 16;
   static constexpr int TILEB = T * L::ROWB, STAGEB = 2 * TILEB;
   static constexpr int SMEM = 2 * STAGEB;
-  static constexpr int kAhead = 4;  // fragments
+  // Fragments in flight, as the registers allow: at D = 128 (255 of them) 244 us with 8 for 2 x 28 heads of 509 rows, 252 with
+  // 4; at D = 256 709 us with 8 for 2 x 16 heads of 1024, 701 with 4; at D = 64 4 spills ten registers where 3 spills four.
+  static constexpr int kAhead = D == 64 ? 3 : (D == 128 ? 8 : 4);
   static constexpr int PER = T * UPR / 256;  // 16-channel units of K, and of V, per thread
   static_assert(PER * 256 == T * UPR, "units");
 
@@ -942,6 +947,7 @@ struct Kv8Chunk {
 #pragma unroll
       for (int n = 0; n < kAhead; ++n) ring[n] = keys_of(n);
       __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);  // before a neighbour's softmax
       floatx4 x[KT][QT];
 #pragma unroll
       for (int n = 0; n < KT * KS; ++n) {
@@ -952,6 +958,7 @@ struct Kv8Chunk {
         if (n + kAhead < KT * KS) ring[n % kAhead] = keys_of(n + kAhead);
         __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_s_setprio(0);
       bool move[QT];
       float tops[QT];
 #pragma unroll
@@ -1030,7 +1037,7 @@ struct Kv8Chunk {
         }
         return m;
       };
-      __builtin_amdgcn_s_setprio(1);  // before a neighbour's softmax
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int n = 0; n < VALUES; ++n) {
         const int d = n / (KT / 2), i = n % (KT / 2);
@@ -1184,8 +1191,8 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttendParams p) {
   join_parts<Tag, D, Kv8Chunk<Tag, D>::BLOCK>(p);
 }
 
-// Workgroups to a CU. At D = 64 the third costs 4 spilled registers, and 1024 rows against 16k keys twice take 207 us
-// where two workgroups take 221.
+// Workgroups to a CU. At D = 64 the third costs 4 spilled registers, and 1024 rows against 16k keys twice took 207 us
+// where two workgroups took 221 (193 now).
 template <int D>
 constexpr int chunk8_waves() {
   return D == 64 ? 3 : 2;
