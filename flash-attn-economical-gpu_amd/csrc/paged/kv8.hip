@@ -97,10 +97,11 @@ __device__ inline int page_at(const Kv8Pages& c, int b, int64_t column) {
 
 // Append: a wave takes a block, 16 channels of a row to a lane and step: the tokens that the block holds already, the
 // new rows, zeros behind them. The largest finite magnitude of all gives the scale (integer compares: any host that
-// follows the definition gets the same bytes), and the block is written whole, so what it holds depends on its tokens
-// only, not on rows that were drafted in vain or on what the page held before. Bound by memory: 4 prompts of 2-4k tokens,
+// follows the definition gets the same bytes), and the block is written whole, so it holds nothing of rows that were
+// drafted in vain or of what the page held before, and its scale is that of its tokens. (Tokens that stay are rounded again
+// where the scale grows.) Bound by memory: 4 prompts of 2-4k tokens,
 // 8 heads, D = 128, values returned (149 MB), 24.5 us, 6.1 TB/s, some of it in the caches. A step of 32 single tokens
-// 5.8 us: a chain of four dependent loads (start, page, the block's scale and codes, all but the last two in turn).
+// 6 us: a chain of four dependent loads (start, page, the block's scale and codes, all but the last two in turn).
 template <typename Tag, int D>
 __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendParams p) {
   typedef Fp8<Tag> F;
