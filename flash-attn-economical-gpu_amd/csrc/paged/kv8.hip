@@ -973,7 +973,9 @@ struct Kv8Chunk {
             top = larger(top, x[i][j][r]);
           }
         tops[j] = row_max(top);
-        move[j] = tops[j] > m[j] + lag;  // a NaN score makes the row NaN through P
+        // the difference, not the sum m + lag: that one rounds to the spacing of the scores. A NaN score makes the row NaN
+        // through P
+        move[j] = tops[j] - m[j] > lag;
       }
       if (__any(QT == 2 ? move[0] || move[QT - 1] : move[0])) {
         bool far = false;

@@ -1,0 +1,63 @@
+"""Attention over the paged 8-bit cache where its running softmax, its joins and its searches come to their ends."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import flash_atten
+import kv8
+from kv8_model import Model
+from test_kv8_gpu import BF16, F16, _deal, _i32, _rand
+
+pytestmark = pytest.mark.gpu
+
+
+def _splits(monkeypatch, n):
+    monkeypatch.setattr(kv8, "choose_splits", lambda *a: n)
+    monkeypatch.setattr(flash_atten, "_plans", {})
+
+
+def _scores(dtype, capacity, H, M, q_channels, k_channels, D=64):
+    """A cache and queries whose scores (scale 1) are the sum of q_channels[i] * k_channels[i] (a number or one for each
+    token), exact in fp32, and random values."""
+    cache = kv8.Kv8Cache(1, H, capacity, D, dtype=dtype)
+    _deal(cache, [capacity])
+    k, v, q = torch.zeros(1, H, capacity, D), _rand(5, 1, H, capacity, D, dtype=dtype), torch.zeros(1, H, M, D)
+    for i, (a, b) in enumerate(zip(q_channels, k_channels)):
+        q[..., i], k[..., i] = a, b
+    held = cache.append(k.to(dtype).cuda(), v.cuda(), _i32(0), return_values=True)[0].cpu()
+    assert torch.equal(held.float(), k) and torch.equal(q.to(dtype).float(), q), "exact operands"
+    return cache, q.to(dtype).cuda()
+
+
+def _check_far(cache, q, start, dtype):
+    """Scores are exact, so are their differences but for half a step of the difference; an exponent is one times
+    fl(log2 e), at most 93 where it counts: 2^-24 x 3 x 93 x ln 2 < 2^-16 on a weight, twice that on a quotient of sums, and
+    the sums of 400 terms take 2^-24 x 400 < 2^-15: 2^-14 in all. P and the result are rounded to the type once; a weight
+    under the type's normal numbers by 2^-25 of a sum of 2^7 at least."""
+    H, M = q.shape[1:3]
+    o, lse = flash_atten.sdpa_kv8(q, cache, _i32(start), scale=1.0, return_lse=True)
+    model = Model(cache)
+    want, want_lse, _ = model.attention(q, [start], scale=1.0)
+    keys, values, _ = model.line(0, 0)
+    u = torch.finfo(dtype).eps / 2
+    assert torch.isfinite(o).all()
+    for h in range(H):
+        s = q[0, h].double().cpu() @ keys[h].t()
+        p = torch.softmax(s.masked_fill(torch.arange(s.shape[1])[None] > start + torch.arange(M)[:, None], -math.inf), -1)
+        bound = (u + 2.0 ** -14) * (p @ values[h].abs()) + u * want[0, h].abs() + 2.0 ** -32 * values[h].abs().sum(0)
+        assert ((o[0, h].double().cpu() - want[0, h]).abs() <= 1.01 * bound).all(), h
+    assert ((lse.double().cpu() - want_lse).abs() <= 2e-5 + 2.0 ** -22 * want_lse.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_a_maximum_that_moves_by_the_spacing_of_the_scores(gpu, monkeypatch, dtype, sign):
+    """Scores of 2^26 are 8 apart: the next larger one is further than the maximum may lag behind."""
+    _splits(monkeypatch, 1)
+    steps = torch.arange(400) // 100 * 8.0
+    cache, q = _scores(dtype, 400, 2, 40, (sign * 2.0 ** 13, 1.0), (2.0 ** 13, steps))
+    for start in (360, 200, 80):
+        _check_far(cache, q, start, dtype)
