@@ -806,7 +806,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv4_chunk_kernel(Kv4Atte
 
 template <typename Tag, int D, int WPR>
 __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void kv4_merge_kernel(Kv4AttendParams p) {
-  merge_splits<Tag, D, WPR>(p);
+  merge_splits<Tag, D, WPR>(p, 1.f);
 }
 
 #define KV4_ENTRY(TAG, DTYPE, D)                                                                                   \

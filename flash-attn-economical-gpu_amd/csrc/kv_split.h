@@ -118,11 +118,13 @@ __device__ inline Split find_split(const Params& p, int slot, int b) {
   return s;
 }
 
-// Joins the splits of a row: weights exp2(m_s - m) of the unnormalised partial sums. WPR waves take a row: one
+// Joins the splits of a row: weights exp2((m_s - m) unit) of the unnormalised partial sums; the maxima m_s are scores with
+// `unit` log2 units to one (the difference comes first: far from zero a product with the unit would be rounded to more than
+// scores may differ by), or in log2 units with 1. WPR waves take a row: one
 // where rows are many and splits few, four or sixteen the other way round (single tokens over long caches). D / 4 lanes read one
 // split's row, so a wave has 256 / D of them in flight at once, times the unrolling.
 template <typename Tag, int D, int WPR, typename Params>
-__device__ inline void merge_splits(const Params& p) {
+__device__ inline void merge_splits(const Params& p, float unit) {
   constexpr int LPS = D / 4, AT_ONCE = WPR * 64 / LPS;
   __shared__ floatx4 part_o[WPR][LPS];
   __shared__ float part_ml[WPR][2];
@@ -146,7 +148,7 @@ __device__ inline void merge_splits(const Params& p) {
 #pragma unroll 4
     for (int s = mine; s < part.used; s += AT_ONCE) {
       const int64_t w = at + s * stride;
-      const float f = fast_exp2(p.ws_ml[2 * w] - base);
+      const float f = fast_exp2((p.ws_ml[2 * w] - base) * unit);
       const floatx4 x = *reinterpret_cast<const floatx4*>(p.ws_o + w * D + 4 * c4);
       sum = fmaf(f, p.ws_ml[2 * w + 1], sum);
 #pragma unroll
@@ -156,7 +158,7 @@ __device__ inline void merge_splits(const Params& p) {
     for (int k = LPS; k < 64; k *= 2) {  // the wave's lane groups
       const float mo = __shfl_xor(m, k, 64), so = __shfl_xor(sum, k, 64);
       const float top = fmaxf(m, mo), ref = top == FA_NEG_INF ? 0.f : top;
-      const float f = fast_exp2(m - ref), fo = fast_exp2(mo - ref);
+      const float f = fast_exp2((m - ref) * unit), fo = fast_exp2((mo - ref) * unit);
       sum = f * sum + fo * so;
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] = f * o[j] + fo * __shfl_xor(o[j], k, 64);
@@ -178,7 +180,7 @@ __device__ inline void merge_splits(const Params& p) {
       o = (floatx4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < WPR; ++w) {
-        const float f = fast_exp2(part_ml[w][0] - ref);
+        const float f = fast_exp2((part_ml[w][0] - ref) * unit);
         sum = fmaf(f, part_ml[w][1], sum);
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[j] = fmaf(f, part_o[w][c4][j], o[j]);
@@ -191,7 +193,7 @@ __device__ inline void merge_splits(const Params& p) {
         (u32x2){DT<Tag>::pack2(o[0] * inv, o[1] * inv), DT<Tag>::pack2(o[2] * inv, o[3] * inv)};
     if (c4 == 0 && p.lse != nullptr)
       p.lse[b * p.sl[0] + h * p.sl[1] + i * p.sl[2]] =
-          sum == 0.f ? FA_NEG_INF : (m + __builtin_amdgcn_logf(sum) - weight_bias<Tag>()) * 0.6931471805599453f;
+          sum == 0.f ? FA_NEG_INF : (m * unit + __builtin_amdgcn_logf(sum) - weight_bias<Tag>()) * 0.6931471805599453f;
   }
 }
 

@@ -555,7 +555,7 @@ struct Kv8Attend {
         *reinterpret_cast<floatx4*>(dst + j) =
             l == 0.f ? (floatx4){0.f, 0.f, 0.f, 0.f} : (floatx4){o[j], o[j + 1], o[j + 2], o[j + 3]};
       if (at == 0) {
-        p.ws_ml[2 * w] = m * p.c;
+        p.ws_ml[2 * w] = m;
         p.ws_ml[2 * w + 1] = l;
       }
     } else {
@@ -1209,7 +1209,7 @@ __global__ __launch_bounds__(256, (chunk8_waves<D>())) void kv8_chunk_kernel(Kv8
 
 template <typename Tag, int D, int WPR>
 __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void kv8_merge_kernel(Kv8AttendParams p) {
-  merge_splits<Tag, D, WPR>(p);
+  merge_splits<Tag, D, WPR>(p, p.c);
 }
 
 #define KV8_ENTRY(TAG, DTYPE, D)                                                                            \

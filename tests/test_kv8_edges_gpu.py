@@ -61,3 +61,17 @@ def test_a_maximum_that_moves_by_the_spacing_of_the_scores(gpu, monkeypatch, dty
     cache, q = _scores(dtype, 400, 2, 40, (sign * 2.0 ** 13, 1.0), (2.0 ** 13, steps))
     for start in (360, 200, 80):
         _check_far(cache, q, start, dtype)
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("M", [1, 20])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("power,spacing", [(12, 2.0), (13, 8.0)])
+def test_parts_whose_maxima_are_far_from_zero(gpu, monkeypatch, power, spacing, dtype, M, splits):
+    """Parts of a row whose maxima differ by steps of scores of 2^24 and 2^26: they are weighed by the difference of the
+    scores, not by that of their rounded products with log2 e."""
+    _splits(monkeypatch, splits)
+    for sign in (1, -1):
+        cache, q = _scores(dtype, 400, 2, M, (sign * 2.0 ** power, 1.0), (2.0 ** power, torch.arange(400) // 50 * spacing))
+        for start in (400 - M, 300 - M, 70):
+            _check_far(cache, q, start, dtype)
