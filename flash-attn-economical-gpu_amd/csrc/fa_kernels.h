@@ -213,7 +213,7 @@ struct Kv8AttendParams {
   const int32_t* start;
   const int32_t* count;  // nullable: all rows
   float* ws_o;           // splits > 1: unnormalised partial sums [slots][H][M][D]
-  float* ws_ml;          // splits > 1: their row maximum (a score; chunks: in log2 units) and sum [slots][H][M][2]
+  float* ws_ml;          // splits > 1: their row maximum (a score; chunks: the reference) and sum [slots][H][M][2]
   int32_t* parts;        // chunks, splits > 1: first workgroup and number of parts [Hkv][B][row_blocks][2]
   int64_t sq[3], so[3], sl[3];
   int32_t B, H, Hkv, M, group, capacity;

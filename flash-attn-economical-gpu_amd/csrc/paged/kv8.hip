@@ -233,6 +233,28 @@ __device__ constexpr float lag_bias<bf16_t>() { return 0.f; }
 // Beyond this R, x c and R cancel to what their rounding leaves: the difference of the scores is taken first, from the
 // score that gave R, which is its product with c as it stands (rounded to a whole number it would be another's).
 constexpr float kLargeR = 0x1p20f;
+// bias - R of a row whose reference score is m.
+template <typename Tag>
+__device__ inline float offset_of(float m, float c) {
+  const float whole = lag_bias<Tag>() - __builtin_rintf(m * c);
+  return fabsf(whole) <= kLargeR ? whole : lag_bias<Tag>() - m * c;
+}
+// The reference itself: R, or the score that gave it.
+struct Reference {
+  float at;
+  bool score;
+  template <typename Tag>
+  __device__ static inline Reference of(float m, float off) {
+    const bool whole = fabsf(off) <= kLargeR;
+    return {whole ? lag_bias<Tag>() - off : m, !whole};
+  }
+  // Less another one, in log2 units, rounded once: scores are subtracted before they are multiplied, and no product is
+  // rounded before it meets an R (to a sixteenth at 2^20: a weight would be off by 4%).
+  __device__ inline float less(const Reference& o, float c) const {
+    if (score == o.score) return score ? (at - o.at) * c : at - o.at;
+    return score ? fmaf(at, c, -o.at) : -fmaf(o.at, c, -at);
+  }
+};
 
 // n / d for 0 <= n < 2^31 (the host's numbers in fa_kernels.h): with `shift` = ceil(log2 d), 2^32 + multiplier is
 // 2^(32 + shift) / d rounded up. Every workgroup runs through its set-up once, from a cold instruction cache: there a
@@ -982,11 +1004,9 @@ struct Kv8Chunk {
 #pragma unroll
         for (int j = 0; j < QT; ++j) {
           // each row by itself: what another row of the wave sees does not change its bits
-          float to = lag_bias<Tag>() - tops[j] * p.c;
-          bool still = fabsf(to) <= kLargeR;
-          if (still) to = lag_bias<Tag>() - __builtin_rintf(tops[j] * p.c);
-          still |= fabsf(off[j]) <= kLargeR;  // the old one or the new one lies in reach
-          const float f = m[j] == FA_NEG_INF ? 0.f : (move[j] ? fast_exp2(still ? to - off[j] : (m[j] - tops[j]) * p.c) : 1.f);
+          float to = offset_of<Tag>(tops[j], p.c);
+          const float back = Reference::of<Tag>(m[j], off[j]).less(Reference::of<Tag>(tops[j], to), p.c);
+          const float f = m[j] == FA_NEG_INF ? 0.f : (move[j] ? fast_exp2(back) : 1.f);
           to = move[j] ? to : off[j];
           l[j] *= f;
 #pragma unroll
@@ -1120,8 +1140,10 @@ struct Kv8Chunk {
         for (int d = 0; d < DT16; ++d)  // a row that saw no key is zeros, whatever values that are no numbers left in o
           *reinterpret_cast<floatx4*>(p.ws_o + w * D + 16 * d + 4 * g) = sum == 0.f ? (floatx4){0.f, 0.f, 0.f, 0.f} : o[d][j];
         if (g == 0) {
-          p.ws_ml[2 * w] = m[j] == FA_NEG_INF ? FA_NEG_INF : lag_bias<Tag>() - off[j];
-          p.ws_ml[2 * w + 1] = sum;
+          // the sum's sign tells what the reference is: a score has a negative one
+          const Reference r = Reference::of<Tag>(m[j], off[j]);
+          p.ws_ml[2 * w] = m[j] == FA_NEG_INF ? FA_NEG_INF : r.at;
+          p.ws_ml[2 * w + 1] = r.score ? -sum : sum;
         }
       } else {
         const float inv = 1.f / sum;
@@ -1139,8 +1161,9 @@ struct Kv8Chunk {
   }
 };
 
-// Joins the parts of a row block: weights exp2(m_s - m) of the unnormalised sums. A wave takes a row, D / 4 lanes a
-// part's row; a workgroup kJoinRows rows of a block. About 700 parts of 64 KB (2 x 28 heads, 509 rows): 12.4 us, 3.9 TB/s.
+// Joins the parts of a row block: weights exp2 of their references' distance to the largest, of the unnormalised sums. A
+// wave takes a row, D / 4 lanes a part's row; a workgroup kJoinRows rows of a block. About 700 parts of 64 KB (2 x 28 heads,
+// 509 rows): 12.4 us, 3.9 TB/s.
 constexpr int kJoinRows = 4;
 template <typename Tag, int D, int BLOCK>
 __device__ inline void join_parts(const Kv8AttendParams& p) {
@@ -1155,28 +1178,49 @@ __device__ inline void join_parts(const Kv8AttendParams& p) {
     const int at = (int)(blockIdx.x % GROUPS) * kJoinRows + k, r = rb * BLOCK + at;
     if (r >= p.M * p.group) return;
     auto place = [&](int s) { return (int64_t)(s == 0 ? 2 * first + 1 : 2 * (first + s)) * BLOCK + at; };
-    float m = FA_NEG_INF, sum = 0.f;
+    float m = FA_NEG_INF, sum = 0.f;  // m: the largest reference
     floatx4 o = (floatx4){0.f, 0.f, 0.f, 0.f};
-    for (int s = lane / LPS; s < n; s += AT_ONCE) m = fmaxf(m, p.ws_ml[2 * place(s)]);
-    const float base = m == FA_NEG_INF ? 0.f : m;
-#pragma unroll 2
+    uint32_t signs = 0;
     for (int s = lane / LPS; s < n; s += AT_ONCE) {
-      const int64_t w = place(s);
-      const float f = fast_exp2(p.ws_ml[2 * w] - base);
+      const u32x2 part = *reinterpret_cast<const u32x2*>(p.ws_ml + 2 * place(s));
+      m = fmaxf(m, __uint_as_float(part[0]));
+      signs |= part[1];
+    }
+    auto add = [&](int64_t w, float f) {
       const floatx4 x = *reinterpret_cast<const floatx4*>(p.ws_o + w * D + 4 * c4);
-      sum = fmaf(f, p.ws_ml[2 * w + 1], sum);
+      sum = fmaf(f, fabsf(p.ws_ml[2 * w + 1]), sum);
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] = fmaf(f, x[j], o[j]);
+    };
+    if (__builtin_expect(__any((int)signs < 0), 0)) {
+      // A part's reference is a score (rare). The largest is looked for by what they are about, by every lane in all parts.
+      Reference top = {0.f, false};
+      m = FA_NEG_INF;
+      auto reference = [&](int s) { return Reference{p.ws_ml[2 * place(s)], __builtin_signbitf(p.ws_ml[2 * place(s) + 1]) != 0}; };
+      for (int s = 0; s < n; ++s) {
+        const Reference r = reference(s);
+        const float about = r.score ? r.at * p.c : r.at;
+        if (about > m) top = r;
+        m = fmaxf(m, about);
+      }
+      for (int s = lane / LPS; s < n; s += AT_ONCE) {
+        const Reference r = reference(s);
+        add(place(s), r.at == FA_NEG_INF ? 0.f : fast_exp2(r.less(top, p.c)));
+      }
+    } else {
+      const float base = m == FA_NEG_INF ? 0.f : m;
+#pragma unroll 2
+      for (int s = lane / LPS; s < n; s += AT_ONCE) add(place(s), fast_exp2(p.ws_ml[2 * place(s)] - base));
     }
 #pragma unroll
     for (int x = LPS; x < 64; x *= 2) {  // the wave's lane groups
       const float mo = __shfl_xor(m, x, 64), so = __shfl_xor(sum, x, 64);
-      const float top = fmaxf(m, mo), ref = top == FA_NEG_INF ? 0.f : top;
+      const float both = fmaxf(m, mo), ref = both == FA_NEG_INF ? 0.f : both;
       const float f = fast_exp2(m - ref), fo = fast_exp2(mo - ref);
       sum = f * sum + fo * so;
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[j] = f * o[j] + fo * __shfl_xor(o[j], x, 64);
-      m = top;
+      m = both;
     }
     if (lane >= LPS) continue;
     const int i = divide(r, p.by_group), h = hk * p.group + r - i * p.group;

@@ -64,7 +64,7 @@ def test_a_maximum_that_moves_by_the_spacing_of_the_scores(gpu, monkeypatch, dty
 
 
 @pytest.mark.parametrize("splits", [1, 3])
-@pytest.mark.parametrize("M", [1, 20])
+@pytest.mark.parametrize("M", [1, 20, 40])
 @pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
 @pytest.mark.parametrize("power,spacing", [(12, 2.0), (13, 8.0)])
 def test_parts_whose_maxima_are_far_from_zero(gpu, monkeypatch, power, spacing, dtype, M, splits):
@@ -75,3 +75,17 @@ def test_parts_whose_maxima_are_far_from_zero(gpu, monkeypatch, power, spacing, 
         cache, q = _scores(dtype, 400, 2, M, (sign * 2.0 ** power, 1.0), (2.0 ** power, torch.arange(400) // 50 * spacing))
         for start in (400 - M, 300 - M, 70):
             _check_far(cache, q, start, dtype)
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("M", [1, 40])
+@pytest.mark.parametrize("dtype,near,far", [(F16, (36.0, 0.0), (36.0, 5.0)), (BF16, (30.0, 1.0), (36.0, 0.0))], ids=["f16", "bf16"])
+def test_a_maximum_that_leaves_the_reach_of_whole_numbers(gpu, monkeypatch, dtype, near, far, M, splits):
+    """Scores round 2^20 / log2 e = 726817.6, where the reference of a chunk's row stops being a whole number: the maximum
+    moves by 5, past that border, when 330 tokens of e^-5 have been summed."""
+    _splits(monkeypatch, splits)
+    late = torch.arange(400) >= 330
+    more = [torch.where(late, b, a) for a, b in zip(near, far)]
+    cache, q = _scores(dtype, 400, 2, M, (708.0, 1.0, 1.0, 1.0), (1024.0, 1792.0, *more))
+    for start in (400 - M, 331):
+        _check_far(cache, q, start, dtype)
