@@ -5,6 +5,7 @@
 // (v_cvt_scalef32_pk_*_fp8), so the products stay 16-bit MFMAs on exact values. A floating code keeps its relative
 // step whatever the scale, so one power of two for 32 rows costs nothing until a channel lies 2^14 below the block's
 // largest value. Blocks never cross a page, and a tile of the attention kernels is one or two whole blocks.
+#include <limits>
 #include <type_traits>
 
 #include "../fa_common.h"
@@ -776,23 +777,25 @@ struct Kv8Chunk {
     int pair;
     int64_t before;
   };
+  typedef uint32_t Tiles;
+  static_assert((uint64_t)(kMaxCapacity / T) * 64 <= std::numeric_limits<Tiles>::max(), "64 row blocks of the longest sequence");
   __device__ static inline Place find(const Kv8AttendParams& p, int64_t at) {
     const int lane = threadIdx.x & 63, pairs = p.B * p.row_blocks;
     int64_t base = 0;
     for (int c = 0; c < pairs; c += 64) {
-      const int n = c + lane < pairs ? tiles_of(p, c + lane) : 0;  // at most 2^25: 64 of them fit 32 bits
-      int end = n;
+      const Tiles n = c + lane < pairs ? (Tiles)tiles_of(p, c + lane) : 0;
+      Tiles end = n;
 #pragma unroll
       for (int k = 1; k < 64; k *= 2) {
-        const int o = __shfl_up(end, k, 64);
+        const Tiles o = __shfl_up(end, k, 64);
         if (lane >= k) end += o;
       }
       const uint64_t hit = __ballot(at < base + end);
       if (hit != 0) {
         const int who = __builtin_ctzll(hit);
-        return {c + who, base + __builtin_amdgcn_readlane(end - n, who)};
+        return {c + who, base + (Tiles)__builtin_amdgcn_readlane((int)(end - n), who)};
       }
-      base += __builtin_amdgcn_readlane(end, 63);
+      base += (Tiles)__builtin_amdgcn_readlane((int)end, 63);
     }
     return {pairs, base};
   }

@@ -8,8 +8,8 @@ import torch
 
 import flash_atten
 import kv8
-from kv8_model import Model
-from test_kv8_gpu import BF16, F16, _deal, _i32, _rand
+from kv8_model import Model, check_attention
+from test_kv8_gpu import BF16, F16, _deal, _full, _i32, _rand
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +89,28 @@ def test_a_maximum_that_leaves_the_reach_of_whole_numbers(gpu, monkeypatch, dtyp
     cache, q = _scores(dtype, 400, 2, M, (708.0, 1.0, 1.0, 1.0), (1024.0, 1792.0, *more))
     for start in (400 - M, 331):
         _check_far(cache, q, start, dtype)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("splits", [5, 97])
+def test_shares_of_many_sequences(gpu, monkeypatch, D, splits):
+    """More than 64 row blocks on the line that workgroups share: 70 sequences of unequal lengths, some without rows."""
+    _splits(monkeypatch, splits)
+    B, H, Hk, M, capacity = 70, 2, 2, 40, 300
+    cache = _full(400 + D, B, Hk, capacity, D, 64, BF16)
+    q = _rand(401, B, H, M, D, dtype=BF16).cuda()
+    starts = [(b * 37) % (capacity - M) - (20 if b % 11 == 0 else 0) for b in range(B)]
+    counts = [0 if b % 9 == 4 else M - b % 3 for b in range(B)]
+    for causal in (True, False):
+        o, lse = flash_atten.sdpa_kv8(q, cache, _i32(*starts), count=_i32(*counts), is_causal=causal, return_lse=True)
+        check_attention(o, lse, *Model(cache).attention(q, starts, counts, causal=causal), (D, splits, causal))
+
+
+@pytest.mark.parametrize("splits", [3, 250])
+def test_shares_of_many_row_blocks(gpu, monkeypatch, splits):
+    """The same with one sequence: 69 blocks of 128 rows, 8 heads that share 1200 keys."""
+    _splits(monkeypatch, splits)
+    cache = _full(410, 1, 1, 1200, 64, 64, F16)
+    q = _rand(411, 1, 8, 1100, 64, dtype=F16).cuda()
+    o, lse = flash_atten.sdpa_kv8(q, cache, _i32(100), return_lse=True)
+    check_attention(o, lse, *Model(cache).attention(q, [100]), splits)
