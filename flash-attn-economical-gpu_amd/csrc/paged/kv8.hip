@@ -1008,7 +1008,9 @@ struct Kv8Chunk {
         for (int j = 0; j < QT; ++j) {
           // each row by itself: what another row of the wave sees does not change its bits
           float to = offset_of<Tag>(tops[j], p.c);
-          const float back = Reference::of<Tag>(m[j], off[j]).less(Reference::of<Tag>(tops[j], to), p.c);
+          float back = to - off[j];
+          if (__builtin_expect(__any(!(fmaxf(fabsf(to), fabsf(off[j])) <= kLargeR)), 0))
+            back = Reference::of<Tag>(m[j], off[j]).less(Reference::of<Tag>(tops[j], to), p.c);
           const float f = m[j] == FA_NEG_INF ? 0.f : (move[j] ? fast_exp2(back) : 1.f);
           to = move[j] ? to : off[j];
           l[j] *= f;
