@@ -425,6 +425,7 @@ def sdpa_kv8(query: torch.Tensor, cache: kv8.Kv8Cache, start: torch.Tensor, *, c
     """Attention of new tokens' queries [B, H, M, D] over a layer of a paged 8-bit cache that already holds their keys:
     `sdpa_kv4`'s rules for rows, lengths, empty rows and NaN, and its layout. Tokens whose page is missing are not seen.
     start and count are int32 [B] on the GPU; nothing synchronises, and the call can be captured into a HIP graph."""
+    cache._layer(layer)  # before the look-up: 1.0 is equal to 1, and no layer
     key = (cache._form, _form(query), kv4._form(start), None if count is None else kv4._form(count), layer, bool(is_causal),
            None if scale is None else float(scale), bool(return_lse))
     plan = _plans.get(key)
@@ -438,7 +439,6 @@ def sdpa_kv8(query: torch.Tensor, cache: kv8.Kv8Cache, start: torch.Tensor, *, c
                              f"heads of {cache.head_dim}")
         if query.dtype != cache.dtype or query.device != cache.device:
             raise ValueError(f"query is {query.dtype} on {query.device}, the cache {cache.dtype} on {cache.device}")
-        cache._layer(layer)
         start, count = cache.positions(start, count)
         query = hip_lib.operand(query, "query")
     B, H, M, D = query.shape

@@ -144,13 +144,14 @@ class Kv8Cache:
         length from here on. Rows outside the capacity, or whose page is missing or shared, are dropped (`reserve`
         comes first). With return_values, returns what the rows now stand for (zeros in rows that were not written), in
         k's type, for a layer that goes on with the values its later steps will see."""
+        self._layer(layer)  # before the look-up: 1.0 is equal to 1, and no layer
         key = (self._form, _form(k), _form(v), _form(start), None if count is None else _form(count), layer,
                bool(return_values))
         plan = _plans.get(key)
         if plan is None or (k.data_ptr() | v.data_ptr()) & 15:
             k, v, start, count = self._append_operands(k, v, start, count)
             values = (hip_lib.dense_like(k), hip_lib.dense_like(v)) if return_values else (None, None)
-            plan = hip_lib.kv8_append_plan(k, v, *values, layer=self._layer(layer))
+            plan = hip_lib.kv8_append_plan(k, v, *values, layer=layer)
             if key == (self._form, _form(k), _form(v), _form(start), None if count is None else _form(count), layer,
                        bool(return_values)):  # nothing had to be copied: calls of this form take the short way
                 keep_plan(key, plan)
@@ -192,10 +193,9 @@ class Kv8Cache:
         start, count = self.positions(start, count)
         return hip_lib.operand(k, "k"), hip_lib.operand(v, "v"), start, count
 
-    def _layer(self, layer: int) -> int:
+    def _layer(self, layer: int) -> None:
         if not isinstance(layer, int) or not 0 <= layer < self.layers:
             raise ValueError(f"layer {layer!r} of a cache with {self.layers}")
-        return layer
 
     def _lengths(self, name: str, t: torch.Tensor) -> torch.Tensor:
         if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or tuple(t.shape) != (self.batch,) or t.device != self.device:

@@ -114,3 +114,17 @@ def test_shares_of_many_row_blocks(gpu, monkeypatch, splits):
     q = _rand(411, 1, 8, 1100, 64, dtype=F16).cuda()
     o, lse = flash_atten.sdpa_kv8(q, cache, _i32(100), return_lse=True)
     check_attention(o, lse, *Model(cache).attention(q, [100]), splits)
+
+
+def test_a_layer_is_a_whole_number(gpu):
+    """Also when a call of the same form has been made for the layer that the number is equal to."""
+    cache = _full(420, 1, 2, 64, 64, 64, F16, layers=2)
+    q, start = _rand(421, 1, 2, 3, 64, dtype=F16).cuda(), _i32(20)
+    for layer in (1, 1.0, torch.tensor(1), "1"):
+        calls = (lambda: cache.append(q, q, start, layer=layer), lambda: flash_atten.sdpa_kv8(q, cache, start, layer=layer))
+        for call in calls:
+            if type(layer) is int:
+                call()
+            else:
+                with pytest.raises(ValueError, match="layer"):
+                    call()
