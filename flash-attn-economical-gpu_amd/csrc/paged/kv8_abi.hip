@@ -31,6 +31,13 @@ int check_buffers(const kv8_cache* c) {
   if (c->pages > 1 && c->page_stride < kv8_page_bytes(c->H_kv, c->page, c->D))
     return fail(FA_EINVAL, "page stride %lld is under a page's %lld bytes", (long long)c->page_stride,
                 (long long)kv8_page_bytes(c->H_kv, c->page, c->D));
+  if (c->layers > 1) {  // whole layers behind each other, or a page's layers
+    const __int128 page = kv8_page_bytes(c->H_kv, c->page, c->D);
+    const __int128 layer = page + (c->pages > 1 ? (c->pages - 1) * (__int128)c->page_stride : 0);
+    const __int128 stack = page + (c->layers - 1) * (__int128)c->layer_stride;
+    if (c->layer_stride < layer && (c->layer_stride < page || c->page_stride < stack))
+      return fail(FA_EINVAL, "layers %lld bytes apart overlap", (long long)c->layer_stride);
+  }
   return FA_OK;
 }
 

@@ -350,7 +350,8 @@ int64_t kv4_attend_workspace_bytes(int32_t B, int32_t H, int32_t M, int32_t D, i
 int32_t kv4_attend_splits(int32_t B, int32_t H, int32_t H_kv, int32_t M, int32_t D, int32_t capacity);
 
 /* Key/value cache of 8-bit codes in pages. A page holds `page` tokens (32, 64, 128 or 256) of every kv head, in each of
- * `layers` layers; `data` is [layers][pages] of them, layer_stride and page_stride bytes apart (multiples of 16). A page is
+ * `layers` layers; `data` is [layers][pages] of them, layer_stride and page_stride bytes apart (multiples of 16; whole
+ * layers, or a page's layers, one behind the other: layers that overlap are refused). A page is
  *   codes   [H_kv][2][page][D]      keys, then values, one byte a channel: e4m3 (sign, 4 exponent bits, 3 mantissa bits;
  *                                   largest 448, 127 and 255 are NaN)
  *   scales  [H_kv][page / 32][2]    keys', then values': byte e stands for 2^(e - 127)
