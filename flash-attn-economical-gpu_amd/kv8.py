@@ -125,7 +125,9 @@ class Kv8Cache:
         without a count). In order of sequence and token, an entry without a page takes the lowest free page; one whose
         page has other holders takes the lowest free page and a copy of it in all layers (but for the last such entry
         of a page whose holders are all among them, which keeps it). Returns how many pages were wanting, int32 [1] on
-        the GPU: those entries stay as they are, and appends to them are dropped."""
+        the GPU: those entries stay as they are, and appends to them are dropped. So are appends to a page that its last
+        holder keeps while one of the others still waits: the page has two holders until a later `reserve` finds
+        it a free one."""
         if not isinstance(rows, int) or rows < 0:
             raise ValueError(f"rows must be a number of tokens, got {rows!r}")
         rows = min(rows, 2 ** 31 - 1)

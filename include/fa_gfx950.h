@@ -425,8 +425,9 @@ int32_t kv8_attend_splits(int32_t B, int32_t H, int32_t H_kv, int32_t M, int32_t
 /* Pages for tokens start[b] .. start[b] + n - 1 inside the capacity, n = min(rows, count[b]) (rows without a count), that
  * append may write. In order of sequence and token: an entry without a page takes the lowest free page; one whose page
  * has other holders takes the lowest free page and a copy of all layers of it, but for the last such entry of a page where
- * all its holders are among them: it keeps the page. Where no page is free any more entries stay as they are.
- * missing (int32 [1], device memory) receives how many. workspace: kv8_reserve_workspace_bytes(), 16-byte aligned. */
+ * all its holders are among them: it keeps the page. Where no page is free any more entries stay as they are,
+ * and a page that is kept has other holders as long as one of them waits. missing (int32 [1], device memory) receives how
+ * many entries wait. workspace: kv8_reserve_workspace_bytes(), 16-byte aligned. */
 typedef struct {
   kv8_cache cache;
   const int32_t* start;

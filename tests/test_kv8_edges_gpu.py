@@ -128,3 +128,30 @@ def test_a_layer_is_a_whole_number(gpu):
             else:
                 with pytest.raises(ValueError, match="layer"):
                     call()
+
+
+def test_a_kept_page_waits_for_its_last_copy(gpu):
+    """Three holders of a page write and one page is free: the first gets its copy, the second is counted as missing, and the
+    last, which keeps the page, cannot write it either until a later call has given the second one a page."""
+    cache = kv8.Kv8Cache(4, 1, 64, 64, dtype=F16, pages=3, page_size=64)
+    start, three = _i32(10, 10, 10, 0), _i32(1, 1, 1, 0)
+    assert int(cache.reserve(_i32(0, 0, 0, 0), 64, count=_i32(10, 0, 0, 64))) == 0
+    rows = _rand(430, 4, 1, 10, 64, dtype=F16).cuda()
+    cache.append(rows, rows, _i32(0, 0, 0, 0), count=_i32(10, 0, 0, 10))
+    cache.fork(_i32(0, 0, 0, 3))
+    model = Model(cache)
+    new = _rand(431, 4, 1, 1, 64, dtype=F16)
+
+    def both():
+        left = int(cache.reserve(start, 1, count=three))
+        assert left == model.reserve([10, 10, 10, 0], 1, [1, 1, 1, 0])
+        held = cache.append(new.cuda(), new.cuda(), start, count=three, return_values=True)[0]
+        want = model.append(new, new, [10, 10, 10, 0], [1, 1, 1, 0])[0]
+        model.check(cache)
+        assert torch.equal(held.double().cpu(), want)
+        return left, [bool(x.any()) for x in held]
+
+    assert both() == (1, [True, False, False, False])
+    cache.truncate(_i32(64, 64, 64, 0))
+    model.truncate([64, 64, 64, 0])
+    assert both() == (0, [True, True, True, False])
