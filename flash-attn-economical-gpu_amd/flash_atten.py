@@ -424,7 +424,8 @@ def sdpa_kv8(query: torch.Tensor, cache: kv8.Kv8Cache, start: torch.Tensor, *, c
              layer: int = 0, is_causal: bool = True, scale: float | None = None, return_lse: bool = False):
     """Attention of new tokens' queries [B, H, M, D] over a layer of a paged 8-bit cache that already holds their keys:
     `sdpa_kv4`'s rules for rows, lengths, empty rows and NaN, and its layout. Tokens whose page is missing are not seen.
-    start and count are int32 [B] on the GPU; nothing synchronises, and the call can be captured into a HIP graph."""
+    start and count are int32 [B] on the GPU; nothing synchronises, and the call can be captured into a HIP graph. The result
+    takes no part in autograd, whatever the query does: rounded keys and values have no gradient."""
     cache._layer(layer)  # before the look-up: 1.0 is equal to 1, and no layer
     key = (cache._form, _form(query), kv4._form(start), None if count is None else kv4._form(count), layer, bool(is_causal),
            None if scale is None else float(scale), bool(return_lse))

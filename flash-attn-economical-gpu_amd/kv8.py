@@ -145,7 +145,7 @@ class Kv8Cache:
         and the new rows; their tokens behind the new ones become zeros, so start[b] + count[b] is the sequence's
         length from here on. Rows outside the capacity, or whose page is missing or shared, are dropped (`reserve`
         comes first). With return_values, returns what the rows now stand for (zeros in rows that were not written), in
-        k's type, for a layer that goes on with the values its later steps will see."""
+        k's type, for a layer that goes on with the values its later steps will see. They take no part in autograd."""
         self._layer(layer)  # before the look-up: 1.0 is equal to 1, and no layer
         key = (self._form, _form(k), _form(v), _form(start), None if count is None else _form(count), layer,
                bool(return_values))

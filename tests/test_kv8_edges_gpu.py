@@ -155,3 +155,16 @@ def test_a_kept_page_waits_for_its_last_copy(gpu):
     cache.truncate(_i32(64, 64, 64, 0))
     model.truncate([64, 64, 64, 0])
     assert both() == (0, [True, True, True, False])
+
+
+def test_results_take_no_part_in_autograd(gpu):
+    """They are the bits of a call without gradients, and nothing of a graph."""
+    cache = _full(440, 1, 2, 64, 64, 64, BF16)
+    q, k = (_rand(441 + i, 1, 2, 3, 64, dtype=BF16).cuda() for i in range(2))
+    held = cache.append(k, k, _i32(20), return_values=True)
+    o, lse = flash_atten.sdpa_kv8(q, cache, _i32(20), return_lse=True)
+    q.requires_grad_()
+    k.requires_grad_()
+    again = (*cache.append(k, k, _i32(20), return_values=True), *flash_atten.sdpa_kv8(q, cache, _i32(20), return_lse=True))
+    for a, b in zip((*held, o, lse), again):
+        assert torch.equal(a, b) and not b.requires_grad
