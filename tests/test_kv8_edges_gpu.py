@@ -168,3 +168,27 @@ def test_results_take_no_part_in_autograd(gpu):
     again = (*cache.append(k, k, _i32(20), return_values=True), *flash_atten.sdpa_kv8(q, cache, _i32(20), return_lse=True))
     for a, b in zip((*held, o, lse), again):
         assert torch.equal(a, b) and not b.requires_grad
+
+
+def test_what_compact_leaves_can_be_moved(gpu):
+    """Pages [0, used) of every layer, the table and the counts are the state: a smaller pool that they are copied into answers
+    with the same bits."""
+    cache = kv8.Kv8Cache(3, 2, 200, 64, dtype=F16, pages=40, page_size=32, layers=2)
+    zero, n = _i32(0, 0, 0), _i32(200, 33, 150)
+    _deal(cache, [200, 33, 150], 4)
+    for layer in range(2):
+        k, v = (_rand(450 + 2 * layer + i, 3, 2, 200, 64, dtype=F16).cuda() for i in range(2))
+        cache.append(k, v, zero, count=n, layer=layer)
+    cache.fork(_i32(0, 1, 0))
+    cache.truncate(_i32(200, 0, 97))
+    q, start = _rand(460, 3, 4, 2, 64, dtype=F16).cuda(), _i32(198, 0, 95)
+    want = [flash_atten.sdpa_kv8(q, cache, start, layer=i) for i in range(2)]
+    used = int(cache.compact())
+    assert used == 7 == int((cache.refs > 0).sum())
+    small = kv8.Kv8Cache(3, 2, 200, 64, dtype=F16, pages=used, page_size=32, layers=2)
+    small.table.copy_(cache.table)
+    small.refs.copy_(cache.refs[:used])
+    for a, b in zip((small.k_codes, small.v_codes, small.k_scales, small.v_scales), (cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales)):
+        a.copy_(b[:, :used])
+    for other in (cache, small):
+        assert all(torch.equal(a, flash_atten.sdpa_kv8(q, other, start, layer=i)) for i, a in enumerate(want))
