@@ -232,8 +232,7 @@ struct Kv8KernelEntry {
   const void* attend[3];  // 16 rows shared by a workgroup's waves, 32 rows shared, chunks of a prompt
   const void* join;       // of the last one's parts
   int32_t per_cu[3];      // workgroups of each that the split rule counts on per CU
-  int32_t chunk_rows;     // query rows of a workgroup of the last, and its keys at a time
-  int32_t chunk_keys;
+  int32_t chunk_rows;     // query rows of a workgroup of the last
   int32_t join_rows;      // rows of a joining workgroup
 };
 

@@ -313,12 +313,6 @@ struct Blocks {
   int at[2];
   float ks, vs;
 
-  struct Place {
-    int64_t at;
-    float ks, vs;
-    bool there;
-  };
-
   __device__ inline Blocks(const Kv8Pages& c, int b, int hk) {
     half = (int64_t)(32 * D) << c.blocks_log2;
     table = c.table + (int64_t)b * c.columns;
@@ -1268,7 +1262,7 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void kv8_merge_kernel(Kv8At
    {(const void*)&kv8_attend_kernel<TAG, D, 1>, attend_two_tiles<TAG, D>(), (const void*)&kv8_chunk_kernel<TAG, D>}, \
    (const void*)&kv8_join_kernel<TAG, D>,                                                                   \
    {attend8_waves<D, 1>(), attend8_waves<D, 2>(), chunk8_waves<D>()},                                       \
-   Kv8Chunk<TAG, D>::BLOCK, Kv8Chunk<TAG, D>::T, kJoinRows}
+   Kv8Chunk<TAG, D>::BLOCK, kJoinRows}
 
 static const Kv8KernelEntry kKv8Entries[] = {
     KV8_ENTRY(f16_t, FA_DTYPE_F16, 64),   KV8_ENTRY(f16_t, FA_DTYPE_F16, 128),   KV8_ENTRY(f16_t, FA_DTYPE_F16, 256),
