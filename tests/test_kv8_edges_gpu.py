@@ -192,3 +192,46 @@ def test_what_compact_leaves_can_be_moved(gpu):
         a.copy_(b[:, :used])
     for other in (cache, small):
         assert all(torch.equal(a, flash_atten.sdpa_kv8(q, other, start, layer=i)) for i, a in enumerate(want))
+
+
+@pytest.mark.parametrize("D,H,M", [(64, 2, 1), (128, 2, 1), (256, 2, 1), (128, 8, 5), (64, 8, 8), (256, 8, 8)])
+def test_many_tiles_in_one_split(gpu, monkeypatch, D, H, M):
+    """9000 tokens by one workgroup: its waves look up their 64 blocks more than once. Pages lie in no order, and some are
+    missing, in the first look-up, in the second, and at the border between them."""
+    _splits(monkeypatch, 1)
+    capacity = 9000
+    cache = _full(470 + D, 1, 2, capacity, D, 64, BF16)
+    for token in (700, 8160, 8192, 8256, 8900):
+        cache.table[0, token // 64] = -1
+    q = _rand(471, 1, H, M, D, dtype=BF16).cuda()
+    for start in (capacity - M, 8192 - M, 8192):
+        o, lse = flash_atten.sdpa_kv8(q, cache, _i32(start), return_lse=True)
+        check_attention(o, lse, *Model(cache).attention(q, [start]), (D, M, start))
+
+
+@pytest.mark.parametrize("splits", [None, 1, 4])
+@pytest.mark.parametrize("B,H,M", [(70, 4, 1), (130, 2, 6)])
+def test_splits_of_many_sequences(gpu, monkeypatch, B, H, M, splits):
+    """More than 64 sequences of unequal lengths, some empty, by single tokens and drafts."""
+    if splits is not None:
+        _splits(monkeypatch, splits)
+    capacity = 1300
+    cache = _full(480, B, 2, capacity, 64, 128, F16)
+    q = _rand(481, B, H, M, 64, dtype=F16).cuda()
+    starts = [(b * 331) % (capacity - M) for b in range(B)]
+    counts = [0 if b % 13 == 5 else M for b in range(B)]
+    o, lse = flash_atten.sdpa_kv8(q, cache, _i32(*starts), count=_i32(*counts), return_lse=True)
+    check_attention(o, lse, *Model(cache).attention(q, starts, counts), (B, M, splits))
+
+
+@pytest.mark.parametrize("D,M", [(128, 33), (256, 65)])
+def test_whole_row_blocks_by_the_rule(gpu, D, M):
+    """So many row blocks that each workgroup takes a whole one, the longest first, without `choose_splits` being told."""
+    B, H, capacity = 128, 8 if M < 64 else 4, 100
+    assert kv8.choose_splits(B, H, H, M, D, capacity) == 1
+    cache = _full(490, B, H, capacity, D, 32, F16)
+    q = _rand(491, B, H, M, D, dtype=F16).cuda()
+    starts = [(b * 7) % (capacity - M + 1) for b in range(B)]
+    counts = [M - b % 40 if b % 10 else 0 for b in range(B)]
+    o, lse = flash_atten.sdpa_kv8(q, cache, _i32(*starts), count=_i32(*counts), return_lse=True)
+    check_attention(o, lse, *Model(cache).attention(q, starts, counts), (D, M))
