@@ -361,8 +361,12 @@ __device__ inline void for_each(Fn& f) {
 //   S^T = K Q^T     A = K rows: lane (key, 16 of each 64 channels) reads its channels and converts them in place
 //   O^T += V^T P^T  A = V^T: lane (channels, 8 keys) reads the keys' codes of its D / 16 channels, converts, and
 //                   regroups them by channel with byte permutes; P^T is S^T's accumulator as it stands
-// so nothing passes through LDS but the waves' sums at the end. A lane keeps the table entries of its wave's next 64
-// tiles, so that a page number costs no load in the loop; a tile without a page is one that no row sees.
+// so nothing passes through LDS but the waves' sums at the end. P is rounded to the type once, on its way to the second
+// product, as the prompt chunks' is: weights in two 16-bit halves would double that product and P's registers. Sums and
+// lse take the unrounded weights. Results are off from 64 bits by 1.9e-3 (bf16) and 2.4e-4 (fp16) of their norm, chunks' by
+// 2.3e-3 and 2.9e-4, where fp32 weights and the result's rounding alone leave 1.6e-3 and 2.1e-4.
+// A lane keeps the table entries of its wave's next 64 tiles, so that a page number costs no load in the loop; a tile
+// without a page is one that no row sees.
 // The four waves hold the same rows and take turns at the tiles. A wave has one tile's registers: the next tile's keys are
 // asked for when the scores stand, its values when the second product does, so that half a tile or more is in flight.
 // Bound by memory where there is enough of it: 8 sequences of 16-32k keys, 8 kv heads, D = 128 (419 MB), 78 us, 5.4 TB/s.
@@ -720,14 +724,14 @@ constexpr const void* attend_two_tiles() {
 // conversion: a tile's codes are loaded a tile ahead, 16 channels of a row to a thread and step, converted once into
 // 16-bit rows in LDS (two stages, one barrier a tile), and both products read their fragments there, V's by the
 // transposing read. S^T = K Q^T and O^T = V^T P^T as above. The chip's workgroups take equal shares of all blocks' tiles,
-// or whole blocks where there are at least two to a place, the longest first: 2 x 32 heads of a first 2048 rows 93 us whole
-// and 167 in shares; 2 x 28 heads of 509 rows against 12-16k keys (not even one to a place) 261 in shares and 598 whole (both
-// before fragments were asked for ahead: 88 and 245 since).
-// Products of 1024 rows against 32k keys, 32/8 heads, D = 128 run at 1000 TFLOP/s, of a first 2048 rows at 775, D = 64 at
-// 690 and D = 256 at 755. Bound by two waves to a SIMD (registers, LDS): matrix unit, vector unit and LDS are busy about
-// half of the time each, and overlap as far as two waves let them. Eight waves in two groups that take turns at products
-// and softmax were 5 to 25% slower than four (without fragments ahead), their barriers cost more than the overlap gave.
+// or whole blocks where there are at least two to a place, the longest first (both sides measured at kv8_attend_splits).
+// Products of 1024 rows against 32k keys, 32/8 heads, bf16, D = 128 run at 970 to 1000 TFLOP/s by card, of a first 2048 rows
+// at 770, fp16 D = 64 at 690 and D = 256 at 755. Bound by two waves to a SIMD (registers, LDS): matrix unit, vector unit and
+// LDS are busy about half of the time each, and overlap as far as two waves let them. Eight waves in two groups that take
+// turns at products and softmax were 5 to 25% slower than four (without fragments ahead), their barriers cost more than the
+// overlap gave.
 // Sums of the rounded weights by the matrix unit gave 1 to 5% and an lse of 16-bit weights: the sums stay in the vector unit.
+
 // Fewest key tiles to a workgroup's share: below, the parts' extra pass costs more than it gives.
 constexpr int kMinShare = 4;
 
@@ -743,8 +747,9 @@ struct Kv8Chunk {
   static constexpr int BLOCK = WAVES * QT * 16;
   static constexpr int TILEB = T * L::ROWB, STAGEB = 2 * TILEB;
   static constexpr int SMEM = 2 * STAGEB;
-  // Fragments in flight, as the registers allow: at D = 128 (255 of them) 244 us with 8 for 2 x 28 heads of 509 rows, 252 with
-  // 4; at D = 256 709 us with 8 for 2 x 16 heads of 1024, 701 with 4; at D = 64 4 spills ten registers where 3 spills four.
+  // Fragments in flight, as the registers allow: at D = 128 (255 of them in bf16, all 256 in fp16) 244 us with 8 for 2 x 28
+  // heads of 509 rows, 252 with 4; at D = 256 709 us with 8 for 2 x 16 heads of 1024, 701 with 4; at D = 64 4 spills ten
+  // registers in bf16, 3 spills four (five in fp16).
   static constexpr int kAhead = D == 64 ? 3 : (D == 128 ? 8 : 4);
   static constexpr int PER = T * UPR / 256;  // 16-channel units of K, and of V, per thread
   static_assert(PER * 256 == T * UPR, "units");
@@ -1195,7 +1200,9 @@ __device__ inline void join_parts(const Kv8AttendParams& p) {
       // A part's reference is a score (rare). The largest is looked for by what they are about, by every lane in all parts.
       Reference top = {0.f, false};
       m = FA_NEG_INF;
-      auto reference = [&](int s) { return Reference{p.ws_ml[2 * place(s)], __builtin_signbitf(p.ws_ml[2 * place(s) + 1]) != 0}; };
+      auto reference = [&](int s) {
+        return Reference{p.ws_ml[2 * place(s)], __builtin_signbitf(p.ws_ml[2 * place(s) + 1]) != 0};
+      };
       for (int s = 0; s < n; ++s) {
         const Reference r = reference(s);
         const float about = r.score ? r.at * p.c : r.at;
@@ -1237,8 +1244,8 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttendParams p) {
   join_parts<Tag, D, Kv8Chunk<Tag, D>::BLOCK>(p);
 }
 
-// Workgroups to a CU. At D = 64 the third costs 4 spilled registers, and 1024 rows against 16k keys twice took 207 us
-// where two workgroups took 221 (193 now).
+// Workgroups to a CU. At D = 64 the third costs 4 spilled registers (5 in fp16), and 1024 rows against 16k keys twice took
+// 207 us where two workgroups took 221 (192 now).
 template <int D>
 constexpr int chunk8_waves() {
   return D == 64 ? 3 : 2;

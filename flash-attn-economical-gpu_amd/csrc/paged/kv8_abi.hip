@@ -237,7 +237,11 @@ int32_t kv8_attend_splits(int32_t B, int32_t H, int32_t H_kv, int32_t M, int32_t
   const int64_t blocks = (int64_t)B * H_kv * k.row_blocks, room = 256LL * e->per_cu[k.kind];
   // as many as the chip (256 CUs) holds at once, none with less than 256 keys of a full cache
   if (k.kind == 2) {
-    // twice as many blocks as fit are given out whole, the longest first: nothing is left to join
+    // Twice as many blocks as fit are given out whole, the longest first: nothing is left to join. Whole / shares, us: two
+    // sequences' first 2048 rows (32/8 heads, 1024 blocks) 88 / 156, one sequence's first 4096 157 / 217; below that, 512 rows
+    // against 32k keys (128 blocks) 736 / 293, 2 x 509 against 16k (224) 537 / 305, 100 rows of 8/2 heads against 4k (8) 133 / 30.
+    // The number of blocks alone does not tell: blocks that fit at once and are short are faster whole too (first 512 rows
+    // 20 / 35, first 2048 rows of one sequence 60 / 97, 1024 rows of 16/4 heads, D = 256, against 16k 670 / 693).
     if (blocks >= 2 * room) return 1;
     const int64_t most = blocks * ((capacity + 255) / 256);
     return (int32_t)(most < room ? most : room);
