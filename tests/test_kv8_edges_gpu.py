@@ -235,3 +235,28 @@ def test_whole_row_blocks_by_the_rule(gpu, D, M):
     counts = [M - b % 40 if b % 10 else 0 for b in range(B)]
     o, lse = flash_atten.sdpa_kv8(q, cache, _i32(*starts), count=_i32(*counts), return_lse=True)
     check_attention(o, lse, *Model(cache).attention(q, starts, counts), (D, M))
+
+
+@pytest.mark.parametrize("M", [1, 40])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_nan_and_missing_pages_in_parts_far_from_zero(gpu, monkeypatch, D, M):
+    """Parts whose references are scores, next to one that holds a NaN key and one without a page: rows that see the key are
+    NaN, the others' bits stay."""
+    _splits(monkeypatch, 3)
+    cache, q = _scores(F16, 700, 2, M, (2.0 ** 12, 1.0), (2.0 ** 12, torch.arange(700) // 100 * 2.0), D)
+    start, nan = 700 - M, 700 - M // 2 - 1
+    for missing in (None, 300 // 64):
+        if missing is not None:
+            cache.table[0, missing] = -1
+        clean, clean_lse = flash_atten.sdpa_kv8(q, cache, _i32(start), scale=1.0, return_lse=True)
+        want, want_lse, bound = Model(cache).attention(q, [start], scale=1.0)
+        assert torch.isfinite(clean).all()
+        assert ((clean.double().cpu() - want).abs() <= 1.01 * bound).all()
+        page = cache.table[0, nan // 64].long()
+        was = cache.k_codes[0, page, :, nan % 64, 3].clone()
+        cache.k_codes[0, page, :, nan % 64, 3] = 127
+        o, lse = flash_atten.sdpa_kv8(q, cache, _i32(start), scale=1.0, return_lse=True)
+        cache.k_codes[0, page, :, nan % 64, 3] = was
+        first = nan - start
+        assert torch.equal(o[:, :, :first], clean[:, :, :first]) and torch.equal(lse[:, :, :first], clean_lse[:, :, :first])
+        assert torch.isnan(o[:, :, first:]).all() and torch.isnan(lse[:, :, first:]).all()
